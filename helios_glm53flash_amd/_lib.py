@@ -30,6 +30,10 @@ class ExpertTablesC(C.Structure):
         "down_trellis", "down_suh", "down_svh", "gate_bits", "up_bits", "down_bits")] + [("bits_mask", C.c_uint32)]
 
 
+class W4WordsC(C.Structure):
+    _fields_ = [("words", C.c_void_p), ("scales", C.c_void_p), ("zeros", C.c_void_p), ("group", C.c_int)]
+
+
 class ExpertLayoutC(C.Structure):
     _fields_ = [("off", C.c_uint64 * 12), ("piece", C.c_uint64 * 12), ("bits", C.c_int * 3), ("stride", C.c_uint64)]
 
@@ -77,6 +81,14 @@ SIGNATURES: dict[str, tuple] = {
                                  C.c_void_p]),
     "hx_gather_rows": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
     "hx_scatter_add_rows": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
+    "hx_w4_gemm": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(W4WordsC), C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
+    "hx_w4_embed": (C.c_int, [C.POINTER(W4WordsC), C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_float, C.c_int,
+                              C.c_void_p]),
+    "hx_beam_select_workspace_size": (C.c_size_t, [C.c_int] * 4),
+    "hx_beam_select": (C.c_int, [C.c_void_p] * 6 + [C.c_int] * 4 + [C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
+                                                                   C.c_size_t]),
+    "hx_beam_reorder": (C.c_int, [C.c_void_p] * 3 + [C.c_int] * 3 + [C.c_int64] * 3 +
+                        [C.POINTER(C.c_int64), C.POINTER(C.c_int64), C.c_void_p]),
     "hx_ckpt_open": (C.c_int, [C.c_char_p, C.POINTER(C.c_void_p)]),
     "hx_ckpt_close": (None, [C.c_void_p]),
     "hx_ckpt_tensor_count": (C.c_int, [C.c_void_p]),

@@ -479,6 +479,140 @@ int hx_gemm_nt_f16(void* y, const void* x, const void* w, int M, int N, int K, i
                       "hx_gemm_nt_f16");
 }
 
+// ------------------------------------------------------------------ 4-bit words with group scales
+
+namespace {
+
+// Checks a linear's words and fills the kernels' arguments; `who` opens the error text.
+int w4_args(const hx_w4_words* w, int N, int K, hx::W4Args* a, const char* who)
+{
+    const char* what = nullptr;
+    if (!w || !w->words || !w->scales) what = "null pointer";
+    else if (N <= 0 || K <= 0 || K % 32) what = "N and K must be positive and K a multiple of 32";
+    else if (K > (1 << 24)) what = "K must be at most 2^24";
+    else if (w->group < 32 || (w->group & (w->group - 1))) what = "group must be a power of two of at least 32";
+    else if ((uintptr_t)w->words & 15) what = "words must be 16-byte aligned";
+    else if ((uintptr_t)w->scales & 1) what = "scales must be 2-byte aligned";
+    if (what) {
+        snprintf(g_err, sizeof(g_err), "%s: %s", who, what);
+        return HX_ERR_INVALID;
+    }
+    *a = {static_cast<const uint32_t*>(w->words), static_cast<const _Float16*>(w->scales),
+          static_cast<const uint8_t*>(w->zeros), N, K, (K + w->group - 1) / w->group, __builtin_ctz((unsigned)w->group)};
+    return 0;
+}
+
+}  // namespace
+
+int hx_w4_gemm(void* y, const void* x, const hx_w4_words* w, int M, int N, int K, int y_fp32, hx_stream_t stream)
+{
+    hx::W4Args a;
+    const int r = w4_args(w, N, K, &a, "hx_w4_gemm");
+    if (r) return r;
+    if (M < 0) return fail(HX_ERR_INVALID, "hx_w4_gemm: negative M");
+    if (M == 0) return 0;
+    if (!y || !x) return fail(HX_ERR_INVALID, "hx_w4_gemm: null pointer");
+    if ((uintptr_t)x & 15) return fail(HX_ERR_INVALID, "hx_w4_gemm: x must be 16-byte aligned");
+    if ((uintptr_t)y & (y_fp32 ? 3 : 1)) return fail(HX_ERR_INVALID, "hx_w4_gemm: y is not aligned to its type");
+    return hip_status(hx::launch_w4_gemm(static_cast<const _Float16*>(x), a, y, M, y_fp32 != 0, (hipStream_t)stream),
+                      "hx_w4_gemm");
+}
+
+int hx_w4_embed(const hx_w4_words* w, const int64_t* tokens, void* out, int n, int N, int K, float scale, int out_fp32,
+                hx_stream_t stream)
+{
+    hx::W4Args a;
+    const int r = w4_args(w, N, K, &a, "hx_w4_embed");
+    if (r) return r;
+    if (n < 0) return fail(HX_ERR_INVALID, "hx_w4_embed: negative number of tokens");
+    if (n == 0) return 0;
+    if (!tokens || !out) return fail(HX_ERR_INVALID, "hx_w4_embed: null pointer");
+    if (((uintptr_t)out & 15) || ((uintptr_t)tokens & 7))
+        return fail(HX_ERR_INVALID, "hx_w4_embed: out must be 16-byte and tokens 8-byte aligned");
+    return hip_status(hx::launch_w4_embed(a, tokens, out, n, scale, out_fp32 != 0, (hipStream_t)stream), "hx_w4_embed");
+}
+
+// ------------------------------------------------------------------ beam search
+
+size_t hx_beam_select_workspace_size(int batch, int beams, int vocab, int n)
+{
+    if (batch <= 0 || beams <= 0 || vocab <= 0 || n <= 0) return 0;
+    return hx::beam_select_workspace_bytes(batch, beams, vocab, n);
+}
+
+int hx_beam_select(const void* logits, const float* cum, const uint8_t* done, float* scores, int64_t* parents,
+                   int64_t* tokens, int batch, int beams, int vocab, int n, int64_t ld, int eos, int dtype,
+                   hx_stream_t stream, void* workspace, size_t workspace_bytes)
+{
+    if (batch < 0 || batch > hx::BEAM_MAX_BATCH || beams <= 0 || vocab <= 0 || n <= 0 || n > hx::BEAM_MAX_N)
+        return fail(HX_ERR_INVALID, "hx_beam_select: batch must be in [0, 4096], n in [1, 128], beams and vocab positive");
+    if (beams > hx::BEAM_MAX_BEAMS) return fail(HX_ERR_INVALID, "hx_beam_select: at most 1024 beams");
+    if (ld < vocab) return fail(HX_ERR_INVALID, "hx_beam_select: rows of logits overlap (ld < vocab)");
+    if (dtype != HX_DTYPE_HALF && dtype != HX_DTYPE_FLOAT)
+        return fail(HX_ERR_INVALID, "hx_beam_select: dtype must be HX_DTYPE_HALF or HX_DTYPE_FLOAT");
+    if (done && (eos < 0 || eos >= vocab)) return fail(HX_ERR_INVALID, "hx_beam_select: eos outside the vocabulary");
+    if (batch == 0) return 0;
+    if (!logits || !cum || !scores || !parents || !tokens) return fail(HX_ERR_INVALID, "hx_beam_select: null pointer");
+    if (((uintptr_t)logits & (dtype == HX_DTYPE_FLOAT ? 3 : 1)) || (((uintptr_t)cum | (uintptr_t)scores) & 3) ||
+        (((uintptr_t)parents | (uintptr_t)tokens) & 7))
+        return fail(HX_ERR_INVALID, "hx_beam_select: a pointer is not aligned to its type");
+    if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < hx::beam_select_workspace_bytes(batch, beams, vocab, n))
+        return fail(HX_ERR_WORKSPACE, "hx_beam_select: workspace missing, not 16-byte aligned or smaller than "
+                                      "hx_beam_select_workspace_size");
+    const hx::BeamArgs a{cum, done, scores, parents, tokens, (long)ld, batch, beams, vocab, n, eos};
+    return hip_status(hx::launch_beam_select(logits, dtype == HX_DTYPE_FLOAT, a, workspace, (hipStream_t)stream),
+                      "hx_beam_select");
+}
+
+namespace {
+
+// Bytes that pieces at these strides span, or -1 where two pieces of different index may share a byte (`apart`), a
+// stride is negative, or the span does not fit 62 bits.
+int64_t reorder_span(int64_t bytes, const int64_t* count, const int64_t* stride, bool apart)
+{
+    int order[3] = {0, 1, 2};
+    for (int i = 0; i < 2; ++i)
+        for (int j = 0; j < 2 - i; ++j)
+            if (stride[order[j]] > stride[order[j + 1]]) {
+                const int t = order[j];
+                order[j] = order[j + 1];
+                order[j + 1] = t;
+            }
+    __int128 span = bytes;
+    for (int i : order) {
+        if (count[i] == 1) continue;
+        if (stride[i] < 0 || (apart && stride[i] < span)) return -1;
+        span += (__int128)(count[i] - 1) * stride[i];
+        if (span >> 62) return -1;
+    }
+    return (int64_t)span;
+}
+
+}  // namespace
+
+int hx_beam_reorder(const void* src, const int64_t* parents, void* dst, int batch, int beams, int out_beams, int64_t outer,
+                    int64_t inner, int64_t bytes, const int64_t src_stride[3], const int64_t dst_stride[3],
+                    hx_stream_t stream)
+{
+    if (batch < 0 || beams <= 0 || out_beams < 0 || outer < 0 || inner < 0 || bytes < 0)
+        return fail(HX_ERR_INVALID, "hx_beam_reorder: negative extent or no beams");
+    if (!batch || !out_beams || !outer || !inner || !bytes) return 0;
+    if (!src || !parents || !dst || !src_stride || !dst_stride) return fail(HX_ERR_INVALID, "hx_beam_reorder: null pointer");
+    if ((uintptr_t)parents & 7) return fail(HX_ERR_INVALID, "hx_beam_reorder: parents must be 8-byte aligned");
+    if ((__int128)outer * batch * out_beams * inner >> 62) return fail(HX_ERR_INVALID, "hx_beam_reorder: extents too large");
+    const int64_t sc[3] = {outer, (int64_t)batch * beams, inner}, dc[3] = {outer, (int64_t)batch * out_beams, inner};
+    const int64_t ss = reorder_span(bytes, sc, src_stride, false), ds = reorder_span(bytes, dc, dst_stride, true);
+    if (ss < 0 || ds < 0) return fail(HX_ERR_INVALID, "hx_beam_reorder: a negative stride, or pieces of dst overlap");
+    const char *s = static_cast<const char*>(src), *d = static_cast<const char*>(dst);
+    if (s < d + ds && d < s + ss) return fail(HX_ERR_INVALID, "hx_beam_reorder: src and dst overlap");
+    hx::ReorderArgs p{outer, inner, bytes, {}, {}, batch, beams, out_beams};
+    for (int i = 0; i < 3; ++i) {  // the stride of an extent of one is never used and says nothing about alignment
+        p.src[i] = sc[i] == 1 ? 0 : src_stride[i];
+        p.dst[i] = dc[i] == 1 ? 0 : dst_stride[i];
+    }
+    return hip_status(hx::launch_beam_reorder(src, parents, dst, p, (hipStream_t)stream), "hx_beam_reorder");
+}
+
 // ------------------------------------------------------------------ MoE
 
 size_t hx_moe_workspace_size(int tokens, int hidden_dim, int intermediate_dim, int num_experts, int topk)

@@ -82,4 +82,37 @@ hipError_t launch_scatter_add_rows(float* y, const float* src, const int64_t* id
 hipError_t launch_gemm_nt_f16(const _Float16* x, const _Float16* w, void* y, int M, int N, int K, bool y_fp32,
                               bool add, hipStream_t st);
 
+
+// linear and row lookup over 4-bit words with group scales (hx_w4.hip; the words' layout is at its top)
+struct W4Args {
+    const uint32_t* words;    // [N][ceil(K / 128) * 16]
+    const _Float16* scales;   // [N][groups]
+    const uint8_t* zeros;     // [N][groups], or null: 8
+    int N, K, groups, group_log2;
+};
+hipError_t launch_w4_gemm(const _Float16* x, const W4Args& a, void* y, int M, bool y_fp32, hipStream_t st);
+hipError_t launch_w4_embed(const W4Args& a, const int64_t* tokens, void* out, long n, float scale, bool out_fp32,
+                           hipStream_t st);
+
+// beam search's selection and reordering of states (hx_beam.hip)
+struct BeamArgs {
+    const float* cum;     // [batch * beams]
+    const uint8_t* done;  // [batch * beams], or null: none is finished
+    float* scores;        // [batch][n], as parents and tokens
+    int64_t *parents, *tokens;
+    long ld;              // elements from one row of logits to the next
+    int batch, beams, vocab, n, eos;
+};
+constexpr int BEAM_MAX_N = 128;       // candidates asked for per sequence
+constexpr int BEAM_MAX_BATCH = 4096;  // sequences per call
+constexpr int BEAM_MAX_BEAMS = 1024;  // beams of a sequence
+size_t beam_select_workspace_bytes(int batch, int beams, int vocab, int n);
+hipError_t launch_beam_select(const void* logits, bool fp32, const BeamArgs& a, void* ws, hipStream_t st);
+struct ReorderArgs {
+    long outer, inner, bytes;  // pieces of `bytes` bytes, [outer][rows][inner] of them
+    long src[3], dst[3];       // byte strides of outer, row, inner
+    int batch, beams, out_beams;
+};
+hipError_t launch_beam_reorder(const void* src, const int64_t* parents, void* dst, const ReorderArgs& p, hipStream_t st);
+
 }  // namespace hx

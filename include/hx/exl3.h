@@ -228,6 +228,53 @@ int hx_scatter_add_rows(float* y, const float* src, const int64_t* idx, const vo
 int hx_gemm_nt_f16(void* y, const void* x, const void* w, int M, int N, int K, int y_fp32, int add,
                    hx_stream_t stream);
 
+/* ---- 4-bit words with group scales --------------------------------------------------------- */
+
+/* One linear W[N][K] of plain 4-bit codes (no trellis, no Hadamard; no counterpart in the reference):
+ *   W[n][k] = scales[n][k / group] * (q(n, k) - zeros[n][k / group])
+ * words: uint32 [N][16 * ceil(K / 128)], 16-byte aligned.  Word 4 g + j of each block of 128 k holds the eight codes
+ * k = 32 j + 8 g + (0, 2, 4, 6, 1, 3, 5, 7) of the block in its nibbles, lowest first; codes past K are not used.
+ * scales: fp16 [N][ceil(K / group)]; zeros: uint8 of that shape, or NULL for 8 everywhere; group: a power of two >= 32
+ * (the last group of a row may be short).  K % 32 == 0, any N. */
+typedef struct hx_w4_words {
+    const void* words;
+    const void* scales;
+    const void* zeros;
+    int group;
+} hx_w4_words;
+
+/* y[M][N] = x W^T: x fp16 [M][K] (16-byte aligned), y fp32 (y_fp32) or fp16, fp32 sums rounded once.  The codes and zero
+ * points enter the products exactly and the scales are applied to fp32 sums.  M == 0 is a no-op (x and y may
+ * then be NULL).  Needs no workspace. */
+int hx_w4_gemm(void* y, const void* x, const hx_w4_words* w, int M, int N, int K, int y_fp32, hx_stream_t stream);
+
+/* out[t][:] = scale * W[tokens[t]][:] for t < n, fp32 (out_fp32) or fp16 rows of K (16-byte aligned); a token outside
+ * [0, N) gives a row of zeros. */
+int hx_w4_embed(const hx_w4_words* w, const int64_t* tokens, void* out, int n, int N, int K, float scale, int out_fp32,
+                hx_stream_t stream);
+
+/* ---- beam search ---------------------------------------------------------------------------- */
+
+/* Selection over beams and vocabulary (no counterpart in the reference, which samples one sequence).  Row
+ * b * beams + w of logits (fp16 or fp32 by dtype, HX_DTYPE_*; ld elements from row to row) is beam w of sequence b:
+ *   score(w, v) = cum[b][w] + logits[w][v] - logsumexp(logits[w][0 .. vocab))
+ * and scores / parents / tokens [batch][n] receive the n best (score, w, v) of each sequence in descending order, the
+ * lowest w * vocab + v first among equal scores; fp32 scores rounded once from 64 bits.  A beam with done != 0 (done may be
+ * NULL) has the one candidate (w, eos) with score cum.  A logit of -inf is no candidate; a beam whose cum is not finite, whose
+ * logits hold a NaN or +inf, or are all -inf, has none.  Places without a candidate get score -inf, parent -1, token -1.
+ * batch <= 4096, beams <= 1024, n <= 128.  batch == 0 is a no-op. */
+size_t hx_beam_select_workspace_size(int batch, int beams, int vocab, int n);
+int hx_beam_select(const void* logits, const float* cum, const uint8_t* done, float* scores, int64_t* parents,
+                   int64_t* tokens, int batch, int beams, int vocab, int n, int64_t ld, int eos, int dtype,
+                   hx_stream_t stream, void* workspace, size_t workspace_bytes);
+
+/* dst[o][b * out_beams + j][i][:] = src[o][b * beams + parents[b][j]][i][:], pieces of `bytes` bytes, o < outer (layers),
+ * i < inner (heads); src_stride and dst_stride are host arrays of the byte strides of o, row and i.  A piece whose parent lies
+ * outside [0, beams) is left as it was.  src and dst may not overlap (their address ranges), nor may the pieces of dst. */
+int hx_beam_reorder(const void* src, const int64_t* parents, void* dst, int batch, int beams, int out_beams, int64_t outer,
+                    int64_t inner, int64_t bytes, const int64_t src_stride[3], const int64_t dst_stride[3],
+                    hx_stream_t stream);
+
 /* ---- MoE layer ---------------------------------------------------------------------------- */
 
 /* Number of expert groups the engine's moe_grouped temp buffers are sized for ([concurrency,

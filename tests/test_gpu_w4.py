@@ -1,0 +1,270 @@
+"""Linear and row lookup over 4-bit words with group scales, through the C ABI, against the definition in 64 bits."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+U32 = 2.0 ** -24  # half a step of fp32, relative
+U16 = 2.0 ** -11  # of fp16
+
+
+@pytest.fixture(scope="module")
+def w4():
+    import torch
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from helios_glm53flash_amd import w4
+    return w4
+
+
+def make(seed, N, K, group, zeros, exact=False):
+    """Codes, scales and zero points as numpy arrays, and the weights in float64.  exact: scales are powers of two, so that
+    sums of integer inputs are exact in fp32."""
+    r = np.random.default_rng(seed)
+    G = -(-K // group)
+    q = r.integers(0, 16, (N, K), dtype=np.uint8)
+    s = (2.0 ** r.integers(-2, 2, (N, G)) if exact else r.uniform(0.2, 2.0, (N, G)) / np.sqrt(K)).astype(np.float16)
+    z = r.integers(0, 16, (N, G), dtype=np.uint8) if zeros else None
+    gi = np.arange(K) // group
+    w = s.astype(np.float64)[:, gi] * (q.astype(np.float64) - (z.astype(np.float64)[:, gi] if zeros else 8.0))
+    return q, s, z, w
+
+
+def dev(a):
+    import torch
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def words(w4, q, s, z, K, group):
+    return w4.W4Words(w4.pack(dev(q)), dev(s), dev(z) if z is not None else None, K, group)
+
+
+def guarded(shape, dtype, rows=2):
+    """An output with rows of a sentinel before and behind it: (whole, view of the output)."""
+    import torch
+    whole = torch.full((shape[0] + 2 * rows, shape[1]), 77.0, dtype=dtype, device="cuda")
+    return whole, whole[rows:rows + shape[0]]
+
+
+def check_guard(whole, rows=2):
+    assert bool((whole[:rows] == 77.0).all()) and bool((whole[-rows:] == 77.0).all())
+
+
+SHAPES = [  # M, K, N, group, zeros
+    (1, 32, 1, 32, False), (1, 128, 16, 128, True), (1, 4096, 2048, 128, False), (1, 160, 33, 32, True),
+    (2, 4128, 47, 64, True), (3, 512, 5, 64, False), (4, 8192, 515, 32, True), (5, 8192, 260, 32, True),
+    (7, 1056, 129, 256, False), (8, 4096, 1000, 128, True), (9, 2048, 96, 64, False), (16, 4224, 300, 128, True),
+    (16, 16416, 70, 128, True), (1, 33024, 40, 256, False), (6, 20000, 24, 64, True),
+    (17, 640, 200, 32, True), (31, 4096, 130, 128, False), (33, 96, 64, 64, True), (45, 4096, 1024, 64, True),
+    (64, 2080, 257, 128, False), (65, 1024, 255, 32, True), (128, 4096, 384, 128, True), (129, 352, 129, 256, True),
+    (200, 2048, 1000, 64, False), (513, 1184, 390, 128, True),
+]
+
+
+@pytest.mark.parametrize("fp32", [True, False])
+@pytest.mark.parametrize("M,K,N,group,zeros", SHAPES)
+def test_gemm_of_integers_is_exact(w4, M, K, N, group, zeros, fp32):
+    """Integer inputs and scales that are powers of two: every product and partial sum is a multiple of 1/4 below 2^22, so
+    fp32 sums are exact in any order and the fp16 result is the one rounding of the exact sum."""
+    import torch
+    q, s, z, w = make(M + K, N, K, group, zeros, exact=True)
+    x = np.random.default_rng(K).integers(-4, 5, (M, K)).astype(np.float16)
+    ref = x.astype(np.float64) @ w.T
+    assert np.abs(x).astype(np.float64).max() * K * 15 * 2 < 2 ** 22
+    whole, y = guarded((M, N), torch.float32 if fp32 else torch.float16)
+    w4.gemm(y, dev(x), words(w4, q, s, z, K, group), M, N, K, fp32)
+    torch.cuda.synchronize()
+    with np.errstate(over="ignore"):
+        want = ref.astype(np.float32 if fp32 else np.float16)
+    assert np.array_equal(y.cpu().numpy(), want)
+    check_guard(whole)
+
+
+@pytest.mark.parametrize("fp32", [True, False])
+@pytest.mark.parametrize("M,K,N,group,zeros", SHAPES[::2] + SHAPES[1:16:2])
+def test_gemm_random(w4, M, K, N, group, zeros, fp32):
+    """Error of a sum of K products in any order with each group's scale applied to its own sum: at most (K + G + 2) roundings of
+    2^-24, each relative to a partial sum, so at most (K + G + 2) 2^-24 sum |x w|; fp16 outputs are rounded once more
+    (2^-11 of the value, or half the smallest step, 2^-25)."""
+    import torch
+    q, s, z, w = make(3 * M + K, N, K, group, zeros)
+    x = np.random.default_rng(K + 1).standard_normal((M, K)).astype(np.float16)
+    x64 = x.astype(np.float64)
+    ref = x64 @ w.T
+    tol = (K + -(-K // group) + 2) * U32 * (np.abs(x64) @ np.abs(w).T)
+    if not fp32:
+        tol = tol * (1 + U16) + U16 * np.abs(ref) + 2.0 ** -25
+    y = torch.empty((M, N), dtype=torch.float32 if fp32 else torch.float16, device="cuda")
+    w4.gemm(y, dev(x), words(w4, q, s, z, K, group), M, N, K, fp32)
+    torch.cuda.synchronize()
+    err = np.abs(y.cpu().numpy().astype(np.float64) - ref)
+    assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("M", [1, 3, 8, 16, 40, 130])
+def test_gemm_zero_points_over_the_whole_byte(w4, M):
+    """Zero points are bytes: values above 15 (outside what 4 bits hold) enter exactly too."""
+    import torch
+    K, N, group = 256, 40, 64
+    q, s, z, _ = make(5, N, K, group, True, exact=True)
+    z = np.random.default_rng(6).integers(0, 256, z.shape, dtype=np.uint8)
+    z[0, 0], z[1, 1] = 255, 0
+    gi = np.arange(K) // group
+    w = s.astype(np.float64)[:, gi] * (q.astype(np.float64) - z.astype(np.float64)[:, gi])
+    x = np.random.default_rng(M).integers(-4, 5, (M, K)).astype(np.float16)
+    y = torch.empty((M, N), dtype=torch.float32, device="cuda")
+    w4.gemm(y, dev(x), words(w4, q, s, z, K, group), M, N, K, True)
+    assert np.array_equal(y.cpu().numpy(), (x.astype(np.float64) @ w.T).astype(np.float32))
+
+
+@pytest.mark.parametrize("M", [1, 4, 6, 16, 20, 70])
+def test_gemm_keeps_infinities_and_nans_in_their_rows(w4, M):
+    """A NaN or infinity in one input row or one weight row's scale stays in that row and column of y."""
+    import torch
+    K, N, group = 1056, 37, 32
+    q, s, z, w = make(11, N, K, group, True, exact=True)
+    x = np.random.default_rng(3).integers(-4, 5, (M, K)).astype(np.float16)
+    ref = x.astype(np.float64) @ w.T
+    s[5, -1] = np.inf   # the last group of a weight row
+    s[9, 0] = np.nan
+    bad_row = M - 1
+    if M > 1:
+        x[bad_row, K - 1] = np.inf
+        x[0, 0] = np.nan
+    y = torch.empty((M, N), dtype=torch.float32, device="cuda")
+    w4.gemm(y, dev(x), words(w4, q, s, z, K, group), M, N, K, True)
+    got = y.cpu().numpy()
+    cols = np.ones(N, bool)
+    cols[[5, 9]] = False
+    rows = np.ones(M, bool)
+    if M > 1:
+        rows[[0, bad_row]] = False
+        assert not np.isfinite(got[0]).any()
+        d = q[:, K - 1].astype(int) - z[:, (K - 1) // group]
+        assert not np.isfinite(got[bad_row][d != 0]).any()
+    assert np.array_equal(got[np.ix_(rows, cols)], ref[np.ix_(rows, cols)].astype(np.float32))
+    assert not np.isfinite(got[:, 9]).any()
+
+
+def test_gemm_empty_batch(w4):
+    import torch
+    q, s, z, _ = make(1, 16, 128, 64, True)
+    w4.gemm(torch.empty((0, 16), device="cuda"), torch.empty((0, 128), dtype=torch.float16, device="cuda"),
+            words(w4, q, s, z, 128, 64), 0, 16, 128, True)
+
+
+@pytest.mark.parametrize("M", [1, 8, 45, 300])
+def test_gemm_rows_do_not_depend_on_the_batch(w4, M):
+    """Two calls give the same bits, and weight rows and outputs may be views that start inside larger tensors."""
+    import torch
+    K, N, group = 2048, 320, 64
+    q, s, z, _ = make(21, N, K, group, True)
+    w = words(w4, q, s, z, K, group)
+    x = torch.randn((M + 3, K), device="cuda").half()
+    y = torch.empty((2, M, N), dtype=torch.float32, device="cuda")
+    w4.gemm(y[0], x[3:], w, M, N, K, True)
+    w4.gemm(y[1], x[3:].clone(), w, M, N, K, True)
+    assert torch.equal(y[0], y[1])
+    part = w4.W4Words(w.words[33:], w.scales[33:], w.zeros[33:], K, group)
+    y2 = torch.empty((M, N - 33), dtype=torch.float32, device="cuda")
+    w4.gemm(y2, x[3:], part, M, N - 33, K, True)
+    # another tile of columns may take another order of sums
+    tol = (K + K // group + 2) * U32 * (x[3:].double().abs() @ weights64(w, K).abs().T)
+    assert bool(((y2.double() - y[0][:, 33:].double()).abs() <= 2 * tol[:, 33:]).all())
+
+
+def weights64(w, K):
+    import torch
+    from helios_glm53flash_amd import w4
+    gi = torch.arange(K, device="cuda") // w.group
+    d = w4.unpack(w.words, K).double() - (w.zeros.double()[:, gi] if w.zeros is not None else 8.0)
+    return d * w.scales.double()[:, gi]
+
+
+def test_gemm_large_table_offsets(w4):
+    """More than 2^32 bytes of words: the last rows of the table."""
+    import torch
+    K, group = 16384, 128
+    N = (1 << 32) // (K // 2) + 70
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(1)
+    wd = torch.zeros((N, K // 8), dtype=torch.int32, device="cuda")
+    wd[-80:] = torch.randint(-2 ** 31, 2 ** 31 - 1, (80, K // 8), generator=gen, device="cuda").to(torch.int32)
+    sc = torch.full((N, K // group), 0.5, dtype=torch.float16, device="cuda")
+    w = w4.W4Words(wd, sc, None, K, group)
+    tail = w4.W4Words(wd[-80:].clone(), sc[-80:].clone(), None, K, group)
+    for M in (1, 20):
+        x = torch.randint(-3, 4, (M, K), generator=gen, device="cuda").half()
+        y = torch.empty((M, N), dtype=torch.float32, device="cuda")
+        w4.gemm(y, x, w, M, N, K, True)
+        ref = x.double() @ weights64(tail, K).T
+        assert torch.equal(y[:, -80:].double(), ref)
+        assert torch.equal(y[:, 0].double(), x.double().sum(dim=1) * -4.0)
+    out = torch.empty((2, K), dtype=torch.float32, device="cuda")
+    w4.embed(w, torch.tensor([N - 1, N - 80], device="cuda"), out, 2)
+    assert torch.equal(out.double(), weights64(tail, K)[[79, 0]])
+
+
+@pytest.mark.parametrize("M", [1, 6, 16, 45, 200])
+def test_gemm_graph_replays_on_another_stream(w4, M):
+    import torch
+    K, N, group = 1024, 300, 128
+    q, s, z, _ = make(31, N, K, group, True)
+    w = words(w4, q, s, z, K, group)
+    x = torch.randn((M, K), device="cuda").half()
+    y = torch.empty((M, N), dtype=torch.float32, device="cuda")
+    want = torch.empty_like(y)
+    w4.gemm(want, x, w, M, N, K, True)
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        w4.gemm(y, x, w, M, N, K, True)
+    for rep in range(3):
+        x.copy_(torch.randn((M, K), device="cuda").half())
+        y.fill_(float("nan"))
+        g.replay()
+        w4.gemm(want, x, w, M, N, K, True)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want), rep
+
+
+@pytest.mark.parametrize("fp32", [True, False])
+@pytest.mark.parametrize("T,K,N,group,zeros", [(1, 4096, 300, 128, False), (7, 160, 50, 32, True), (33, 2080, 1000, 64, True),
+                                              (1000, 512, 17, 256, False)])
+def test_embed(w4, T, K, N, group, zeros, fp32):
+    """scale * s is rounded once, its product with the integer once: 2 x 2^-24 relative; fp16 outputs once more."""
+    import torch
+    q, s, z, w = make(T, N, K, group, zeros)
+    tok = np.random.default_rng(T).integers(0, N, T)
+    tok[0], tok[-1] = N - 1, 0
+    scale = float(np.float32(np.sqrt(K)))
+    whole, out = guarded((T, K), torch.float32 if fp32 else torch.float16)
+    w4.embed(words(w4, q, s, z, K, group), dev(tok), out, T, scale)
+    ref = w[tok] * scale
+    tol = 2.01 * U32 * np.abs(ref)
+    if not fp32:
+        tol = tol + U16 * np.abs(ref) * 1.001 + 2.0 ** -25
+    assert (np.abs(out.cpu().numpy().astype(np.float64) - ref) <= tol).all()
+    check_guard(whole)
+
+
+def test_embed_tokens_outside_the_table(w4):
+    import torch
+    q, s, z, w = make(2, 20, 128, 64, True, exact=True)
+    tok = torch.tensor([3, -1, 19, 20, 1 << 40, -(1 << 40), 0], device="cuda")
+    out = torch.full((7, 128), 5.0, device="cuda")
+    w4.embed(words(w4, q, s, z, 128, 64), tok, out, 7)
+    got = out.cpu().numpy()
+    assert (got[[1, 3, 4, 5]] == 0).all()
+    assert np.array_equal(got[[0, 2, 6]], w[[3, 19, 0]].astype(np.float32))
+    w4.embed(words(w4, q, s, z, 128, 64), tok[:0], out[:0], 0)
+
+
+def test_another_device_is_refused(w4):
+    """The entry points launch on the current device: tensors elsewhere (here the host) are refused."""
+    import torch
+    q, s, z, _ = make(1, 16, 128, 64, True)
+    w = words(w4, q, s, z, 128, 64)
+    with pytest.raises(ValueError, match="device"):
+        w4.gemm(torch.empty((1, 16)), torch.empty((1, 128), dtype=torch.float16), w, 1, 16, 128, True)
