@@ -552,11 +552,13 @@ int hx_beam_select(const void* logits, const float* cum, const uint8_t* done, fl
         return fail(HX_ERR_INVALID, "hx_beam_select: dtype must be HX_DTYPE_HALF or HX_DTYPE_FLOAT");
     if (done && (eos < 0 || eos >= vocab)) return fail(HX_ERR_INVALID, "hx_beam_select: eos outside the vocabulary");
     if (batch == 0) return 0;
+    const size_t need = hx::beam_select_workspace_bytes(batch, beams, vocab, n);
+    if (!need) return fail(HX_ERR_INVALID, "hx_beam_select: extents too large for one call");
     if (!logits || !cum || !scores || !parents || !tokens) return fail(HX_ERR_INVALID, "hx_beam_select: null pointer");
     if (((uintptr_t)logits & (dtype == HX_DTYPE_FLOAT ? 3 : 1)) || (((uintptr_t)cum | (uintptr_t)scores) & 3) ||
         (((uintptr_t)parents | (uintptr_t)tokens) & 7))
         return fail(HX_ERR_INVALID, "hx_beam_select: a pointer is not aligned to its type");
-    if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < hx::beam_select_workspace_bytes(batch, beams, vocab, n))
+    if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)
         return fail(HX_ERR_WORKSPACE, "hx_beam_select: workspace missing, not 16-byte aligned or smaller than "
                                       "hx_beam_select_workspace_size");
     const hx::BeamArgs a{cum, done, scores, parents, tokens, (long)ld, batch, beams, vocab, n, eos};
