@@ -81,7 +81,9 @@ SIGNATURES: dict[str, tuple] = {
                                  C.c_void_p]),
     "hx_gather_rows": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
     "hx_scatter_add_rows": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
-    "hx_w4_gemm": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(W4WordsC), C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
+    "hx_w4_gemm": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(W4WordsC), C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p,
+                             C.c_void_p, C.c_size_t]),
+    "hx_w4_gemm_workspace_size": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
     "hx_w4_embed": (C.c_int, [C.POINTER(W4WordsC), C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_float, C.c_int,
                               C.c_void_p]),
     "hx_beam_select_workspace_size": (C.c_size_t, [C.c_int] * 4),

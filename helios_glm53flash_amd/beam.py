@@ -12,8 +12,8 @@ from typing import Optional
 import torch
 
 from ._lib import check, lib
-from .exl3 import _need, _ptr, _stream, workspace
-from .w4 import _on_one_device
+from .exl3 import _need, _ptr, _stream
+from .w4 import _on_one_device, call_workspace
 
 _DTYPES = {torch.float16: 0, torch.float32: 1}
 
@@ -51,7 +51,7 @@ def select(logits: torch.Tensor, cum: torch.Tensor, done: Optional[torch.Tensor]
         raise ValueError("select: cum / outputs smaller than batch * beams / batch * n")
     _on_one_device(logits, cum, done, scores, parents, tokens)
     st = _stream(stream)
-    ws = workspace(_select_workspace_bytes(batch, beams, vocab, n), logits.device, st)
+    ws = call_workspace(_select_workspace_bytes(batch, beams, vocab, n), logits.device, st)
     check(lib.hx_beam_select(logits.data_ptr(), cum.data_ptr(), _ptr(done), scores.data_ptr(), parents.data_ptr(),
                              tokens.data_ptr(), batch, beams, vocab, n, ld, eos, _DTYPES[logits.dtype], st, ws.data_ptr(),
                              ws.numel()), "hx_beam_select")

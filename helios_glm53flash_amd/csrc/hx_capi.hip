@@ -489,7 +489,7 @@ int w4_args(const hx_w4_words* w, int N, int K, hx::W4Args* a, const char* who)
     const char* what = nullptr;
     if (!w || !w->words || !w->scales) what = "null pointer";
     else if (N <= 0 || K <= 0 || K % 32) what = "N and K must be positive and K a multiple of 32";
-    else if (K > (1 << 24)) what = "K must be at most 2^24";
+    else if (K > (1 << 22)) what = "K must be at most 2^22";
     else if (w->group < 32 || (w->group & (w->group - 1))) what = "group must be a power of two of at least 32";
     else if ((uintptr_t)w->words & 15) what = "words must be 16-byte aligned";
     else if ((uintptr_t)w->scales & 1) what = "scales must be 2-byte aligned";
@@ -504,7 +504,14 @@ int w4_args(const hx_w4_words* w, int N, int K, hx::W4Args* a, const char* who)
 
 }  // namespace
 
-int hx_w4_gemm(void* y, const void* x, const hx_w4_words* w, int M, int N, int K, int y_fp32, hx_stream_t stream)
+size_t hx_w4_gemm_workspace_size(int M, int N, int K)
+{
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    return hx::w4_gemm_workspace_bytes(M, N, K);
+}
+
+int hx_w4_gemm(void* y, const void* x, const hx_w4_words* w, int M, int N, int K, int y_fp32, hx_stream_t stream,
+               void* workspace, size_t workspace_bytes)
 {
     hx::W4Args a;
     const int r = w4_args(w, N, K, &a, "hx_w4_gemm");
@@ -514,7 +521,9 @@ int hx_w4_gemm(void* y, const void* x, const hx_w4_words* w, int M, int N, int K
     if (!y || !x) return fail(HX_ERR_INVALID, "hx_w4_gemm: null pointer");
     if ((uintptr_t)x & 15) return fail(HX_ERR_INVALID, "hx_w4_gemm: x must be 16-byte aligned");
     if ((uintptr_t)y & (y_fp32 ? 3 : 1)) return fail(HX_ERR_INVALID, "hx_w4_gemm: y is not aligned to its type");
-    return hip_status(hx::launch_w4_gemm(static_cast<const _Float16*>(x), a, y, M, y_fp32 != 0, (hipStream_t)stream),
+    if ((uintptr_t)workspace & 15) return fail(HX_ERR_WORKSPACE, "hx_w4_gemm: workspace must be 16-byte aligned");
+    return hip_status(hx::launch_w4_gemm(static_cast<const _Float16*>(x), a, y, M, y_fp32 != 0, workspace, workspace_bytes,
+                                         (hipStream_t)stream),
                       "hx_w4_gemm");
 }
 

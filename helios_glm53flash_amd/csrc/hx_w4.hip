@@ -55,52 +55,64 @@ HX_INLINE hx_h8 word_operand(uint32_t w, ZeroPair z)
     return o.v;
 }
 
-// Scales (fp16, one per 16 bits) and zero points (one per 8 bits) of a block of 128 k, lowest group first.  GS: groups in a
-// block, 1 where the group is 128 or longer.
-template <int GS>
+// Buffer accesses return 0 beyond a descriptor's bytes (and beyond 2^30 always, which marks what must read as 0).  Everything
+// that decides about that is in the per-lane offset.
+constexpr int W4_NONE = 0x7ffffff0;
+HX_INLINE __amdgpu_buffer_rsrc_t w4_rsrc(const void* base, long bytes)
+{
+    return mf_rsrc(base, (size_t)(bytes < 0 ? 0 : bytes > 0x40000000l ? 0x40000000l : bytes));
+}
+
+// Scales (fp16) and zero points of a block of 128 k, lowest group first.  GS: groups in a block, 1 where the group is 128 or
+// longer.  V: the GS groups of a block are one aligned piece (K a multiple of 128, aligned pointers); without, each group is
+// loaded by itself.  Which of the two is not decided in the kernels: branches between the loads of a ring make the compiler
+// wait for all of them.
+template <int GS, bool Z, bool V>
 struct BlockScale {
-    uint64_t s;
-    uint32_t z;
-    HX_INLINE float scale(int g) const { return (float)u16_as_h((uint16_t)(s >> (16 * g))); }
-    HX_INLINE ZeroPair zero(int g) const { return zero_pair((z >> (8 * g)) & 255u); }
+    static constexpr int NS = GS == 1 ? 1 : V ? GS / 2 : GS, NZ = GS == 1 || V ? 1 : GS;
+    uint32_t s[NS], z[NZ];  // as loaded: converted where they are used, since anything earlier would wait for the load
+    HX_INLINE float scale(int g) const
+    {
+        if constexpr (NS == GS) return (float)u16_as_h((uint16_t)s[g]);
+        else return (float)u16_as_h((uint16_t)(s[g >> 1] >> (16 * (g & 1))));
+    }
+    HX_INLINE ZeroPair zero(int g) const
+    {
+        if constexpr (!Z) return {u32_as_h2(0x64086408u), u32_as_h2(0x54805480u)};  // 1032, 72
+        else if constexpr (NZ == GS) return zero_pair(z[g]);
+        else return zero_pair((z[0] >> (8 * g)) & 255u);
+    }
 };
 
-// Of block blk of row `row` (both inside the matrix).  A short last block reads the GS groups that end with the row and shifts
-// them down, so groups past K have scale 0; a row of fewer than GS groups reads them one by one.
-template <int GS, bool Z>
-HX_INLINE BlockScale<GS> block_scale(const W4Args& a, size_t row, int blk)
+// Of block blk of the row whose first group lies `first` groups behind the descriptors' base.  Groups past K, and rows past the
+// descriptors, have scale 0.
+template <int GS, bool Z, bool V>
+HX_INLINE BlockScale<GS, Z, V> block_scale(__amdgpu_buffer_rsrc_t rs, __amdgpu_buffer_rsrc_t rz, const W4Args& a, int first,
+                                           int blk)
 {
-    typedef uint32_t u32a2 __attribute__((aligned(2)));
-    typedef uint64_t u64a2 __attribute__((aligned(2)));
-    typedef uint16_t u16a1 __attribute__((aligned(1)));
-    typedef uint32_t u32a1 __attribute__((aligned(1)));
-    BlockScale<GS> r{0, 0};
+    BlockScale<GS, Z, V> r;
     if constexpr (GS == 1) {
-        const size_t i = row * a.groups + ((blk * 128) >> a.group_log2);
-        r.s = h_as_u16(a.scales[i]);
-        if constexpr (Z) r.z = a.zeros[i];
-    } else {
-        const int g0 = blk * GS;
-        const _Float16* s = a.scales + row * a.groups;
-        const uint8_t* z = a.zeros + row * a.groups;
-        if (a.groups >= GS) {
-            const int g = min(g0, a.groups - GS), off = g0 - g;
-            if constexpr (GS == 2) r.s = *reinterpret_cast<const u32a2*>(s + g);
-            else r.s = *reinterpret_cast<const u64a2*>(s + g);
-            r.s >>= 16 * off;
-            if constexpr (Z) {
-                if constexpr (GS == 2) r.z = *reinterpret_cast<const u16a1*>(z + g);
-                else r.z = *reinterpret_cast<const u32a1*>(z + g);
-                r.z >>= 8 * off;
-            }
+        const int g = (blk * 128) >> a.group_log2, i = g < a.groups ? first + g : W4_NONE >> 1;
+        r.s[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rs, 2 * i, 0, 0);
+        if constexpr (Z) r.z[0] = __builtin_amdgcn_raw_buffer_load_b8(rz, i, 0, 0);
+    } else if constexpr (V) {
+        const int i = blk * GS < a.groups ? first + blk * GS : W4_NONE >> 1;
+        if constexpr (GS == 2) {
+            r.s[0] = __builtin_amdgcn_raw_buffer_load_b32(rs, 2 * i, 0, 0);
+            if constexpr (Z) r.z[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rz, i, 0, 0);
         } else {
-            for (int g = g0; g < a.groups; ++g) {
-                r.s |= (uint64_t)h_as_u16(s[g]) << (16 * (g - g0));
-                if constexpr (Z) r.z |= (uint32_t)z[g] << (8 * (g - g0));
-            }
+            const auto v = __builtin_amdgcn_raw_buffer_load_b64(rs, 2 * i, 0, 0);
+            r.s[0] = v[0], r.s[1] = v[1];
+            if constexpr (Z) r.z[0] = __builtin_amdgcn_raw_buffer_load_b32(rz, i, 0, 0);
+        }
+    } else {
+#pragma unroll
+        for (int g = 0; g < GS; ++g) {
+            const int i = blk * GS + g < a.groups ? first + blk * GS + g : W4_NONE >> 1;
+            r.s[g] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rs, 2 * i, 0, 0);
+            if constexpr (Z) r.z[g] = __builtin_amdgcn_raw_buffer_load_b8(rz, i, 0, 0);
         }
     }
-    if constexpr (!Z) r.z = 0x08080808u;
     return r;
 }
 
@@ -121,53 +133,57 @@ HX_INLINE void store_y(void* y, size_t i, float v, bool y_fp32)
 // A wave owns NS spans (S blocks each) of every WK NS, keeps x for them in registers and goes over tiles of NT R rows; each word
 // is replaced by the next tile's as soon as it is decoded.  Per group the products are summed by the matrix
 // instructions from zero, then scaled into the fp32 sums.
-template <int S, int MT, int NS, int NT, int GS, bool Z>
-__global__ __launch_bounds__(512) void w4_rows_kernel(const _Float16* x, W4Args a, void* y, int M, bool y_fp32, int wk)
+template <int S, int MT, int WAVES, int NS, int NT, int GS, bool Z, bool V>
+__device__ __forceinline__ void w4_rows(const _Float16* x, const W4Args& a, void* y, int M, bool y_fp32, int wk)
 {
-    constexpr int R = 16 / S, H = 4 / S, SLOTS = 16 * H;  // rows of a load; 4-token pieces of a column; pieces kept per tile
-    __shared__ hx_f4 red[2][8][NT * MT][SLOTS];
+    constexpr int R = 16 / S, H = 4 / S;  // rows of a load; 4-token pieces of a column
+    __shared__ float red[WAVES][NT * MT][4 * H][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kw = wave & (wk - 1), rw = wave / wk, wr = 8 / wk;  // the wave's place in K and in rows
+    const int kw = wave & (wk - 1), rw = wave / wk, wr = WAVES / wk;  // the wave's place in K and in rows
     const int col = lane & 15, kg = lane >> 4, s = col / R, r = col % R;
     const int nb = (a.K + 127) / 128, nkb = ((nb + S - 1) / S + wk * NS - 1) / (wk * NS);  // blocks; rounds over K
     const int row_bytes = nb * 64, rows_wg = wr * NT * R;
     const int tiles = (a.N + rows_wg - 1) / rows_wg;
 
+    const __amdgpu_buffer_rsrc_t rx = w4_rsrc(x, (long)M * a.K * 2);
     hx_h8 xa[NS][MT][4];
     auto load_x = [&](int kb) {
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            const int blk = ((kb * NS + i) * wk + kw) * S + s;
+            const int k = (((kb * NS + i) * wk + kw) * S + s) * 128 + 8 * kg;
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const int t = 16 * m + r;
+            for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int k = blk * 128 + 32 * j + 8 * kg;
-                    xa[i][m][j] = hx_h8{};
-                    if (t < M && k < a.K) xa[i][m][j] = *reinterpret_cast<const hx_h8*>(x + (size_t)t * a.K + k);
+                    const int off = k + 32 * j < a.K ? ((16 * m + r) * a.K + k + 32 * j) * 2 : W4_NONE;
+                    xa[i][m][j] = __builtin_bit_cast(hx_h8, __builtin_amdgcn_raw_buffer_load_b128(rx, off, 0, 0));
                 }
-            }
         }
     };
     hx_u4 w[NS][NT];
-    BlockScale<GS> sc[NS][NT];
-    auto load_w = [&](int i, int n, int tile, int kb) {
-        const int row0 = (tile * wr + rw) * NT * R;
-        const int blk = ((kb * NS + i) * wk + kw) * S + s, bc = min(blk, nb - 1);
-        const size_t row = min(row0 + n * R + r, a.N - 1);
-        w[i][n] = *reinterpret_cast<const hx_u4*>(reinterpret_cast<const char*>(a.words) + row * row_bytes + bc * 64 + kg * 16);
-        sc[i][n] = block_scale<GS, Z>(a, row, bc);
-        if (blk != bc) sc[i][n].s = 0;
+    BlockScale<GS, Z, V> sc[NS][NT];
+    __amdgpu_buffer_rsrc_t rw_, rs, rz;
+    auto aim = [&](int tile) {  // descriptors of the tile's rows (nothing left of the matrix: every load is 0)
+        const long row0 = (long)(tile * wr + rw) * NT * R, left = tile < tiles ? a.N - row0 : 0;
+        rw_ = w4_rsrc(reinterpret_cast<const char*>(a.words) + row0 * row_bytes, left * row_bytes);
+        rs = w4_rsrc(a.scales + row0 * a.groups, left * a.groups * 2);
+        rz = w4_rsrc(Z ? a.zeros + row0 * a.groups : nullptr, Z ? left * a.groups : 0);
     };
-    load_x(0);
+    const int lane_off = r * row_bytes + s * 64 + kg * 16;
+    auto load_w = [&](int i, int n, int kb) {
+        const int span = (kb * NS + i) * wk + kw;
+        // a block past K reads the next row's words: x is 0 there, and the scale
+        w[i][n] = __builtin_bit_cast(hx_u4, __builtin_amdgcn_raw_buffer_load_b128(rw_, lane_off + n * R * row_bytes + span * (S * 64), 0, 0));
+        sc[i][n] = block_scale<GS, Z, V>(rs, rz, a, (n * R + r) * a.groups, span * S + s);
+    };
     int tile = blockIdx.x;
+    aim(tile);
+    load_x(0);
 #pragma unroll
     for (int i = 0; i < NS; ++i)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) load_w(i, n, tile, 0);
-    int buf = 0;
-    for (; tile < tiles; tile += gridDim.x, buf ^= 1) {
+        for (int n = 0; n < NT; ++n) load_w(i, n, 0);
+    for (; tile < tiles; tile += gridDim.x) {
         hx_f4 acc[NT][MT];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -176,17 +192,18 @@ __global__ __launch_bounds__(512) void w4_rows_kernel(const _Float16* x, W4Args 
         for (int kb = 0; kb < nkb; ++kb) {
             if (nkb > 1) load_x(kb);
             const bool wrap = kb + 1 == nkb;
-            const int next_tile = wrap ? min(tile + (int)gridDim.x, tiles - 1) : tile, next_kb = wrap ? 0 : kb + 1;
+            const int next_kb = wrap ? 0 : kb + 1;
+            if (wrap) aim(tile + gridDim.x);
 #pragma unroll
             for (int i = 0; i < NS; ++i)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const hx_u4 wv = w[i][n];
-                    const BlockScale<GS> sv = sc[i][n];
+                    const BlockScale<GS, Z, V> sv = sc[i][n];
                     hx_h8 b[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) b[j] = word_operand(wv[j], sv.zero(j * GS / 4));
-                    load_w(i, n, next_tile, next_kb);
+                    load_w(i, n, next_kb);
 #pragma unroll
                     for (int g = 0; g < GS; ++g) {
                         const float f = sv.scale(g);
@@ -207,142 +224,219 @@ __global__ __launch_bounds__(512) void w4_rows_kernel(const _Float16* x, W4Args 
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int m = 0; m < MT; ++m) red[buf][wave][n * MT + m][col * H + kg % H] = acc[n][m];
-        __syncthreads();  // the other buffer was read before the previous tile's barrier
-        constexpr int ITEMS = NT * MT * R * H;  // pieces of 4 tokens of one row, per row part of the workgroup
-        for (int i = threadIdx.x; i < ITEMS * wr; i += 512) {
-            const int part = i / ITEMS, q = i % ITEMS;
-            const int h = q % H, rr = q / H % R, m = q / H / R % MT, n = q / H / R / MT;
-            hx_f4 v{0.f, 0.f, 0.f, 0.f};
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) red[wave][n * MT + m][kg % H * 4 + e][col] = acc[n][m][e];
+        hx_lds_barrier();
+        constexpr int ITEMS = NT * MT * 4 * H * R;  // outputs per row part of the workgroup
+        for (int i = threadIdx.x; i < ITEMS * wr; i += 64 * WAVES) {
+            const int part = i / ITEMS, q = i % ITEMS, rr = q % R, t4 = q / R % (4 * H), m = q / R / (4 * H) % MT, n = q / R / (4 * H) / MT;
+            const int row = (tile * wr + part) * NT * R + n * R + rr, t = 16 * m + t4;
+            float v = 0.0f;
             for (int k = 0; k < wk; ++k)
 #pragma unroll
-                for (int ss = 0; ss < S; ++ss) v += red[buf][part * wk + k][n * MT + m][(ss * R + rr) * H + h];
-            const int row = (tile * wr + part) * NT * R + n * R + rr;
-            if (row < a.N)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int t = 16 * m + 4 * h + e;
-                    if (t < M) store_y(y, (size_t)t * a.N + row, v[e], y_fp32);
-                }
+                for (int ss = 0; ss < S; ++ss) v += red[part * wk + k][n * MT + m][t4][ss * R + rr];
+            if (row < a.N && t < M) store_y(y, (size_t)t * a.N + row, v, y_fp32);
         }
+        hx_lds_barrier();  // the sums are read before the next tile's overwrite them
     }
 }
 
-// ---- M > 64
-//
-// A workgroup of 4 waves computes BM x 128 outputs; wave w the 32 columns (weight rows) 32 w.. for all BM rows.  x goes through a
-// ring of LDS buffers of BM x 128 k, loaded by buffer loads with an LDS destination; 16-byte piece u of row m lies at
-// piece u ^ (m & 15), so the 16 rows of a fragment read touch all banks.  The words go from memory into registers, PF chunks
-// ahead, and become operands there: no wave decodes a weight another wave of the workgroup uses.
-constexpr int W4T_BN = 128;
-
-template <int BM, int GS, bool Z>
-__device__ __forceinline__ void w4_tile(const _Float16* x, const W4Args& a, void* y, int M, bool y_fp32)
+template <int S, int MT, int WAVES, int NS, int NT, int GS, bool Z, bool V>
+__global__ __launch_bounds__(64 * WAVES) void w4_rows_kernel(const _Float16* x, W4Args a, void* y, int M, bool y_fp32, int wk)
 {
-    constexpr int NBUF = 2, RB = BM / 16, NL = BM / 16;  // loads of 4 rows per wave: BM / 4 rows / 4 waves
-    extern __shared__ __align__(16) _Float16 w4_lds[];   // [NBUF][BM][128]
+    w4_rows<S, MT, WAVES, NS, NT, GS, Z, V>(x, a, y, M, y_fp32, wk);
+}
+
+// ---- more rows
+//
+// A workgroup computes BM x 64 NT outputs; its waves are KS parts of K by four column groups of 16 NT weight rows.  A step takes
+// KS consecutive blocks of 128 k, one for each part.  x goes through a ring of PF LDS stages [KS][BM][128], filled by buffer loads
+// with an LDS destination (256 consecutive bytes of a row); 16-byte piece u of row m lies at piece u ^ (m & 15), so the 16
+// rows of a fragment read touch all banks.  The words go from memory into registers, as many steps ahead, and become operands
+// there: no wave decodes a weight that another wave of the workgroup uses.
+struct W4Split {
+    int splits, steps;  // workgroups that share a tile's K, steps of each
+    hx_f4* partial;     // [tiles][splits][RB][NT][4][64]
+    int* counters;      // arrivals per tile, zero between calls
+};
+
+template <int BM, int NT, int KS, int PF, int GS, bool Z, bool V>
+__device__ __forceinline__ void w4_tile(const _Float16* x, const W4Args& a, void* y, int M, bool y_fp32, W4Split sp)
+{
+    constexpr int RB = BM / 16, NL = BM / 16;  // row blocks; x loads (4 rows each) of a wave per step
+    constexpr int NVM = NL + NT * (1 + (V || GS == 1 ? 1 : GS) * (Z ? 2 : 1));  // vector memory instructions of a wave per step
+    extern __shared__ __align__(16) _Float16 w4_lds[];  // [PF][KS][BM][128]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, kg = lane >> 4;
+    const int part = wave >> 2, cw = wave & 3, col = lane & 15, kg = lane >> 4;
     const int nb = (a.K + 127) / 128, row_bytes = nb * 64;
+    const int tile = (int)(blockIdx.x / sp.splits), split = (int)(blockIdx.x % sp.splits);
+    const int first = split * sp.steps, steps = min(first + sp.steps, (nb + KS - 1) / KS);  // this split's steps
     const int mt = (M + BM - 1) / BM;
-    const int m0 = (int)(blockIdx.x % mt) * BM, n0 = (int)(blockIdx.x / mt) * W4T_BN;
-    const __amdgpu_buffer_rsrc_t rx = mf_rsrc(x + (size_t)m0 * a.K, (size_t)min(M - m0, BM) * a.K * sizeof(_Float16));
-    int voff[NL];
+    const int m0 = tile % mt * BM, n0 = tile / mt * (64 * NT);
+    const __amdgpu_buffer_rsrc_t rx = w4_rsrc(x + (size_t)m0 * a.K, (long)min(M - m0, BM) * a.K * 2);
+    const long left = a.N - n0;
+    const __amdgpu_buffer_rsrc_t rw = w4_rsrc(reinterpret_cast<const char*>(a.words) + (size_t)n0 * row_bytes, left * row_bytes);
+    const __amdgpu_buffer_rsrc_t rs = w4_rsrc(a.scales + (size_t)n0 * a.groups, left * a.groups * 2);
+    const __amdgpu_buffer_rsrc_t rz = w4_rsrc(Z ? a.zeros + (size_t)n0 * a.groups : nullptr, Z ? left * a.groups : 0);
+    // rows past M and pieces past K hold anything: the former are not stored, the products of the latter are skipped
+    int xoff[NL];
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-        const int r = 4 * (wave * NL + i) + (lane >> 4);  // rows past M (clamped) are computed but not stored
-        voff[i] = (int)(((size_t)min(r, M - m0 - 1) * a.K + 8 * ((lane & 15) ^ (r & 15))) * sizeof(_Float16));
+        const int r = 4 * (cw * NL + i) + (lane >> 4);
+        xoff[i] = (r * a.K + part * 128 + 8 * ((lane & 15) ^ (r & 15))) * 2;
     }
-    // past K a piece is the next row's or, past the end, zeros; its products are skipped below
-    auto load_a = [&](int c) {
-        _Float16* d = w4_lds + (size_t)(c % NBUF) * BM * 128 + wave * NL * 512;
+    auto load_x = [&](int slot, int c) {
+        _Float16* d = w4_lds + (slot * KS + part) * (BM * 128) + cw * NL * 512;
 #pragma unroll
         for (int i = 0; i < NL; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (__attribute__((address_space(3))) void*)(d + 512 * i), 16, voff[i],
-                                                     c * 256, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (__attribute__((address_space(3))) void*)(d + 512 * i), 16,
+                                                     c < steps ? xoff[i] + c * (KS * 256) : W4_NONE, 0, 0, 0);
     };
-    size_t row[2];
-    const char* wp[2];
+    hx_u4 w[PF][NT];
+    BlockScale<GS, Z, V> sc[PF][NT];
+    auto load_w = [&](int slot, int c) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        row[n] = min(n0 + 32 * wave + 16 * n + col, a.N - 1);
-        wp[n] = reinterpret_cast<const char*>(a.words) + row[n] * row_bytes + kg * 16;
-    }
-    hx_f4 acc[RB][2];
+        for (int n = 0; n < NT; ++n) {
+            const int row = 16 * (cw * NT + n) + col, blk = c * KS + part;
+            w[slot][n] = __builtin_bit_cast(hx_u4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                       rw, c < steps ? row * row_bytes + blk * 64 + kg * 16 : W4_NONE, 0, 0));
+            sc[slot][n] = block_scale<GS, Z, V>(rs, rz, a, row * a.groups, blk);
+        }
+    };
+    hx_f4 acc[RB][NT];
 #pragma unroll
     for (int i = 0; i < RB; ++i)
 #pragma unroll
-        for (int n = 0; n < 2; ++n) acc[i][n] = hx_f4{0.f, 0.f, 0.f, 0.f};
-    hx_u4 w[2];
-    BlockScale<GS> sc[2];
-    auto load_w = [&](int c) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            w[n] = *reinterpret_cast<const hx_u4*>(wp[n] + c * 64);
-            sc[n] = block_scale<GS, Z>(a, row[n], c);
-        }
+        for (int n = 0; n < NT; ++n) acc[i][n] = hx_f4{0.f, 0.f, 0.f, 0.f};
+    // The waits below, and the compiler's, count a step's loads: steps stay apart, the x loads come first in each, and every step
+    // issues its loads, past the end as accesses that touch no memory (where they depended on the step, each use of the words
+    // waited for all loads in flight: 13 us instead of x at 16 rows of 4096 -> 2048).
+    auto load = [&](int slot, int c) {
+        asm volatile("" ::: "memory");
+        load_x(slot, c);
+        asm volatile("" ::: "memory");
+        load_w(slot, c);
+        asm volatile("" ::: "memory");
     };
-    load_a(0);
-    load_w(0);
-    for (int c = 0; c < nb; ++c) {
-        __syncthreads();  // waits for this wave's loads of chunk c, then for the others'; buffer c + 1 is no longer read
-        hx_h8 b[2][4];
-        float f[2][GS];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
+    for (int u = 0; u < PF - 1; ++u) load(u, first + u);
+    auto step = [&](int u, int c, bool whole) {
+        // the decode of a later step's words would wait for their loads here
+        __builtin_amdgcn_sched_barrier(0);
+        // x of step c has arrived once at most the loads of the PF - 2 later steps in flight are outstanding
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(qt_vmcnt((PF - 2) * NVM));
+        hx_lds_barrier();  // and the other waves'; the stage of step c - 1 is no longer read
+        hx_h8 b[NT][4];
+        float f[NT][GS];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) b[n][j] = word_operand(w[n][j], sc[n].zero(j * GS / 4));
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int g = 0; g < GS; ++g) f[n][g] = sc[n].scale(g);
+            for (int j = 0; j < 4; ++j) b[n][j] = word_operand(w[u][n][j], sc[u][n].zero(j * GS / 4));
+#pragma unroll
+            for (int g = 0; g < GS; ++g) f[n][g] = sc[u][n].scale(g);
         }
-        if (c + 1 < nb) {
-            load_a(c + 1);
-            load_w(c + 1);
-        }
-        const _Float16* s = w4_lds + (size_t)(c % NBUF) * BM * 128;
-        auto products = [&](int i, int nj) {
+        load((u + PF - 1) % PF, c + PF - 1);
+        const _Float16* s = w4_lds + (u * KS + part) * (BM * 128);
+        const int left_k = whole ? 128 : a.K - 128 * (c * KS + part);  // of K in this block
+#pragma unroll
+        for (int i = 0; i < RB; ++i) {
             hx_h8 xa[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 xa[j] = *reinterpret_cast<const hx_h8*>(s + (16 * i + col) * 128 + 8 * ((4 * j + kg) ^ col));
+            if (!whole)  // what lies behind a row's K, x of another row or nothing, counts as 0 (as do the scales there)
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+                for (int j = 0; j < 4; ++j)
+                    if (32 * j >= left_k) xa[j] = hx_h8{};
+            if constexpr (GS > 1) __builtin_amdgcn_sched_barrier(0);  // the row blocks' products would all be started at once
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int g = 0; g < GS; ++g) {
                     hx_f4 t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int j = g * 4 / GS; j < (g + 1) * 4 / GS; ++j)
-                        if (j < nj) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(xa[j], b[n][j], t, 0, 0, 0);
+                        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(xa[j], b[n][j], t, 0, 0, 0);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[i][n][e] = __builtin_fmaf(f[n][g], t[e], acc[i][n][e]);
                 }
-        };
-        const int nj = min(4, (a.K - 128 * c) / 32);
-        if (nj == 4) {
-#pragma unroll
-            for (int i = 0; i < RB; ++i) products(i, 4);
-        } else {
-#pragma unroll
-            for (int i = 0; i < RB; ++i) products(i, nj);
         }
+    };
+    // Whole rounds of the ring have no branches, so that every wait in them is for the step's own loads only.
+    const int whole = min(steps, a.K / (128 * KS));  // the end of the steps without a part past K
+    int c0 = first;
+    for (; c0 + PF <= whole; c0 += PF)
+#pragma unroll
+        for (int u = 0; u < PF; ++u) step(u, c0 + u, true);
+    for (; c0 < steps; c0 += PF)
+#pragma unroll
+        for (int u = 0; u < PF; ++u)
+            if (c0 + u < steps) step(u, c0 + u, false);
+    // the accesses behind the last step are done with the stages too
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(qt_vmcnt(0));
+    hx_lds_barrier();
+    if constexpr (KS > 1) {  // the parts' sums, in order; part p finishes row blocks p, p + KS, ..
+        static_assert(NT <= PF, "the sums fit the stages");
+        hx_f4* red = reinterpret_cast<hx_f4*>(w4_lds);  // [KS][4][RB][NT][64]
+#pragma unroll
+        for (int i = 0; i < RB; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) red[((wave * RB + i) * NT + n) * 64 + lane] = acc[i][n];
+        hx_lds_barrier();
+#pragma unroll
+        for (int i = 0; i < RB; ++i)
+            if (i % KS == part)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    hx_f4 v = red[((cw * RB + i) * NT + n) * 64 + lane];
+#pragma unroll
+                    for (int p = 1; p < KS; ++p) v += red[(((4 * p + cw) * RB + i) * NT + n) * 64 + lane];
+                    acc[i][n] = v;
+                }
+    }
+    if (sp.splits > 1) {  // the splits' sums, in order: the last workgroup of a tile to arrive adds them
+        constexpr int PIECES = RB * NT * 256;
+        hx_f4* mine = sp.partial + (size_t)tile * sp.splits * PIECES;
+        const __amdgpu_buffer_rsrc_t rp = coherent_rsrc(mine);
+#pragma unroll
+        for (int i = 0; i < RB; ++i)
+            if (i % KS == part)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    coherent_store4(rp, (split * PIECES + ((i * NT + n) * 4 + cw) * 64 + lane) * 16, acc[i][n]);
+        if (!arrive_last(sp.counters + tile, sp.splits)) return;
+#pragma unroll
+        for (int i = 0; i < RB; ++i)
+            if (i % KS == part)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const int at = (((i * NT + n) * 4 + cw) * 64 + lane) * 16;
+                    hx_f4 v = coherent_load4(rp, at);
+                    for (int p = 1; p < sp.splits; ++p) v += coherent_load4(rp, at + p * PIECES * 16);
+                    acc[i][n] = v;
+                }
     }
 #pragma unroll
     for (int i = 0; i < RB; ++i)
+        if (i % KS == part)
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const int nn = n0 + 32 * wave + 16 * n + col;
+            for (int n = 0; n < NT; ++n) {
+                const int nn = n0 + 16 * (cw * NT + n) + col;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int m = m0 + 16 * i + 4 * kg + e;
-                if (m < M && nn < a.N) store_y(y, (size_t)m * a.N + nn, acc[i][n][e], y_fp32);
+                for (int e = 0; e < 4; ++e) {
+                    const int m = m0 + 16 * i + 4 * kg + e;
+                    if (m < M && nn < a.N) store_y(y, (size_t)m * a.N + nn, acc[i][n][e], y_fp32);
+                }
             }
-        }
 }
 
-template <int BM, int GS, bool Z>
-__global__ __launch_bounds__(256) void w4_tile_kernel(const _Float16* x, W4Args a, void* y, int M, bool y_fp32)
+template <int BM, int NT, int KS, int PF, int GS, bool Z, bool V>
+__global__ __launch_bounds__(256 * KS) void w4_tile_kernel(const _Float16* x, W4Args a, void* y, int M, bool y_fp32, W4Split sp)
 {
-    w4_tile<BM, GS, Z>(x, a, y, M, y_fp32);
+    w4_tile<BM, NT, KS, PF, GS, Z, V>(x, a, y, M, y_fp32, sp);
 }
 
 // out[t][k] = scale * weight(tokens[t], k), the product in fp32 and rounded once; zeros for a token outside [0, N).
@@ -378,39 +472,132 @@ struct W4Call {
     void* y;
     int M;
     bool y_fp32;
+    void* ws;  // counters and the splits' sums, or null
     hipStream_t st;
 };
 
-template <int S, int MT, int NS, int NT, int GS, bool Z>
-hipError_t rows_launch(const W4Call& c)
+// Which kernel takes a call of M rows, by measured shapes (us, 4-bit, group 128, weights from memory).
+struct W4Plan {
+    enum Kind { ROWS4_FEW, ROWS4, ROWS8_FEW, ROWS8, ROWS16, TILE16, TILE32, TILE64, TILE64W, TILE128 } kind;
+    int splits, steps;  // of a tile kernel
+    long tiles;
+};
+struct W4Tile {
+    int bm, nt, ks;
+};
+constexpr W4Tile W4_TILES[] = {{16, 1, 2}, {32, 1, 2}, {64, 1, 2}, {64, 2, 1}, {128, 2, 1}};  // TILE16 ..
+constexpr int W4_SLOTS = 256;  // workgroups that splitting fills the chip with, one per CU
+
+W4Plan w4_tile_plan(int kind, int M, int N, int K, bool split)
+{
+    const W4Tile t = W4_TILES[kind - W4Plan::TILE16];
+    W4Plan p{(W4Plan::Kind)kind, 1, (K + 128 * t.ks - 1) / (128 * t.ks), 0};
+    p.tiles = (long)((M + t.bm - 1) / t.bm) * ((N + 64 * t.nt - 1) / (64 * t.nt));
+    // K is split while that fills idle CUs and leaves each split 4 steps: 32 rows, 8192 -> 4096, 27 us unsplit, 12.5 in 4, 15 in
+    // 8; 2048 -> 2048 7.7, 7.5 in 2, 8.0 in 4.
+    if (split && t.ks > 1) {
+        const int most = (int)(W4_SLOTS / p.tiles) < p.steps / 4 ? (int)(W4_SLOTS / p.tiles) : p.steps / 4;
+        if (most > 1) {
+            p.steps = (p.steps + most - 1) / most;
+            p.splits = ((K + 128 * t.ks - 1) / (128 * t.ks) + p.steps - 1) / p.steps;
+        }
+    }
+    return p;
+}
+
+// pieces: the kernels for groups in aligned pieces are among the choice; the others are built for the basic shapes only.
+W4Plan w4_plan(int M, int N, int K, bool split, bool pieces)
+{
+    const bool few = !pieces || (long)N * K <= 1l << 24;
+    // Few weights: 2 loads per wave, so that more waves share them (1 row, 4096 -> 2048: 3.9 us, 5.2 with 4 loads; 4096 -> 12288:
+    // 10.4 / 9.7, 4096 -> 151552: 76 / 59).
+    if (M <= 4) return {few ? W4Plan::ROWS4_FEW : W4Plan::ROWS4, 1, 0, 0};
+    if (M <= 8) return {few ? W4Plan::ROWS8_FEW : W4Plan::ROWS8, 1, 0, 0};
+    // 16 rows: 4096 -> 151552 87 us in rows, 99 in tiles; 4096 -> 12288 12.6 / 12.1; 8192 -> 4096 13.8 / 10.7
+    if (M <= 16) return pieces && N >= 32768 ? W4Plan{W4Plan::ROWS16, 1, 0, 0} : w4_tile_plan(W4Plan::TILE16, M, N, K, split);
+    if (M <= 32) return w4_tile_plan(W4Plan::TILE32, M, N, K, split);
+    // A step of a workgroup takes as long as its share of the CU lets it, or its own latency where it is alone.
+    struct Cost {
+        int kind;
+        float alone, shared;  // us per step: one workgroup on a CU, and per workgroup where a CU has several
+    };
+    constexpr Cost cost[] = {{W4Plan::TILE64, 0.85f, 0.95f}, {W4Plan::TILE64W, 0.82f, 0.74f}, {W4Plan::TILE128, 1.25f, 1.0f}};
+    W4Plan best{};
+    float least = 0.0f;
+    for (const Cost& c : cost) {
+        if (!pieces && c.kind != W4Plan::TILE64) continue;
+        const W4Plan p = w4_tile_plan(c.kind, M, N, K, split);
+        const float rounds = (float)((p.tiles * p.splits + 255) / 256) * c.shared;
+        const float t = p.steps * (rounds > c.alone ? rounds : c.alone) + (p.splits > 1 ? 3.0f : 0.0f);
+        if (c.kind == W4Plan::TILE64 || t < least) least = t, best = p;
+    }
+    return best;
+}
+
+size_t w4_partial_bytes(const W4Plan& p)
+{
+    const W4Tile t = W4_TILES[p.kind - W4Plan::TILE16];
+    return (size_t)p.tiles * p.splits * t.bm * 64 * t.nt * sizeof(float);
+}
+
+template <int S, int MT, int WAVES, int NS, int NT, int GS, bool Z, bool V>
+hipError_t rows_launch(const W4Call& c, int slots)
 {
     const int spans = ((c.a.K + 127) / 128 + S - 1) / S;
-    int wk = 1;  // waves along K: as many as have spans, up to all 8
-    while (wk < 8 && wk * NS < spans) wk *= 2;
-    const int rows = 8 / wk * NT * 16 / S, tiles = (c.a.N + rows - 1) / rows;
-    hipLaunchKernelGGL((w4_rows_kernel<S, MT, NS, NT, GS, Z>), dim3(tiles < 512 ? tiles : 512), dim3(512), 0, c.st, c.x, c.a,
-                       c.y, c.M, c.y_fp32, wk);
+    int wk = 1;  // waves along K: as many as have spans, up to all
+    while (wk < WAVES && wk * NS < spans) wk *= 2;
+    const int rows = WAVES / wk * NT * 16 / S, tiles = (c.a.N + rows - 1) / rows;
+    const int rounds = (tiles + slots - 1) / slots, grid = (tiles + rounds - 1) / rounds;  // equal rounds for all workgroups
+    hipLaunchKernelGGL((w4_rows_kernel<S, MT, WAVES, NS, NT, GS, Z, V>), dim3(grid), dim3(64 * WAVES), 0, c.st, c.x, c.a, c.y,
+                       c.M, c.y_fp32, wk);
     return hipGetLastError();
 }
 
-template <int BM, int GS, bool Z>
-hipError_t tile_launch(const W4Call& c)
+template <int BM, int NT, int KS, int PF, int GS, bool Z, bool V>
+hipError_t tile_launch(const W4Call& c, const W4Plan& p)
 {
-    constexpr size_t lds = sizeof(_Float16) * 2 * BM * 128;
-    const long tiles = (long)((c.M + BM - 1) / BM) * ((c.a.N + W4T_BN - 1) / W4T_BN);
-    hipLaunchKernelGGL((w4_tile_kernel<BM, GS, Z>), dim3((unsigned)tiles), dim3(256), lds, c.st, c.x, c.a, c.y, c.M, c.y_fp32);
+    constexpr size_t lds = sizeof(_Float16) * PF * KS * BM * 128;
+    if (p.tiles * p.splits > 0x7fffffl) return hipErrorInvalidValue;  // threads of a launch
+    const W4Split sp{p.splits, p.steps, reinterpret_cast<hx_f4*>(static_cast<char*>(c.ws) + HX_COUNTER_BYTES),
+                     static_cast<int*>(c.ws)};
+    hipLaunchKernelGGL((w4_tile_kernel<BM, NT, KS, PF, GS, Z, V>), dim3((unsigned)(p.tiles * p.splits)), dim3(256 * KS), lds,
+                       c.st, c.x, c.a, c.y, c.M, c.y_fp32, sp);
     return hipGetLastError();
+}
+
+template <int GS, bool Z, bool V>
+hipError_t gemm_launch(const W4Call& c)
+{
+    const W4Plan p = w4_plan(c.M, c.a.N, c.a.K, c.ws != nullptr, V || GS == 1);
+    if constexpr (V || GS == 1) {
+        switch (p.kind) {
+            case W4Plan::ROWS4: return rows_launch<4, 1, 8, 2, 2, GS, Z, V>(c, 512);
+            case W4Plan::ROWS8: return rows_launch<2, 1, 8, 2, 2, GS, Z, V>(c, 512);
+            case W4Plan::ROWS16: return rows_launch<2, 2, 16, 1, 2, GS, Z, V>(c, 256);
+            case W4Plan::TILE64W: return tile_launch<64, 2, 1, 3, GS, Z, V>(c, p);
+            case W4Plan::TILE128: return tile_launch<128, 2, 1, 2, GS, Z, V>(c, p);
+            default: break;
+        }
+    }
+    switch (p.kind) {
+        case W4Plan::ROWS4_FEW: return rows_launch<4, 1, 8, 1, 2, GS, Z, V>(c, 512);
+        case W4Plan::ROWS8_FEW: return rows_launch<2, 1, 8, 2, 1, GS, Z, V>(c, 512);
+        case W4Plan::TILE16: return tile_launch<16, 1, 2, 4, GS, Z, V>(c, p);
+        case W4Plan::TILE32: return tile_launch<32, 1, 2, 4, GS, Z, V>(c, p);
+        default: return tile_launch<64, 1, 2, 3, GS, Z, V>(c, p);
+    }
 }
 
 template <int GS, bool Z>
 hipError_t gemm_launch(const W4Call& c)
 {
-    if (c.M <= 4) return rows_launch<4, 1, 2, 4, GS, Z>(c);
-    if (c.M <= 8) return rows_launch<2, 1, 2, 4, GS, Z>(c);
-    if (c.M <= 16) return rows_launch<1, 1, 4, 2, GS, Z>(c);
-    if (c.M <= 32) return rows_launch<1, 2, 2, 2, GS, Z>(c);
-    if (c.M <= 64) return rows_launch<1, 4, 1, 2, GS, Z>(c);
-    return tile_launch<128, GS, Z>(c);
+    if constexpr (GS == 1) {
+        return gemm_launch<GS, Z, true>(c);
+    } else {
+        const bool pieces = c.a.groups % GS == 0 && reinterpret_cast<uintptr_t>(c.a.scales) % (2 * GS) == 0 &&
+                            reinterpret_cast<uintptr_t>(c.a.zeros) % GS == 0;
+        return pieces ? gemm_launch<GS, Z, true>(c) : gemm_launch<GS, Z, false>(c);
+    }
 }
 
 template <int GS>
@@ -421,10 +608,22 @@ hipError_t gemm_launch(const W4Call& c)
 
 }  // namespace
 
-hipError_t launch_w4_gemm(const _Float16* x, const W4Args& a, void* y, int M, bool y_fp32, hipStream_t st)
+// Bytes of workspace with which calls of M rows split K; 0 where none do.
+size_t w4_gemm_workspace_bytes(int M, int N, int K)
+{
+    size_t most = 0;
+    for (const bool pieces : {false, true}) {
+        const W4Plan p = w4_plan(M, N, K, true, pieces);
+        if (p.splits > 1 && w4_partial_bytes(p) > most) most = w4_partial_bytes(p);
+    }
+    return most ? HX_COUNTER_BYTES + most : 0;
+}
+
+hipError_t launch_w4_gemm(const _Float16* x, const W4Args& a, void* y, int M, bool y_fp32, void* ws, size_t ws_bytes,
+                          hipStream_t st)
 {
     if (M <= 0 || a.N <= 0) return hipSuccess;
-    const W4Call c{x, a, y, M, y_fp32, st};
+    const W4Call c{x, a, y, M, y_fp32, ws && ws_bytes >= w4_gemm_workspace_bytes(M, a.N, a.K) ? ws : nullptr, st};
     return a.group_log2 == 5 ? gemm_launch<4>(c) : a.group_log2 == 6 ? gemm_launch<2>(c) : gemm_launch<1>(c);
 }
 

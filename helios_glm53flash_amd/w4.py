@@ -9,13 +9,15 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import Optional
 
 import torch
 
 from ._lib import W4WordsC, check, lib
-from .exl3 import _get_device, _need, _ptr, _stream
+from .exl3 import _GEMM_EXTRA, _get_device, _need, _ptr, _stream, workspace
 
+COUNTER_BYTES = 64 * 1024  # arrival counters at the start of a workspace
 _NIBBLE_K = (0, 2, 4, 6, 1, 3, 5, 7)  # the k of an octet that each nibble of its word holds, lowest nibble first
 
 
@@ -88,8 +90,25 @@ def _on_one_device(*tensors) -> None:
             raise ValueError(f"tensors must be on the current device (cuda:{dev}), got {t.device}")
 
 
+@lru_cache(maxsize=4096)
+def _gemm_workspace_bytes(M: int, N: int, K: int) -> int:
+    return lib.hx_w4_gemm_workspace_size(M, N, K)
+
+
+def call_workspace(nbytes: int, device: torch.device, st: int) -> torch.Tensor:
+    """A call's workspace on stream st: the stream's own one, or, where the current stream is being captured, memory of the
+    graph's with counters that each replay clears, so that the graph depends on no buffer that a later call may replace."""
+    if torch.cuda.is_current_stream_capturing() and st == _stream(None):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws[:COUNTER_BYTES].zero_()
+        return ws
+    # the bytes behind every workspace, which hold a linear's splits, are enough here too
+    return workspace(max(0, nbytes - _GEMM_EXTRA), device, st)
+
+
 def gemm(y: torch.Tensor, x: torch.Tensor, w: W4Words, M: int, N: int, K: int, y_fp32: bool = False, stream=None) -> None:
-    """y[m][n] = sum_k x[m][k] W[n][k]: x fp16 [M][K], y fp32 or fp16 [M][N], any M (M = 0 is a no-op)."""
+    """y[m][n] = sum_k x[m][k] W[n][k]: x fp16 [M][K], y fp32 or fp16 [M][N], any M (M = 0 is a no-op).  Shapes that split K
+    over workgroups do so in the stream's workspace (exl3.workspace, which never grows for it)."""
     _need(x, "x", (torch.float16,))
     _need(y, "y", (torch.float32,) if y_fp32 else (torch.float16,))
     if M < 0 or x.numel() < M * K or y.numel() < M * N:
@@ -97,7 +116,11 @@ def gemm(y: torch.Tensor, x: torch.Tensor, w: W4Words, M: int, N: int, K: int, y
     if w.in_features != K or w.out_features != N:
         raise ValueError("W4Words shapes do not match K, N")
     _on_one_device(x, y, w.words)
-    check(lib.hx_w4_gemm(y.data_ptr(), x.data_ptr(), C.byref(w.c()), M, N, K, int(y_fp32), _stream(stream)), "hx_w4_gemm")
+    st = _stream(stream)
+    need = _gemm_workspace_bytes(M, N, K)
+    ws = call_workspace(need, x.device, st) if need else None
+    check(lib.hx_w4_gemm(y.data_ptr(), x.data_ptr(), C.byref(w.c()), M, N, K, int(y_fp32), st, _ptr(ws),
+                         ws.numel() if ws is not None else 0), "hx_w4_gemm")
 
 
 def embed(w: W4Words, tokens: torch.Tensor, out: torch.Tensor, n: int, scale: float = 1.0, stream=None) -> None:

@@ -235,7 +235,7 @@ int hx_gemm_nt_f16(void* y, const void* x, const void* w, int M, int N, int K, i
  * words: uint32 [N][16 * ceil(K / 128)], 16-byte aligned.  Word 4 g + j of each block of 128 k holds the eight codes
  * k = 32 j + 8 g + (0, 2, 4, 6, 1, 3, 5, 7) of the block in its nibbles, lowest first; codes past K are not used.
  * scales: fp16 [N][ceil(K / group)]; zeros: uint8 of that shape, or NULL for 8 everywhere; group: a power of two >= 32
- * (the last group of a row may be short).  K % 32 == 0, any N. */
+ * (the last group of a row may be short).  K % 32 == 0, K <= 2^22, any N. */
 typedef struct hx_w4_words {
     const void* words;
     const void* scales;
@@ -245,8 +245,12 @@ typedef struct hx_w4_words {
 
 /* y[M][N] = x W^T: x fp16 [M][K] (16-byte aligned), y fp32 (y_fp32) or fp16, fp32 sums rounded once.  The codes and zero
  * points enter the products exactly and the scales are applied to fp32 sums.  M == 0 is a no-op (x and y may
- * then be NULL).  Needs no workspace. */
-int hx_w4_gemm(void* y, const void* x, const hx_w4_words* w, int M, int N, int K, int y_fp32, hx_stream_t stream);
+ * then be NULL).  The workspace is optional: a call with at least hx_w4_gemm_workspace_size(M, N, K) bytes (0: the shape has no
+ * use for it; at most 9 MiB) splits K over more workgroups where there are few (up to three times as fast from 9 rows on),
+ * with the fp32 sums in another order than without; NULL or fewer bytes do without. */
+size_t hx_w4_gemm_workspace_size(int M, int N, int K);
+int hx_w4_gemm(void* y, const void* x, const hx_w4_words* w, int M, int N, int K, int y_fp32, hx_stream_t stream,
+               void* workspace, size_t workspace_bytes);
 
 /* out[t][:] = scale * W[tokens[t]][:] for t < n, fp32 (out_fp32) or fp16 rows of K (16-byte aligned); a token outside
  * [0, N) gives a row of zeros. */

@@ -42,9 +42,9 @@ def test_pack_refusals():
     assert w4.pack(torch.zeros((0, 64), dtype=torch.uint8)).shape == (0, 16)
 
 
-def gemm(y=16, x=16, words=16, scales=16, zeros=None, group=64, M=1, N=16, K=128, null=False):
+def gemm(y=16, x=16, words=16, scales=16, zeros=None, group=64, M=1, N=16, K=128, null=False, ws=None):
     w = _lib.W4WordsC(words, scales, zeros, group)
-    return LIB.hx_w4_gemm(y, x, None if null else C.byref(w), M, N, K, 1, None)
+    return LIB.hx_w4_gemm(y, x, None if null else C.byref(w), M, N, K, 1, None, ws, 1 << 30)
 
 
 @pytest.mark.parametrize("bad,text", [
@@ -52,7 +52,7 @@ def gemm(y=16, x=16, words=16, scales=16, zeros=None, group=64, M=1, N=16, K=128
     (dict(x=None), "null"), (dict(K=100), "multiple of 32"), (dict(K=0), "positive"), (dict(K=-128), "positive"),
     (dict(N=0), "positive"), (dict(M=-1), "negative"), (dict(group=16), "power of two"), (dict(group=96), "power of two"),
     (dict(group=0), "power of two"), (dict(group=-64), "power of two"), (dict(words=24), "16-byte"), (dict(x=8), "16-byte"),
-    (dict(y=18), "aligned"), (dict(scales=17), "aligned"), (dict(K=(1 << 24) + 32), "2^24")])
+    (dict(y=18), "aligned"), (dict(scales=17), "aligned"), (dict(K=(1 << 22) + 32), "2^22")])
 def test_gemm_refusals(bad, text):
     assert gemm(**bad) == _lib.HX_ERR_INVALID and text in err()
 
@@ -142,3 +142,14 @@ def test_reorder_refuses_irreducible_strides():
     dims = [(n, s * 4, s * 4) for n, s in zip(t.shape, t.stride())]
     with pytest.raises(ValueError):
         beam._merge(dims[1:], 4)
+
+
+def test_gemm_workspace():
+    size = LIB.hx_w4_gemm_workspace_size
+    assert gemm(ws=24) == _lib.HX_ERR_WORKSPACE and "16-byte" in err()
+    assert size(1, 4096, 8192) == 0 and size(0, 4096, 8192) == 0  # single tokens need none
+    assert size(64, 4096, 8192) > 65536
+    for M in (9, 16, 17, 32, 33, 64, 65, 128, 200, 512, 2000):
+        for N in (1, 64, 2048, 4096, 12288, 151552):
+            for K in (32, 2048, 4096, 16384, 1 << 22):
+                assert size(M, N, K) <= 9 << 20, (M, N, K)
