@@ -204,6 +204,9 @@ __device__ __forceinline__ void w4_rows(const _Float16* x, const W4Args& a, void
 #pragma unroll
                     for (int j = 0; j < 4; ++j) b[j] = word_operand(wv[j], sv.zero(j * GS / 4));
                     load_w(i, n, next_kb);
+                    // the loads stay here, ahead of this word's products: sunk to the end of the tile they cost 10 % of a long walk
+                    // (4096 -> 151552, 1 row: 65 -> 59 us)
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int g = 0; g < GS; ++g) {
                         const float f = sv.scale(g);
@@ -508,9 +511,9 @@ W4Plan w4_tile_plan(int kind, int M, int N, int K, bool split)
 // pieces: the kernels for groups in aligned pieces are among the choice; the others are built for the basic shapes only.
 W4Plan w4_plan(int M, int N, int K, bool split, bool pieces)
 {
-    const bool few = !pieces || (long)N * K <= 1l << 24;
-    // Few weights: 2 loads per wave, so that more waves share them (1 row, 4096 -> 2048: 3.9 us, 5.2 with 4 loads; 4096 -> 12288:
-    // 10.4 / 9.7, 4096 -> 151552: 76 / 59).
+    // Few weights: 2 loads per wave, so that more waves share them (1 row, 4096 -> 2048: 3.9 us, 4.7 with 4 loads; 8192 -> 4096
+    // 7.6 / 7.9, with 4 rows 10.8 / 9.1; 4096 -> 12288 9.7 / 9.1, 4096 -> 151552 73 / 62).
+    const bool few = !pieces || (long)N * K <= 1l << (M <= 2 ? 25 : 24);
     if (M <= 4) return {few ? W4Plan::ROWS4_FEW : W4Plan::ROWS4, 1, 0, 0};
     if (M <= 8) return {few ? W4Plan::ROWS8_FEW : W4Plan::ROWS8, 1, 0, 0};
     // 16 rows: 4096 -> 151552 87 us in rows, 99 in tiles; 4096 -> 12288 12.6 / 12.1; 8192 -> 4096 13.8 / 10.7
@@ -547,8 +550,7 @@ hipError_t rows_launch(const W4Call& c, int slots)
     int wk = 1;  // waves along K: as many as have spans, up to all
     while (wk < WAVES && wk * NS < spans) wk *= 2;
     const int rows = WAVES / wk * NT * 16 / S, tiles = (c.a.N + rows - 1) / rows;
-    const int rounds = (tiles + slots - 1) / slots, grid = (tiles + rounds - 1) / rounds;  // equal rounds for all workgroups
-    hipLaunchKernelGGL((w4_rows_kernel<S, MT, WAVES, NS, NT, GS, Z, V>), dim3(grid), dim3(64 * WAVES), 0, c.st, c.x, c.a, c.y,
+    hipLaunchKernelGGL((w4_rows_kernel<S, MT, WAVES, NS, NT, GS, Z, V>), dim3(tiles < slots ? tiles : slots), dim3(64 * WAVES), 0, c.st, c.x, c.a, c.y,
                        c.M, c.y_fp32, wk);
     return hipGetLastError();
 }
@@ -571,7 +573,7 @@ hipError_t gemm_launch(const W4Call& c)
     const W4Plan p = w4_plan(c.M, c.a.N, c.a.K, c.ws != nullptr, V || GS == 1);
     if constexpr (V || GS == 1) {
         switch (p.kind) {
-            case W4Plan::ROWS4: return rows_launch<4, 1, 8, 2, 2, GS, Z, V>(c, 512);
+            case W4Plan::ROWS4: return rows_launch<4, 1, 8, 1, 4, GS, Z, V>(c, 512);
             case W4Plan::ROWS8: return rows_launch<2, 1, 8, 2, 2, GS, Z, V>(c, 512);
             case W4Plan::ROWS16: return rows_launch<2, 2, 16, 1, 2, GS, Z, V>(c, 256);
             case W4Plan::TILE64W: return tile_launch<64, 2, 1, 3, GS, Z, V>(c, p);
