@@ -76,9 +76,25 @@ def _merge(dims, run):
     return (merged[0] if merged else (1, 0, 0)), run
 
 
+@lru_cache(maxsize=1024)
+def _geometry(src_shape, src_stride, dst_shape, dst_stride, e, dim, rows, out_rows):
+    """(outer, inner, bytes, source strides, destination strides) for the C call."""
+    want = list(src_shape)
+    want[dim] = out_rows
+    if src_shape[dim] != rows or list(dst_shape) != want:
+        raise ValueError("reorder: src must have batch * beams rows along dim, dst batch * out_beams and src's other extents")
+    if 0 in want:
+        return None
+    dims = [(n, s * e, d * e) for n, s, d in zip(src_shape, src_stride, dst_stride)]
+    (inner, si, di), run = _merge(dims[dim + 1:], e)
+    (outer, so, do), _ = _merge(dims[:dim], None)
+    three = C.c_int64 * 3
+    return outer, inner, run, three(so, dims[dim][1], si), three(do, dims[dim][2], di)
+
+
 def reorder(src: torch.Tensor, parents: torch.Tensor, dst: torch.Tensor, batch: int, beams: int, out_beams: int,
             dim: int = 0, stream=None) -> None:
-    """dst[.., b * out_beams + j, ..] = src[.., b * beams + parents[b][j], ..] along dimension dim, for states of any type
+    """dst[.., b * out_beams + j, ..] = src[.., b * beams + parents[b][j], ..] along dimension dim, for states of any real type
     and shape: dim counts batch * beams rows in src and batch * out_beams in dst, the other dimensions agree.  Views are
     accepted (a cache filled below its capacity) as long as the dimensions on either side of dim reduce to one stride each.
     Rows whose parent lies outside [0, beams) are left as they were; src and dst may not overlap."""
@@ -86,25 +102,18 @@ def reorder(src: torch.Tensor, parents: torch.Tensor, dst: torch.Tensor, batch: 
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise ValueError(f"reorder: {name} must be a device tensor")
     _need(parents, "parents", (torch.int64,))
-    if src.dtype != dst.dtype or src.dim() != dst.dim() or not -src.dim() <= dim < src.dim():
-        raise ValueError("reorder: src and dst must have the same type and dimensions, dim among them")
-    dim %= src.dim()
+    if src.dtype != dst.dtype or src.is_complex() or src.dim() != dst.dim() or not -src.dim() <= dim < src.dim():
+        raise ValueError("reorder: src and dst must have the same (real) type and dimensions, dim among them")
     if batch < 0 or beams < 1 or out_beams < 0 or parents.numel() < batch * out_beams:
         raise ValueError("reorder: parents smaller than batch * out_beams")
-    want = list(src.shape)
-    want[dim] = batch * out_beams
-    if src.shape[dim] != batch * beams or list(dst.shape) != want:
-        raise ValueError("reorder: src must have batch * beams rows along dim, dst batch * out_beams and src's other extents")
     _on_one_device(src, parents, dst)
-    if dst.numel() == 0:
+    g = _geometry(src.shape, src.stride(), dst.shape, dst.stride(), src.element_size(), dim % src.dim(), batch * beams,
+                  batch * out_beams)
+    if g is None:
         return
-    e = src.element_size()
-    dims = [(n, s * e, d * e) for n, s, d in zip(src.shape, src.stride(), dst.stride())]
-    (inner, si, di), run = _merge(dims[dim + 1:], e)
-    (outer, so, do), _ = _merge(dims[:dim], None)
-    three = C.c_int64 * 3
+    outer, inner, run, ss, ds = g
     check(lib.hx_beam_reorder(src.data_ptr(), parents.data_ptr(), dst.data_ptr(), batch, beams, out_beams, outer, inner, run,
-                              three(so, dims[dim][1], si), three(do, dims[dim][2], di), _stream(stream)), "hx_beam_reorder")
+                              ss, ds, _stream(stream)), "hx_beam_reorder")
 
 
 __all__ = ["select", "reorder"]

@@ -49,22 +49,18 @@ def unpack(words: torch.Tensor, K: int) -> torch.Tensor:
     return q.reshape(words.shape[0], words.shape[1] * 8)[:, :K].contiguous()
 
 
-@dataclass
+@dataclass(frozen=True)
 class W4Words:
     """One linear: words int32 [N][16 * ceil(K / 128)] (see pack), scales fp16 [N][ceil(K / group)], zeros uint8 of that
-    shape or None (8), the number K of input features, the group size (a power of two >= 32)."""
+    shape or None (8), the number K of input features, the group size (a power of two >= 32).  The tensors are checked and
+    the C descriptor is made once, here: that took 1.6 of the 7 us that a small call costs on the host."""
     words: torch.Tensor
     scales: torch.Tensor
     zeros: Optional[torch.Tensor]
     in_features: int
     group: int
 
-    @property
-    def out_features(self) -> int:
-        return self.words.shape[0]
-
-    def c(self) -> W4WordsC:
-        """The C descriptor, its tensors checked."""
+    def __post_init__(self):
         z, K, group = self.zeros, self.in_features, self.group
         if K <= 0 or K % 32 or group < 32 or group & (group - 1):
             raise ValueError("W4Words: K must be a positive multiple of 32 and group a power of two of at least 32")
@@ -79,8 +75,19 @@ class W4Words:
             _need(z, "zeros", (torch.uint8,))
             if z.shape != shape:
                 raise ValueError(f"W4Words: zeros must be {shape}")
-        _on_one_device(self.words, self.scales, z)
-        return W4WordsC(self.words.data_ptr(), self.scales.data_ptr(), _ptr(z), group)
+        if len({t.get_device() for t in (self.words, self.scales, z) if t is not None}) != 1:
+            raise ValueError("W4Words: words, scales and zeros must be on one device")
+        ptrs = (self.words.data_ptr(), self.scales.data_ptr(), _ptr(z))
+        object.__setattr__(self, "_ptrs", ptrs)
+        object.__setattr__(self, "_c", W4WordsC(*ptrs, group))
+        object.__setattr__(self, "device_index", self.words.get_device())
+        object.__setattr__(self, "out_features", shape[0])
+
+    def c(self) -> W4WordsC:
+        """The C descriptor (made again if a tensor was given other memory)."""
+        if (self.words.data_ptr(), self.scales.data_ptr(), _ptr(self.zeros)) != self._ptrs:
+            self.__post_init__()
+        return self._c
 
 
 def _on_one_device(*tensors) -> None:
@@ -88,6 +95,11 @@ def _on_one_device(*tensors) -> None:
     for t in tensors:
         if t is not None and t.get_device() != dev:
             raise ValueError(f"tensors must be on the current device (cuda:{dev}), got {t.device}")
+
+
+def _weights_here(w: W4Words) -> None:
+    if w.device_index != _get_device():
+        raise ValueError(f"the weights are on cuda:{w.device_index}, the current device is cuda:{_get_device()}")
 
 
 @lru_cache(maxsize=4096)
@@ -115,7 +127,8 @@ def gemm(y: torch.Tensor, x: torch.Tensor, w: W4Words, M: int, N: int, K: int, y
         raise ValueError("x / y smaller than M*K / M*N")
     if w.in_features != K or w.out_features != N:
         raise ValueError("W4Words shapes do not match K, N")
-    _on_one_device(x, y, w.words)
+    _on_one_device(x, y)
+    _weights_here(w)
     st = _stream(stream)
     need = _gemm_workspace_bytes(M, N, K)
     ws = call_workspace(need, x.device, st) if need else None
@@ -130,7 +143,8 @@ def embed(w: W4Words, tokens: torch.Tensor, out: torch.Tensor, n: int, scale: fl
     _need(out, "out", (torch.float16, torch.float32))
     if n < 0 or tokens.numel() < n or out.numel() < n * w.in_features:
         raise ValueError("embed: tokens / out smaller than n / n*K")
-    _on_one_device(tokens, out, w.words)
+    _on_one_device(tokens, out)
+    _weights_here(w)
     check(lib.hx_w4_embed(C.byref(w.c()), tokens.data_ptr(), out.data_ptr(), n, w.out_features, w.in_features, scale,
                           int(out.dtype == torch.float32), _stream(stream)), "hx_w4_embed")
 
