@@ -8,13 +8,15 @@
 // hold a NaN or +inf, or are all -inf, has none (its log-softmax is not defined); a logit of -inf is no candidate.
 // Sequences with fewer than n candidates get score -inf, parent -1 and token -1 behind them.
 //
-// Selection is one launch.  A workgroup takes one chunk of one row: it reads the chunk once into registers, and from there
-// come the chunk's maximum, the sum of its exponentials and its n largest logits.  The last workgroup of a sequence to
-// arrive merges the chunks: the rows' log-sum-exp in 64 bits, the candidates' scores in 64 bits, the n best of them.
+// Selection is one launch.  A workgroup takes one chunk of one row and reads it once, 4096 logits at a time with the next ones
+// in flight: running maximum and sum of exponentials per thread, and the logits that may be among the n largest.  The last
+// workgroup of a sequence to arrive merges the chunks: the rows' log-sum-exp in 64 bits, the candidates' scores in 64 bits, the n
+// best of them.
 //
 // The n largest of a set spread over threads, without sorting it: the n-th largest of the threads' maxima is a lower bound of
-// the n-th largest of all, and only elements that reach it (n to 2n of random ones) are ranked against each other.  Sets with more
-// ties at that bound than the candidate buffer holds are picked one by one instead.
+// the n-th largest of all, and only elements that reach it (n to 2n of random ones) are ranked against each other.  A chunk's
+// bound comes from its first 4096 logits, and again whenever the candidates overflow their buffer; where ties at the bound alone
+// overflow it, the n largest are picked one by one.
 #include "hx_gemv.hpp"
 #include "hx_kernels.hpp"
 
@@ -44,8 +46,8 @@ HX_INLINE uint32_t div_by(uint32_t i, FastDiv f)
     return q * (u64)f.d > i ? q - 1 : q;
 }
 
-// The n-th largest of 64 P keys in LDS, for one wave (0 where fewer than n are above 0): the key's bits from the top, each kept if
-// n keys still reach the value.
+// The n-th largest of 64 P keys in LDS, for one wave (0 where fewer than n are above 0): the key's bits from the top, two at a time,
+// each pair as large as still leaves n keys at or above the value.
 template <int P>
 HX_INLINE uint32_t nth_largest(const uint32_t* keys, int n)
 {
@@ -54,12 +56,13 @@ HX_INLINE uint32_t nth_largest(const uint32_t* keys, int n)
 #pragma unroll
     for (int p = 0; p < P; ++p) k[p] = keys[64 * p + lane];
     uint32_t t = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t c = t | (1u << bit);
-        int count = 0;
+    for (int bit = 30; bit >= 0; bit -= 2) {
+        int count[4] = {};
 #pragma unroll
-        for (int p = 0; p < P; ++p) count += __popcll(__ballot(k[p] >= c));
-        if (count >= n) t = c;
+        for (int d = 1; d < 4; ++d)
+#pragma unroll
+            for (int p = 0; p < P; ++p) count[d] += __popcll(__ballot(k[p] >= (t | (uint32_t)d << bit)));
+        t |= (uint32_t)(count[3] >= n ? 3 : count[2] >= n ? 2 : count[1] >= n ? 1 : 0) << bit;
     }
     return t;
 }
@@ -99,7 +102,7 @@ HX_INLINE float wave_sum(float v)
 }
 
 struct BeamPlan {
-    int chunks, lists;         // chunks of a row; beams * chunks, the lists of a sequence
+    int subs, chunks, lists;   // pieces of 4096 logits in a chunk; chunks of a row; beams * chunks, the lists of a sequence
     FastDiv by_chunks, by_lists;
     int cap;                   // candidates (16 bytes) that the LDS buffer holds
     u64* entries;              // [batch][n][lists]: the r-th best of each list, key << 32 | ~token, 0: none
@@ -108,7 +111,9 @@ struct BeamPlan {
 };
 
 constexpr int SEL_THREADS = 256;
-constexpr int MERGE_E = 16;                         // candidates of a thread in one round of the merge
+constexpr int SEL_E = 16;                           // logits of a thread in a piece
+constexpr int PIECE = SEL_THREADS * SEL_E;
+constexpr int MERGE_E = 8;                          // candidates of a thread in one round of the merge
 constexpr int MERGE = SEL_THREADS * MERGE_E;        // and of the workgroup
 
 // A candidate of the merge: its score (-inf: none) and w * vocab + token.
@@ -128,105 +133,168 @@ HX_INLINE void coherent_store8(__amdgpu_buffer_rsrc_t r, int off, u64 v)
     __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2v, v), r, off, 0, HX_BUF_SC1);
 }
 
-// One chunk of SEL_THREADS * E logits of row w of sequence b, as list `list` of the sequence.
-template <typename T, int E>
+// SEL_E logits of a thread: element i is logit (i / VEC * SEL_THREADS + thread) * VEC + i % VEC of its piece.
+template <typename T>
+struct Piece {
+    static constexpr int VEC = 16 / sizeof(T), NV = SEL_E / VEC;
+    typedef T vec __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
+    vec v[NV];
+    static HX_INLINE int offset(int i) { return (i / VEC * SEL_THREADS + (int)threadIdx.x) * VEC + i % VEC; }
+    // room: logits from x to the row's end; what lies behind is -inf
+    HX_INLINE void load(const T* x, int room)
+    {
+        if (room >= PIECE) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] = *reinterpret_cast<const vec*>(x + offset(i * VEC));
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int o = offset(i * VEC);
+                if (o + VEC <= room) {
+                    v[i] = *reinterpret_cast<const vec*>(x + o);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) v[i][j] = o + j < room ? x[o + j] : (T)-INFINITY;
+                }
+            }
+        }
+    }
+};
+
+HX_INLINE u64 wave_max_u64(u64 m)
+{
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        const u64 q = __shfl_xor(m, o, 64);
+        m = q > m ? q : m;
+    }
+    return m;
+}
+
+// Ranks the c candidates in LDS and puts the n best, in order, into `sorted`; returns how many there are.  The buffer is filled up
+// with zeros to the next 16, which the loop takes at a time: one by one, each waited for the LDS (7 us for 184).  Starts and ends
+// with a barrier.
+HX_INLINE int rank_entries(u64* cand, int c, int n, u64* sorted)
+{
+    if ((int)threadIdx.x < (-c & 15)) cand[c + threadIdx.x] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < c; i += SEL_THREADS) {
+        const u64 mine = cand[i];
+        int r = 0;
+        for (int j = 0; j < c; j += 16) {
+            ulonglong2 t[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) t[u] = reinterpret_cast<const ulonglong2*>(cand + j)[u];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) r += (t[u].x > mine) + (t[u].y > mine);
+        }
+        if (r < n) sorted[r] = mine;
+    }
+    __syncthreads();
+    return min(c, n);
+}
+
+// Chunk `chunk` of a row, as list `list` of sequence b.
+template <typename T>
 HX_INLINE void select_chunk(const T* x, int chunk, int list, const BeamArgs& a, const BeamPlan& p, long b, char* lds)
 {
-    constexpr int VEC = 16 / sizeof(T);
-    typedef T vec __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
     __shared__ uint32_t keys[SEL_THREADS];
+    __shared__ u64 sorted[BEAM_MAX_N];
+    __shared__ u64 best[4];
     __shared__ float part[2][4];
     __shared__ int count;
     u64* cand = reinterpret_cast<u64*>(lds);
     const int cap = 2 * p.cap;  // entries of 8 bytes
-    const int tid = threadIdx.x, wave = tid >> 6;
-    const int base = chunk * (SEL_THREADS * E), room = a.vocab - base;  // logits from the chunk's start to the row's end
-    float v[E];
-    if (room >= SEL_THREADS * E) {
-#pragma unroll
-        for (int i = 0; i < E / VEC; ++i) {
-            const vec t = *reinterpret_cast<const vec*>(x + base + (i * SEL_THREADS + tid) * VEC);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) v[i * VEC + j] = (float)t[j];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < E / VEC; ++i) {
-            const int o = (i * SEL_THREADS + tid) * VEC;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) v[i * VEC + j] = -INFINITY;
-            if (o + VEC <= room) {
-                const vec t = *reinterpret_cast<const vec*>(x + base + o);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) v[i * VEC + j] = (float)t[j];
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    if (o + j < room) v[i * VEC + j] = (float)x[base + o + j];
-            }
-        }
-    }
-    float most = -INFINITY;  // a NaN is skipped here and makes the sum a NaN below
-#pragma unroll
-    for (int i = 0; i < E; ++i) most = fmaxf(most, v[i]);
-    const float wm = wave_max(most);
-    if ((tid & 63) == 0) part[0][wave] = wm;
+    const int tid = threadIdx.x, wave = tid >> 6, n = a.n;
+    const int first = chunk * p.subs * PIECE;
+    const int pieces = min(p.subs, (a.vocab - first + PIECE - 1) / PIECE);
+    float m = -INFINITY, sum = 0.0f;  // of this thread: its maximum, its exponentials relative to that
+    uint32_t bound = 0;               // what a candidate has to reach
+    int c = 0;                        // candidates
     if (tid == 0) count = 0;
-    const uint32_t bound = bound_of(float_key(most), a.n, keys);  // its barriers publish part[0] and count
-    const float top = fmaxf(fmaxf(part[0][0], part[0][1]), fmaxf(part[0][2], part[0][3]));
-    // elements that reach the bound
-    if (float_key(most) >= bound && most > -INFINITY) {
-        const float least = bound > KEY_NEG_INF ? key_float(bound) : -INFINITY;
+    Piece<T> next;
+    next.load(x + first, a.vocab - first);
+    for (int s = 0; s < pieces; ++s) {
+        const int base = first + s * PIECE;
+        float v[SEL_E];
 #pragma unroll
-        for (int i = 0; i < E; ++i)
-            if (v[i] >= least && v[i] > -INFINITY) {
-                const int at = atomicAdd(&count, 1);
-                const uint32_t token = base + (i / VEC * SEL_THREADS + tid) * VEC + i % VEC;
-                if (at < cap) cand[at] = (u64)float_key(v[i]) << 32 | (uint32_t)~token;
+        for (int i = 0; i < SEL_E; ++i) v[i] = (float)next.v[i / Piece<T>::VEC][i % Piece<T>::VEC];
+        if (s + 1 < pieces) next.load(x + base + PIECE, a.vocab - base - PIECE);
+        float most = -INFINITY;  // a NaN is skipped here and makes the sum a NaN below
+#pragma unroll
+        for (int i = 0; i < SEL_E; ++i) most = fmaxf(most, v[i]);
+        auto append = [&] {
+            if (most > -INFINITY && float_key(most) >= bound) {
+                const float least = bound > KEY_NEG_INF ? key_float(bound) : -INFINITY;
+#pragma unroll
+                for (int i = 0; i < SEL_E; ++i)
+                    if (v[i] >= least && v[i] > -INFINITY) {
+                        const int at = atomicAdd(&count, 1);
+                        if (at < cap) cand[at] = (u64)float_key(v[i]) << 32 | (uint32_t)~(uint32_t)(base + Piece<T>::offset(i));
+                    }
             }
-    }
-    // exp of the exact difference to the maximum (0 in its place in a chunk of -inf, whose sum is 0)
-    const float sub = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;
+        };
+        if (s == 0) bound = bound_of(float_key(most), n, keys);  // its barriers publish count
+        append();
+        // exponentials of exact differences to the maximum (while that is -inf, of the logits: 0)
+        const float top = fmaxf(m, most), sub = top == -INFINITY ? 0.0f : top;
+        float add = 0.0f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) sum += __builtin_amdgcn_exp2f((v[i] - sub) * 1.44269504f);
-    sum = wave_sum(sum);
-    if ((tid & 63) == 0) part[1][wave] = sum;
-    __syncthreads();
-    const int c = count;
-    const __amdgpu_buffer_rsrc_t out = coherent_rsrc(p.entries + (size_t)b * a.n * p.lists + list);
-    if (c <= cap) {
-        for (int i = tid; i < c; i += SEL_THREADS) {
-            const u64 mine = cand[i];
-            int r = 0;
-            for (int j = 0; j < c; ++j) r += cand[j] > mine;
-            if (r < a.n) coherent_store8(out, r * p.lists * 8, mine);
-        }
-        for (int r = c + tid; r < a.n; r += SEL_THREADS) coherent_store8(out, r * p.lists * 8, 0);
-    } else {  // more ties than the buffer holds: one after the other
-        u64* best = cand;  // [4]
-        u64 last = ~0ull;
-        for (int r = 0; r < a.n; ++r) {
-            u64 m = 0;
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const uint32_t token = base + (i / VEC * SEL_THREADS + tid) * VEC + i % VEC;
-                const u64 k = v[i] > -INFINITY ? (u64)float_key(v[i]) << 32 | (uint32_t)~token : 0;
-                if (k < last && k > m) m = k;
-            }
-#pragma unroll
-            for (int o = 32; o >= 1; o >>= 1) {
-                const u64 q = __shfl_xor(m, o, 64);
-                m = q > m ? q : m;
-            }
-            __syncthreads();  // every thread is done with the buffer
-            if ((tid & 63) == 0) best[wave] = m;
+        for (int i = 0; i < SEL_E; ++i) add += __builtin_amdgcn_exp2f((v[i] - sub) * 1.44269504f);
+        sum = (m == top ? sum : sum * __builtin_amdgcn_exp2f((m - sub) * 1.44269504f)) + add;
+        m = top;
+        __syncthreads();
+        const int had = c;
+        c = count;
+        __syncthreads();  // every thread has read count
+        if (c > cap) {
+            // the candidates so far give a higher bound, and so does this piece by itself
+            c = rank_entries(cand, had, n, sorted);
+            if (c == n) bound = max(bound, (uint32_t)(sorted[n - 1] >> 32) + 1);  // equals come after them: later tokens
+            for (int i = tid; i < c; i += SEL_THREADS) cand[i] = sorted[i];
+            if (tid == 0) count = c;
+            bound = max(bound, bound_of(float_key(most), n, keys));
+            append();
             __syncthreads();
-            const u64 h = best[0] > best[1] ? best[0] : best[1], g = best[2] > best[3] ? best[2] : best[3];
-            last = h > g ? h : g;
-            if (tid == 0) coherent_store8(out, r * p.lists * 8, last);
+            const int now = count;
+            __syncthreads();
+            if (now > cap) {  // ties: the piece's n best, one after the other
+                u64 last = ~0ull;
+                int r = 0;
+                for (; r < n; ++r) {
+                    u64 k = 0;
+#pragma unroll
+                    for (int i = 0; i < SEL_E; ++i) {
+                        const u64 e = v[i] > -INFINITY
+                                          ? (u64)float_key(v[i]) << 32 | (uint32_t)~(uint32_t)(base + Piece<T>::offset(i)) : 0;
+                        if (e < last && e > k) k = e;
+                    }
+                    k = wave_max_u64(k);
+                    if ((tid & 63) == 0) best[wave] = k;
+                    __syncthreads();
+                    const u64 h = best[0] > best[1] ? best[0] : best[1], g = best[2] > best[3] ? best[2] : best[3];
+                    last = h > g ? h : g;
+                    if (tid == 0) cand[c + r] = last;
+                    __syncthreads();  // best is read before the next round's
+                }
+                c += r;
+                if (tid == 0) count = c;
+                __syncthreads();
+            } else {
+                c = now;
+            }
         }
     }
+    const float wm = wave_max(m);
+    if ((tid & 63) == 0) part[0][wave] = wm;
+    const int found = rank_entries(cand, c, n, sorted);
+    const float top = fmaxf(fmaxf(part[0][0], part[0][1]), fmaxf(part[0][2], part[0][3]));
+    // a thread without finite logits has m = -inf and a sum of 0 (or a NaN)
+    sum = wave_sum(m == top ? sum : sum * __builtin_amdgcn_exp2f((m - (top == -INFINITY ? 0.0f : top)) * 1.44269504f));
+    if ((tid & 63) == 0) part[1][wave] = sum;
+    const __amdgpu_buffer_rsrc_t out = coherent_rsrc(p.entries + (size_t)b * n * p.lists + list);
+    for (int r = tid; r < n; r += SEL_THREADS) coherent_store8(out, r * p.lists * 8, r < found ? sorted[r] : 0);
+    __syncthreads();
     if (tid == 0) {
         const float2 st = {top, (part[1][0] + part[1][1]) + (part[1][2] + part[1][3])};
         coherent_store8(coherent_rsrc(p.stats + (size_t)b * p.lists + list), 0, __builtin_bit_cast(u64, st));
@@ -246,42 +314,54 @@ HX_INLINE void select_merge(const BeamArgs& a, const BeamPlan& p, long b, char* 
     const int tid = threadIdx.x, lane = tid & 63, n = a.n;
     const __amdgpu_buffer_rsrc_t rs = coherent_rsrc(p.stats + (size_t)b * p.lists);
     const __amdgpu_buffer_rsrc_t re = coherent_rsrc(p.entries + (size_t)b * n * p.lists);
+    const int total = n * p.lists;
+    u64 e[MERGE_E];  // the first round's candidates come while the rows' sums are formed
+#pragma unroll
+    for (int i = 0; i < MERGE_E; ++i) {
+        const int q = i * SEL_THREADS + tid;
+        e[i] = q < total ? coherent_load8(re, q * 8) : 0;
+    }
     // score = offset[w] + (logit - tops[w]); offset NaN: the row has no candidates
     for (int w = tid >> 6; w < a.beams; w += 4) {
-        const double cum = (double)a.cum[b * a.beams + w];
-        double off = NAN;
-        float top = 0.0f;
-        if (!(fabs(cum) < INFINITY)) {
-        } else if (a.done && a.done[b * a.beams + w]) {
-            off = cum;
-        } else {
-            float m = -INFINITY;
-            for (int c = lane; c < p.chunks; c += 64)
-                m = fmaxf(m, __builtin_bit_cast(float2, coherent_load8(rs, (w * p.chunks + c) * 8)).x);
-            m = wave_max(m);
-            double s = 0.0;
-            for (int c = lane; c < p.chunks; c += 64) {
-                const float2 st = __builtin_bit_cast(float2, coherent_load8(rs, (w * p.chunks + c) * 8));
-                s += (double)st.y * exp((double)st.x - (double)m);
-            }
-#pragma unroll
-            for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
-            if (fabsf(m) < INFINITY && s < INFINITY) off = cum - log(s), top = m;  // a NaN fails both tests
+        const float cum = a.cum[b * a.beams + w];
+        const bool fin = a.done && a.done[b * a.beams + w];
+        // a chunk per lane, further ones by running maximum and sum (of finished and dead rows: whatever is there)
+        float m = -INFINITY;
+        double s = 0.0;
+        for (int c = lane; c < p.chunks; c += 64) {
+            const float2 st = __builtin_bit_cast(float2, coherent_load8(rs, (w * p.chunks + c) * 8));
+            const float top = fmaxf(m, st.x);
+            s = (m == top ? s : s * exp((double)m - (double)top)) +
+                (double)st.y * (st.x == top ? 1.0 : exp((double)st.x - (double)top));
+            m = top;
         }
-        if (lane == 0) offset[w] = off, tops[w] = top;
+        const float top = wave_max(m);
+        if (m != top) s *= exp((double)m - (double)top);
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+        if (lane == 0) {
+            double off = NAN;
+            float t = 0.0f;
+            if (!(fabsf(cum) < INFINITY)) {
+            } else if (fin) {
+                off = cum;
+            } else if (fabsf(top) < INFINITY && s < INFINITY) {  // a NaN fails both tests
+                off = (double)cum - log(s), t = top;
+            }
+            offset[w] = off, tops[w] = t;
+        }
     }
-    const int total = n * p.lists;
     int kept = 0;  // entries of carry
     __syncthreads();
     for (int done = 0; done < total;) {
         const int fresh = min(total - done, MERGE - kept);
         Cand v[MERGE_E];
-        u64 e[MERGE_E];
+        if (done > 0)
 #pragma unroll
-        for (int i = 0; i < MERGE_E; ++i) {
-            const int q = i * SEL_THREADS + tid;
-            e[i] = q < fresh ? coherent_load8(re, (done + q) * 8) : 0;
-        }
+            for (int i = 0; i < MERGE_E; ++i) {
+                const int q = i * SEL_THREADS + tid;
+                e[i] = q < fresh ? coherent_load8(re, (done + q) * 8) : 0;
+            }
         double most = -INFINITY;
 #pragma unroll
         for (int i = 0; i < MERGE_E; ++i) {
@@ -319,10 +399,18 @@ HX_INLINE void select_merge(const BeamArgs& a, const BeamPlan& p, long b, char* 
         __syncthreads();
         const int c = count;
         if (c <= p.cap) {
+            if (tid < (-c & 7)) cand[c + tid] = {-INFINITY, ~0ull};
+            __syncthreads();
             for (int i = tid; i < c; i += SEL_THREADS) {
                 const Cand mine = cand[i];
                 int r = 0;
-                for (int j = 0; j < c; ++j) r += better(cand[j].s, cand[j].at, mine.s, mine.at);
+                for (int j = 0; j < c; j += 8) {  // 8 at a time, as in rank_entries
+                    Cand t[8];
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) t[u] = cand[j + u];
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) r += better(t[u].s, t[u].at, mine.s, mine.at);
+                }
                 if (r < n) carry[r] = mine;
             }
             kept = min(c, n);
@@ -364,7 +452,7 @@ HX_INLINE void select_merge(const BeamArgs& a, const BeamPlan& p, long b, char* 
 }  // namespace
 
 // grid: [batch][beams][chunks]
-template <typename T, int E>
+template <typename T>
 __global__ __launch_bounds__(SEL_THREADS) void beam_select_kernel(const T* logits, BeamArgs a, BeamPlan p)
 {
     extern __shared__ __align__(16) char beam_lds[];
@@ -372,24 +460,23 @@ __global__ __launch_bounds__(SEL_THREADS) void beam_select_kernel(const T* logit
     const uint32_t b = div_by(blockIdx.x, p.by_lists), list = blockIdx.x - b * p.lists;
     // rows that are finished or dead are not read
     if (!(a.done && a.done[row]) && fabsf(a.cum[row]) < INFINITY)
-        select_chunk<T, E>(logits + row * a.ld, chunk, list, a, p, b, beam_lds);
+        select_chunk(logits + row * a.ld, chunk, list, a, p, b, beam_lds);
     if (!arrive_last(p.counters + b, p.lists)) return;
     select_merge(a, p, b, beam_lds);
 }
 
 namespace {
 
-// Logits of a chunk: 8192 (32 per thread), or 2048 where that leaves fewer than 4 workgroups per CU.
-int select_elems(long rows, int vocab) { return rows * ((vocab + 8191) / 8192) >= 1024 ? 32 : 8; }
-
+// A chunk is as many pieces as leave about 4 workgroups per CU, which is what their registers allow at once.
 struct SelectLayout {
-    int elems;
-    long chunks, lists;
+    long subs, chunks, lists;
     size_t entries, stats, total;  // bytes
     SelectLayout(int batch, int beams, int vocab, int n)
     {
-        elems = select_elems((long)batch * beams, vocab);
-        chunks = ((long)vocab + SEL_THREADS * elems - 1) / (SEL_THREADS * elems);
+        const long pieces = ((long)vocab + PIECE - 1) / PIECE, rows = (long)batch * beams;
+        const long per_row = 1024 / rows > 1 ? 1024 / rows : 1;  // chunks
+        subs = (pieces + per_row - 1) / per_row;
+        chunks = (pieces + subs - 1) / subs;
         lists = beams * chunks;
         entries = (size_t)batch * n * lists * sizeof(u64);
         stats = (size_t)batch * lists * sizeof(float2);
@@ -398,14 +485,6 @@ struct SelectLayout {
 };
 
 FastDiv fast_div(uint32_t d) { return {d, (uint32_t)(((1ull << 32) + d - 1) / d)}; }
-
-template <typename T, int E>
-hipError_t select_launch(const void* logits, const BeamArgs& a, const BeamPlan& p, size_t lds, hipStream_t st)
-{
-    hipLaunchKernelGGL((beam_select_kernel<T, E>), dim3(a.batch * p.lists), dim3(SEL_THREADS), lds, st,
-                       static_cast<const T*>(logits), a, p);
-    return hipGetLastError();
-}
 
 }  // namespace
 
@@ -422,15 +501,20 @@ hipError_t launch_beam_select(const void* logits, bool fp32, const BeamArgs& a, 
     if (a.batch <= 0) return hipSuccess;
     const SelectLayout l(a.batch, a.beams, a.vocab, a.n);
     char* base = static_cast<char*>(ws);
-    // the candidate buffer, 16 times what is asked for (32 times in a chunk's 8-byte entries): ties aside the bound is reached by
-    // n threads (or quads) at most, each with at most 32 elements or MERGE_E candidates, and by n to 2n elements as a rule
-    const BeamPlan p{(int)l.chunks, (int)l.lists, fast_div(l.chunks), fast_div(l.lists), a.n * MERGE_E,
+    // the candidate buffer, 16 times what is asked for (32 times in a chunk's 8-byte entries) and more for few: ties aside a bound
+    // is reached by n threads (or quads) at most, and by n to 2n elements as a rule
+    const int cap = a.n > 8 ? 16 * a.n : 128;
+    const BeamPlan p{(int)l.subs, (int)l.chunks, (int)l.lists, fast_div(l.chunks), fast_div(l.lists), cap,
                      reinterpret_cast<u64*>(base + HX_COUNTER_BYTES),
                      reinterpret_cast<float2*>(base + HX_COUNTER_BYTES + l.entries), reinterpret_cast<int*>(base)};
     const size_t lds = ((size_t)a.beams * 12 + 15) / 16 * 16 + (size_t)p.cap * sizeof(Cand);
-    if (l.elems == 32)
-        return fp32 ? select_launch<float, 32>(logits, a, p, lds, st) : select_launch<_Float16, 32>(logits, a, p, lds, st);
-    return fp32 ? select_launch<float, 8>(logits, a, p, lds, st) : select_launch<_Float16, 8>(logits, a, p, lds, st);
+    const dim3 grid(a.batch * p.lists);
+    if (fp32)
+        hipLaunchKernelGGL((beam_select_kernel<float>), grid, dim3(SEL_THREADS), lds, st, static_cast<const float*>(logits), a, p);
+    else
+        hipLaunchKernelGGL((beam_select_kernel<_Float16>), grid, dim3(SEL_THREADS), lds, st,
+                           static_cast<const _Float16*>(logits), a, p);
+    return hipGetLastError();
 }
 
 // dst[o][b * out_beams + j][i][:] = src[o][b * beams + parents[b][j]][i][:], pieces of p.bytes bytes at byte strides.
