@@ -80,9 +80,9 @@ HX_INLINE uint32_t bound_of(uint32_t key, int n, uint32_t* keys)
         keys[threadIdx.x] = key;
     }
     __syncthreads();
-    if (threadIdx.x < 64) {
+    if (hx_vwave() == 0) {  // another SIMD for each of the workgroups that share a CU
         const uint32_t t = n <= 32 ? nth_largest<1>(keys, n) : nth_largest<4>(keys, n);
-        if (threadIdx.x == 0) bound = t;
+        if ((threadIdx.x & 63) == 0) bound = t;
     }
     __syncthreads();
     return bound;
@@ -116,7 +116,7 @@ constexpr int PIECE = SEL_THREADS * SEL_E;
 constexpr int MERGE_E = 8;                          // candidates of a thread in one round of the merge
 constexpr int MERGE = SEL_THREADS * MERGE_E;        // and of the workgroup
 
-// A candidate of the merge: its score (-inf: none) and w * vocab + token.
+// A candidate of the merge: its score (-inf: none) and beam << 32 | token, in whose order equal scores come.
 struct Cand {
     double s;
     u64 at;
@@ -309,82 +309,100 @@ HX_INLINE void select_merge(const BeamArgs& a, const BeamPlan& p, long b, char* 
     __shared__ Cand best[4];
     __shared__ int count;
     double* offset = reinterpret_cast<double*>(lds);
-    float* tops = reinterpret_cast<float*>(offset + a.beams);
+    float* tops = reinterpret_cast<float*>(offset + a.beams);  // NaN: the beam is finished
     Cand* cand = reinterpret_cast<Cand*>(lds + ((size_t)a.beams * 12 + 15) / 16 * 16);
-    const int tid = threadIdx.x, lane = tid & 63, n = a.n;
+    const int tid = threadIdx.x, lane = tid & 63, n = a.n, total = n * p.lists;
     const __amdgpu_buffer_rsrc_t rs = coherent_rsrc(p.stats + (size_t)b * p.lists);
     const __amdgpu_buffer_rsrc_t re = coherent_rsrc(p.entries + (size_t)b * n * p.lists);
-    const int total = n * p.lists;
-    u64 e[MERGE_E];  // the first round's candidates come while the rows' sums are formed
+    u64 e[MERGE_E];  // the first round's entries come while the rows' sums are formed
 #pragma unroll
     for (int i = 0; i < MERGE_E; ++i) {
         const int q = i * SEL_THREADS + tid;
         e[i] = q < total ? coherent_load8(re, q * 8) : 0;
     }
-    // score = offset[w] + (logit - tops[w]); offset NaN: the row has no candidates
-    for (int w = tid >> 6; w < a.beams; w += 4) {
-        const float cum = a.cum[b * a.beams + w];
-        const bool fin = a.done && a.done[b * a.beams + w];
-        // a chunk per lane, further ones by running maximum and sum (of finished and dead rows: whatever is there)
+    // score = offset[w] + (logit - tops[w]); offset NaN: the row has no candidates.  g lanes per row, a chunk each (further ones
+    // by running maximum and sum).
+    int g = 1;
+    while (g < 64 && g < p.chunks) g *= 2;
+    for (int w0 = 0; w0 < a.beams; w0 += SEL_THREADS / g) {
+        const int w = w0 + tid / g;
+        const bool mine = w < a.beams;
+        const float cum = mine ? a.cum[b * a.beams + w] : NAN;
+        const bool fin = mine && a.done && a.done[b * a.beams + w];
         float m = -INFINITY;
         double s = 0.0;
-        for (int c = lane; c < p.chunks; c += 64) {
+        // of finished and dead rows: whatever is there
+        for (int c = tid % g; mine && c < p.chunks; c += g) {
             const float2 st = __builtin_bit_cast(float2, coherent_load8(rs, (w * p.chunks + c) * 8));
-            const float top = fmaxf(m, st.x);
-            s = (m == top ? s : s * exp((double)m - (double)top)) +
-                (double)st.y * (st.x == top ? 1.0 : exp((double)st.x - (double)top));
-            m = top;
+            if (c < g) {
+                m = st.x, s = (double)st.y;
+            } else {
+                const float top = fmaxf(m, st.x);
+                s = s * exp((double)m - (double)top) + (double)st.y * exp((double)st.x - (double)top);
+                m = top;
+            }
         }
-        const float top = wave_max(m);
+        float top = m;
+        for (int o = g / 2; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
         if (m != top) s *= exp((double)m - (double)top);
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
-        if (lane == 0) {
+        for (int o = g / 2; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+        if (mine && tid % g == 0) {
             double off = NAN;
-            float t = 0.0f;
             if (!(fabsf(cum) < INFINITY)) {
             } else if (fin) {
-                off = cum;
+                off = (double)cum, top = NAN;
             } else if (fabsf(top) < INFINITY && s < INFINITY) {  // a NaN fails both tests
-                off = (double)cum - log(s), t = top;
+                off = (double)cum - log(s);
             }
-            offset[w] = off, tops[w] = t;
+            offset[w] = off, tops[w] = top;
         }
     }
-    int kept = 0;  // entries of carry
+    int kept = 0, nothing = 0;  // entries of carry; entries in a row that were no better than those
     __syncthreads();
-    for (int done = 0; done < total;) {
-        const int fresh = min(total - done, MERGE - kept);
+    for (int at = 0; at < total;) {
+        const int fresh = min(total - at, MERGE - kept);
         Cand v[MERGE_E];
-        if (done > 0)
+        if (at > 0)
 #pragma unroll
             for (int i = 0; i < MERGE_E; ++i) {
                 const int q = i * SEL_THREADS + tid;
-                e[i] = q < fresh ? coherent_load8(re, (done + q) * 8) : 0;
+                e[i] = q < fresh ? coherent_load8(re, (at + q) * 8) : 0;
             }
+        const Cand last_kept = kept == n ? carry[n - 1] : Cand{-INFINITY, ~0ull};
         double most = -INFINITY;
+        bool any = false;  // an entry that would be among the n best so far
 #pragma unroll
         for (int i = 0; i < MERGE_E; ++i) {
             const int q = i * SEL_THREADS + tid;
             v[i] = {-INFINITY, 0};
             if (q < fresh) {
-                const uint32_t at = done + q, rank = div_by(at, p.by_lists), list = at - rank * p.lists;
+                const uint32_t f = at + q, rank = div_by(f, p.by_lists), list = f - rank * p.lists;
                 const uint32_t w = div_by(list, p.by_chunks);
                 const double off = offset[w];
-                const bool fin = a.done && a.done[b * a.beams + w];
+                const float top = tops[w];
                 if (off == off) {
-                    if (fin) {
-                        if (rank == 0 && list == w * p.chunks) v[i] = {off, w * (u64)a.vocab + a.eos};
+                    if (top != top) {
+                        if (rank == 0 && list == w * p.chunks) v[i] = {off, (u64)w << 32 | (uint32_t)a.eos};
                     } else if (e[i]) {
-                        v[i] = {off + ((double)key_float((uint32_t)(e[i] >> 32)) - (double)tops[w]),
-                                w * (u64)a.vocab + (uint32_t)~(uint32_t)e[i]};
+                        v[i] = {off + ((double)key_float((uint32_t)(e[i] >> 32)) - (double)top),
+                                (u64)w << 32 | (uint32_t)~(uint32_t)e[i]};
                     }
                 }
+                any |= better(v[i].s, v[i].at, last_kept.s, last_kept.at);
             } else if (q < fresh + kept) {
                 v[i] = carry[q - fresh];
             }
             most = fmax(most, v[i].s);
         }
+        at += fresh;
+        if (!__syncthreads_or(any)) {
+            // Every list is in descending order and the r-th entries of all lists come before the r+1-st: once an entry of each
+            // list in turn was no better, none behind them is.
+            nothing += fresh;
+            if (nothing >= p.lists) break;
+            continue;
+        }
+        nothing = 0;
         if (tid == 0) count = 0;
         // scores rounded to fp32 keep their order (not strictly): the bound holds for the rounded ones
         const uint32_t bound = bound_of(most > -INFINITY ? float_key((float)most) : 0, n, keys);
@@ -392,8 +410,8 @@ HX_INLINE void select_merge(const BeamArgs& a, const BeamPlan& p, long b, char* 
 #pragma unroll
             for (int i = 0; i < MERGE_E; ++i)
                 if (v[i].s > -INFINITY && float_key((float)v[i].s) >= bound) {
-                    const int at = atomicAdd(&count, 1);
-                    if (at < p.cap) cand[at] = v[i];
+                    const int to = atomicAdd(&count, 1);
+                    if (to < p.cap) cand[to] = v[i];
                 }
         }
         __syncthreads();
@@ -425,8 +443,8 @@ HX_INLINE void select_merge(const BeamArgs& a, const BeamPlan& p, long b, char* 
 #pragma unroll
                 for (int o = 32; o >= 1; o >>= 1) {
                     const double s = __shfl_xor(m.s, o, 64);
-                    const u64 at = __shfl_xor(m.at, o, 64);
-                    if (better(s, at, m.s, m.at)) m = {s, at};
+                    const u64 i = __shfl_xor(m.at, o, 64);
+                    if (better(s, i, m.s, m.at)) m = {s, i};
                 }
                 if (lane == 0) best[tid >> 6] = m;
                 __syncthreads();
@@ -438,14 +456,12 @@ HX_INLINE void select_merge(const BeamArgs& a, const BeamPlan& p, long b, char* 
             }
             kept = n;
         }
-        done += fresh;
     }
     for (int r = tid; r < n; r += SEL_THREADS) {
         const bool found = r < kept;
-        const u64 at = found ? carry[r].at : 0;
         a.scores[b * n + r] = found ? (float)carry[r].s : -INFINITY;
-        a.parents[b * n + r] = found ? (int64_t)(at / a.vocab) : -1;
-        a.tokens[b * n + r] = found ? (int64_t)(at % a.vocab) : -1;
+        a.parents[b * n + r] = found ? (int64_t)(carry[r].at >> 32) : -1;
+        a.tokens[b * n + r] = found ? (int64_t)(uint32_t)carry[r].at : -1;
     }
 }
 
