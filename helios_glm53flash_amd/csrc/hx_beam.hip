@@ -8,15 +8,14 @@
 // hold a NaN or +inf, or are all -inf, has none (its log-softmax is not defined); a logit of -inf is no candidate.
 // Sequences with fewer than n candidates get score -inf, parent -1 and token -1 behind them.
 //
-// Selection is one launch.  A workgroup takes one chunk of one row and reads it once, 4096 logits at a time with the next ones
-// in flight: running maximum and sum of exponentials per thread, and the logits that may be among the n largest.  The last
-// workgroup of a sequence to arrive merges the chunks: the rows' log-sum-exp in 64 bits, the candidates' scores in 64 bits, the n
-// best of them.
+// Selection is one launch.  A workgroup takes one chunk of one row and reads it once, in pieces of 4096 logits with the next
+// two in flight: running maximum and sum of exponentials per thread, and which blocks (the 16 logits of a thread and piece) may
+// hold some of the n largest.  Few blocks are left at the end; their logits are read again and ranked.  The last workgroup of
+// a sequence to arrive merges the chunks: the rows' log-sum-exp in 64 bits, the candidates' scores in 64 bits, the n best of them.
 //
 // The n largest of a set spread over threads, without sorting it: the n-th largest of the threads' maxima is a lower bound of
-// the n-th largest of all, and only elements that reach it (n to 2n of random ones) are ranked against each other.  A chunk's
-// bound comes from its first 4096 logits, and again whenever the candidates overflow their buffer; where ties at the bound alone
-// overflow it, the n largest are picked one by one.
+// the n-th largest of all, and only what reaches it (n to 2n of random elements) is ranked.  The bound is renewed after 1, 2,
+// 4, .. pieces.
 #include "hx_gemv.hpp"
 #include "hx_kernels.hpp"
 
@@ -79,32 +78,36 @@ HX_INLINE uint32_t bound_of(uint32_t key, int n, uint32_t* keys)
     } else {
         keys[threadIdx.x] = key;
     }
-    __syncthreads();
+    hx_lds_barrier();
     if (hx_vwave() == 0) {  // another SIMD for each of the workgroups that share a CU
         const uint32_t t = n <= 32 ? nth_largest<1>(keys, n) : nth_largest<4>(keys, n);
         if ((threadIdx.x & 63) == 0) bound = t;
     }
-    __syncthreads();
+    hx_lds_barrier();
     return bound;
 }
 
-HX_INLINE float wave_max(float v)
-{
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
-}
+// Over the 64 lanes, with lane-permuted operands instead of round trips through the LDS crossbar; every lane gets the result.
+HX_INLINE float wave_max(float v) { return key_float(hx_wave_max_u32(float_key(v))); }
 HX_INLINE float wave_sum(float v)
 {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+    auto add = [&](auto ctrl, auto rows) {
+        v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value,
+                                                                   decltype(rows)::value, 0xf, false));
+    };
+    add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});  // row_shr:1
+    add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});  // row_shr:2
+    add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});  // row_shr:4
+    add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});  // row_shr:8
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // row_bcast:15
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // row_bcast:31
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 struct BeamPlan {
     int subs, chunks, lists;   // pieces of 4096 logits in a chunk; chunks of a row; beams * chunks, the lists of a sequence
     FastDiv by_chunks, by_lists;
-    int cap;                   // candidates (16 bytes) that the LDS buffer holds
+    int cap;                   // candidates (16 bytes) that the merge's LDS buffer holds
     u64* entries;              // [batch][n][lists]: the r-th best of each list, key << 32 | ~token, 0: none
     float2* stats;             // [batch][lists]: the chunk's maximum, the sum of exp(logit - maximum)
     int* counters;             // arrivals per sequence
@@ -113,6 +116,7 @@ struct BeamPlan {
 constexpr int SEL_THREADS = 256;
 constexpr int SEL_E = 16;                           // logits of a thread in a piece
 constexpr int PIECE = SEL_THREADS * SEL_E;
+constexpr int BLOCKS = 4 * SEL_THREADS;              // entries of a chunk's list of blocks
 constexpr int MERGE_E = 8;                          // candidates of a thread in one round of the merge
 constexpr int MERGE = SEL_THREADS * MERGE_E;        // and of the workgroup
 
@@ -133,31 +137,75 @@ HX_INLINE void coherent_store8(__amdgpu_buffer_rsrc_t r, int off, u64 v)
     __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2v, v), r, off, 0, HX_BUF_SC1);
 }
 
-// SEL_E logits of a thread: element i is logit (i / VEC * SEL_THREADS + thread) * VEC + i % VEC of its piece.
+// Sums of exponentials are relative to 2^ref(top), top log2 e in fp32, or where that overflows (a maximum beyond REF_MAX) relative
+// to e^top.  ref_rest(top) is what the rounding of ref left out: relative to e^top the former are 2^-ref_rest times as much.
+// A maximum of +inf or a NaN makes the sum a NaN.  log2 e itself rounded to fp32 is off by 1.3e-8, which changes a
+// log-sum-exp by that times the row's entropy, at most 2e-7.
+constexpr float LOG2E = 1.44269504f, REF_MAX = 2e38f;
+HX_INLINE bool ref_fits(float top) { return fabsf(top) < REF_MAX; }
+HX_INLINE float ref_rest(float top) { return ref_fits(top) ? __builtin_fmaf(top, LOG2E, -(top * LOG2E)) : 0.0f; }
+// Factor that takes a sum relative to `from` to one relative to the larger `to`.
+HX_INLINE float rescale(float from, float to)
+{
+    return __builtin_amdgcn_exp2f(ref_fits(from) && ref_fits(to) ? from * LOG2E - to * LOG2E : (from - to) * LOG2E);
+}
+
+// SEL_E logits of a thread: element i is logit (i / VEC * SEL_THREADS + t) * VEC + i % VEC of its piece.
 template <typename T>
 struct Piece {
     static constexpr int VEC = 16 / sizeof(T), NV = SEL_E / VEC;
     typedef T vec __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
     vec v[NV];
-    static HX_INLINE int offset(int i) { return (i / VEC * SEL_THREADS + (int)threadIdx.x) * VEC + i % VEC; }
-    // room: logits from x to the row's end; what lies behind is -inf
-    HX_INLINE void load(const T* x, int room)
+    static HX_INLINE int offset(int t, int i) { return (i / VEC * SEL_THREADS + t) * VEC + i % VEC; }
+    HX_INLINE void load(const T* x)
     {
-        if (room >= PIECE) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) v[i] = *reinterpret_cast<const vec*>(x + offset(i * VEC));
-        } else {
+        for (int i = 0; i < NV; ++i) v[i] = *reinterpret_cast<const vec*>(x + offset(threadIdx.x, i * VEC));
+    }
+    // Thread t's share of a piece of which only `room` logits are there; what lies behind is -inf.
+    HX_INLINE void load_end(const T* x, int t, int room)
+    {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int o = offset(i * VEC);
-                if (o + VEC <= room) {
-                    v[i] = *reinterpret_cast<const vec*>(x + o);
-                } else {
+        for (int i = 0; i < NV; ++i) {
+            const int o = offset(t, i * VEC);
+            if (o + VEC <= room) {
+                v[i] = *reinterpret_cast<const vec*>(x + o);
+            } else {
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) v[i][j] = o + j < room ? x[o + j] : (T)-INFINITY;
-                }
+                for (int j = 0; j < VEC; ++j) v[i][j] = o + j < room ? x[o + j] : (T)-INFINITY;
             }
         }
+    }
+    HX_INLINE float operator[](int i) const { return (float)v[i / VEC][i % VEC]; }
+    HX_INLINE float most() const
+    {
+        vec t = v[0];
+#pragma unroll
+        for (int i = 1; i < NV; ++i) t = __builtin_elementwise_max(t, v[i]);
+        float r = (float)t[0];
+        if constexpr (sizeof(T) == 2) {  // two at a time down to the last pair
+            hx_h4 h = __builtin_elementwise_max(hx_h4{t[0], t[1], t[2], t[3]}, hx_h4{t[4], t[5], t[6], t[7]});
+            hx_h2 q = __builtin_elementwise_max(hx_h2{h[0], h[1]}, hx_h2{h[2], h[3]});
+            r = fmaxf((float)q[0], (float)q[1]);
+        } else {
+#pragma unroll
+            for (int j = 1; j < VEC; ++j) r = fmaxf(r, (float)t[j]);
+        }
+        return r;
+    }
+    // Sum of the exponentials relative to top (0 where that is -inf): one multiply-add and one exponential per logit.
+    HX_INLINE float sum(float top) const
+    {
+        float s = 0.0f;
+        if (ref_fits(top) || top == -INFINITY) {
+            const float r = top == -INFINITY ? 0.0f : top * LOG2E;
+#pragma unroll
+            for (int i = 0; i < SEL_E; ++i) s += __builtin_amdgcn_exp2f(__builtin_fmaf((*this)[i], LOG2E, -r));
+        } else {
+#pragma unroll
+            for (int i = 0; i < SEL_E; ++i) s += __builtin_amdgcn_exp2f(((*this)[i] - top) * LOG2E);
+        }
+        return s;
     }
 };
 
@@ -177,7 +225,7 @@ HX_INLINE u64 wave_max_u64(u64 m)
 HX_INLINE int rank_entries(u64* cand, int c, int n, u64* sorted)
 {
     if ((int)threadIdx.x < (-c & 15)) cand[c + threadIdx.x] = 0;
-    __syncthreads();
+    hx_lds_barrier();
     for (int i = threadIdx.x; i < c; i += SEL_THREADS) {
         const u64 mine = cand[i];
         int r = 0;
@@ -190,111 +238,177 @@ HX_INLINE int rank_entries(u64* cand, int c, int n, u64* sorted)
         }
         if (r < n) sorted[r] = mine;
     }
-    __syncthreads();
+    hx_lds_barrier();
     return min(c, n);
 }
 
 // Chunk `chunk` of a row, as list `list` of sequence b.
+//
+// Blocks are ordered by their maximum, then by their piece: logits of an earlier piece have lower tokens, so a block with n
+// blocks before it in that order holds none of the n best.  (Blocks of one piece with equal maxima are not told apart.)
 template <typename T>
 HX_INLINE void select_chunk(const T* x, int chunk, int list, const BeamArgs& a, const BeamPlan& p, long b, char* lds)
 {
     __shared__ uint32_t keys[SEL_THREADS];
-    __shared__ u64 sorted[BEAM_MAX_N];
+    __shared__ u64 sorted[BEAM_MAX_N + SEL_THREADS];
     __shared__ u64 best[4];
     __shared__ float part[2][4];
     __shared__ int count;
-    u64* cand = reinterpret_cast<u64*>(lds);
-    const int cap = 2 * p.cap;  // entries of 8 bytes
+    u64* cand = reinterpret_cast<u64*>(lds);  // [BLOCKS]: key of the maximum << 32 | ~(piece * SEL_THREADS + thread)
     const int tid = threadIdx.x, wave = tid >> 6, n = a.n;
-    const int first = chunk * p.subs * PIECE;
-    const int pieces = min(p.subs, (a.vocab - first + PIECE - 1) / PIECE);
-    float m = -INFINITY, sum = 0.0f;  // of this thread: its maximum, its exponentials relative to that
-    uint32_t bound = 0;               // what a candidate has to reach
-    int c = 0;                        // candidates
+    const int first = chunk * p.subs * PIECE, end = min(first + p.subs * PIECE, a.vocab);
+    const int whole = (end - first) / PIECE;  // pieces; what is left over ends the row
+    const bool over = first + whole * PIECE < end;
+    float m = -INFINITY, sum = 0.0f;  // of this thread: its maximum; its exponentials, relative to that
+    uint32_t need = 1, bound = 0;     // keys: what a block has to reach, what n logits reach
+    int free = 0;                     // pieces that the list has room for in any case
     if (tid == 0) count = 0;
-    Piece<T> next;
-    next.load(x + first, a.vocab - first);
-    for (int s = 0; s < pieces; ++s) {
-        const int base = first + s * PIECE;
-        float v[SEL_E];
-#pragma unroll
-        for (int i = 0; i < SEL_E; ++i) v[i] = (float)next.v[i / Piece<T>::VEC][i % Piece<T>::VEC];
-        if (s + 1 < pieces) next.load(x + base + PIECE, a.vocab - base - PIECE);
-        float most = -INFINITY;  // a NaN is skipped here and makes the sum a NaN below
-#pragma unroll
-        for (int i = 0; i < SEL_E; ++i) most = fmaxf(most, v[i]);
-        auto append = [&] {
-            if (most > -INFINITY && float_key(most) >= bound) {
-                const float least = bound > KEY_NEG_INF ? key_float(bound) : -INFINITY;
-#pragma unroll
-                for (int i = 0; i < SEL_E; ++i)
-                    if (v[i] >= least && v[i] > -INFINITY) {
-                        const int at = atomicAdd(&count, 1);
-                        if (at < cap) cand[at] = (u64)float_key(v[i]) << 32 | (uint32_t)~(uint32_t)(base + Piece<T>::offset(i));
-                    }
-            }
-        };
-        if (s == 0) bound = bound_of(float_key(most), n, keys);  // its barriers publish count
-        append();
-        // exponentials of exact differences to the maximum (while that is -inf, of the logits: 0)
-        const float top = fmaxf(m, most), sub = top == -INFINITY ? 0.0f : top;
-        float add = 0.0f;
-#pragma unroll
-        for (int i = 0; i < SEL_E; ++i) add += __builtin_amdgcn_exp2f((v[i] - sub) * 1.44269504f);
-        sum = (m == top ? sum : sum * __builtin_amdgcn_exp2f((m - sub) * 1.44269504f)) + add;
+    auto take = [&](const Piece<T>& piece, int s) {
+        const float most = piece.most();  // a NaN is skipped here and makes the sum a NaN below
+        const float top = fmaxf(m, most);
+        sum = (m == top ? sum : sum * rescale(m, top)) + piece.sum(top);
         m = top;
-        __syncthreads();
-        const int had = c;
-        c = count;
-        __syncthreads();  // every thread has read count
-        if (c > cap) {
-            // the candidates so far give a higher bound, and so does this piece by itself
-            c = rank_entries(cand, had, n, sorted);
-            if (c == n) bound = max(bound, (uint32_t)(sorted[n - 1] >> 32) + 1);  // equals come after them: later tokens
-            for (int i = tid; i < c; i += SEL_THREADS) cand[i] = sorted[i];
-            if (tid == 0) count = c;
-            bound = max(bound, bound_of(float_key(most), n, keys));
-            append();
-            __syncthreads();
-            const int now = count;
-            __syncthreads();
-            if (now > cap) {  // ties: the piece's n best, one after the other
-                u64 last = ~0ull;
-                int r = 0;
-                for (; r < n; ++r) {
-                    u64 k = 0;
-#pragma unroll
-                    for (int i = 0; i < SEL_E; ++i) {
-                        const u64 e = v[i] > -INFINITY
-                                          ? (u64)float_key(v[i]) << 32 | (uint32_t)~(uint32_t)(base + Piece<T>::offset(i)) : 0;
-                        if (e < last && e > k) k = e;
-                    }
-                    k = wave_max_u64(k);
-                    if ((tid & 63) == 0) best[wave] = k;
-                    __syncthreads();
-                    const u64 h = best[0] > best[1] ? best[0] : best[1], g = best[2] > best[3] ? best[2] : best[3];
-                    last = h > g ? h : g;
-                    if (tid == 0) cand[c + r] = last;
-                    __syncthreads();  // best is read before the next round's
-                }
-                c += r;
-                if (tid == 0) count = c;
-                __syncthreads();
-            } else {
-                c = now;
-            }
+        // The threads' maxima so far give a bound that n blocks reach: from then on equals come too late.
+        uint32_t now = need;
+        if ((s & (s + 1)) == 0) {
+            bound = max(bound, bound_of(float_key(m), n, keys));  // its barriers publish count
+            now = max(need, bound), need = bound + 1;
         }
+        if (free == 0) {
+            int c = 0;
+            if (s > 0) {
+                hx_lds_barrier();
+                c = count;
+                hx_lds_barrier();  // every thread has read count
+                if (c > BLOCKS - SEL_THREADS) {
+                    c = rank_entries(cand, c, n + SEL_THREADS - 1, sorted);
+                    for (int i = tid; i < c; i += SEL_THREADS) cand[i] = sorted[i];
+                    if (tid == 0) count = c;
+                    hx_lds_barrier();
+                }
+            }
+            free = (BLOCKS - c) / SEL_THREADS;
+        }
+        --free;
+        const uint32_t key = float_key(most);
+        if (key >= now && most > -INFINITY)
+            cand[atomicAdd(&count, 1)] = (u64)key << 32 | (uint32_t)~(uint32_t)(s * SEL_THREADS + tid);
+    };
+    Piece<T> block[2];  // the blocks that may hold some of the n largest, two per thread at most
+    int base[2] = {first, first}, own[2] = {tid, tid};
+    bool two = false;
+    if (end - first <= PIECE) {
+        if (over) block[0].load_end(x + first, tid, end - first);
+        else block[0].load(x + first);
+        take(block[0], 0);  // every thread keeps its block
+    } else {
+        // Two pieces in flight.  Every step loads one (past the end the last again), so that the waits are for the piece's own
+        // loads.
+        Piece<T> odd;
+        block[0].load(x + first);
+        odd.load(x + first + min(1, whole - 1) * PIECE);
+        for (int s = 0; s < whole; s += 2) {
+            take(block[0], s);
+            block[0].load(x + first + min(s + 2, whole - 1) * PIECE);
+            if (s + 1 < whole) take(odd, s + 1);
+            odd.load(x + first + min(s + 3, whole - 1) * PIECE);
+        }
+        if (over) {
+            block[0].load_end(x + first + whole * PIECE, tid, end - first - whole * PIECE);
+            take(block[0], whole);
+        }
+        hx_lds_barrier();
+        int c = count;
+        hx_lds_barrier();
+        if (c > SEL_THREADS) {
+            // more than one per thread: those that reach the bound of all, or where they are many, the n + 255 first in order
+            bound = max(bound, bound_of(float_key(m), n, keys));
+            u64 mine[BLOCKS / SEL_THREADS];
+#pragma unroll
+            for (int i = 0; i < BLOCKS / SEL_THREADS; ++i) {
+                const int at = i * SEL_THREADS + tid;
+                mine[i] = at < c && (uint32_t)(cand[at] >> 32) >= bound ? cand[at] : 0;
+            }
+            if (tid == 0) count = 0;
+            hx_lds_barrier();  // the list is read
+#pragma unroll
+            for (int i = 0; i < BLOCKS / SEL_THREADS; ++i)
+                if (mine[i]) cand[atomicAdd(&count, 1)] = mine[i];
+            hx_lds_barrier();
+            c = count;
+            hx_lds_barrier();
+            if (c > 2 * SEL_THREADS) {
+                c = rank_entries(cand, c, n + SEL_THREADS - 1, sorted);  // < 2 SEL_THREADS
+                for (int i = tid; i < c; i += SEL_THREADS) cand[i] = sorted[i];
+                hx_lds_barrier();
+            }
+            two = c > SEL_THREADS;
+        }
+        // their logits again
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (k == 0 || two) {
+                const int at = k * SEL_THREADS + tid;
+                const uint32_t id = at < c ? (uint32_t)~(uint32_t)cand[at] : 0;
+                own[k] = id % SEL_THREADS;
+                base[k] = first + (int)(id / SEL_THREADS) * PIECE;
+                block[k].load_end(x + base[k], own[k], at < c ? end - base[k] : 0);
+            }
     }
     const float wm = wave_max(m);
     if ((tid & 63) == 0) part[0][wave] = wm;
-    const int found = rank_entries(cand, c, n, sorted);
+    hx_lds_barrier();  // the list is read
+    if (tid == 0) count = 0;
+    hx_lds_barrier();
+    const float least = bound > KEY_NEG_INF ? key_float(bound) : -3.402823466e38f;
+    auto entry = [&](int k, int i) {
+        const int token = base[k] + Piece<T>::offset(own[k], i);
+        return (u64)float_key(block[k][i]) << 32 | (uint32_t)~(uint32_t)token;
+    };
+    auto reach = [&](int k) {
+#pragma unroll
+        for (int i = 0; i < SEL_E; ++i)
+            if (block[k][i] >= least) {
+                const int at = atomicAdd(&count, 1);
+                if (at < BLOCKS) cand[at] = entry(k, i);
+            }
+    };
+    reach(0);
+    if (two) reach(1);
+    hx_lds_barrier();
+    int found = count;
+    if (found <= BLOCKS) {
+        found = rank_entries(cand, found, n, sorted);
+    } else {  // ties at the bound: one after the other
+        u64 last = ~0ull;
+        for (int r = 0; r < n; ++r) {
+            u64 q = 0;
+            auto next = [&](int k) {
+#pragma unroll
+                for (int i = 0; i < SEL_E; ++i) {
+                    const u64 e = block[k][i] >= least ? entry(k, i) : 0;
+                    if (e < last && e > q) q = e;
+                }
+            };
+            next(0);
+            if (two) next(1);
+            q = wave_max_u64(q);
+            if ((tid & 63) == 0) best[wave] = q;
+            hx_lds_barrier();
+            const u64 h = best[0] > best[1] ? best[0] : best[1], g = best[2] > best[3] ? best[2] : best[3];
+            last = h > g ? h : g;
+            if (tid == 0) sorted[r] = last;
+            hx_lds_barrier();  // best is read before the next round's
+        }
+        found = n;  // more than n reach the bound
+    }
     const float top = fmaxf(fmaxf(part[0][0], part[0][1]), fmaxf(part[0][2], part[0][3]));
     // a thread without finite logits has m = -inf and a sum of 0 (or a NaN)
-    sum = wave_sum(m == top ? sum : sum * __builtin_amdgcn_exp2f((m - (top == -INFINITY ? 0.0f : top)) * 1.44269504f));
+    sum = wave_sum((m == top ? sum : sum * rescale(m, top)) * __builtin_amdgcn_exp2f(-ref_rest(top)));
     if ((tid & 63) == 0) part[1][wave] = sum;
-    const __amdgpu_buffer_rsrc_t out = coherent_rsrc(p.entries + (size_t)b * n * p.lists + list);
+    const __amdgpu_buffer_rsrc_t out = coherent_rsrc(p.entries + (size_t)b * a.n * p.lists + list);
     for (int r = tid; r < n; r += SEL_THREADS) coherent_store8(out, r * p.lists * 8, r < found ? sorted[r] : 0);
-    __syncthreads();
+    hx_lds_barrier();
     if (tid == 0) {
         const float2 st = {top, (part[1][0] + part[1][1]) + (part[1][2] + part[1][3])};
         coherent_store8(coherent_rsrc(p.stats + (size_t)b * p.lists + list), 0, __builtin_bit_cast(u64, st));
@@ -358,7 +472,7 @@ HX_INLINE void select_merge(const BeamArgs& a, const BeamPlan& p, long b, char* 
         }
     }
     int kept = 0, nothing = 0;  // entries of carry; entries in a row that were no better than those
-    __syncthreads();
+    hx_lds_barrier();
     for (int at = 0; at < total;) {
         const int fresh = min(total - at, MERGE - kept);
         Cand v[MERGE_E];
@@ -414,11 +528,11 @@ HX_INLINE void select_merge(const BeamArgs& a, const BeamPlan& p, long b, char* 
                     if (to < p.cap) cand[to] = v[i];
                 }
         }
-        __syncthreads();
+        hx_lds_barrier();
         const int c = count;
         if (c <= p.cap) {
             if (tid < (-c & 7)) cand[c + tid] = {-INFINITY, ~0ull};
-            __syncthreads();
+            hx_lds_barrier();
             for (int i = tid; i < c; i += SEL_THREADS) {
                 const Cand mine = cand[i];
                 int r = 0;
@@ -432,7 +546,7 @@ HX_INLINE void select_merge(const BeamArgs& a, const BeamPlan& p, long b, char* 
                 if (r < n) carry[r] = mine;
             }
             kept = min(c, n);
-            __syncthreads();
+            hx_lds_barrier();
         } else {
             Cand last = {INFINITY, 0};
             for (int r = 0; r < n; ++r) {  // c > n: there are n to take
@@ -447,12 +561,12 @@ HX_INLINE void select_merge(const BeamArgs& a, const BeamPlan& p, long b, char* 
                     if (better(s, i, m.s, m.at)) m = {s, i};
                 }
                 if (lane == 0) best[tid >> 6] = m;
-                __syncthreads();
+                hx_lds_barrier();
                 last = best[0];
                 for (int i = 1; i < 4; ++i)
                     if (better(best[i].s, best[i].at, last.s, last.at)) last = best[i];
                 if (tid == 0) carry[r] = last;
-                __syncthreads();
+                hx_lds_barrier();
             }
             kept = n;
         }
@@ -469,7 +583,7 @@ HX_INLINE void select_merge(const BeamArgs& a, const BeamPlan& p, long b, char* 
 
 // grid: [batch][beams][chunks]
 template <typename T>
-__global__ __launch_bounds__(SEL_THREADS) void beam_select_kernel(const T* logits, BeamArgs a, BeamPlan p)
+__global__ __launch_bounds__(SEL_THREADS, 4) void beam_select_kernel(const T* logits, BeamArgs a, BeamPlan p)
 {
     extern __shared__ __align__(16) char beam_lds[];
     const uint32_t row = div_by(blockIdx.x, p.by_chunks), chunk = blockIdx.x - row * p.chunks;
@@ -517,13 +631,13 @@ hipError_t launch_beam_select(const void* logits, bool fp32, const BeamArgs& a, 
     if (a.batch <= 0) return hipSuccess;
     const SelectLayout l(a.batch, a.beams, a.vocab, a.n);
     char* base = static_cast<char*>(ws);
-    // the candidate buffer, 16 times what is asked for (32 times in a chunk's 8-byte entries) and more for few: ties aside a bound
-    // is reached by n threads (or quads) at most, and by n to 2n elements as a rule
+    // the merge's candidates, 16 times what is asked for and more for few: ties aside a bound is reached by n to 2n as a rule
     const int cap = a.n > 8 ? 16 * a.n : 128;
     const BeamPlan p{(int)l.subs, (int)l.chunks, (int)l.lists, fast_div(l.chunks), fast_div(l.lists), cap,
                      reinterpret_cast<u64*>(base + HX_COUNTER_BYTES),
                      reinterpret_cast<float2*>(base + HX_COUNTER_BYTES + l.entries), reinterpret_cast<int*>(base)};
-    const size_t lds = ((size_t)a.beams * 12 + 15) / 16 * 16 + (size_t)p.cap * sizeof(Cand);
+    const size_t merge = ((size_t)a.beams * 12 + 15) / 16 * 16 + (size_t)p.cap * sizeof(Cand);
+    const size_t lds = merge > BLOCKS * sizeof(u64) ? merge : BLOCKS * sizeof(u64);
     const dim3 grid(a.batch * p.lists);
     if (fp32)
         hipLaunchKernelGGL((beam_select_kernel<float>), grid, dim3(SEL_THREADS), lds, st, static_cast<const float*>(logits), a, p);
