@@ -648,37 +648,53 @@ hipError_t launch_beam_select(const void* logits, bool fp32, const BeamArgs& a, 
 }
 
 // dst[o][b * out_beams + j][i][:] = src[o][b * beams + parents[b][j]][i][:], pieces of p.bytes bytes at byte strides.
-// A workgroup takes one piece (o, row, i); pieces whose parent lies outside the beams are left alone.
+// A workgroup takes a part of one piece (o, row, i), `part` elements of V; pieces whose parent lies outside the beams are left alone.
 template <typename V>
-__global__ __launch_bounds__(256) void beam_reorder_kernel(const char* src, const int64_t* parents, char* dst, ReorderArgs p)
+__global__ __launch_bounds__(256) void beam_reorder_kernel(const char* src, const int64_t* parents, char* dst, ReorderArgs p, long part)
 {
     const long rows = (long)p.batch * p.out_beams;
-    for (long q = blockIdx.x; q < p.outer * rows * p.inner; q += gridDim.x) {
+    const long length = p.bytes / (long)sizeof(V), parts = (length + part - 1) / part;
+    for (long u = blockIdx.x; u < p.outer * rows * p.inner * parts; u += gridDim.x) {
+        const long q = u / parts, c0 = u % parts * part;
         const long i = q % p.inner, r = q / p.inner % rows, o = q / p.inner / rows;
         const int64_t parent = parents[r];
         if (parent < 0 || parent >= p.beams) continue;
         const char* s = src + o * p.src[0] + (r / p.out_beams * p.beams + parent) * p.src[1] + i * p.src[2];
         char* d = dst + o * p.dst[0] + r * p.dst[1] + i * p.dst[2];
-        for (long c = threadIdx.x; c < p.bytes / (long)sizeof(V); c += 256)
+        for (long c = c0 + threadIdx.x; c < min(c0 + part, length); c += 256)
             reinterpret_cast<V*>(d)[c] = reinterpret_cast<const V*>(s)[c];
     }
 }
 
+namespace {
+
+// Few large pieces are divided among workgroups, 8 per CU in all, into no less than one access per thread.
+template <typename V>
+hipError_t reorder_launch(const char* src, const int64_t* parents, char* dst, const ReorderArgs& p, hipStream_t st)
+{
+    constexpr long SLOTS = 2048;
+    const long pieces = p.outer * p.batch * p.out_beams * p.inner, length = p.bytes / (long)sizeof(V);
+    const long most = pieces < SLOTS ? (SLOTS + pieces - 1) / pieces : 1;
+    const long part = ((length + most - 1) / most + 255) / 256 * 256, units = pieces * ((length + part - 1) / part);
+    hipLaunchKernelGGL((beam_reorder_kernel<V>), dim3((unsigned)(units < 65536 ? units : 65536)), dim3(256), 0, st, src, parents,
+                       dst, p, part);
+    return hipGetLastError();
+}
+
+}  // namespace
+
 hipError_t launch_beam_reorder(const void* src, const int64_t* parents, void* dst, const ReorderArgs& p, hipStream_t st)
 {
-    const long pieces = p.outer * p.batch * p.out_beams * p.inner;
-    if (pieces == 0 || p.bytes == 0) return hipSuccess;
+    if (p.outer == 0 || p.batch == 0 || p.out_beams == 0 || p.inner == 0 || p.bytes == 0) return hipSuccess;
     // the widest access that every piece's address and length allow
     uint64_t low = reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst) | (uint64_t)p.bytes;
     for (int i = 0; i < 3; ++i) low |= (uint64_t)p.src[i] | (uint64_t)p.dst[i];
-    const dim3 grid((unsigned)(pieces < 65536 ? pieces : 65536));
     const char* s = static_cast<const char*>(src);
     char* d = static_cast<char*>(dst);
-    if (low % 16 == 0) hipLaunchKernelGGL((beam_reorder_kernel<hx_u4>), grid, dim3(256), 0, st, s, parents, d, p);
-    else if (low % 4 == 0) hipLaunchKernelGGL((beam_reorder_kernel<uint32_t>), grid, dim3(256), 0, st, s, parents, d, p);
-    else if (low % 2 == 0) hipLaunchKernelGGL((beam_reorder_kernel<uint16_t>), grid, dim3(256), 0, st, s, parents, d, p);
-    else hipLaunchKernelGGL((beam_reorder_kernel<uint8_t>), grid, dim3(256), 0, st, s, parents, d, p);
-    return hipGetLastError();
+    return low % 16 == 0  ? reorder_launch<hx_u4>(s, parents, d, p, st)
+           : low % 4 == 0 ? reorder_launch<uint32_t>(s, parents, d, p, st)
+           : low % 2 == 0 ? reorder_launch<uint16_t>(s, parents, d, p, st)
+                          : reorder_launch<uint8_t>(s, parents, d, p, st);
 }
 
 }  // namespace hx

@@ -489,7 +489,7 @@ int w4_args(const hx_w4_words* w, int N, int K, hx::W4Args* a, const char* who)
     const char* what = nullptr;
     if (!w || !w->words || !w->scales) what = "null pointer";
     else if (N <= 0 || K <= 0 || K % 32) what = "N and K must be positive and K a multiple of 32";
-    else if (K > (1 << 22)) what = "K must be at most 2^22";
+    else if (K > (1 << 22) || N > (1 << 28)) what = "K must be at most 2^22 and N at most 2^28";
     else if (w->group < 32 || (w->group & (w->group - 1))) what = "group must be a power of two of at least 32";
     else if ((uintptr_t)w->words & 15) what = "words must be 16-byte aligned";
     else if ((uintptr_t)w->scales & 1) what = "scales must be 2-byte aligned";
@@ -506,7 +506,7 @@ int w4_args(const hx_w4_words* w, int N, int K, hx::W4Args* a, const char* who)
 
 size_t hx_w4_gemm_workspace_size(int M, int N, int K)
 {
-    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || K > (1 << 22) || N > (1 << 28)) return 0;
     return hx::w4_gemm_workspace_bytes(M, N, K);
 }
 
@@ -545,7 +545,7 @@ int hx_w4_embed(const hx_w4_words* w, const int64_t* tokens, void* out, int n, i
 
 size_t hx_beam_select_workspace_size(int batch, int beams, int vocab, int n)
 {
-    if (batch <= 0 || beams <= 0 || vocab <= 0 || n <= 0) return 0;
+    if (batch <= 0 || beams <= 0 || vocab <= 0 || vocab > hx::BEAM_MAX_VOCAB || n <= 0) return 0;
     return hx::beam_select_workspace_bytes(batch, beams, vocab, n);
 }
 
@@ -555,7 +555,8 @@ int hx_beam_select(const void* logits, const float* cum, const uint8_t* done, fl
 {
     if (batch < 0 || batch > hx::BEAM_MAX_BATCH || beams <= 0 || vocab <= 0 || n <= 0 || n > hx::BEAM_MAX_N)
         return fail(HX_ERR_INVALID, "hx_beam_select: batch must be in [0, 4096], n in [1, 128], beams and vocab positive");
-    if (beams > hx::BEAM_MAX_BEAMS) return fail(HX_ERR_INVALID, "hx_beam_select: at most 1024 beams");
+    if (beams > hx::BEAM_MAX_BEAMS || vocab > hx::BEAM_MAX_VOCAB)
+        return fail(HX_ERR_INVALID, "hx_beam_select: at most 1024 beams and 2^30 tokens");
     if (ld < vocab) return fail(HX_ERR_INVALID, "hx_beam_select: rows of logits overlap (ld < vocab)");
     if (dtype != HX_DTYPE_HALF && dtype != HX_DTYPE_FLOAT)
         return fail(HX_ERR_INVALID, "hx_beam_select: dtype must be HX_DTYPE_HALF or HX_DTYPE_FLOAT");

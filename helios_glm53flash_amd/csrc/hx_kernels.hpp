@@ -108,6 +108,7 @@ struct BeamArgs {
 constexpr int BEAM_MAX_N = 128;       // candidates asked for per sequence
 constexpr int BEAM_MAX_BATCH = 4096;  // sequences per call
 constexpr int BEAM_MAX_BEAMS = 1024;  // beams of a sequence
+constexpr int BEAM_MAX_VOCAB = 1 << 30;
 size_t beam_select_workspace_bytes(int batch, int beams, int vocab, int n);
 hipError_t launch_beam_select(const void* logits, bool fp32, const BeamArgs& a, void* ws, hipStream_t st);
 struct ReorderArgs {

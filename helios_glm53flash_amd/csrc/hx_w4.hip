@@ -449,22 +449,22 @@ __global__ __launch_bounds__(256) void w4_embed_kernel(W4Args a, const int64_t* 
 {
     typedef T v8 __attribute__((ext_vector_type(8)));
     const int nw = (a.K + 127) / 128 * 16;
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n * nw) return;
-    const long t = i / nw;
-    const int w = (int)(i % nw), k = word_k(w);
-    if (k >= a.K) return;
-    const int64_t row = tokens[t];
-    v8 o = {};
-    if (row >= 0 && row < a.N) {
-        const size_t g = (size_t)row * a.groups + (k >> a.group_log2);
-        float v[8];
-        word_values(a.words[(size_t)row * nw + w], a.zeros ? (float)a.zeros[g] : 8.0f, v);
-        const float s = (float)a.scales[g] * scale;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n * nw; i += (long)gridDim.x * 256) {
+        const long t = i / nw;
+        const int w = (int)(i % nw), k = word_k(w);
+        if (k >= a.K) continue;
+        const int64_t row = tokens[t];
+        v8 o = {};
+        if (row >= 0 && row < a.N) {
+            const size_t g = (size_t)row * a.groups + (k >> a.group_log2);
+            float v[8];
+            word_values(a.words[(size_t)row * nw + w], a.zeros ? (float)a.zeros[g] : 8.0f, v);
+            const float s = (float)a.scales[g] * scale;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = (T)(s * v[j]);
+            for (int j = 0; j < 8; ++j) o[j] = (T)(s * v[j]);
+        }
+        *reinterpret_cast<v8*>(out + (size_t)t * a.K + k) = o;
     }
-    *reinterpret_cast<v8*>(out + (size_t)t * a.K + k) = o;
 }
 
 namespace {
@@ -481,7 +481,7 @@ struct W4Call {
 
 // Which kernel takes a call of M rows, by measured shapes (us, 4-bit, group 128, weights from memory).
 struct W4Plan {
-    enum Kind { ROWS4_FEW, ROWS4, ROWS8_FEW, ROWS8, ROWS16, TILE16, TILE32, TILE64, TILE64W, TILE128 } kind;
+    enum Kind { ROWS4_FEW, ROWS4, ROWS8_FEW, ROWS8, ROWS8_WIDE, ROWS16, TILE16, TILE32, TILE64, TILE64W, TILE128 } kind;
     int splits, steps;  // of a tile kernel
     long tiles;
 };
@@ -495,7 +495,7 @@ W4Plan w4_tile_plan(int kind, int M, int N, int K, bool split)
 {
     const W4Tile t = W4_TILES[kind - W4Plan::TILE16];
     W4Plan p{(W4Plan::Kind)kind, 1, (K + 128 * t.ks - 1) / (128 * t.ks), 0};
-    p.tiles = (long)((M + t.bm - 1) / t.bm) * ((N + 64 * t.nt - 1) / (64 * t.nt));
+    p.tiles = ((long)M + t.bm - 1) / t.bm * (((long)N + 64 * t.nt - 1) / (64 * t.nt));
     // K is split while that fills idle CUs and leaves each split 4 steps: 32 rows, 8192 -> 4096, 27 us unsplit, 12.5 in 4, 15 in
     // 8; 2048 -> 2048 7.7, 7.5 in 2, 8.0 in 4.
     if (split && t.ks > 1) {
@@ -515,7 +515,13 @@ W4Plan w4_plan(int M, int N, int K, bool split, bool pieces)
     // 7.6 / 7.9, with 4 rows 10.8 / 9.1; 4096 -> 12288 9.7 / 9.1, 4096 -> 151552 73 / 62).
     const bool few = !pieces || (long)N * K <= 1l << (M <= 2 ? 25 : 24);
     if (M <= 4) return {few ? W4Plan::ROWS4_FEW : W4Plan::ROWS4, 1, 0, 0};
-    if (M <= 8) return {few ? W4Plan::ROWS8_FEW : W4Plan::ROWS8, 1, 0, 0};
+    // 5 rows, groups of 32 with zero points, as 16 waves of one load / 8 waves of 2 / 8 waves of 2 in each of two spans: 4096 ->
+    // 2048 5.4 / 7.2 / 7.7, 8192 -> 4096 14.0 / 11.2 / 12.5, 2048 -> 8192 7.3 / 7.1 / 7.8, 4096 -> 12288 17.5 / 15.3 / 14.3; groups
+    // of 128 without them 4.9 / 6.2 / 6.1, 12.2 / 9.7 / 10.3, 6.2 / 5.9 / 6.2, 14.2 / 13.0 / 11.1.
+    if (M <= 8) {
+        const W4Plan::Kind kind = (long)N * K <= 1l << 23 ? W4Plan::ROWS8_FEW : N <= 8192 ? W4Plan::ROWS8 : W4Plan::ROWS8_WIDE;
+        return {pieces ? kind : W4Plan::ROWS8, 1, 0, 0};
+    }
     // 16 rows: 4096 -> 151552 87 us in rows, 99 in tiles; 4096 -> 12288 12.6 / 12.1; 8192 -> 4096 13.8 / 10.7
     if (M <= 16) return pieces && N >= 32768 ? W4Plan{W4Plan::ROWS16, 1, 0, 0} : w4_tile_plan(W4Plan::TILE16, M, N, K, split);
     if (M <= 32) return w4_tile_plan(W4Plan::TILE32, M, N, K, split);
@@ -559,7 +565,6 @@ template <int BM, int NT, int KS, int PF, int GS, bool Z, bool V>
 hipError_t tile_launch(const W4Call& c, const W4Plan& p)
 {
     constexpr size_t lds = sizeof(_Float16) * PF * KS * BM * 128;
-    if (p.tiles * p.splits > 0x7fffffl) return hipErrorInvalidValue;  // threads of a launch
     const W4Split sp{p.splits, p.steps, reinterpret_cast<hx_f4*>(static_cast<char*>(c.ws) + HX_COUNTER_BYTES),
                      static_cast<int*>(c.ws)};
     hipLaunchKernelGGL((w4_tile_kernel<BM, NT, KS, PF, GS, Z, V>), dim3((unsigned)(p.tiles * p.splits)), dim3(256 * KS), lds,
@@ -574,7 +579,8 @@ hipError_t gemm_launch(const W4Call& c)
     if constexpr (V || GS == 1) {
         switch (p.kind) {
             case W4Plan::ROWS4: return rows_launch<4, 1, 8, 1, 4, GS, Z, V>(c, 512);
-            case W4Plan::ROWS8: return rows_launch<2, 1, 8, 2, 2, GS, Z, V>(c, 512);
+            case W4Plan::ROWS8_FEW: return rows_launch<2, 1, 16, 1, 1, GS, Z, V>(c, 512);
+            case W4Plan::ROWS8_WIDE: return rows_launch<2, 1, 8, 2, 2, GS, Z, V>(c, 512);
             case W4Plan::ROWS16: return rows_launch<2, 2, 16, 1, 2, GS, Z, V>(c, 256);
             case W4Plan::TILE64W: return tile_launch<64, 2, 1, 3, GS, Z, V>(c, p);
             case W4Plan::TILE128: return tile_launch<128, 2, 1, 2, GS, Z, V>(c, p);
@@ -583,7 +589,7 @@ hipError_t gemm_launch(const W4Call& c)
     }
     switch (p.kind) {
         case W4Plan::ROWS4_FEW: return rows_launch<4, 1, 8, 1, 2, GS, Z, V>(c, 512);
-        case W4Plan::ROWS8_FEW: return rows_launch<2, 1, 8, 2, 1, GS, Z, V>(c, 512);
+        case W4Plan::ROWS8: return rows_launch<2, 1, 8, 1, 2, GS, Z, V>(c, 512);
         case W4Plan::TILE16: return tile_launch<16, 1, 2, 4, GS, Z, V>(c, p);
         case W4Plan::TILE32: return tile_launch<32, 1, 2, 4, GS, Z, V>(c, p);
         default: return tile_launch<64, 1, 2, 3, GS, Z, V>(c, p);
@@ -624,9 +630,17 @@ size_t w4_gemm_workspace_bytes(int M, int N, int K)
 hipError_t launch_w4_gemm(const _Float16* x, const W4Args& a, void* y, int M, bool y_fp32, void* ws, size_t ws_bytes,
                           hipStream_t st)
 {
-    if (M <= 0 || a.N <= 0) return hipSuccess;
-    const W4Call c{x, a, y, M, y_fp32, ws && ws_bytes >= w4_gemm_workspace_bytes(M, a.N, a.K) ? ws : nullptr, st};
-    return a.group_log2 == 5 ? gemm_launch<4>(c) : a.group_log2 == 6 ? gemm_launch<2>(c) : gemm_launch<1>(c);
+    // 2^20 tiles of 64 x 64 and fewer in a launch: one takes at most 2^32 threads
+    const long columns = ((long)a.N + 63) / 64, most = 64 * (columns < 1l << 20 ? (1l << 20) / columns : 1);
+    for (long m = 0; m < M; m += most) {
+        const int rows = (int)(M - m < most ? M - m : most);
+        const size_t need = w4_gemm_workspace_bytes(rows, a.N, a.K);
+        const W4Call c{x + m * a.K, a, static_cast<char*>(y) + m * a.N * (y_fp32 ? 4 : 2), rows, y_fp32,
+                       need && ws && ws_bytes >= need ? ws : nullptr, st};
+        const hipError_t e = a.group_log2 == 5 ? gemm_launch<4>(c) : a.group_log2 == 6 ? gemm_launch<2>(c) : gemm_launch<1>(c);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 hipError_t launch_w4_embed(const W4Args& a, const int64_t* tokens, void* out, long n, float scale, bool out_fp32,
@@ -634,7 +648,7 @@ hipError_t launch_w4_embed(const W4Args& a, const int64_t* tokens, void* out, lo
 {
     if (n <= 0) return hipSuccess;
     const long work = n * ((a.K + 127) / 128 * 16);
-    const dim3 grid((unsigned)((work + 255) / 256));
+    const dim3 grid((unsigned)((work + 255) / 256 < 65536 ? (work + 255) / 256 : 65536));
     if (out_fp32)
         hipLaunchKernelGGL((w4_embed_kernel<float>), grid, dim3(256), 0, st, a, tokens, static_cast<float*>(out), n, scale);
     else

@@ -8,6 +8,7 @@ that are not trellis coded, and the lookup of single rows (a head that is the em
 from __future__ import annotations
 
 import ctypes as C
+from contextlib import nullcontext
 from dataclasses import dataclass
 from functools import lru_cache
 from typing import Optional
@@ -108,12 +109,15 @@ def _gemm_workspace_bytes(M: int, N: int, K: int) -> int:
 
 
 def call_workspace(nbytes: int, device: torch.device, st: int) -> torch.Tensor:
-    """A call's workspace on stream st: the stream's own one, or, where the current stream is being captured, memory of the
+    """A call's workspace on stream st: the stream's own one, or, where it is being captured, memory of the
     graph's with counters that each replay clears, so that the graph depends on no buffer that a later call may replace."""
-    if torch.cuda.is_current_stream_capturing() and st == _stream(None):
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        ws[:COUNTER_BYTES].zero_()
-        return ws
+    if torch.cuda.is_current_stream_capturing():
+        here = st == _stream(None)
+        with nullcontext() if here else torch.cuda.stream(torch.cuda.ExternalStream(st, device=device)):
+            if here or torch.cuda.is_current_stream_capturing():  # another stream may have been forked into the capture
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+                ws[:COUNTER_BYTES].zero_()
+                return ws
     # the bytes behind every workspace, which hold a linear's splits, are enough here too
     return workspace(max(0, nbytes - _GEMM_EXTRA), device, st)
 

@@ -235,7 +235,7 @@ int hx_gemm_nt_f16(void* y, const void* x, const void* w, int M, int N, int K, i
  * words: uint32 [N][16 * ceil(K / 128)], 16-byte aligned.  Word 4 g + j of each block of 128 k holds the eight codes
  * k = 32 j + 8 g + (0, 2, 4, 6, 1, 3, 5, 7) of the block in its nibbles, lowest first; codes past K are not used.
  * scales: fp16 [N][ceil(K / group)]; zeros: uint8 of that shape, or NULL for 8 everywhere; group: a power of two >= 32
- * (the last group of a row may be short).  K % 32 == 0, K <= 2^22, any N. */
+ * (the last group of a row may be short).  K % 32 == 0, K <= 2^22, N <= 2^28. */
 typedef struct hx_w4_words {
     const void* words;
     const void* scales;
@@ -266,7 +266,7 @@ int hx_w4_embed(const hx_w4_words* w, const int64_t* tokens, void* out, int n, i
  * lowest w * vocab + v first among equal scores; fp32 scores rounded once from 64 bits.  A beam with done != 0 (done may be
  * NULL) has the one candidate (w, eos) with score cum.  A logit of -inf is no candidate; a beam whose cum is not finite, whose
  * logits hold a NaN or +inf, or are all -inf, has none.  Places without a candidate get score -inf, parent -1, token -1.
- * batch <= 4096, beams <= 1024, n <= 128.  batch == 0 is a no-op. */
+ * batch <= 4096, beams <= 1024, vocab <= 2^30, n <= 128.  batch == 0 is a no-op. */
 size_t hx_beam_select_workspace_size(int batch, int beams, int vocab, int n);
 int hx_beam_select(const void* logits, const float* cum, const uint8_t* done, float* scores, int64_t* parents,
                    int64_t* tokens, int batch, int beams, int vocab, int n, int64_t ld, int eos, int dtype,

@@ -165,6 +165,38 @@ def test_select_equal_logits_go_to_the_lowest_token(beam, dtype, V, n):
     assert np.array_equal(t[0][:k], top[:k]) and (p[0][:k] == 0).all()
 
 
+def shaped_rows(r, rows, V, dtype):
+    """Rows that a bound found on the way meets in every manner: ascending and descending, equal in all or most places, steps
+    of hundreds of equal logits, the largest at the very end or start, hardly any finite, of the type's lowest value."""
+    x = (r.standard_normal((rows, V)) * 3).astype(np.float32)
+    ramp = np.arange(V) * np.float32(60.0 / V)
+    x[1::11] = ramp
+    x[2::11] = -ramp
+    x[3::11] = np.floor(ramp)
+    x[4::11] = -np.floor(ramp)
+    x[5::11] = -1.5
+    x[6::11] = r.integers(0, 3, x[6::11].shape)
+    x[7::11, V - 7:] += 30
+    x[8::11] = np.where(r.random(x[8::11].shape) < 0.0005, x[8::11], -np.inf)
+    x[9::11] = np.where(r.random(x[9::11].shape) < 0.5, x[9::11], -np.inf)
+    x = x.astype(dtype)
+    x[10::11] = np.finfo(dtype).min
+    x[10::22, V // 2:] = 1.0
+    x[1, -1], x[12, V // 2], x[23, 0] = np.nan, np.inf, -np.inf
+    return x
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("batch,beams,V,n", [(600, 1, 20001, 1), (600, 1, 20001, 128), (130, 4, 33000, 33), (260, 2, 8193, 8),
+                                             (1, 520, 12289, 128), (520, 1, 36864, 20)])
+def test_select_many_rows(beam, dtype, batch, beams, V, n):
+    """More rows than workgroups fit the chip, so that a workgroup walks over several pieces of its row."""
+    r = np.random.default_rng(V + n)
+    x = shaped_rows(r, batch * beams, V, dtype)
+    cum = (-r.uniform(0, 6, batch * beams)).astype(np.float32)
+    check(beam, x, cum, None, batch, beams, V, n)
+
+
 def test_select_padded_and_strided_rows(beam):
     """Rows at a stride beyond the vocabulary, starting at any element: what lies between them is never read into a result."""
     import torch
@@ -219,6 +251,34 @@ def test_select_graph_and_streams(beam):
         torch.cuda.synchronize()
         for a, b in zip(o, w):
             assert torch.equal(a, b), rep
+
+
+def test_select_on_a_forked_stream_of_a_capture(beam):
+    """A captured call on a stream that was forked from the capturing one depends on no workspace of that stream."""
+    import torch
+    batch, beams, V, n = 2, 4, 20000, 8
+    x = torch.randn((batch * beams, V), device="cuda") * 3
+    cum = -torch.rand(batch * beams, device="cuda")
+    outs = [[torch.empty((batch, n), dtype=d, device="cuda") for d in (torch.float32, torch.int64, torch.int64)]
+            for _ in range(3)]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        beam.select(x, cum, None, *outs[0], batch, beams, V, n, stream=side)
+        beam.select(x, cum, None, *outs[1], batch, beams, V, n)
+        here.wait_stream(side)
+    for rep in range(4):
+        x.copy_(torch.randn_like(x) * 3)
+        torch.cuda.synchronize()
+        g.replay()
+        with torch.cuda.stream(side):
+            beam.select(x, cum, None, *outs[2], batch, beams, V, n)
+        torch.cuda.synchronize()
+        for a, b, c in zip(*outs):
+            assert torch.equal(a, c) and torch.equal(b, c), rep
 
 
 def test_select_leaves_the_counters_zero(beam):
@@ -286,6 +346,12 @@ def test_reorder_unaligned_and_large(beam):
             p = torch.tensor([[1, 1, 0], [2, 0, 2]], device="cuda")
             beam.reorder(src, p, dst, 2, 3, 3)
             assert torch.equal(dst, src[[1, 1, 0, 5, 3, 5]])
+    for width in (300_000, 1_000_003):  # few large pieces, each in parts
+        src = torch.randint(0, 255, (6, width), device="cuda").to(torch.uint8)
+        dst = torch.full((8, width), 255, dtype=torch.uint8, device="cuda")
+        beam.reorder(src, p, dst[1:-1], 2, 3, 3)
+        assert torch.equal(dst[1:-1], src[[1, 1, 0, 5, 3, 5]])
+        assert bool((dst[0] == 255).all()) and bool((dst[-1] == 255).all())
     big = torch.zeros((3, (1 << 31) + 48), dtype=torch.uint8, device="cuda")  # offsets past 2^32 bytes
     big[2, -100:] = torch.arange(100, dtype=torch.uint8, device="cuda")
     big[1, -1] = 9

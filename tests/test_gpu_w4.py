@@ -249,6 +249,36 @@ def test_embed(w4, T, K, N, group, zeros, fp32):
     check_guard(whole)
 
 
+@pytest.mark.parametrize("n,K", [(1_200_000, 32), (540_000, 8192)])
+def test_embed_many_tokens(w4, n, K):
+    """More words than threads of a launch; an output of more than 2^32 elements."""
+    import torch
+    q, s, z, w = make(5, 50, K, 32, True, exact=True)
+    tok = torch.randint(0, 50, (n,), device="cuda")
+    out = torch.full((n, K), 99.0, dtype=torch.float16, device="cuda")
+    w4.embed(words(w4, q, s, z, K, 32), tok, out, n)
+    table = dev(w.astype(np.float16))
+    for a in range(0, n, 60_000):
+        assert torch.equal(out[a:a + 60_000], table[tok[a:a + 60_000]])
+
+
+def test_gemm_large_batches(w4):
+    """Several launches of tiles, an output of more than 2^32 elements, an input of more than 2^31."""
+    import torch
+    for M, N, K in ((4200, 1 << 20, 32), (70_000, 64, 32768)):
+        gen = torch.Generator(device="cuda")
+        gen.manual_seed(N)
+        wd = torch.randint(-2 ** 31, 2 ** 31 - 1, (N, -(-K // 128) * 16), generator=gen, device="cuda").to(torch.int32)
+        w = w4.W4Words(wd, torch.full((N, K // 32), 0.5, dtype=torch.float16, device="cuda"), None, K, 32)
+        x = torch.randint(-2, 3, (M, K), generator=gen, device="cuda", dtype=torch.int8).half()
+        y = torch.full((M, N), float("nan"), dtype=torch.float16, device="cuda")
+        w4.gemm(y, x, w, M, N, K)
+        for rows in ([0, 63, 64, M // 2], [4095 % M, 4096 % M, M - 2, M - 1]):
+            ref = x[rows].double() @ weights64(w, K).T  # integers and halves: exact but for the output's rounding
+            assert torch.equal(y[rows], ref.half())
+        assert not bool(y[:, 0].isnan().any()) and not bool(y[:, -1].isnan().any())
+
+
 def test_embed_tokens_outside_the_table(w4):
     import torch
     q, s, z, w = make(2, 20, 128, 64, True, exact=True)

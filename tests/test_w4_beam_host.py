@@ -153,3 +153,12 @@ def test_gemm_workspace():
         for N in (1, 64, 2048, 4096, 12288, 151552):
             for K in (32, 2048, 4096, 16384, 1 << 22):
                 assert size(M, N, K) <= 9 << 20, (M, N, K)
+
+
+def test_extents_beyond_a_call():
+    assert gemm(N=(1 << 28) + 1) == _lib.HX_ERR_INVALID and "2^28" in err()
+    assert select(vocab=(1 << 30) + 1, ld=1 << 31) == _lib.HX_ERR_INVALID and "2^30" in err()
+    assert LIB.hx_w4_gemm_workspace_size(64, (1 << 28) + 1, 128) == 0
+    assert LIB.hx_w4_gemm_workspace_size((1 << 31) - 1, 64, 128) == 0
+    assert LIB.hx_w4_gemm_workspace_size(64, 4096, (1 << 31) - 1) == 0
+    assert LIB.hx_beam_select_workspace_size(1, 1, (1 << 31) - 1, 8) == 0
