@@ -58,9 +58,9 @@ HX_INLINE hx_h8 word_operand(uint32_t w, ZeroPair z)
 // Buffer accesses return 0 beyond a descriptor's bytes (and beyond 2^30 always, which marks what must read as 0).  Everything
 // that decides about that is in the per-lane offset.
 constexpr int W4_NONE = 0x7ffffff0;
-HX_INLINE __amdgpu_buffer_rsrc_t w4_rsrc(const void* base, long bytes)
+HX_INLINE __amdgpu_buffer_rsrc_t w4_rsrc(const void* base, long bytes, long most = 0x40000000l)
 {
-    return mf_rsrc(base, (size_t)(bytes < 0 ? 0 : bytes > 0x40000000l ? 0x40000000l : bytes));
+    return mf_rsrc(base, (size_t)(bytes < 0 ? 0 : bytes > most ? most : bytes));
 }
 
 // Scales (fp16) and zero points of a block of 128 k, lowest group first.  GS: groups in a block, 1 where the group is 128 or
@@ -83,6 +83,49 @@ struct BlockScale {
         else return zero_pair((z[0] >> (8 * g)) & 255u);
     }
 };
+
+// The scales of NT <= 4 columns' blocks are loaded together: lane group kg those of column kg, `first` that column's, or W4_NO_SCALE
+// (zero points are read through descriptors of at most 2^29 bytes) in lane groups past NT; then every lane group gets all NT.
+// A load whose lanes are in 16 rows takes the address unit 62 cycles with the row's value in all four lane groups (the words, 16
+// bytes a lane, 33) and 19 in one, which bounded everything here while each column had a load of its own.
+constexpr int W4_NO_SCALE = 1 << 29;
+template <int NT>
+HX_INLINE void spread(uint32_t v, uint32_t (&o)[NT])
+{
+    const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);  // columns 0 1 0 1 | 2 3 2 3 by lane group
+    const auto a = __builtin_amdgcn_permlane16_swap(h[0], h[0], false, false);
+    o[0] = a[0];
+    if constexpr (NT > 1) o[1] = a[1];
+    if constexpr (NT > 2) {
+        const auto b = __builtin_amdgcn_permlane16_swap(h[1], h[1], false, false);
+        o[2] = b[0];
+        if constexpr (NT > 3) o[3] = b[1];
+    }
+}
+template <int NT, int GS, bool Z, bool V>
+HX_INLINE void spread_scale(const BlockScale<GS, Z, V>& v, BlockScale<GS, Z, V> (&o)[NT])
+{
+    uint32_t t[NT];
+    if constexpr (GS == 1 && Z) {
+        spread<NT>(v.s[0] | v.z[0] << 16, t);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) o[n].s[0] = t[n], o[n].z[0] = t[n] >> 16;
+    } else {
+#pragma unroll
+        for (int i = 0; i < BlockScale<GS, Z, V>::NS; ++i) {
+            spread<NT>(v.s[i], t);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) o[n].s[i] = t[n];
+        }
+        if constexpr (Z)
+#pragma unroll
+            for (int i = 0; i < BlockScale<GS, Z, V>::NZ; ++i) {
+                spread<NT>(v.z[i], t);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) o[n].z[i] = t[n];
+            }
+    }
+}
 
 // Of block blk of the row whose first group lies `first` groups behind the descriptors' base.  Groups past K, and rows past the
 // descriptors, have scale 0.
@@ -161,20 +204,20 @@ __device__ __forceinline__ void w4_rows(const _Float16* x, const W4Args& a, void
         }
     };
     hx_u4 w[NS][NT];
-    BlockScale<GS, Z, V> sc[NS][NT];
+    BlockScale<GS, Z, V> sc[NS];
     __amdgpu_buffer_rsrc_t rw_, rs, rz;
     auto aim = [&](int tile) {  // descriptors of the tile's rows (nothing left of the matrix: every load is 0)
         const long row0 = (long)(tile * wr + rw) * NT * R, left = tile < tiles ? a.N - row0 : 0;
         rw_ = w4_rsrc(reinterpret_cast<const char*>(a.words) + row0 * row_bytes, left * row_bytes);
         rs = w4_rsrc(a.scales + row0 * a.groups, left * a.groups * 2);
-        rz = w4_rsrc(Z ? a.zeros + row0 * a.groups : nullptr, Z ? left * a.groups : 0);
+        rz = w4_rsrc(Z ? a.zeros + row0 * a.groups : nullptr, Z ? left * a.groups : 0, W4_NO_SCALE);
     };
-    const int lane_off = r * row_bytes + s * 64 + kg * 16;
+    const int lane_off = r * row_bytes + s * 64 + kg * 16, lane_group = kg < NT ? (kg * R + r) * a.groups : W4_NO_SCALE;
     auto load_w = [&](int i, int n, int kb) {
         const int span = (kb * NS + i) * wk + kw;
         // a block past K reads the next row's words: x is 0 there, and the scale
         w[i][n] = __builtin_bit_cast(hx_u4, __builtin_amdgcn_raw_buffer_load_b128(rw_, lane_off + n * R * row_bytes + span * (S * 64), 0, 0));
-        sc[i][n] = block_scale<GS, Z, V>(rs, rz, a, (n * R + r) * a.groups, span * S + s);
+        if (n == 0) sc[i] = block_scale<GS, Z, V>(rs, rz, a, lane_group, span * S + s);
     };
     int tile = blockIdx.x;
     aim(tile);
@@ -195,11 +238,13 @@ __device__ __forceinline__ void w4_rows(const _Float16* x, const W4Args& a, void
             const int next_kb = wrap ? 0 : kb + 1;
             if (wrap) aim(tile + gridDim.x);
 #pragma unroll
-            for (int i = 0; i < NS; ++i)
+            for (int i = 0; i < NS; ++i) {
+                BlockScale<GS, Z, V> all[NT];
+                spread_scale<NT>(sc[i], all);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const hx_u4 wv = w[i][n];
-                    const BlockScale<GS, Z, V> sv = sc[i][n];
+                    const BlockScale<GS, Z, V> sv = all[n];
                     hx_h8 b[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) b[j] = word_operand(wv[j], sv.zero(j * GS / 4));
@@ -221,6 +266,7 @@ __device__ __forceinline__ void w4_rows(const _Float16* x, const W4Args& a, void
                         }
                     }
                 }
+            }
         }
         // lane: column col, rows 4 kg + e of the products; wanted where their blocks agree
         if (kg / H == s)
@@ -268,7 +314,7 @@ template <int BM, int NT, int KS, int PF, int GS, bool Z, bool V>
 __device__ __forceinline__ void w4_tile(const _Float16* x, const W4Args& a, void* y, int M, bool y_fp32, W4Split sp)
 {
     constexpr int RB = BM / 16, NL = BM / 16;  // row blocks; x loads (4 rows each) of a wave per step
-    constexpr int NVM = NL + NT * (1 + (V || GS == 1 ? 1 : GS) * (Z ? 2 : 1));  // vector memory instructions of a wave per step
+    constexpr int NVM = NL + NT + (V || GS == 1 ? 1 : GS) * (Z ? 2 : 1);  // vector memory instructions of a wave per step
     extern __shared__ __align__(16) _Float16 w4_lds[];  // [PF][KS][BM][128]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int part = wave >> 2, cw = wave & 3, col = lane & 15, kg = lane >> 4;
@@ -281,7 +327,7 @@ __device__ __forceinline__ void w4_tile(const _Float16* x, const W4Args& a, void
     const long left = a.N - n0;
     const __amdgpu_buffer_rsrc_t rw = w4_rsrc(reinterpret_cast<const char*>(a.words) + (size_t)n0 * row_bytes, left * row_bytes);
     const __amdgpu_buffer_rsrc_t rs = w4_rsrc(a.scales + (size_t)n0 * a.groups, left * a.groups * 2);
-    const __amdgpu_buffer_rsrc_t rz = w4_rsrc(Z ? a.zeros + (size_t)n0 * a.groups : nullptr, Z ? left * a.groups : 0);
+    const __amdgpu_buffer_rsrc_t rz = w4_rsrc(Z ? a.zeros + (size_t)n0 * a.groups : nullptr, Z ? left * a.groups : 0, W4_NO_SCALE);
     // rows past M and pieces past K hold anything: the former are not stored, the products of the latter are skipped
     int xoff[NL];
 #pragma unroll
@@ -289,41 +335,39 @@ __device__ __forceinline__ void w4_tile(const _Float16* x, const W4Args& a, void
         const int r = 4 * (cw * NL + i) + (lane >> 4);
         xoff[i] = (r * a.K + part * 128 + 8 * ((lane & 15) ^ (r & 15))) * 2;
     }
-    auto load_x = [&](int slot, int c) {
+    auto load_x = [&](int i, int slot, int c) {
         _Float16* d = w4_lds + (slot * KS + part) * (BM * 128) + cw * NL * 512;
-#pragma unroll
-        for (int i = 0; i < NL; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (__attribute__((address_space(3))) void*)(d + 512 * i), 16,
-                                                     c < steps ? xoff[i] + c * (KS * 256) : W4_NONE, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (__attribute__((address_space(3))) void*)(d + 512 * i), 16,
+                                                 c < steps ? xoff[i] + c * (KS * 256) : W4_NONE, 0, 0, 0);
     };
     hx_u4 w[PF][NT];
-    BlockScale<GS, Z, V> sc[PF][NT];
+    BlockScale<GS, Z, V> sc[PF];
+    const int lane_group = kg < NT ? (16 * (cw * NT + kg) + col) * a.groups : W4_NO_SCALE;
     auto load_w = [&](int slot, int c) {
+        const int blk = c * KS + part;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int row = 16 * (cw * NT + n) + col, blk = c * KS + part;
-            w[slot][n] = __builtin_bit_cast(hx_u4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                       rw, c < steps ? row * row_bytes + blk * 64 + kg * 16 : W4_NONE, 0, 0));
-            sc[slot][n] = block_scale<GS, Z, V>(rs, rz, a, row * a.groups, blk);
-        }
+        for (int n = 0; n < NT; ++n)
+            w[slot][n] = __builtin_bit_cast(
+                hx_u4, __builtin_amdgcn_raw_buffer_load_b128(
+                           rw, c < steps ? (16 * (cw * NT + n) + col) * row_bytes + blk * 64 + kg * 16 : W4_NONE, 0, 0));
+        sc[slot] = block_scale<GS, Z, V>(rs, rz, a, lane_group, blk);
     };
     hx_f4 acc[RB][NT];
 #pragma unroll
     for (int i = 0; i < RB; ++i)
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[i][n] = hx_f4{0.f, 0.f, 0.f, 0.f};
-    // The waits below, and the compiler's, count a step's loads: steps stay apart, the x loads come first in each, and every step
+    // The waits below, and the compiler's, count a step's loads: steps stay apart, the words come first in each, and every step
     // issues its loads, past the end as accesses that touch no memory (where they depended on the step, each use of the words
     // waited for all loads in flight: 13 us instead of x at 16 rows of 4096 -> 2048).
-    auto load = [&](int slot, int c) {
-        asm volatile("" ::: "memory");
-        load_x(slot, c);
-        asm volatile("" ::: "memory");
-        load_w(slot, c);
-        asm volatile("" ::: "memory");
-    };
 #pragma unroll
-    for (int u = 0; u < PF - 1; ++u) load(u, first + u);
+    for (int u = 0; u < PF - 1; ++u) {
+        asm volatile("" ::: "memory");
+        load_w(u, first + u);
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < NL; ++i) load_x(i, u, first + u);
+    }
     auto step = [&](int u, int c, bool whole) {
         // the decode of a later step's words would wait for their loads here
         __builtin_amdgcn_sched_barrier(0);
@@ -333,27 +377,38 @@ __device__ __forceinline__ void w4_tile(const _Float16* x, const W4Args& a, void
         hx_lds_barrier();  // and the other waves'; the stage of step c - 1 is no longer read
         hx_h8 b[NT][4];
         float f[NT][GS];
+        BlockScale<GS, Z, V> sv[NT];
+        spread_scale<NT>(sc[u], sv);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) b[n][j] = word_operand(w[u][n][j], sc[u][n].zero(j * GS / 4));
+            for (int j = 0; j < 4; ++j) b[n][j] = word_operand(w[u][n][j], sv[n].zero(j * GS / 4));
 #pragma unroll
-            for (int g = 0; g < GS; ++g) f[n][g] = sc[u][n].scale(g);
+            for (int g = 0; g < GS; ++g) f[n][g] = sv[n].scale(g);
         }
-        load((u + PF - 1) % PF, c + PF - 1);
+        asm volatile("" ::: "memory");
+        load_w((u + PF - 1) % PF, c + PF - 1);
+        asm volatile("" ::: "memory");
         const _Float16* s = w4_lds + (u * KS + part) * (BM * 128);
         const int left_k = whole ? 128 : a.K - 128 * (c * KS + part);  // of K in this block
-#pragma unroll
-        for (int i = 0; i < RB; ++i) {
-            hx_h8 xa[4];
+        hx_h8 xa[2][4];
+        auto fragment = [&](int i) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                xa[j] = *reinterpret_cast<const hx_h8*>(s + (16 * i + col) * 128 + 8 * ((4 * j + kg) ^ col));
+                xa[i & 1][j] = *reinterpret_cast<const hx_h8*>(s + (16 * i + col) * 128 + 8 * ((4 * j + kg) ^ col));
+        };
+        fragment(0);
+#pragma unroll
+        for (int i = 0; i < RB; ++i) {
+            // One row block's products, the next one's fragments and one x load at a time: the eight waves' loads, all issued at
+            // the start of a step, kept them from their products for a third of it.
+            __builtin_amdgcn_sched_barrier(0);
+            load_x(i, (u + PF - 1) % PF, c + PF - 1);
+            if (i + 1 < RB) fragment(i + 1);
             if (!whole)  // what lies behind a row's K, x of another row or nothing, counts as 0 (as do the scales there)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (32 * j >= left_k) xa[j] = hx_h8{};
-            if constexpr (GS > 1) __builtin_amdgcn_sched_barrier(0);  // the row blocks' products would all be started at once
+                    if (32 * j >= left_k) xa[i & 1][j] = hx_h8{};
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -361,7 +416,7 @@ __device__ __forceinline__ void w4_tile(const _Float16* x, const W4Args& a, void
                     hx_f4 t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int j = g * 4 / GS; j < (g + 1) * 4 / GS; ++j)
-                        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(xa[j], b[n][j], t, 0, 0, 0);
+                        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(xa[i & 1][j], b[n][j], t, 0, 0, 0);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[i][n][e] = __builtin_fmaf(f[n][g], t[e], acc[i][n][e]);
                 }
