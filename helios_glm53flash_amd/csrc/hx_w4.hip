@@ -314,7 +314,9 @@ template <int BM, int NT, int KS, int PF, int GS, bool Z, bool V>
 __device__ __forceinline__ void w4_tile(const _Float16* x, const W4Args& a, void* y, int M, bool y_fp32, W4Split sp)
 {
     constexpr int RB = BM / 16, NL = BM / 16;  // row blocks; x loads (4 rows each) of a wave per step
-    constexpr int NVM = NL + NT + (V || GS == 1 ? 1 : GS) * (Z ? 2 : 1);  // vector memory instructions of a wave per step
+    // vector memory instructions of a wave: per step, and for the scales of every SP-th
+    constexpr int NVM = NL + NT, NSC = (V || GS == 1 ? 1 : GS) * (Z ? 2 : 1), SP = 4 / NT;
+    static_assert(PF % SP == 0);
     extern __shared__ __align__(16) _Float16 w4_lds[];  // [PF][KS][BM][128]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int part = wave >> 2, cw = wave & 3, col = lane & 15, kg = lane >> 4;
@@ -323,9 +325,13 @@ __device__ __forceinline__ void w4_tile(const _Float16* x, const W4Args& a, void
     const int first = split * sp.steps, steps = min(first + sp.steps, (nb + KS - 1) / KS);  // this split's steps
     const int mt = (M + BM - 1) / BM;
     const int m0 = tile % mt * BM, n0 = tile / mt * (64 * NT);
-    const __amdgpu_buffer_rsrc_t rx = w4_rsrc(x + (size_t)m0 * a.K, (long)min(M - m0, BM) * a.K * 2);
-    const long left = a.N - n0;
-    const __amdgpu_buffer_rsrc_t rw = w4_rsrc(reinterpret_cast<const char*>(a.words) + (size_t)n0 * row_bytes, left * row_bytes);
+    const long left = min(a.N - n0, 64 * NT);
+    const char *xb = reinterpret_cast<const char*>(x + (size_t)m0 * a.K), *wb = reinterpret_cast<const char*>(a.words) + (size_t)n0 * row_bytes;
+    const int x_bytes = min(M - m0, BM) * a.K * 2, w_bytes = (int)left * row_bytes;
+    // From byte `at` on; nothing from step `steps` on.  The lanes' offsets are the same in all steps, and nothing branches.
+    auto stepped = [&](const char* base, int at, int bytes, int c) {
+        return mf_rsrc(base + at, (size_t)(max(bytes - at, 0) & ((c - steps) >> 31)));
+    };
     const __amdgpu_buffer_rsrc_t rs = w4_rsrc(a.scales + (size_t)n0 * a.groups, left * a.groups * 2);
     const __amdgpu_buffer_rsrc_t rz = w4_rsrc(Z ? a.zeros + (size_t)n0 * a.groups : nullptr, Z ? left * a.groups : 0, W4_NO_SCALE);
     // rows past M and pieces past K hold anything: the former are not stored, the products of the latter are skipped
@@ -333,24 +339,26 @@ __device__ __forceinline__ void w4_tile(const _Float16* x, const W4Args& a, void
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
         const int r = 4 * (cw * NL + i) + (lane >> 4);
-        xoff[i] = (r * a.K + part * 128 + 8 * ((lane & 15) ^ (r & 15))) * 2;
+        xoff[i] = (r * a.K + 8 * ((lane & 15) ^ (r & 15))) * 2;
     }
     auto load_x = [&](int i, int slot, int c) {
         _Float16* d = w4_lds + (slot * KS + part) * (BM * 128) + cw * NL * 512;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (__attribute__((address_space(3))) void*)(d + 512 * i), 16,
-                                                 c < steps ? xoff[i] + c * (KS * 256) : W4_NONE, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(stepped(xb, (c * KS + part) * 256, x_bytes, c),
+                                                 (__attribute__((address_space(3))) void*)(d + 512 * i), 16, xoff[i], 0, 0, 0);
     };
     hx_u4 w[PF][NT];
-    BlockScale<GS, Z, V> sc[PF];
-    const int lane_group = kg < NT ? (16 * (cw * NT + kg) + col) * a.groups : W4_NO_SCALE;
+    BlockScale<GS, Z, V> sc;
+    const int lane_group = (16 * (cw * NT + kg % NT) + col) * a.groups;
+    auto load_scales = [&](int c) {  // of steps c .. c + SP - 1: lane group kg takes column kg % NT, step c + kg / NT
+        sc = block_scale<GS, Z, V>(rs, rz, a, lane_group, (c + kg / NT) * KS + part);
+        asm volatile("" ::: "memory");
+    };
     auto load_w = [&](int slot, int c) {
-        const int blk = c * KS + part;
+        const __amdgpu_buffer_rsrc_t rw = stepped(wb, (c * KS + part) * 64, w_bytes, c);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
             w[slot][n] = __builtin_bit_cast(
-                hx_u4, __builtin_amdgcn_raw_buffer_load_b128(
-                           rw, c < steps ? (16 * (cw * NT + n) + col) * row_bytes + blk * 64 + kg * 16 : W4_NONE, 0, 0));
-        sc[slot] = block_scale<GS, Z, V>(rs, rz, a, lane_group, blk);
+                hx_u4, __builtin_amdgcn_raw_buffer_load_b128(rw, (16 * (cw * NT + n) + col) * row_bytes + kg * 16, 0, 0));
     };
     hx_f4 acc[RB][NT];
 #pragma unroll
@@ -360,33 +368,43 @@ __device__ __forceinline__ void w4_tile(const _Float16* x, const W4Args& a, void
     // The waits below, and the compiler's, count a step's loads: steps stay apart, the words come first in each, and every step
     // issues its loads, past the end as accesses that touch no memory (where they depended on the step, each use of the words
     // waited for all loads in flight: 13 us instead of x at 16 rows of 4096 -> 2048).
+    if constexpr (SP >= PF) load_scales(first);
 #pragma unroll
     for (int u = 0; u < PF - 1; ++u) {
         asm volatile("" ::: "memory");
+        if ((u + 1) % SP == 0 && u + 1 == PF - SP) load_scales(first);
         load_w(u, first + u);
         asm volatile("" ::: "memory");
 #pragma unroll
         for (int i = 0; i < NL; ++i) load_x(i, u, first + u);
     }
-    auto step = [&](int u, int c, bool whole) {
+    BlockScale<GS, Z, V> sv[4];  // of SP steps
+    auto step = [&](auto slot, int c, bool whole) {
+        constexpr int u = decltype(slot)::value;
         // the decode of a later step's words would wait for their loads here
         __builtin_amdgcn_sched_barrier(0);
-        // x of step c has arrived once at most the loads of the PF - 2 later steps in flight are outstanding
+        // x of step c has arrived once at most what the PF - 2 steps before this one have loaded is outstanding
+        constexpr int later = [] {
+            int n = 0;
+            for (int d = 1; d <= PF - 2; ++d) n += NVM + ((u + PF - d) % SP == 0 ? NSC : 0);
+            return n;
+        }();
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(qt_vmcnt((PF - 2) * NVM));
+        __builtin_amdgcn_s_waitcnt(qt_vmcnt(later));
         hx_lds_barrier();  // and the other waves'; the stage of step c - 1 is no longer read
         hx_h8 b[NT][4];
         float f[NT][GS];
-        BlockScale<GS, Z, V> sv[NT];
-        spread_scale<NT>(sc[u], sv);
+        if constexpr (u % SP == 0) spread_scale<4>(sc, sv);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
+            const BlockScale<GS, Z, V>& s = sv[u % SP * NT + n];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) b[n][j] = word_operand(w[u][n][j], sv[n].zero(j * GS / 4));
+            for (int j = 0; j < 4; ++j) b[n][j] = word_operand(w[u][n][j], s.zero(j * GS / 4));
 #pragma unroll
-            for (int g = 0; g < GS; ++g) f[n][g] = sv[n].scale(g);
+            for (int g = 0; g < GS; ++g) f[n][g] = s.scale(g);
         }
         asm volatile("" ::: "memory");
+        if constexpr (u % SP == 0) load_scales(c + SP);
         load_w((u + PF - 1) % PF, c + PF - 1);
         asm volatile("" ::: "memory");
         const _Float16* s = w4_lds + (u * KS + part) * (BM * 128);
@@ -426,12 +444,13 @@ __device__ __forceinline__ void w4_tile(const _Float16* x, const W4Args& a, void
     const int whole = min(steps, a.K / (128 * KS));  // the end of the steps without a part past K
     int c0 = first;
     for (; c0 + PF <= whole; c0 += PF)
-#pragma unroll
-        for (int u = 0; u < PF; ++u) step(u, c0 + u, true);
+        [&]<int... U>(std::integer_sequence<int, U...>) {
+            (step(std::integral_constant<int, U>{}, c0 + U, true), ...);
+        }(std::make_integer_sequence<int, PF>{});
     for (; c0 < steps; c0 += PF)
-#pragma unroll
-        for (int u = 0; u < PF; ++u)
-            if (c0 + u < steps) step(u, c0 + u, false);
+        [&]<int... U>(std::integer_sequence<int, U...>) {
+            ((c0 + U < steps && (step(std::integral_constant<int, U>{}, c0 + U, false), true)) && ...);
+        }(std::make_integer_sequence<int, PF>{});
     // the accesses behind the last step are done with the stages too
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(qt_vmcnt(0));
@@ -637,7 +656,7 @@ hipError_t gemm_launch(const W4Call& c)
             case W4Plan::ROWS8_FEW: return rows_launch<2, 1, 16, 1, 1, GS, Z, V>(c, 512);
             case W4Plan::ROWS8_WIDE: return rows_launch<2, 1, 8, 2, 2, GS, Z, V>(c, 512);
             case W4Plan::ROWS16: return rows_launch<2, 2, 16, 1, 2, GS, Z, V>(c, 256);
-            case W4Plan::TILE64W: return tile_launch<64, 2, 1, 3, GS, Z, V>(c, p);
+            case W4Plan::TILE64W: return tile_launch<64, 2, 1, 4, GS, Z, V>(c, p);
             case W4Plan::TILE128: return tile_launch<128, 2, 1, 2, GS, Z, V>(c, p);
             default: break;
         }
@@ -647,7 +666,7 @@ hipError_t gemm_launch(const W4Call& c)
         case W4Plan::ROWS8: return rows_launch<2, 1, 8, 1, 2, GS, Z, V>(c, 512);
         case W4Plan::TILE16: return tile_launch<16, 1, 2, 4, GS, Z, V>(c, p);
         case W4Plan::TILE32: return tile_launch<32, 1, 2, 4, GS, Z, V>(c, p);
-        default: return tile_launch<64, 1, 2, 3, GS, Z, V>(c, p);
+        default: return tile_launch<64, 1, 2, 4, GS, Z, V>(c, p);
     }
 }
 

@@ -146,6 +146,22 @@ def test_gemm_keeps_infinities_and_nans_in_their_rows(w4, M):
     assert not np.isfinite(got[:, 9]).any()
 
 
+@pytest.mark.parametrize("M", [9, 17, 33, 65, 129])
+@pytest.mark.parametrize("K", [1120, 32, 2336])
+def test_gemm_single_rows_behind_a_tile(w4, M, K):
+    """A last tile of one row, a part of K without a block, and a last block cut short; the memory behind x holds NaN."""
+    import torch
+    N, group = 70, 32
+    q, s, z, w = make(M + K, N, K, group, True, exact=True)
+    whole = torch.full((M + 4, K), float("nan"), dtype=torch.float16, device="cuda")
+    x = whole[2:-2]
+    x.copy_(torch.from_numpy(np.random.default_rng(M).integers(-3, 4, (M, K))))
+    guard, y = guarded((M, N), torch.float32)
+    w4.gemm(y, x, words(w4, q, s, z, K, group), M, N, K, True)
+    assert np.array_equal(y.cpu().numpy().astype(np.float64), x.cpu().numpy().astype(np.float64) @ w.T)
+    check_guard(guard)
+
+
 def test_gemm_empty_batch(w4):
     import torch
     q, s, z, _ = make(1, 16, 128, 64, True)
