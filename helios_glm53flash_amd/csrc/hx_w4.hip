@@ -167,20 +167,20 @@ HX_INLINE void store_y(void* y, size_t i, float v, bool y_fp32)
 
 }  // namespace
 
-// ---- M <= 64
+// ---- up to 8 rows
 //
 // One wave load covers 16 / S weight rows over S consecutive blocks of 128 k (S * 64 bytes of each row): column n = s R + r of
 // the matrix instruction is row r (R = 16 / S), block s, and row a = s R + t of the other operand is token t's x in block s.  Of
 // the products those with equal s are wanted; for few tokens the unused rows so buy whole cache lines per row and four times
-// as many rows to spread over the chip.  S = 4 serves 4 tokens, 2 serves 8, 1 serves 16 MT.
+// as many rows to spread over the chip.  S = 4 serves 4 tokens, 2 serves 8.
 // A wave owns NS spans (S blocks each) of every WK NS, keeps x for them in registers and goes over tiles of NT R rows; each word
 // is replaced by the next tile's as soon as it is decoded.  Per group the products are summed by the matrix
 // instructions from zero, then scaled into the fp32 sums.
-template <int S, int MT, int WAVES, int NS, int NT, int GS, bool Z, bool V>
+template <int S, int WAVES, int NS, int NT, int GS, bool Z, bool V>
 __device__ __forceinline__ void w4_rows(const _Float16* x, const W4Args& a, void* y, int M, bool y_fp32, int wk)
 {
     constexpr int R = 16 / S, H = 4 / S;  // rows of a load; 4-token pieces of a column
-    __shared__ float red[WAVES][NT * MT][4 * H][16];
+    __shared__ float red[WAVES][NT][4 * H][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kw = wave & (wk - 1), rw = wave / wk, wr = WAVES / wk;  // the wave's place in K and in rows
     const int col = lane & 15, kg = lane >> 4, s = col / R, r = col % R;
@@ -189,18 +189,16 @@ __device__ __forceinline__ void w4_rows(const _Float16* x, const W4Args& a, void
     const int tiles = (a.N + rows_wg - 1) / rows_wg;
 
     const __amdgpu_buffer_rsrc_t rx = w4_rsrc(x, (long)M * a.K * 2);
-    hx_h8 xa[NS][MT][4];
+    hx_h8 xa[NS][4];
     auto load_x = [&](int kb) {
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             const int k = (((kb * NS + i) * wk + kw) * S + s) * 128 + 8 * kg;
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int off = k + 32 * j < a.K ? ((16 * m + r) * a.K + k + 32 * j) * 2 : W4_NONE;
-                    xa[i][m][j] = __builtin_bit_cast(hx_h8, __builtin_amdgcn_raw_buffer_load_b128(rx, off, 0, 0));
-                }
+            for (int j = 0; j < 4; ++j) {
+                const int off = k + 32 * j < a.K ? (r * a.K + k + 32 * j) * 2 : W4_NONE;
+                xa[i][j] = __builtin_bit_cast(hx_h8, __builtin_amdgcn_raw_buffer_load_b128(rx, off, 0, 0));
+            }
         }
     };
     hx_u4 w[NS][NT];
@@ -227,11 +225,9 @@ __device__ __forceinline__ void w4_rows(const _Float16* x, const W4Args& a, void
 #pragma unroll
         for (int n = 0; n < NT; ++n) load_w(i, n, 0);
     for (; tile < tiles; tile += gridDim.x) {
-        hx_f4 acc[NT][MT];
+        hx_f4 acc[NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int m = 0; m < MT; ++m) acc[n][m] = hx_f4{0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < NT; ++n) acc[n] = hx_f4{0.f, 0.f, 0.f, 0.f};
         for (int kb = 0; kb < nkb; ++kb) {
             if (nkb > 1) load_x(kb);
             const bool wrap = kb + 1 == nkb;
@@ -255,15 +251,12 @@ __device__ __forceinline__ void w4_rows(const _Float16* x, const W4Args& a, void
 #pragma unroll
                     for (int g = 0; g < GS; ++g) {
                         const float f = sv.scale(g);
+                        hx_f4 c{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int m = 0; m < MT; ++m) {
-                            hx_f4 c{0.f, 0.f, 0.f, 0.f};
+                        for (int j = g * 4 / GS; j < (g + 1) * 4 / GS; ++j)
+                            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(xa[i][j], b[j], c, 0, 0, 0);
 #pragma unroll
-                            for (int j = g * 4 / GS; j < (g + 1) * 4 / GS; ++j)
-                                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(xa[i][m][j], b[j], c, 0, 0, 0);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) acc[n][m][e] = __builtin_fmaf(f, c[e], acc[n][m][e]);
-                        }
+                        for (int e = 0; e < 4; ++e) acc[n][e] = __builtin_fmaf(f, c[e], acc[n][e]);
                     }
                 }
             }
@@ -273,28 +266,26 @@ __device__ __forceinline__ void w4_rows(const _Float16* x, const W4Args& a, void
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) red[wave][n * MT + m][kg % H * 4 + e][col] = acc[n][m][e];
+                for (int e = 0; e < 4; ++e) red[wave][n][kg % H * 4 + e][col] = acc[n][e];
         hx_lds_barrier();
-        constexpr int ITEMS = NT * MT * 4 * H * R;  // outputs per row part of the workgroup
+        constexpr int ITEMS = NT * 4 * H * R;  // outputs per row part of the workgroup
         for (int i = threadIdx.x; i < ITEMS * wr; i += 64 * WAVES) {
-            const int part = i / ITEMS, q = i % ITEMS, rr = q % R, t4 = q / R % (4 * H), m = q / R / (4 * H) % MT, n = q / R / (4 * H) / MT;
-            const int row = (tile * wr + part) * NT * R + n * R + rr, t = 16 * m + t4;
+            const int part = i / ITEMS, q = i % ITEMS, rr = q % R, t = q / R % (4 * H), n = q / R / (4 * H);
+            const int row = (tile * wr + part) * NT * R + n * R + rr;
             float v = 0.0f;
             for (int k = 0; k < wk; ++k)
 #pragma unroll
-                for (int ss = 0; ss < S; ++ss) v += red[part * wk + k][n * MT + m][t4][ss * R + rr];
+                for (int ss = 0; ss < S; ++ss) v += red[part * wk + k][n][t][ss * R + rr];
             if (row < a.N && t < M) store_y(y, (size_t)t * a.N + row, v, y_fp32);
         }
         hx_lds_barrier();  // the sums are read before the next tile's overwrite them
     }
 }
 
-template <int S, int MT, int WAVES, int NS, int NT, int GS, bool Z, bool V>
+template <int S, int WAVES, int NS, int NT, int GS, bool Z, bool V>
 __global__ __launch_bounds__(64 * WAVES) void w4_rows_kernel(const _Float16* x, W4Args a, void* y, int M, bool y_fp32, int wk)
 {
-    w4_rows<S, MT, WAVES, NS, NT, GS, Z, V>(x, a, y, M, y_fp32, wk);
+    w4_rows<S, WAVES, NS, NT, GS, Z, V>(x, a, y, M, y_fp32, wk);
 }
 
 // ---- more rows
@@ -555,14 +546,14 @@ struct W4Call {
 
 // Which kernel takes a call of M rows, by measured shapes (us, 4-bit, group 128, weights from memory).
 struct W4Plan {
-    enum Kind { ROWS4_FEW, ROWS4, ROWS8_FEW, ROWS8, ROWS8_WIDE, ROWS16, TILE16, TILE32, TILE64, TILE64W, TILE128 } kind;
+    enum Kind { ROWS4_FEW, ROWS4, ROWS8_FEW, ROWS8, ROWS8_WIDE, TILE16, TILE32, TILE64, TILE64W, TILE64W2, TILE128 } kind;
     int splits, steps;  // of a tile kernel
     long tiles;
 };
 struct W4Tile {
     int bm, nt, ks;
 };
-constexpr W4Tile W4_TILES[] = {{16, 1, 2}, {32, 1, 2}, {64, 1, 2}, {64, 2, 1}, {128, 2, 1}};  // TILE16 ..
+constexpr W4Tile W4_TILES[] = {{16, 1, 2}, {32, 1, 2}, {64, 1, 2}, {64, 2, 1}, {64, 2, 2}, {128, 2, 1}};  // TILE16 ..
 constexpr int W4_SLOTS = 256;  // workgroups that splitting fills the chip with, one per CU
 
 W4Plan w4_tile_plan(int kind, int M, int N, int K, bool split)
@@ -570,9 +561,9 @@ W4Plan w4_tile_plan(int kind, int M, int N, int K, bool split)
     const W4Tile t = W4_TILES[kind - W4Plan::TILE16];
     W4Plan p{(W4Plan::Kind)kind, 1, (K + 128 * t.ks - 1) / (128 * t.ks), 0};
     p.tiles = ((long)M + t.bm - 1) / t.bm * (((long)N + 64 * t.nt - 1) / (64 * t.nt));
-    // K is split while that fills idle CUs and leaves each split 4 steps: 32 rows, 8192 -> 4096, 27 us unsplit, 12.5 in 4, 15 in
-    // 8; 2048 -> 2048 7.7, 7.5 in 2, 8.0 in 4.
-    if (split && t.ks > 1) {
+    // K is split while that fills idle CUs and leaves each split 4 steps: 64 rows, 16384 -> 4096, 41 us unsplit, 21.5 in 4; 8192
+    // -> 4096 25 and 14.4; 32 rows of the former 27 and 16.
+    if (split && t.nt == 1) {
         const int most = (int)(W4_SLOTS / p.tiles) < p.steps / 4 ? (int)(W4_SLOTS / p.tiles) : p.steps / 4;
         if (most > 1) {
             p.steps = (p.steps + most - 1) / most;
@@ -582,36 +573,42 @@ W4Plan w4_tile_plan(int kind, int M, int N, int K, bool split)
     return p;
 }
 
-// pieces: the kernels for groups in aligned pieces are among the choice; the others are built for the basic shapes only.
-W4Plan w4_plan(int M, int N, int K, bool split, bool pieces)
+// gs: groups in a block of 128 k.  pieces: the kernels for groups in aligned pieces are among the choice; the others are built for the
+// basic shapes only.  Measured as groups of 128 without zero points / of 32 with.
+W4Plan w4_plan(int M, int N, int K, int gs, bool split, bool pieces)
 {
-    // Few weights: 2 loads per wave, so that more waves share them (1 row, 4096 -> 2048: 3.9 us, 4.7 with 4 loads; 8192 -> 4096
-    // 7.6 / 7.9, with 4 rows 10.8 / 9.1; 4096 -> 12288 9.7 / 9.1, 4096 -> 151552 73 / 62).
-    const bool few = !pieces || (long)N * K <= 1l << (M <= 2 ? 25 : 24);
-    if (M <= 4) return {few ? W4Plan::ROWS4_FEW : W4Plan::ROWS4, 1, 0, 0};
-    // 5 rows, groups of 32 with zero points, as 16 waves of one load / 8 waves of 2 / 8 waves of 2 in each of two spans: 4096 ->
-    // 2048 5.4 / 7.2 / 7.7, 8192 -> 4096 14.0 / 11.2 / 12.5, 2048 -> 8192 7.3 / 7.1 / 7.8, 4096 -> 12288 17.5 / 15.3 / 14.3; groups
-    // of 128 without them 4.9 / 6.2 / 6.1, 12.2 / 9.7 / 10.3, 6.2 / 5.9 / 6.2, 14.2 / 13.0 / 11.1.
+    // Few weights: 2 loads per wave, so that more waves share them (1 row, 4096 -> 2048: 3.9 / 4.4 us, 4.4 / 4.9 with 4 loads; 8192 ->
+    // 4096 7.3 / 8.7 and 7.4 / 8.3, with 4 rows 10.6 / 11.5 and 8.6 / 9.5).  Of many, the groups of 32 take the place that
+    // more loads need (1 row, 4096 -> 12288 9.7 / 11.3 and 9.1 / 12.5; -> 32768 20.4 / 23.6 and 18.6 / 25.9).
+    if (M <= 4) return {!pieces || N < 4096 || (gs == 4 && N > 8192) ? W4Plan::ROWS4_FEW : W4Plan::ROWS4, 1, 0, 0};
+    // 5 rows as 16 waves of one load / 8 waves of 2 / 8 waves of 2 in each of two spans: 4096 -> 2048 4.9, 5.8, 6.0 us (groups of 32
+    // 5.1, 6.2, 6.7); 2048 -> 2048 4.7, 4.2, 5.8; 8192 -> 4096 13.5, 8.5, 9.9; 2048 -> 8192 8.1, 5.6, 6.1; 4096 -> 12288
+    // 15.5, 11.4, 10.5 (17.3, 12.4, 15.5); -> 32768 33, 25, 20.5 (38, 27.6, 29.6).
     if (M <= 8) {
-        const W4Plan::Kind kind = (long)N * K <= 1l << 23 ? W4Plan::ROWS8_FEW : N <= 8192 ? W4Plan::ROWS8 : W4Plan::ROWS8_WIDE;
+        const W4Plan::Kind kind = N < 4096 && K >= 4096 ? W4Plan::ROWS8_FEW : N > 8192 && gs < 4 ? W4Plan::ROWS8_WIDE : W4Plan::ROWS8;
         return {pieces ? kind : W4Plan::ROWS8, 1, 0, 0};
     }
-    // 16 rows: 4096 -> 151552 87 us in rows, 99 in tiles; 4096 -> 12288 12.6 / 12.1; 8192 -> 4096 13.8 / 10.7
-    if (M <= 16) return pieces && N >= 32768 ? W4Plan{W4Plan::ROWS16, 1, 0, 0} : w4_tile_plan(W4Plan::TILE16, M, N, K, split);
+    if (M <= 16) return w4_tile_plan(W4Plan::TILE16, M, N, K, split);
     if (M <= 32) return w4_tile_plan(W4Plan::TILE32, M, N, K, split);
-    // A step of a workgroup takes as long as its share of the CU lets it, or its own latency where it is alone.
+    // A step of a tile, in us, where there is less than one workgroup for two CUs, where there is one per CU, and per workgroup where
+    // there are more; how much longer groups of 32 with zero points take.  Of 42 shapes (64 to 256 rows) the choice is 0.5 %
+    // slower than the best each time, and 5 % at most.
     struct Cost {
         int kind;
-        float alone, shared;  // us per step: one workgroup on a CU, and per workgroup where a CU has several
+        float few, one, more, fine;
     };
-    constexpr Cost cost[] = {{W4Plan::TILE64, 0.85f, 0.95f}, {W4Plan::TILE64W, 0.82f, 0.74f}, {W4Plan::TILE128, 1.25f, 1.0f}};
+    constexpr Cost cost[] = {{W4Plan::TILE64, 0.68f, 0.86f, 0.92f, 1.2f},
+                             {W4Plan::TILE64W, 0.56f, 0.77f, 0.62f, 1.4f},
+                             {W4Plan::TILE64W2, 1.15f, 1.32f, 1.4f, 1.42f},
+                             {W4Plan::TILE128, 0.96f, 1.36f, 1.03f, 1.25f}};
     W4Plan best{};
     float least = 0.0f;
     for (const Cost& c : cost) {
-        if (!pieces && c.kind != W4Plan::TILE64) continue;
+        if (c.kind != W4Plan::TILE64 && (!pieces || (M <= 64 && c.kind == W4Plan::TILE128))) continue;
         const W4Plan p = w4_tile_plan(c.kind, M, N, K, split);
-        const float rounds = (float)((p.tiles * p.splits + 255) / 256) * c.shared;
-        const float t = p.steps * (rounds > c.alone ? rounds : c.alone) + (p.splits > 1 ? 3.0f : 0.0f);
+        const long n = p.tiles * p.splits;
+        const float step = n <= 128 ? c.few : n <= 256 ? c.one : (float)((n + 255) / 256) * c.more;
+        const float t = p.steps * step * (gs == 4 ? c.fine : gs == 2 ? 0.5f + 0.5f * c.fine : 1.0f) + (p.splits > 1 ? 1.5f : 0.0f);
         if (c.kind == W4Plan::TILE64 || t < least) least = t, best = p;
     }
     return best;
@@ -623,14 +620,14 @@ size_t w4_partial_bytes(const W4Plan& p)
     return (size_t)p.tiles * p.splits * t.bm * 64 * t.nt * sizeof(float);
 }
 
-template <int S, int MT, int WAVES, int NS, int NT, int GS, bool Z, bool V>
-hipError_t rows_launch(const W4Call& c, int slots)
+template <int S, int WAVES, int NS, int NT, int GS, bool Z, bool V>
+hipError_t rows_launch(const W4Call& c)
 {
     const int spans = ((c.a.K + 127) / 128 + S - 1) / S;
     int wk = 1;  // waves along K: as many as have spans, up to all
     while (wk < WAVES && wk * NS < spans) wk *= 2;
     const int rows = WAVES / wk * NT * 16 / S, tiles = (c.a.N + rows - 1) / rows;
-    hipLaunchKernelGGL((w4_rows_kernel<S, MT, WAVES, NS, NT, GS, Z, V>), dim3(tiles < slots ? tiles : slots), dim3(64 * WAVES), 0, c.st, c.x, c.a, c.y,
+    hipLaunchKernelGGL((w4_rows_kernel<S, WAVES, NS, NT, GS, Z, V>), dim3(tiles < 2 * W4_SLOTS ? tiles : 2 * W4_SLOTS), dim3(64 * WAVES), 0, c.st, c.x, c.a, c.y,
                        c.M, c.y_fp32, wk);
     return hipGetLastError();
 }
@@ -649,21 +646,21 @@ hipError_t tile_launch(const W4Call& c, const W4Plan& p)
 template <int GS, bool Z, bool V>
 hipError_t gemm_launch(const W4Call& c)
 {
-    const W4Plan p = w4_plan(c.M, c.a.N, c.a.K, c.ws != nullptr, V || GS == 1);
+    const W4Plan p = w4_plan(c.M, c.a.N, c.a.K, GS, c.ws != nullptr, V || GS == 1);
     if constexpr (V || GS == 1) {
         switch (p.kind) {
-            case W4Plan::ROWS4: return rows_launch<4, 1, 8, 1, 4, GS, Z, V>(c, 512);
-            case W4Plan::ROWS8_FEW: return rows_launch<2, 1, 16, 1, 1, GS, Z, V>(c, 512);
-            case W4Plan::ROWS8_WIDE: return rows_launch<2, 1, 8, 2, 2, GS, Z, V>(c, 512);
-            case W4Plan::ROWS16: return rows_launch<2, 2, 16, 1, 2, GS, Z, V>(c, 256);
+            case W4Plan::ROWS4: return rows_launch<4, 8, 1, 4, GS, Z, V>(c);
+            case W4Plan::ROWS8_FEW: return rows_launch<2, 16, 1, 1, GS, Z, V>(c);
+            case W4Plan::ROWS8_WIDE: return rows_launch<2, 8, 2, 2, GS, Z, V>(c);
             case W4Plan::TILE64W: return tile_launch<64, 2, 1, 4, GS, Z, V>(c, p);
+            case W4Plan::TILE64W2: return tile_launch<64, 2, 2, 4, GS, Z, V>(c, p);
             case W4Plan::TILE128: return tile_launch<128, 2, 1, 2, GS, Z, V>(c, p);
             default: break;
         }
     }
     switch (p.kind) {
-        case W4Plan::ROWS4_FEW: return rows_launch<4, 1, 8, 1, 2, GS, Z, V>(c, 512);
-        case W4Plan::ROWS8: return rows_launch<2, 1, 8, 1, 2, GS, Z, V>(c, 512);
+        case W4Plan::ROWS4_FEW: return rows_launch<4, 8, 1, 2, GS, Z, V>(c);
+        case W4Plan::ROWS8: return rows_launch<2, 8, 1, 2, GS, Z, V>(c);
         case W4Plan::TILE16: return tile_launch<16, 1, 2, 4, GS, Z, V>(c, p);
         case W4Plan::TILE32: return tile_launch<32, 1, 2, 4, GS, Z, V>(c, p);
         default: return tile_launch<64, 1, 2, 4, GS, Z, V>(c, p);
@@ -694,10 +691,11 @@ hipError_t gemm_launch(const W4Call& c)
 size_t w4_gemm_workspace_bytes(int M, int N, int K)
 {
     size_t most = 0;
-    for (const bool pieces : {false, true}) {
-        const W4Plan p = w4_plan(M, N, K, true, pieces);
-        if (p.splits > 1 && w4_partial_bytes(p) > most) most = w4_partial_bytes(p);
-    }
+    for (const int gs : {1, 2, 4})
+        for (const bool pieces : {false, true}) {
+            const W4Plan p = w4_plan(M, N, K, gs, true, pieces);
+            if (p.splits > 1 && w4_partial_bytes(p) > most) most = w4_partial_bytes(p);
+        }
     return most ? HX_COUNTER_BYTES + most : 0;
 }
 

@@ -37,8 +37,8 @@ def test_every_step_is_complete_at_its_barrier(tmp_path, monkeypatch):
         __graft_entry__.build()
     monkeypatch.setattr(waits, "KERNELS", ("w4_tile_kernel",))
     kernels = waits.tile_kernels(waits.LIB, tmp_path)
-    # five tiles, three group classes, with and without zero points; three tiles for groups loaded one by one
-    assert len(kernels) == 5 * 3 * 2 + 3 * 2 * 2
+    # six tiles, three group classes, with and without zero points; three tiles for groups loaded one by one
+    assert len(kernels) == 6 * 3 * 2 + 3 * 2 * 2
     for name, bb in kernels.items():
         bm = int(re.search(r"w4_tile_kernelILi(\d+)E", name).group(1))
         first = min(bb)
