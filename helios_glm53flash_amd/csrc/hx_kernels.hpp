@@ -93,7 +93,7 @@ struct W4Args {
 size_t w4_gemm_workspace_bytes(int M, int N, int K);
 hipError_t launch_w4_gemm(const _Float16* x, const W4Args& a, void* y, int M, bool y_fp32, void* ws, size_t ws_bytes,
                           hipStream_t st);
-hipError_t launch_w4_embed(const W4Args& a, const int64_t* tokens, void* out, long n, float scale, bool out_fp32,
+hipError_t launch_w4_embed(const W4Args& a, const int64_t* tokens, void* out, int n, float scale, bool out_fp32,
                            hipStream_t st);
 
 // beam search's selection and reordering of states (hx_beam.hip)

@@ -508,28 +508,27 @@ __global__ __launch_bounds__(256 * KS) void w4_tile_kernel(const _Float16* x, W4
 }
 
 // out[t][k] = scale * weight(tokens[t], k), the product in fp32 and rounded once; zeros for a token outside [0, N).
-// One thread per word: 8 consecutive outputs.
+// One thread per word: 8 consecutive outputs.  total: words, below 2^31, so that a division of 32 bits finds the row.
 template <typename T>
-__global__ __launch_bounds__(256) void w4_embed_kernel(W4Args a, const int64_t* tokens, T* out, long n, float scale)
+__global__ __launch_bounds__(256) void w4_embed_kernel(W4Args a, const int64_t* tokens, T* out, uint32_t total, float scale)
 {
     typedef T v8 __attribute__((ext_vector_type(8)));
-    const int nw = (a.K + 127) / 128 * 16;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n * nw; i += (long)gridDim.x * 256) {
-        const long t = i / nw;
-        const int w = (int)(i % nw), k = word_k(w);
-        if (k >= a.K) continue;
-        const int64_t row = tokens[t];
-        v8 o = {};
-        if (row >= 0 && row < a.N) {
-            const size_t g = (size_t)row * a.groups + (k >> a.group_log2);
-            float v[8];
-            word_values(a.words[(size_t)row * nw + w], a.zeros ? (float)a.zeros[g] : 8.0f, v);
-            const float s = (float)a.scales[g] * scale;
+    const uint32_t nw = (uint32_t)(a.K + 127) / 128 * 16, i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;
+    const uint32_t t = i / nw, w = i % nw;
+    const int k = word_k((int)w);
+    if (k >= a.K) return;
+    const int64_t row = tokens[t];
+    v8 o = {};
+    if (row >= 0 && row < a.N) {
+        const size_t g = (size_t)row * a.groups + (k >> a.group_log2);
+        float v[8];
+        word_values(a.words[(size_t)row * nw + w], a.zeros ? (float)a.zeros[g] : 8.0f, v);
+        const float s = (float)a.scales[g] * scale;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) o[j] = (T)(s * v[j]);
-        }
-        *reinterpret_cast<v8*>(out + (size_t)t * a.K + k) = o;
+        for (int j = 0; j < 8; ++j) o[j] = (T)(s * v[j]);
     }
+    *reinterpret_cast<v8*>(out + (size_t)t * a.K + k) = o;
 }
 
 namespace {
@@ -715,17 +714,22 @@ hipError_t launch_w4_gemm(const _Float16* x, const W4Args& a, void* y, int M, bo
     return hipSuccess;
 }
 
-hipError_t launch_w4_embed(const W4Args& a, const int64_t* tokens, void* out, long n, float scale, bool out_fp32,
+hipError_t launch_w4_embed(const W4Args& a, const int64_t* tokens, void* out, int n, float scale, bool out_fp32,
                            hipStream_t st)
 {
     if (n <= 0) return hipSuccess;
-    const long work = n * ((a.K + 127) / 128 * 16);
-    const dim3 grid((unsigned)((work + 255) / 256 < 65536 ? (work + 255) / 256 : 65536));
-    if (out_fp32)
-        hipLaunchKernelGGL((w4_embed_kernel<float>), grid, dim3(256), 0, st, a, tokens, static_cast<float*>(out), n, scale);
-    else
-        hipLaunchKernelGGL((w4_embed_kernel<_Float16>), grid, dim3(256), 0, st, a, tokens, static_cast<_Float16*>(out), n,
-                           scale);
+    const int nw = (a.K + 127) / 128 * 16, most = (int)((1u << 31) / nw) - 1;  // rows of a launch
+    for (int t = 0; t < n; t += most) {
+        const uint32_t total = (uint32_t)(n - t < most ? n - t : most) * nw;
+        const dim3 grid((total + 255) / 256);
+        if (out_fp32)
+            hipLaunchKernelGGL((w4_embed_kernel<float>), grid, dim3(256), 0, st, a, tokens + t,
+                               static_cast<float*>(out) + (size_t)t * a.K, total, scale);
+        else
+            hipLaunchKernelGGL((w4_embed_kernel<_Float16>), grid, dim3(256), 0, st, a, tokens + t,
+                               static_cast<_Float16*>(out) + (size_t)t * a.K, total, scale);
+        if (n - t <= most) break;
+    }
     return hipGetLastError();
 }
 

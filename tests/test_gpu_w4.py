@@ -265,17 +265,18 @@ def test_embed(w4, T, K, N, group, zeros, fp32):
     check_guard(whole)
 
 
-@pytest.mark.parametrize("n,K", [(1_200_000, 32), (540_000, 8192)])
+@pytest.mark.parametrize("n,K", [(1_200_000, 32), (540_000, 8192), (140_000_000, 32)])
 def test_embed_many_tokens(w4, n, K):
-    """More words than threads of a launch; an output of more than 2^32 elements."""
+    """Several launches (2^31 words each); an output of more than 2^32 elements."""
     import torch
     q, s, z, w = make(5, 50, K, 32, True, exact=True)
     tok = torch.randint(0, 50, (n,), device="cuda")
     out = torch.full((n, K), 99.0, dtype=torch.float16, device="cuda")
     w4.embed(words(w4, q, s, z, K, 32), tok, out, n)
     table = dev(w.astype(np.float16))
-    for a in range(0, n, 60_000):
-        assert torch.equal(out[a:a + 60_000], table[tok[a:a + 60_000]])
+    part = 500_000_000 // K
+    for a in range(0, n, part):
+        assert torch.equal(out[a:a + part], table[tok[a:a + part]])
 
 
 def test_gemm_large_batches(w4):
