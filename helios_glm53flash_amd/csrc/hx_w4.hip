@@ -555,20 +555,13 @@ struct W4Tile {
 constexpr W4Tile W4_TILES[] = {{16, 1, 2}, {32, 1, 2}, {64, 1, 2}, {64, 2, 1}, {64, 2, 2}, {128, 2, 1}};  // TILE16 ..
 constexpr int W4_SLOTS = 256;  // workgroups that splitting fills the chip with, one per CU
 
-W4Plan w4_tile_plan(int kind, int M, int N, int K, bool split)
+W4Plan w4_tile_plan(int kind, int M, int N, int K, int splits)
 {
     const W4Tile t = W4_TILES[kind - W4Plan::TILE16];
-    W4Plan p{(W4Plan::Kind)kind, 1, (K + 128 * t.ks - 1) / (128 * t.ks), 0};
+    const int steps = (K + 128 * t.ks - 1) / (128 * t.ks);
+    W4Plan p{(W4Plan::Kind)kind, 1, (steps + splits - 1) / splits, 0};
+    p.splits = (steps + p.steps - 1) / p.steps;
     p.tiles = ((long)M + t.bm - 1) / t.bm * (((long)N + 64 * t.nt - 1) / (64 * t.nt));
-    // K is split while that fills idle CUs and leaves each split 4 steps: 64 rows, 16384 -> 4096, 41 us unsplit, 21.5 in 4; 8192
-    // -> 4096 25 and 14.4; 32 rows of the former 27 and 16.
-    if (split && t.nt == 1) {
-        const int most = (int)(W4_SLOTS / p.tiles) < p.steps / 4 ? (int)(W4_SLOTS / p.tiles) : p.steps / 4;
-        if (most > 1) {
-            p.steps = (p.steps + most - 1) / most;
-            p.splits = ((K + 128 * t.ks - 1) / (128 * t.ks) + p.steps - 1) / p.steps;
-        }
-    }
     return p;
 }
 
@@ -587,28 +580,32 @@ W4Plan w4_plan(int M, int N, int K, int gs, bool split, bool pieces)
         const W4Plan::Kind kind = N < 4096 && K >= 4096 ? W4Plan::ROWS8_FEW : N > 8192 && gs < 4 ? W4Plan::ROWS8_WIDE : W4Plan::ROWS8;
         return {pieces ? kind : W4Plan::ROWS8, 1, 0, 0};
     }
-    if (M <= 16) return w4_tile_plan(W4Plan::TILE16, M, N, K, split);
-    if (M <= 32) return w4_tile_plan(W4Plan::TILE32, M, N, K, split);
-    // A step of a tile, in us, where there is less than one workgroup for two CUs, where there is one per CU, and per workgroup where
-    // there are more; how much longer groups of 32 with zero points take.  Of 42 shapes (64 to 256 rows) the choice is 0.5 %
-    // slower than the best each time, and 5 % at most.
+    // A step of a tile, in us, where there is at most one workgroup for two CUs, where there is one per CU, and per workgroup where
+    // there are more; how much longer groups of 32 with zero points take.  K is split among workgroups of the tiles with one
+    // column group per wave where CUs are idle.  64 rows, 64-row tiles: 16384 -> 4096 41 us unsplit, 21.5 in 4; 8192 -> 4096 25 and 14.7.
+    // 64 rows of 2048 -> 8192 9.1 us in tiles of 64, 7.8 of 32; 128 rows of 4096 -> 12288 32 us in tiles of 64, 28 and 24 in the two of 64 x
+    // 128, 34 of 128; 256 rows of 4096 -> 32768 122, 83, 93 and 70 us.
     struct Cost {
         int kind;
         float few, one, more, fine;
     };
-    constexpr Cost cost[] = {{W4Plan::TILE64, 0.68f, 0.86f, 0.92f, 1.2f},
-                             {W4Plan::TILE64W, 0.56f, 0.77f, 0.62f, 1.4f},
-                             {W4Plan::TILE64W2, 1.15f, 1.32f, 1.4f, 1.42f},
-                             {W4Plan::TILE128, 0.96f, 1.36f, 1.03f, 1.25f}};
+    constexpr Cost cost[] = {{W4Plan::TILE16, 0.35f, 0.45f, 0.51f, 1.25f}, {W4Plan::TILE32, 0.43f, 0.56f, 0.62f, 1.25f},
+                             {W4Plan::TILE64, 0.68f, 0.86f, 0.92f, 1.2f},  {W4Plan::TILE64W, 0.56f, 0.77f, 0.62f, 1.4f},
+                             {W4Plan::TILE64W2, 1.15f, 1.32f, 1.4f, 1.42f}, {W4Plan::TILE128, 0.96f, 1.36f, 1.03f, 1.25f}};
     W4Plan best{};
-    float least = 0.0f;
+    float least = 1e30f;
     for (const Cost& c : cost) {
-        if (c.kind != W4Plan::TILE64 && (!pieces || (M <= 64 && c.kind == W4Plan::TILE128))) continue;
-        const W4Plan p = w4_tile_plan(c.kind, M, N, K, split);
-        const long n = p.tiles * p.splits;
-        const float step = n <= 128 ? c.few : n <= 256 ? c.one : (float)((n + 255) / 256) * c.more;
-        const float t = p.steps * step * (gs == 4 ? c.fine : gs == 2 ? 0.5f + 0.5f * c.fine : 1.0f) + (p.splits > 1 ? 1.5f : 0.0f);
-        if (c.kind == W4Plan::TILE64 || t < least) least = t, best = p;
+        const W4Tile t = W4_TILES[c.kind - W4Plan::TILE16];
+        if ((c.kind == W4Plan::TILE16 ? M > 16 : M <= t.bm / 2) || (t.nt > 1 && !pieces)) continue;
+        for (int splits = 1; splits <= (split && t.nt == 1 ? 8 : 1); splits *= 2) {
+            const W4Plan p = w4_tile_plan(c.kind, M, N, K, splits);
+            const long n = p.tiles * p.splits;
+            if (splits > 1 && (n > W4_SLOTS || p.steps < 2)) break;
+            const float step = n <= W4_SLOTS / 2 ? c.few : n <= W4_SLOTS ? c.one : (float)((n + W4_SLOTS - 1) / W4_SLOTS) * c.more;
+            const float join = splits > 1 ? 0.6f + (float)splits * (0.55f + 0.005f * (float)t.bm) : 0.0f;
+            const float us = (float)p.steps * step * (gs == 4 ? c.fine : gs == 2 ? 0.5f + 0.5f * c.fine : 1.0f) + join;
+            if (us < least) least = us, best = p;
+        }
     }
     return best;
 }
