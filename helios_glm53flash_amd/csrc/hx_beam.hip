@@ -16,6 +16,10 @@
 // The n largest of a set spread over threads, without sorting it: the n-th largest of the threads' maxima is a lower bound of
 // the n-th largest of all, and only what reaches it (n to 2n of random elements) is ranked.  The bound is renewed after 1, 2,
 // 4, .. pieces.
+//
+// 4 rows of 151552 fp32 logits, n = 8: 14 us, a chain of latencies beside 0.5 us of traffic (of a single launch traced at 17.7 us the last
+// chunk arrives at 7, after a piece's load, 1.7, and a bound, 1.1; the merge takes the rows' sums 3, the candidates 2.7, a bound 2.2
+// and their ranking 1.8).  256 rows in fp16, n = 16, some finished: 31 us, 2.5 TB/s, of which the reading is 18.
 #include "hx_gemv.hpp"
 #include "hx_kernels.hpp"
 
@@ -668,7 +672,8 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(const char* src, cons
 
 namespace {
 
-// Few large pieces are divided among workgroups, 8 per CU in all, into no less than one access per thread.
+// Few large pieces are divided among workgroups, 8 per CU in all, into no less than one access per thread: 4 pieces of 64 MiB 111 us, 4.9
+// TB/s, undivided 6980; 32 of 8 MiB 110 and 920.  A cache's pieces (42 layers of 32 rows, 3.1 GB both ways) 550 us, 5.6 TB/s.
 template <typename V>
 hipError_t reorder_launch(const char* src, const int64_t* parents, char* dst, const ReorderArgs& p, hipStream_t st)
 {

@@ -8,9 +8,9 @@
 // consecutive 32-k matrix instructions (lane group g of each holds 8 consecutive k): no group of 32 k and more spans two
 // instructions, whatever its size.
 //
-//   M <= 64  w4_rows_kernel: the waves of a workgroup split K and keep their part of x in registers; they walk over the
-//            weight rows, every word read once, and add their sums through LDS.
-//   M > 64   w4_tile_kernel: tiles of 128 (or 64) x 128 outputs, x through LDS, the words straight into operands.
+//   M <= 8  w4_rows_kernel: the waves of a workgroup split K and keep their part of x in registers; they walk over the
+//           weight rows, every word read once, and add their sums through LDS.
+//   M > 8   w4_tile_kernel: tiles of 16 to 128 by 64 or 128 outputs, x through LDS, the words straight into operands.
 #include "hx_mfma.hpp"
 #include "hx_kernels.hpp"
 
@@ -176,6 +176,9 @@ HX_INLINE void store_y(void* y, size_t i, float v, bool y_fp32)
 // A wave owns NS spans (S blocks each) of every WK NS, keeps x for them in registers and goes over tiles of NT R rows; each word
 // is replaced by the next tile's as soon as it is decoded.  Per group the products are summed by the matrix
 // instructions from zero, then scaled into the fp32 sums.
+// Bound by memory where the weights are many: 8 rows of 4096 -> 151552 in groups of 128 take 66 us, 4.9 TB/s (a copy of 4 GiB runs at 4.8).
+// Of the 8.0 us of one row of 4096 -> 12288 (26 MB, 5.4 us) and the 8.8 of five of 8192 -> 4096 in groups of 32 (20 MB, 4.2 us) about
+// 4 are launch and the first load's latency, which a call of 4 MB also takes.
 template <int S, int WAVES, int NS, int NT, int GS, bool Z, bool V>
 __device__ __forceinline__ void w4_rows(const _Float16* x, const W4Args& a, void* y, int M, bool y_fp32, int wk)
 {
@@ -295,6 +298,10 @@ __global__ __launch_bounds__(64 * WAVES) void w4_rows_kernel(const _Float16* x, 
 // with an LDS destination (256 consecutive bytes of a row); 16-byte piece u of row m lies at piece u ^ (m & 15), so the 16
 // rows of a fragment read touch all banks.  The words go from memory into registers, as many steps ahead, and become operands
 // there: no wave decodes a weight that another wave of the workgroup uses.
+// With few rows the address unit is the busiest (70 % of a step of 64 x 64 outputs by 256 k in groups of 64: x takes 512 of its 1900 cycles,
+// the words 264, scales and zero points 248), the VALU half as much: 45 rows of 4096 -> 12288 15.5 us, 29 MB.  With many it is the
+// matrix instructions at what clock the power limit leaves (1.7 GHz, 52 % busy): 2000 rows of 4096 -> 24576 in groups of 128
+// 383 us, 1.05 PFLOP/s, where the library's fp16 product of 8192^3 runs at 1.26.
 struct W4Split {
     int splits, steps;  // workgroups that share a tile's K, steps of each
     hx_f4* partial;     // [tiles][splits][RB][NT][4][64]
@@ -508,7 +515,8 @@ __global__ __launch_bounds__(256 * KS) void w4_tile_kernel(const _Float16* x, W4
 }
 
 // out[t][k] = scale * weight(tokens[t], k), the product in fp32 and rounded once; zeros for a token outside [0, N).
-// One thread per word: 8 consecutive outputs.  total: words, below 2^31, so that a division of 32 bits finds the row.
+// One thread per word: 8 consecutive outputs.  total: words, below 2^31, so that a division of 32 bits finds the row.  Memory
+// bound: 20000 rows of 4096 43 us, 4.8 TB/s; 2000 6.5 us, of which launch and latency are 2.5.
 template <typename T>
 __global__ __launch_bounds__(256) void w4_embed_kernel(W4Args a, const int64_t* tokens, T* out, uint32_t total, float scale)
 {
