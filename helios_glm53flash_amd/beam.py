@@ -30,7 +30,7 @@ def select(logits: torch.Tensor, cum: torch.Tensor, done: Optional[torch.Tensor]
     beam * vocab + token first among equals, into scores (fp32), parents (beam within the sequence) and tokens (int64),
     each [batch][n].  logits [batch * beams][>= vocab] fp16 or fp32, rows at any stride >= vocab; cum fp32 [batch * beams]; done
     (uint8 or bool, optional) marks finished beams, which go on with eos at an unchanged score.  Forbidden tokens have logit
-    -inf, dead beams cum -inf; places that no candidate fills get -inf, -1, -1."""
+    -inf, dead beams cum -inf; places that no candidate fills get -inf, -1, -1.  scores may be cum itself where n == beams."""
     if not isinstance(logits, torch.Tensor) or logits.dtype not in _DTYPES or not logits.is_cuda or logits.dim() != 2:
         raise ValueError("select: logits must be a 2-d float16 or float32 device tensor")
     rows = batch * beams

@@ -571,6 +571,9 @@ int hx_beam_select(const void* logits, const float* cum, const uint8_t* done, fl
     if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)
         return fail(HX_ERR_WORKSPACE, "hx_beam_select: workspace missing, not 16-byte aligned or smaller than "
                                       "hx_beam_select_workspace_size");
+    // a sequence's scores are written when its cum has been read, so scores may take cum's place where they lie alike
+    if ((scores != cum || n != beams) && scores < cum + (size_t)batch * beams && cum < scores + (size_t)batch * n)
+        return fail(HX_ERR_INVALID, "hx_beam_select: scores and cum overlap");
     const hx::BeamArgs a{cum, done, scores, parents, tokens, (long)ld, batch, beams, vocab, n, eos};
     return hip_status(hx::launch_beam_select(logits, dtype == HX_DTYPE_FLOAT, a, workspace, (hipStream_t)stream),
                       "hx_beam_select");

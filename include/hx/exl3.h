@@ -266,6 +266,7 @@ int hx_w4_embed(const hx_w4_words* w, const int64_t* tokens, void* out, int n, i
  * lowest w * vocab + v first among equal scores; fp32 scores rounded once from 64 bits.  A beam with done != 0 (done may be
  * NULL) has the one candidate (w, eos) with score cum.  A logit of -inf is no candidate; a beam whose cum is not finite, whose
  * logits hold a NaN or +inf, or are all -inf, has none.  Places without a candidate get score -inf, parent -1, token -1.
+ * scores may be cum itself where n == beams; otherwise outputs and inputs may not overlap.
  * batch <= 4096, beams <= 1024, vocab <= 2^30, n <= 128.  batch == 0 is a no-op. */
 size_t hx_beam_select_workspace_size(int batch, int beams, int vocab, int n);
 int hx_beam_select(const void* logits, const float* cum, const uint8_t* done, float* scores, int64_t* parents,

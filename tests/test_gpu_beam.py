@@ -197,6 +197,35 @@ def test_select_many_rows(beam, dtype, batch, beams, V, n):
     check(beam, x, cum, None, batch, beams, V, n)
 
 
+def test_select_large_vocabulary(beam):
+    """300 million tokens: places next to both ends and around multiples of the pieces that workgroups read."""
+    import torch
+    V, n = 300_000_001, 12
+    x = torch.zeros((1, V), dtype=torch.float16, device="cuda")
+    at = [0, 1, 4095, 4096, (1 << 28) - 1, 1 << 28, V - 1, V - 2, 299_999_232, 123_456_789, 4096 * 5000, 7]
+    for i, a in enumerate(at):
+        x[0, a] = 12.0 - i * 0.5
+    s, p, t = (torch.empty((1, n), dtype=d, device="cuda") for d in (torch.float32, torch.int64, torch.int64))
+    beam.select(x, torch.zeros(1, device="cuda"), None, s, p, t, 1, 1, V, n)
+    assert t[0].tolist() == at and bool((p == 0).all())
+    v = 12.0 - 0.5 * np.arange(n)
+    lse = np.log(np.exp(v).sum() + (V - n))
+    # a thread adds some thousand exponentials of fp32: a relative error of 4096 x 2^-24 at most
+    assert (np.abs(s[0].cpu().numpy() - (v - lse)) <= 2.5e-4).all()
+
+
+def test_select_scores_in_place_of_cum(beam):
+    import torch
+    batch, beams, V = 5, 6, 20000
+    x = torch.randn((batch * beams, V), device="cuda") * 3
+    cum = -torch.rand((batch, beams), device="cuda")
+    want = [torch.empty((batch, beams), dtype=d, device="cuda") for d in (torch.float32, torch.int64, torch.int64)]
+    got = [torch.empty_like(o) for o in want]
+    beam.select(x, cum, None, *want, batch, beams, V, beams)
+    beam.select(x, cum, None, cum, *got[1:], batch, beams, V, beams)
+    assert torch.equal(cum, want[0]) and all(torch.equal(a, b) for a, b in zip(got[1:], want[1:]))
+
+
 def test_select_padded_and_strided_rows(beam):
     """Rows at a stride beyond the vocabulary, starting at any element: what lies between them is never read into a result."""
     import torch

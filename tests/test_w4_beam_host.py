@@ -162,3 +162,8 @@ def test_extents_beyond_a_call():
     assert LIB.hx_w4_gemm_workspace_size((1 << 31) - 1, 64, 128) == 0
     assert LIB.hx_w4_gemm_workspace_size(64, 4096, (1 << 31) - 1) == 0
     assert LIB.hx_beam_select_workspace_size(1, 1, (1 << 31) - 1, 8) == 0
+
+
+@pytest.mark.parametrize("kw", [dict(scores=16), dict(scores=28, n=4), dict(scores=4, n=4, beams=4), dict(scores=16, n=3, beams=4)])
+def test_select_refuses_overlapping_scores(kw):
+    assert select(**{"cum": 16, "n": 8, **kw}) == _lib.HX_ERR_INVALID and "overlap" in err()
