@@ -34,10 +34,13 @@ def select(logits: torch.Tensor, cum: torch.Tensor, done: Optional[torch.Tensor]
     if not isinstance(logits, torch.Tensor) or logits.dtype not in _DTYPES or not logits.is_cuda or logits.dim() != 2:
         raise ValueError("select: logits must be a 2-d float16 or float32 device tensor")
     rows = batch * beams
-    if batch < 0 or beams < 1 or vocab < 1 or n < 1 or logits.shape[0] < rows or logits.shape[1] < vocab:
+    height, width = logits.shape
+    if batch < 0 or beams < 1 or vocab < 1 or n < 1 or height < rows or width < vocab:
         raise ValueError("select: logits smaller than [batch * beams][vocab]")
-    ld = logits.stride(0) if logits.shape[0] > 1 else max(vocab, logits.stride(0))
-    if vocab > 1 and logits.stride(1) != 1 or ld < vocab:
+    ld, step = logits.stride()
+    if height < 2:
+        ld = max(vocab, ld)
+    if vocab > 1 and step != 1 or ld < vocab:
         raise ValueError("select: the logits of a row must be consecutive and rows must not overlap")
     _need(cum, "cum", (torch.float32,))
     _need(scores, "scores", (torch.float32,))
@@ -47,7 +50,8 @@ def select(logits: torch.Tensor, cum: torch.Tensor, done: Optional[torch.Tensor]
         _need(done, "done", (torch.uint8, torch.bool))
         if done.numel() < rows:
             raise ValueError("select: done smaller than batch * beams")
-    if cum.numel() < rows or min(scores.numel(), parents.numel(), tokens.numel()) < batch * n:
+    places = batch * n
+    if cum.numel() < rows or scores.numel() < places or parents.numel() < places or tokens.numel() < places:
         raise ValueError("select: cum / outputs smaller than batch * beams / batch * n")
     _on_one_device(logits, cum, done, scores, parents, tokens)
     st = _stream(stream)

@@ -16,8 +16,9 @@ from typing import Optional
 import torch
 
 from ._lib import W4WordsC, check, lib
-from .exl3 import _GEMM_EXTRA, _get_device, _need, _ptr, _stream, workspace
+from .exl3 import _GEMM_EXTRA, _get_device, _need, _ptr, _stream, _workspaces, workspace
 
+_is_capturing = torch._C._cuda_isCurrentStreamCapturing
 COUNTER_BYTES = 64 * 1024  # arrival counters at the start of a workspace
 _NIBBLE_K = (0, 2, 4, 6, 1, 3, 5, 7)  # the k of an octet that each nibble of its word holds, lowest nibble first
 
@@ -111,13 +112,16 @@ def _gemm_workspace_bytes(M: int, N: int, K: int) -> int:
 def call_workspace(nbytes: int, device: torch.device, st: int) -> torch.Tensor:
     """A call's workspace on stream st: the stream's own one, or, where it is being captured, memory of the
     graph's with counters that each replay clears, so that the graph depends on no buffer that a later call may replace."""
-    if torch.cuda.is_current_stream_capturing():
+    if _is_capturing():
         here = st == _stream(None)
         with nullcontext() if here else torch.cuda.stream(torch.cuda.ExternalStream(st, device=device)):
             if here or torch.cuda.is_current_stream_capturing():  # another stream may have been forked into the capture
                 ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
                 ws[:COUNTER_BYTES].zero_()
                 return ws
+    ws = _workspaces.get((_get_device(), st))
+    if ws is not None and ws.numel() >= nbytes:
+        return ws
     # the bytes behind every workspace, which hold a linear's splits, are enough here too
     return workspace(max(0, nbytes - _GEMM_EXTRA), device, st)
 
