@@ -49,8 +49,9 @@ HX_INLINE uint32_t div_by(uint32_t i, FastDiv f)
     return q * (u64)f.d > i ? q - 1 : q;
 }
 
-// The n-th largest of 64 P keys in LDS, for one wave (0 where fewer than n are above 0): the key's bits from the top, two at a time,
-// each pair as large as still leaves n keys at or above the value.
+// A lower bound of the n-th largest of 64 P keys in LDS, for one wave (0 where fewer than n are above 0): the key's 20 high bits from the
+// top, two at a time, each pair as large as still leaves n keys at or above the value, then the least of the keys that reach it (equal
+// keys give their own value).  Keys above 0 are no less than KEY_NEG_INF.
 template <int P>
 HX_INLINE uint32_t nth_largest(const uint32_t* keys, int n)
 {
@@ -59,7 +60,7 @@ HX_INLINE uint32_t nth_largest(const uint32_t* keys, int n)
 #pragma unroll
     for (int p = 0; p < P; ++p) k[p] = keys[64 * p + lane];
     uint32_t t = 0;
-    for (int bit = 30; bit >= 0; bit -= 2) {
+    for (int bit = 30; bit >= 12; bit -= 2) {
         int count[4] = {};
 #pragma unroll
         for (int d = 1; d < 4; ++d)
@@ -67,7 +68,10 @@ HX_INLINE uint32_t nth_largest(const uint32_t* keys, int n)
             for (int p = 0; p < P; ++p) count[d] += __popcll(__ballot(k[p] >= (t | (uint32_t)d << bit)));
         t |= (uint32_t)(count[3] >= n ? 3 : count[2] >= n ? 2 : count[1] >= n ? 1 : 0) << bit;
     }
-    return t;
+    uint32_t most = 0;
+#pragma unroll
+    for (int p = 0; p < P; ++p) most = max(most, k[p] >= t ? ~k[p] : 0u);
+    return t ? ~hx_wave_max_u32(most) : 0u;
 }
 
 // Lower bound of the n-th largest of all elements from the threads' largest keys (0: none): the n-th largest of the 256, or for
@@ -106,6 +110,38 @@ HX_INLINE float wave_sum(float v)
     add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // row_bcast:15
     add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // row_bcast:31
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
+// Over groups of g lanes (a power of two), every lane gets the result: partners by lane permutations up to 16 lanes, then rows swapped.
+template <typename T, typename F>
+HX_INLINE T group_reduce(T v, int g, F f)
+{
+    struct Words {
+        uint32_t w[sizeof(T) / 4];
+    };
+    auto with = [&](auto ctrl) {
+        Words a = __builtin_bit_cast(Words, v);
+#pragma unroll
+        for (uint32_t& x : a.w) x = (uint32_t)__builtin_amdgcn_mov_dpp((int)x, decltype(ctrl)::value, 0xf, 0xf, true);
+        v = f(v, __builtin_bit_cast(T, a));
+    };
+    auto swapped = [&](auto half) {  // 32 lanes or rows of 16: the two results are the two sides, in all lanes
+        Words a = __builtin_bit_cast(Words, v), b;
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(T) / 4); ++i) {
+            const auto r = decltype(half)::value ? __builtin_amdgcn_permlane32_swap(a.w[i], a.w[i], false, false)
+                                                 : __builtin_amdgcn_permlane16_swap(a.w[i], a.w[i], false, false);
+            a.w[i] = r[0], b.w[i] = r[1];
+        }
+        v = f(__builtin_bit_cast(T, a), __builtin_bit_cast(T, b));
+    };
+    if (g > 1) with(std::integral_constant<int, 0xb1>{});   // quad_perm 1 0 3 2
+    if (g > 2) with(std::integral_constant<int, 0x4e>{});   // quad_perm 2 3 0 1
+    if (g > 4) with(std::integral_constant<int, 0x141>{});  // row_half_mirror
+    if (g > 8) with(std::integral_constant<int, 0x140>{});  // row_mirror
+    if (g > 16) swapped(std::integral_constant<int, 0>{});
+    if (g > 32) swapped(std::integral_constant<int, 1>{});
+    return v;
 }
 
 struct BeamPlan {
@@ -425,19 +461,25 @@ HX_INLINE void select_merge(const BeamArgs& a, const BeamPlan& p, long b, char* 
     __shared__ uint32_t keys[SEL_THREADS];
     __shared__ Cand carry[BEAM_MAX_N];  // the best so far
     __shared__ Cand best[4];
-    __shared__ int count;
+    __shared__ int count, wanted[2][4];  // wanted: by round and wave
     double* offset = reinterpret_cast<double*>(lds);
     float* tops = reinterpret_cast<float*>(offset + a.beams);  // NaN: the beam is finished
     Cand* cand = reinterpret_cast<Cand*>(lds + ((size_t)a.beams * 12 + 15) / 16 * 16);
     const int tid = threadIdx.x, lane = tid & 63, n = a.n, total = n * p.lists;
     const __amdgpu_buffer_rsrc_t rs = coherent_rsrc(p.stats + (size_t)b * p.lists);
     const __amdgpu_buffer_rsrc_t re = coherent_rsrc(p.entries + (size_t)b * n * p.lists);
-    u64 e[MERGE_E];  // the first round's entries come while the rows' sums are formed
+    // A round takes the same number of entries beside the best so far, so that the next one's are on their way in each; the first
+    // round's come while the rows' sums are formed.
+    u64 e[MERGE_E];
+    auto load = [&](int at) {
+        const int fresh = min(total - at, MERGE - n);
 #pragma unroll
-    for (int i = 0; i < MERGE_E; ++i) {
-        const int q = i * SEL_THREADS + tid;
-        e[i] = q < total ? coherent_load8(re, q * 8) : 0;
-    }
+        for (int i = 0; i < MERGE_E; ++i) {
+            const int q = i * SEL_THREADS + tid;
+            e[i] = q < fresh ? coherent_load8(re, (at + q) * 8) : 0;
+        }
+    };
+    load(0);
     // score = offset[w] + (logit - tops[w]); offset NaN: the row has no candidates.  g lanes per row, a chunk each (further ones
     // by running maximum and sum).
     int g = 1;
@@ -460,32 +502,25 @@ HX_INLINE void select_merge(const BeamArgs& a, const BeamPlan& p, long b, char* 
                 m = top;
             }
         }
-        float top = m;
-        for (int o = g / 2; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+        const float top = group_reduce(m, g, [](float x, float y) { return fmaxf(x, y); });
         if (m != top) s *= exp((double)m - (double)top);
-        for (int o = g / 2; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+        s = group_reduce(s, g, [](double x, double y) { return x + y; });
         if (mine && tid % g == 0) {
             double off = NAN;
             if (!(fabsf(cum) < INFINITY)) {
             } else if (fin) {
-                off = (double)cum, top = NAN;
+                off = (double)cum;
             } else if (fabsf(top) < INFINITY && s < INFINITY) {  // a NaN fails both tests
                 off = (double)cum - log(s);
             }
-            offset[w] = off, tops[w] = top;
+            offset[w] = off, tops[w] = fin ? NAN : top;
         }
     }
     int kept = 0, nothing = 0;  // entries of carry; entries in a row that were no better than those
     hx_lds_barrier();
-    for (int at = 0; at < total;) {
-        const int fresh = min(total - at, MERGE - kept);
+    for (int at = 0, round = 0; at < total; ++round) {
+        const int fresh = min(total - at, MERGE - n);
         Cand v[MERGE_E];
-        if (at > 0)
-#pragma unroll
-            for (int i = 0; i < MERGE_E; ++i) {
-                const int q = i * SEL_THREADS + tid;
-                e[i] = q < fresh ? coherent_load8(re, (at + q) * 8) : 0;
-            }
         const Cand last_kept = kept == n ? carry[n - 1] : Cand{-INFINITY, ~0ull};
         double most = -INFINITY;
         bool any = false;  // an entry that would be among the n best so far
@@ -513,7 +548,14 @@ HX_INLINE void select_merge(const BeamArgs& a, const BeamPlan& p, long b, char* 
             most = fmax(most, v[i].s);
         }
         at += fresh;
-        if (!__syncthreads_or(any)) {
+        if (at < total) load(at);
+        // so few that ranking them all costs less than a bound (1.5 us)
+        const bool few = total <= 128;
+        const u64 ask = __ballot(any);
+        if (lane == 0) wanted[round & 1][tid >> 6] = ask != 0;
+        hx_lds_barrier();
+        const int* asked = wanted[round & 1];
+        if (!(asked[0] | asked[1] | asked[2] | asked[3])) {
             // Every list is in descending order and the r-th entries of all lists come before the r+1-st: once an entry of each
             // list in turn was no better, none behind them is.
             nothing += fresh;
@@ -523,7 +565,8 @@ HX_INLINE void select_merge(const BeamArgs& a, const BeamPlan& p, long b, char* 
         nothing = 0;
         if (tid == 0) count = 0;
         // scores rounded to fp32 keep their order (not strictly): the bound holds for the rounded ones
-        const uint32_t bound = bound_of(most > -INFINITY ? float_key((float)most) : 0, n, keys);
+        if (few) hx_lds_barrier();  // count
+        const uint32_t bound = few ? 0 : bound_of(most > -INFINITY ? float_key((float)most) : 0, n, keys);
         if (most > -INFINITY && float_key((float)most) >= bound) {
 #pragma unroll
             for (int i = 0; i < MERGE_E; ++i)
