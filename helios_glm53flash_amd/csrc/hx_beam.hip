@@ -480,30 +480,34 @@ HX_INLINE void select_merge(const BeamArgs& a, const BeamPlan& p, long b, char* 
         }
     };
     load(0);
-    // score = offset[w] + (logit - tops[w]); offset NaN: the row has no candidates.  g lanes per row, a chunk each (further ones
-    // by running maximum and sum).
+    // score = offset[w] + (logit - tops[w]); offset NaN: the row has no candidates.  g lanes per row, as many as take all rows at once
+    // (16 rows of 37 chunks, 32 candidates: 24 us, 28 with 64 lanes a row); first the maxima, then the sums relative to the row's.
     int g = 1;
-    while (g < 64 && g < p.chunks) g *= 2;
+    while (g < 64 && g < p.chunks && 2 * g * a.beams <= SEL_THREADS) g *= 2;
     for (int w0 = 0; w0 < a.beams; w0 += SEL_THREADS / g) {
         const int w = w0 + tid / g;
         const bool mine = w < a.beams;
         const float cum = mine ? a.cum[b * a.beams + w] : NAN;
         const bool fin = mine && a.done && a.done[b * a.beams + w];
-        float m = -INFINITY;
-        double s = 0.0;
         // of finished and dead rows: whatever is there
-        for (int c = tid % g; mine && c < p.chunks; c += g) {
-            const float2 st = __builtin_bit_cast(float2, coherent_load8(rs, (w * p.chunks + c) * 8));
-            if (c < g) {
-                m = st.x, s = (double)st.y;
-            } else {
-                const float top = fmaxf(m, st.x);
-                s = s * exp((double)m - (double)top) + (double)st.y * exp((double)st.x - (double)top);
-                m = top;
-            }
-        }
+        auto chunk = [&](int c) {
+            float2 st = {-INFINITY, 0.0f};
+            if (mine && c < p.chunks) st = __builtin_bit_cast(float2, coherent_load8(rs, (w * p.chunks + c) * 8));
+            return st;
+        };
+        float2 st = chunk(tid % g);
+        float m = st.x;
+#pragma unroll 4
+        for (int c = tid % g + g; c < p.chunks; c += g) m = fmaxf(m, chunk(c).x);
         const float top = group_reduce(m, g, [](float x, float y) { return fmaxf(x, y); });
-        if (m != top) s *= exp((double)m - (double)top);
+        double s = 0.0;
+        for (int c = tid % g; c < p.chunks; c += g) {
+            const float2 next = chunk(c + g);
+            double e = (double)st.y;  // of a chunk without finite logits 0, or a NaN
+            if (st.x != top && st.x > -INFINITY) e *= exp((double)st.x - (double)top);
+            s += e;
+            st = next;
+        }
         s = group_reduce(s, g, [](double x, double y) { return x + y; });
         if (mine && tid % g == 0) {
             double off = NAN;
