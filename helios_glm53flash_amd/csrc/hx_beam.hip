@@ -17,9 +17,9 @@
 // the n-th largest of all, and only what reaches it (n to 2n of random elements) is ranked.  The bound is renewed after 1, 2,
 // 4, .. pieces.
 //
-// 4 rows of 151552 fp32 logits, n = 8: 14 us, a chain of latencies beside 0.5 us of traffic (of a single launch traced at 17.7 us the last
-// chunk arrives at 7, after a piece's load, 1.7, and a bound, 1.1; the merge takes the rows' sums 3, the candidates 2.7, a bound 2.2
-// and their ranking 1.8).  256 rows in fp16, n = 16, some finished: 31 us, 2.5 TB/s, of which the reading is 18.
+// 4 rows of 151552 fp32 logits, n = 8: 13 us, a chain of latencies beside 0.5 us of traffic (of a single launch traced at 16.5 us the last
+// chunk arrives at 7, after a piece's load, 1.6, and a bound, 0.9; the merge takes the rows' sums 3.1, the candidates 3.0, a bound 1.7
+// and their ranking 1.1).  256 rows in fp16, n = 16, some finished: 31 us, 2.5 TB/s, of which the reading is 18.
 #include "hx_gemv.hpp"
 #include "hx_kernels.hpp"
 
