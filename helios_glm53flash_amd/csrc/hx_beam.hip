@@ -17,9 +17,8 @@
 // the n-th largest of all, and only what reaches it (n to 2n of random elements) is ranked.  The bound is renewed after 1, 2,
 // 4, .. pieces.
 //
-// 4 rows of 151552 fp32 logits, n = 8: 13 us, a chain of latencies beside 0.5 us of traffic (of a single launch traced at 16.5 us the last
-// chunk arrives at 7, after a piece's load, 1.6, and a bound, 0.9; the merge takes the rows' sums 3.1, the candidates 3.0, a bound 1.7
-// and their ranking 1.1).  256 rows in fp16, n = 16, some finished: 31 us, 2.5 TB/s, of which the reading is 18.
+// 4 rows of 151552 fp32 logits, n = 8: 12.4 us, a chain of latencies beside 0.5 us of traffic: a piece's load, a bound and the ranking, the
+// last arrival half way through; then the merge's sums of rows, candidates, bound and ranking.  256 rows in fp16, n = 16, some finished: 30 us, 2.5 TB/s, of which the reading is 18.
 #include "hx_gemv.hpp"
 #include "hx_kernels.hpp"
 
@@ -481,7 +480,7 @@ HX_INLINE void select_merge(const BeamArgs& a, const BeamPlan& p, long b, char* 
     };
     load(0);
     // score = offset[w] + (logit - tops[w]); offset NaN: the row has no candidates.  g lanes per row, as many as take all rows at once
-    // (16 rows of 37 chunks, 32 candidates: 24 us, 28 with 64 lanes a row); first the maxima, then the sums relative to the row's.
+    // (16 rows of 37 chunks, 32 candidates: 3 us less than with 64 lanes a row); first the maxima, then the sums relative to the row's.
     int g = 1;
     while (g < 64 && g < p.chunks && 2 * g * a.beams <= SEL_THREADS) g *= 2;
     for (int w0 = 0; w0 < a.beams; w0 += SEL_THREADS / g) {
@@ -529,28 +528,41 @@ HX_INLINE void select_merge(const BeamArgs& a, const BeamPlan& p, long b, char* 
         double most = -INFINITY;
         bool any = false;  // an entry that would be among the n best so far
 #pragma unroll
-        for (int i = 0; i < MERGE_E; ++i) {
-            const int q = i * SEL_THREADS + tid;
-            v[i] = {-INFINITY, 0};
-            if (q < fresh) {
-                const uint32_t f = at + q, rank = div_by(f, p.by_lists), list = f - rank * p.lists;
-                const uint32_t w = div_by(list, p.by_chunks);
-                const double off = offset[w];
-                const float top = tops[w];
-                if (off == off) {
-                    if (top != top) {
-                        if (rank == 0 && list == w * p.chunks) v[i] = {off, (u64)w << 32 | (uint32_t)a.eos};
-                    } else if (e[i]) {
-                        v[i] = {off + ((double)key_float((uint32_t)(e[i] >> 32)) - (double)top),
-                                (u64)w << 32 | (uint32_t)~(uint32_t)e[i]};
-                    }
-                }
-                any |= better(v[i].s, v[i].at, last_kept.s, last_kept.at);
-            } else if (q < fresh + kept) {
-                v[i] = carry[q - fresh];
+        for (int h = 0; h < MERGE_E; h += 2) {
+            v[h] = v[h + 1] = {-INFINITY, 0};
+            if (h * SEL_THREADS >= fresh) continue;
+            // two at a time without branches, so that they do not wait for each other's reads
+            double off[2];
+            float top[2];
+            uint32_t beam[2];
+            bool head[2];  // the row's first entry, which stands for a finished beam's only candidate
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t f = at + min((h + u) * SEL_THREADS + tid, fresh - 1), rank = div_by(f, p.by_lists), list = f - rank * p.lists;
+                beam[u] = div_by(list, p.by_chunks);
+                head[u] = rank == 0 && list == beam[u] * p.chunks;
+                off[u] = offset[beam[u]];
+                top[u] = tops[beam[u]];
             }
-            most = fmax(most, v[i].s);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const u64 entry = e[h + u];
+                const bool fin = top[u] != top[u];
+                const bool is = (h + u) * SEL_THREADS + tid < fresh && off[u] == off[u] && (fin ? head[u] : entry != 0);
+                const double score = off[u] + ((double)key_float((uint32_t)(entry >> 32)) - (double)top[u]);
+                Cand& c = v[h + u];
+                c.s = is ? fin ? off[u] : score : -INFINITY;
+                c.at = (u64)beam[u] << 32 | (fin ? (uint32_t)a.eos : (uint32_t)~(uint32_t)entry);
+                any |= is && better(c.s, c.at, last_kept.s, last_kept.at);
+                most = fmax(most, c.s);
+            }
         }
+        if (kept)
+#pragma unroll
+            for (int i = 0; i < MERGE_E; ++i) {
+                const int q = i * SEL_THREADS + tid - fresh;
+                if (q >= 0 && q < kept) v[i] = carry[q], most = fmax(most, v[i].s);
+            }
         at += fresh;
         if (at < total) load(at);
         // so few that ranking them all costs less than a bound (1.5 us)
