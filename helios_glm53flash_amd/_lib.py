@@ -42,6 +42,7 @@ class ExpertLayoutC(C.Structure):
 SIGNATURES: dict[str, tuple] = {
     "hx_version": (C.c_char_p, []),
     "hx_last_error": (C.c_char_p, []),
+    "hx_capture_id": (C.c_ulonglong, [C.c_void_p]),
     "hx_workspace_init": (C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p]),
     "hx_profile_enable": (C.c_int, [C.c_int]),
     "hx_profile_read": (C.c_int, [C.POINTER(C.c_double), C.POINTER(C.c_int), C.c_int]),

@@ -126,6 +126,17 @@ const char* hx_profile_phase_name(int phase)
     return (phase >= 0 && phase < k_nphases) ? k_phase_names[phase] : "";
 }
 
+unsigned long long hx_capture_id(hx_stream_t stream)
+{
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id) != hipSuccess) {
+        (void)hipGetLastError();  // the null stream while another one is captured: not part of it
+        return 0;
+    }
+    return status == hipStreamCaptureStatusActive ? id + 1 : 0;
+}
+
 int hx_workspace_init(void* workspace, size_t bytes, hx_stream_t stream)
 {
     if (!workspace && bytes) return fail(HX_ERR_INVALID, "hx_workspace_init: null workspace");

@@ -109,16 +109,25 @@ def _gemm_workspace_bytes(M: int, N: int, K: int) -> int:
     return lib.hx_w4_gemm_workspace_size(M, N, K)
 
 
+# (device, stream) -> (capture, workspace) of the last capture there.  Held so that a capture's calls share it and its counters are
+# cleared once (2 us a call otherwise).
+_captured: dict[tuple, tuple] = {}
+
+
 def call_workspace(nbytes: int, device: torch.device, st: int) -> torch.Tensor:
-    """A call's workspace on stream st: the stream's own one, or, where it is being captured, memory of the
-    graph's with counters that each replay clears, so that the graph depends on no buffer that a later call may replace."""
-    if _is_capturing():
-        here = st == _stream(None)
-        with nullcontext() if here else torch.cuda.stream(torch.cuda.ExternalStream(st, device=device)):
-            if here or torch.cuda.is_current_stream_capturing():  # another stream may have been forked into the capture
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-                ws[:COUNTER_BYTES].zero_()
-                return ws
+    """A call's workspace on stream st: the stream's own one, or, where st is being captured, memory of the graph's whose
+    counters each replay clears ahead of the first call, so that the graph depends on no buffer that a later call may replace."""
+    here = st == _stream(None)
+    if not here or _is_capturing():
+        capture, key = lib.hx_capture_id(st), (_get_device(), st)
+        if capture:
+            held = _captured.get(key)
+            if held is None or held[0] != capture or held[1].numel() < nbytes:
+                with nullcontext() if here else torch.cuda.stream(torch.cuda.ExternalStream(st, device=device)):
+                    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+                    ws[:COUNTER_BYTES].zero_()
+                _captured[key] = held = (capture, ws)
+            return held[1]
     ws = _workspaces.get((_get_device(), st))
     if ws is not None and ws.numel() >= nbytes:
         return ws

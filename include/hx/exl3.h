@@ -76,6 +76,10 @@ const char* hx_version(void);
 const char* hx_last_error(void);
 int hx_workspace_init(void* workspace, size_t bytes, hx_stream_t stream);
 
+/* A number that tells the graph captures of a process apart, or 0 where `stream` is not being captured.  For callers that give each
+ * captured graph a workspace of its own. */
+unsigned long long hx_capture_id(hx_stream_t stream);
+
 /* Whether a bounded wait inside the few-token MoE layer (hx_moe_layer / hx_moe_grouped with T <= 8:
  * a down-projection workgroup waiting for its activations) gave up since the last check: synchronizes
  * `stream`, clears the flag, returns HX_ERR_TIMEOUT if it was set (the results of those calls are

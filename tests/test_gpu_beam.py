@@ -282,6 +282,71 @@ def test_select_graph_and_streams(beam):
             assert torch.equal(a, b), rep
 
 
+def test_captures_are_told_apart(beam):
+    import torch
+    from helios_glm53flash_amd._lib import lib
+    st, side = torch.cuda.Stream(), torch.cuda.Stream()
+    x = torch.zeros(8, device="cuda")
+    torch.cuda.synchronize()
+    ids = []
+    for _ in range(4):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            side.wait_stream(st)
+            with torch.cuda.stream(side):
+                x.add_(1)
+            ids.append(lib.hx_capture_id(st.cuda_stream))
+            assert lib.hx_capture_id(side.cuda_stream) == ids[-1]
+            st.wait_stream(side)
+        assert lib.hx_capture_id(st.cuda_stream) == 0 and lib.hx_capture_id(None) == 0
+        del g
+    assert 0 not in ids and len(set(ids)) == 4
+
+
+def test_calls_of_two_captures_on_one_stream(beam):
+    """Calls of a capture share memory of its graph, small ones first, with other tensors made and dropped between them; two graphs
+    of one stream replay in any order, beside eager calls."""
+    import torch
+    from helios_glm53flash_amd import w4
+    K, N, group = 4096, 256, 64
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(2)
+    q = torch.randint(0, 16, (N, K), generator=gen, device="cuda").to(torch.uint8)
+    w = w4.W4Words(w4.pack(q), torch.full((N, K // group), 0.125, dtype=torch.float16, device="cuda"), None, K, group)
+    batch, beams, n = 2, 4, 8
+    cum = -torch.rand(batch * beams, device="cuda")
+    st = torch.cuda.Stream()
+    graphs = []
+
+    def calls(x, y, logits, outs):
+        for M in (16, 64, 16):
+            w4.gemm(y[M], x, w, M, N, K, True)
+            torch.full((1 << 20,), 255, dtype=torch.uint8, device="cuda")
+            beam.select(logits, cum, None, *outs, batch, beams, 50000, n)
+
+    for g in range(2):
+        x = torch.randn((64, K), device="cuda").half()
+        y = {M: torch.zeros((M, N), device="cuda") for M in (16, 64)}
+        logits = torch.randn((batch * beams, 50000), device="cuda")
+        outs = [torch.zeros((batch, n), dtype=d, device="cuda") for d in (torch.float32, torch.int64, torch.int64)]
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            calls(x, y, logits, outs)
+        graphs.append((graph, x, y, logits, outs))
+    for rep in range(6):
+        graph, x, y, logits, outs = graphs[(0, 1, 1, 0, 1, 0)[rep]]
+        x.copy_(torch.randn_like(x))
+        logits.copy_(torch.randn_like(logits) * 3)
+        torch.cuda.synchronize()
+        graph.replay()
+        want_y = {M: torch.empty((M, N), device="cuda") for M in (16, 64)}
+        want = [torch.empty_like(o) for o in outs]
+        calls(x, want_y, logits, want)
+        torch.cuda.synchronize()
+        assert all(torch.equal(y[M], want_y[M]) for M in y) and all(torch.equal(a, b) for a, b in zip(outs, want)), rep
+
+
 def test_select_on_a_forked_stream_of_a_capture(beam):
     """A captured call on a stream that was forked from the capturing one depends on no workspace of that stream."""
     import torch
