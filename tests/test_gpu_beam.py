@@ -375,6 +375,25 @@ def test_select_on_a_forked_stream_of_a_capture(beam):
             assert torch.equal(a, c) and torch.equal(b, c), rep
 
 
+@pytest.mark.parametrize("batch,beams,V,n", [(1, 4, 20001, 8), (3, 1, 5, 128), (600, 1, 9000, 3), (2, 300, 5000, 33)])
+def test_select_in_a_workspace_of_the_least_size(beam, batch, beams, V, n):
+    import torch
+    from helios_glm53flash_amd._lib import lib
+    x = torch.randn((batch * beams, V), device="cuda")
+    cum = -torch.rand(batch * beams, device="cuda")
+    want = [torch.empty((batch, n), dtype=d, device="cuda") for d in (torch.float32, torch.int64, torch.int64)]
+    beam.select(x, cum, None, *want, batch, beams, V, n)
+    need = lib.hx_beam_select_workspace_size(batch, beams, V, n)
+    ws = torch.full((need + 4096,), 0x5A, dtype=torch.uint8, device="cuda")
+    ws[:65536].zero_()
+    for _ in range(3):
+        got = [torch.empty_like(o) for o in want]
+        assert lib.hx_beam_select(x.data_ptr(), cum.data_ptr(), None, *(o.data_ptr() for o in got), batch, beams, V, n, V, 0, 1,
+                                  torch.cuda.current_stream().cuda_stream, ws.data_ptr(), need) == 0
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert bool((ws[need:] == 0x5A).all()) and bool((ws[:65536] == 0).all())
+
+
 def test_select_leaves_the_counters_zero(beam):
     import torch
     from helios_glm53flash_amd import exl3

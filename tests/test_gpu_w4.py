@@ -296,6 +296,25 @@ def test_gemm_large_batches(w4):
         assert not bool(y[:, 0].isnan().any()) and not bool(y[:, -1].isnan().any())
 
 
+@pytest.mark.parametrize("M", [1, 5, 12, 40, 130])
+def test_gemm_longest_rows(w4, M):
+    """K at its limit; x is nonzero in few places, the row's ends among them, so that the sums are exact."""
+    import torch
+    K, N, group = 1 << 22, 70, 64
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(M)
+    wd = torch.randint(-2 ** 31, 2 ** 31 - 1, (N, K // 8), generator=gen, device="cuda").to(torch.int32)
+    w = w4.W4Words(wd, torch.full((N, K // group), 0.5, dtype=torch.float16, device="cuda"), None, K, group)
+    x = torch.zeros((M, K), dtype=torch.float16, device="cuda")
+    at = torch.randint(0, K, (300,), generator=gen, device="cuda").unique()
+    at = torch.cat([at, torch.tensor([0, 1, K - 1, K - 129, K // 2], device="cuda")]).unique()
+    x[:, at] = torch.randint(-3, 4, (M, len(at)), generator=gen, device="cuda").half()
+    y = torch.empty((M, N), device="cuda")
+    w4.gemm(y, x, w, M, N, K, True)
+    codes = torch.stack([w4.unpack(wd[n:n + 1], K)[0, at] for n in range(N)]).double()
+    assert torch.equal(y.double(), x[:, at].double() @ ((codes - 8) * 0.5).T)
+
+
 def test_embed_tokens_outside_the_table(w4):
     import torch
     q, s, z, w = make(2, 20, 128, 64, True, exact=True)
@@ -306,6 +325,32 @@ def test_embed_tokens_outside_the_table(w4):
     assert (got[[1, 3, 4, 5]] == 0).all()
     assert np.array_equal(got[[0, 2, 6]], w[[3, 19, 0]].astype(np.float32))
     w4.embed(words(w4, q, s, z, 128, 64), tok[:0], out[:0], 0)
+
+
+@pytest.mark.parametrize("M,K,N,group", [(9, 8192, 300, 32), (16, 4224, 64, 128), (32, 16384, 200, 64), (45, 8192, 4096, 64),
+                                         (64, 4096, 2048, 128), (100, 4096, 1000, 32), (128, 8192, 4096, 128), (300, 2048, 512, 64)])
+def test_gemm_workspaces_through_the_c_entry(w4, M, K, N, group):
+    """A workspace of exactly the size asked for, none, and one that is too small: right each time, nothing written behind it and
+    its counters left at zero."""
+    import ctypes as C
+    import torch
+    from helios_glm53flash_amd._lib import lib
+    q, s, z, w = make(M, N, K, group, True, exact=True)
+    ww = words(w4, q, s, z, K, group)
+    x = np.random.default_rng(K).integers(-2, 3, (M, K))
+    ref = dev(x).double() @ dev(w).T
+    xd = dev(x.astype(np.float16))
+    need = lib.hx_w4_gemm_workspace_size(M, N, K)
+    st = torch.cuda.current_stream().cuda_stream
+    for size in {need, 0, max(need - 16, 0)}:
+        ws = torch.full((size + 4096,), 0x5A, dtype=torch.uint8, device="cuda")
+        ws[:min(size, 65536)].zero_()
+        for _ in range(3):
+            y = torch.full((M, N), float("nan"), device="cuda")
+            assert lib.hx_w4_gemm(y.data_ptr(), xd.data_ptr(), C.byref(ww.c()), M, N, K, 1, st, ws.data_ptr() if size else None,
+                                  size) == 0
+            assert torch.equal(y.double(), ref)
+        assert bool((ws[size:] == 0x5A).all()) and bool((ws[:min(size, 65536)] == 0).all())
 
 
 def test_another_device_is_refused(w4):
