@@ -197,6 +197,40 @@ def test_select_many_rows(beam, dtype, batch, beams, V, n):
     check(beam, x, cum, None, batch, beams, V, n)
 
 
+# The bound on a log-sum-exp does not grow with the logits: exponentials are relative to the largest, and each change of what
+# they are relative to is a factor of 2^(a difference of two fp32 values), 2^-23 off.  A thread here meets up to 3 such changes.
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("offset", [0.0, 20.0, -100.0, 300.0, 1000.0, -3000.0, 30000.0, -60000.0, 60000.0, 1e6])
+def test_select_of_logits_far_from_zero(beam, dtype, offset):
+    """Rows about a common offset: normal ones, one logit above a constant row, two finite logits in different threads, waves or
+    pieces, steps up and down; alone, and as beams whose best scores differ by 1e-4."""
+    if dtype == np.float16 and abs(offset) > 60000:
+        pytest.skip("beyond fp16")
+    r = np.random.default_rng(int(abs(offset)) + 3)
+    for batch, V in ((3, 151552), (65, 12289)):  # chunks of one piece, and workgroups that walk over four
+        rows = 8 * batch
+        x = np.full((rows, V), offset, np.float32)
+        x[0::8] += r.standard_normal(x[0::8].shape).astype(np.float32) * 3
+        step = max(3.0, 1.001 * float(np.spacing(dtype(abs(offset)))))
+        at = r.integers(0, V, rows)
+        x[np.arange(rows), at] += step
+        x[2::8] += np.arange(V) // (V // 5) * np.float32(step)
+        x[3::8] -= np.arange(V) // (V // 5) * np.float32(step)
+        x[4::8, 0] = offset + step
+        for i, gap in ((5, 16), (6, 1024), (7, V - 1)):  # all of the row but two logits forbidden
+            two = np.full_like(x[i::8], -np.inf)
+            two[:, 0], two[:, gap] = offset, offset + step
+            x[i::8] = two
+        x = x.astype(dtype)
+        x64 = x.astype(np.float64)
+        top = x64.max(axis=1)
+        best = -np.log(np.exp(x64 - top[:, None]).sum(axis=1))
+        cum = np.zeros(rows, np.float32)
+        check(beam, x, cum, None, rows, 1, V, 5)
+        want = -20.0 + 1e-4 * r.permuted(np.tile(np.arange(8), (batch, 1)), axis=1).reshape(-1)
+        check(beam, x, (want - best).astype(np.float32), None, batch, 8, V, 16)
+
+
 def test_select_large_vocabulary(beam):
     """300 million tokens: places next to both ends and around multiples of the pieces that workgroups read."""
     import torch
