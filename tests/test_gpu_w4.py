@@ -265,6 +265,28 @@ def test_embed(w4, T, K, N, group, zeros, fp32):
     check_guard(whole)
 
 
+@pytest.mark.parametrize("K,N,group,zeros,scale", [(4128, 70, 32, True, 4128 ** 0.5), (1280, 40, 128, False, 1280 ** 0.5), (160, 33, 64, True, 1 / 3),
+                                                   (256, 20, 256, True, -1e-3)])
+def test_embed_rounds_once(w4, K, N, group, zeros, scale):
+    """A weight is exact in fp32 (9 bits times 11), so its product with the scale is rounded once; fp16 outputs once more."""
+    import torch
+    q, s, z, _ = make(K + N, N, K, group, zeros)
+    if zeros:
+        z = np.random.default_rng(K).integers(0, 256, z.shape, dtype=np.uint8)
+    gi = np.arange(K) // group
+    w = s.astype(np.float64)[:, gi] * (q.astype(np.float64) - (z.astype(np.float64)[:, gi] if zeros else 8.0))
+    ref = w * np.float64(np.float32(scale))  # 20 bits times 24: exact
+    tok = torch.arange(N, device="cuda")
+    ww = words(w4, q, s, z if zeros else None, K, group)
+    out = torch.empty((N, K), device="cuda")
+    w4.embed(ww, tok, out, N, scale)
+    assert np.array_equal(out.cpu().numpy(), ref.astype(np.float32))
+    half = torch.empty((N, K), dtype=torch.float16, device="cuda")
+    w4.embed(ww, tok, half, N, scale)
+    err = np.abs(half.cpu().numpy().astype(np.float64) - ref)
+    assert (err <= (U16 * (1 + U32) + U32) * np.abs(ref) + 2.0 ** -25).all()
+
+
 @pytest.mark.parametrize("n,K", [(1_200_000, 32), (540_000, 8192), (140_000_000, 32)])
 def test_embed_many_tokens(w4, n, K):
     """Several launches (2^31 words each); an output of more than 2^32 elements."""
