@@ -33,6 +33,8 @@ def select(logits: torch.Tensor, cum: torch.Tensor, done: Optional[torch.Tensor]
     -inf, dead beams cum -inf; places that no candidate fills get -inf, -1, -1.  scores may be cum itself where n == beams."""
     if not isinstance(logits, torch.Tensor) or logits.dtype not in _DTYPES or not logits.is_cuda or logits.dim() != 2:
         raise ValueError("select: logits must be a 2-d float16 or float32 device tensor")
+    if max(batch, beams, vocab, n) >> 31 or done is not None and eos >> 31 not in (0, -1):
+        raise ValueError("select: batch, beams, vocab, n and eos must fit 32 bits")
     rows = batch * beams
     height, width = logits.shape
     if batch < 0 or beams < 1 or vocab < 1 or n < 1 or height < rows or width < vocab:
@@ -108,6 +110,8 @@ def reorder(src: torch.Tensor, parents: torch.Tensor, dst: torch.Tensor, batch: 
     _need(parents, "parents", (torch.int64,))
     if src.dtype != dst.dtype or src.is_complex() or src.dim() != dst.dim() or not -src.dim() <= dim < src.dim():
         raise ValueError("reorder: src and dst must have the same (real) type and dimensions, dim among them")
+    if max(batch, beams, out_beams) >> 31:
+        raise ValueError("reorder: batch, beams and out_beams must fit 32 bits")
     if batch < 0 or beams < 1 or out_beams < 0 or parents.numel() < batch * out_beams:
         raise ValueError("reorder: parents smaller than batch * out_beams")
     _on_one_device(src, parents, dst)

@@ -140,7 +140,9 @@ def gemm(y: torch.Tensor, x: torch.Tensor, w: W4Words, M: int, N: int, K: int, y
     over workgroups do so in the stream's workspace (exl3.workspace, which never grows for it)."""
     _need(x, "x", (torch.float16,))
     _need(y, "y", (torch.float32,) if y_fp32 else (torch.float16,))
-    if M < 0 or x.numel() < M * K or y.numel() < M * N:
+    if M >> 31:
+        raise ValueError("gemm: M must be non-negative and fit 32 bits")
+    if x.numel() < M * K or y.numel() < M * N:
         raise ValueError("x / y smaller than M*K / M*N")
     if w.in_features != K or w.out_features != N:
         raise ValueError("W4Words shapes do not match K, N")
@@ -158,7 +160,9 @@ def embed(w: W4Words, tokens: torch.Tensor, out: torch.Tensor, n: int, scale: fl
     [0, N)."""
     _need(tokens, "tokens", (torch.int64,))
     _need(out, "out", (torch.float16, torch.float32))
-    if n < 0 or tokens.numel() < n or out.numel() < n * w.in_features:
+    if n >> 31:
+        raise ValueError("embed: n must be non-negative and fit 32 bits")
+    if tokens.numel() < n or out.numel() < n * w.in_features:
         raise ValueError("embed: tokens / out smaller than n / n*K")
     _on_one_device(tokens, out)
     _weights_here(w)

@@ -248,6 +248,31 @@ def test_select_large_vocabulary(beam):
     assert (np.abs(s[0].cpu().numpy() - (v - lse)) <= 2.5e-4).all()
 
 
+def test_extents_beyond_32_bits_are_refused(beam):
+    """They would reach the C entries modulo 2^32: an eos of 2^32 + 5 as 5, a vocabulary of 2^32 + 100 tokens as 100."""
+    import torch
+    V = 50
+    cum, done = torch.zeros(2, device="cuda"), torch.zeros(2, dtype=torch.uint8, device="cuda")
+    out = [torch.full((1, 2), 9, dtype=d, device="cuda") for d in (torch.float32, torch.int64, torch.int64)]
+    x = torch.randn((2, V), device="cuda")
+    for eos in ((1 << 32) + 5, -(1 << 32), 1 << 31):
+        with pytest.raises(ValueError, match="32 bits"):
+            beam.select(x, cum, done, *out, 1, 2, V, 2, eos)
+    big = torch.zeros((1, (1 << 32) + 100), dtype=torch.float16, device="cuda")
+    with pytest.raises(ValueError, match="32 bits"):
+        beam.select(big, cum[:1], None, *out, 1, 1, big.shape[1], 2)
+    rows = big.view(-1, 1)
+    with pytest.raises(ValueError, match="32 bits"):
+        beam.select(rows, cum, None, *out, rows.shape[0], 1, 1, 2)
+    with pytest.raises(ValueError, match="32 bits"):
+        beam.select(x, cum, None, *out, 1, 2, V, 1 << 32)
+    assert all(bool((o == 9).all()) for o in out)
+    parents = torch.zeros((1, 2), dtype=torch.int64, device="cuda")
+    for extents in ((1 << 32, 1, 1), (1, 1 << 32, 1), (1, 1, 1 << 32)):
+        with pytest.raises(ValueError, match="32 bits"):
+            beam.reorder(x, parents, torch.zeros_like(x), *extents)
+
+
 def test_select_scores_in_place_of_cum(beam):
     import torch
     batch, beams, V = 5, 6, 20000

@@ -375,6 +375,18 @@ def test_gemm_workspaces_through_the_c_entry(w4, M, K, N, group):
         assert bool((ws[size:] == 0x5A).all()) and bool((ws[:min(size, 65536)] == 0).all())
 
 
+def test_counts_beyond_32_bits_are_refused(w4):
+    import torch
+    q, s, z, _ = make(1, 16, 128, 64, True)
+    w = words(w4, q, s, z, 128, 64)
+    x, y = torch.zeros((1, 128), dtype=torch.float16, device="cuda"), torch.zeros((1, 16), device="cuda")
+    for M in (1 << 32, 1 << 31, -1):
+        with pytest.raises(ValueError, match="32 bits"):
+            w4.gemm(y, x, w, M, 16, 128, True)
+        with pytest.raises(ValueError, match="32 bits"):
+            w4.embed(w, torch.zeros(1, dtype=torch.int64, device="cuda"), x, M)
+
+
 def test_another_device_is_refused(w4):
     """The entry points launch on the current device: tensors elsewhere (here the host) are refused."""
     import torch
