@@ -696,7 +696,8 @@ hipError_t gemm_launch(const W4Call& c)
 
 }  // namespace
 
-// Bytes of workspace with which calls of M rows split K; 0 where none do.
+// Bytes of workspace with which calls of M rows split K; 0 where none do.  Splits come in W4_SLOTS workgroups of 64 x 64 sums at most:
+// 4 MiB and the counters.
 size_t w4_gemm_workspace_bytes(int M, int N, int K)
 {
     size_t most = 0;

@@ -250,7 +250,7 @@ typedef struct hx_w4_words {
 /* y[M][N] = x W^T: x fp16 [M][K] (16-byte aligned), y fp32 (y_fp32) or fp16, fp32 sums rounded once.  The codes and zero
  * points enter the products exactly and the scales are applied to fp32 sums.  M == 0 is a no-op (x and y may
  * then be NULL).  The workspace is optional: a call with at least hx_w4_gemm_workspace_size(M, N, K) bytes (0: the shape has no
- * use for it; at most 9 MiB) splits K over more workgroups where there are few (up to three times as fast from 9 rows on),
+ * use for it; at most 64 KiB + 4 MiB) splits K over more workgroups where there are few (up to three times as fast from 9 rows on),
  * with the fp32 sums in another order than without; NULL or fewer bytes do without. */
 size_t hx_w4_gemm_workspace_size(int M, int N, int K);
 int hx_w4_gemm(void* y, const void* x, const hx_w4_words* w, int M, int N, int K, int y_fp32, hx_stream_t stream,

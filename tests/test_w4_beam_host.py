@@ -167,3 +167,13 @@ def test_extents_beyond_a_call():
 @pytest.mark.parametrize("kw", [dict(scores=16), dict(scores=28, n=4), dict(scores=4, n=4, beams=4), dict(scores=16, n=3, beams=4)])
 def test_select_refuses_overlapping_scores(kw):
     assert select(**{"cum": 16, "n": 8, **kw}) == _lib.HX_ERR_INVALID and "overlap" in err()
+
+
+def test_gemm_workspace_bound():
+    """The counters and 256 workgroups' 64 x 64 fp32 sums: never more, and reached."""
+    size, most = LIB.hx_w4_gemm_workspace_size, 65536 + 256 * 64 * 64 * 4
+    assert size(33, 2048, 65536) == most
+    for M in (9, 16, 17, 32, 33, 48, 64, 65, 128, 129, 256, 512, 600):
+        for N in [64 * i + j for i in range(1, 70, 3) for j in (0, 1)] + [8192, 12288, 16384, 24576, 151552]:
+            for K in (2048, 4096, 16384, 65536, 1 << 22):
+                assert size(M, N, K) <= most, (M, N, K)
