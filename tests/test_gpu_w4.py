@@ -394,3 +394,53 @@ def test_another_device_is_refused(w4):
     w = words(w4, q, s, z, 128, 64)
     with pytest.raises(ValueError, match="device"):
         w4.gemm(torch.empty((1, 16)), torch.empty((1, 128), dtype=torch.float16), w, 1, 16, 128, True)
+
+
+def test_gemm_of_the_same_rows_in_other_batches(w4):
+    """Batches on both sides of where another kernel or tile takes over: a row's sums may come in another order, each within the
+    bound of test_gemm_random, and the first rows' results lie within two of it."""
+    import torch
+    K, N, group = 4128, 300, 32
+    q, s, z, w = make(51, N, K, group, True)
+    ww = words(w4, q, s, z, K, group)
+    x = np.random.default_rng(52).standard_normal((130, K)).astype(np.float16)
+    x64 = x.astype(np.float64)
+    ref = x64 @ w.T
+    tol = (K + -(-K // group) + 2) * U32 * (np.abs(x64) @ np.abs(w).T)
+    first = None
+    for M in (1, 4, 5, 8, 9, 16, 17, 32, 33, 64, 65, 128, 129, 130):
+        y = torch.full((M, N), float("nan"), device="cuda")
+        w4.gemm(y, dev(x[:M]), ww, M, N, K, True)
+        got = y.cpu().numpy().astype(np.float64)
+        assert (np.abs(got - ref[:M]) <= tol[:M]).all(), M
+        first = got[0] if first is None else first
+        assert (np.abs(got[0] - first) <= 2 * tol[0]).all(), M
+
+
+def test_tensors_of_another_device_than_the_current_one_are_refused(w4, monkeypatch):
+    """With the current device said to be another one, which is all that the checks look at; nothing is launched."""
+    import torch
+    from helios_glm53flash_amd import beam
+    q, s, z, _ = make(1, 16, 128, 64, True)
+    w = words(w4, q, s, z, 128, 64)
+    x, y = torch.zeros((1, 128), dtype=torch.float16, device="cuda"), torch.full((1, 16), 7.0, device="cuda")
+    tok, par = (torch.full((1, 1), 7, dtype=torch.int64, device="cuda") for _ in range(2))
+    score = torch.full((1, 1), 7.0, device="cuda")
+    here = torch.cuda.current_device()
+    monkeypatch.setattr(w4, "_get_device", lambda: here + 1)
+    other = f"current device \\(cuda:{here + 1}\\)"
+    with pytest.raises(ValueError, match=other):
+        w4.gemm(y, x, w, 1, 16, 128, True)
+    with pytest.raises(ValueError, match=other):
+        w4.embed(w, tok.view(-1), x, 1)
+    with pytest.raises(ValueError, match=other):
+        beam.select(y, torch.zeros(1, device="cuda"), None, score, par, tok, 1, 1, 16, 1)
+    with pytest.raises(ValueError, match=other):
+        beam.reorder(x, par, torch.zeros_like(x), 1, 1, 1)
+    monkeypatch.undo()
+    object.__setattr__(w, "device_index", here + 1)
+    for call in (lambda: w4.gemm(y, x, w, 1, 16, 128, True), lambda: w4.embed(w, tok.view(-1), x, 1)):
+        with pytest.raises(ValueError, match=f"weights are on cuda:{here + 1}"):
+            call()
+    torch.cuda.synchronize()
+    assert all(bool((t == 7).all()) for t in (y, tok, par, score))
