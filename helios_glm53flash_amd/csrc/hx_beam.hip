@@ -11,14 +11,19 @@
 // Selection is one launch.  A workgroup takes one chunk of one row and reads it once, in pieces of 4096 logits with the next
 // two in flight: running maximum and sum of exponentials per thread, and which blocks (the 16 logits of a thread and piece) may
 // hold some of the n largest.  Few blocks are left at the end; their logits are read again and ranked.  The last workgroup of
-// a sequence to arrive merges the chunks: the rows' log-sum-exp in 64 bits, the candidates' scores in 64 bits, the n best of them.
+// a sequence to arrive merges the chunks: the rows' log-sum-exp and the candidates' scores from their sums in 64 bits, the n best.
+//
+// Error of a log-sum-exp, with p pieces in a chunk: 1e-6 from the exponentials' fp32 arguments (2^-24 + 2^-26 of x - max, whose mean under
+// the softmax is at most ln vocab), 15 + p additions of a thread, 9 of a workgroup, p + 1 rescalings of 2^-22 at most, two roundings of the
+// reference: 4e-6 + 3e-7 p.  It does not depend on the logits' size.
 //
 // The n largest of a set spread over threads, without sorting it: the n-th largest of the threads' maxima is a lower bound of
 // the n-th largest of all, and only what reaches it (n to 2n of random elements) is ranked.  The bound is renewed after 1, 2,
 // 4, .. pieces.
 //
-// 4 rows of 151552 fp32 logits, n = 8: 12.4 us, a chain of latencies beside 0.5 us of traffic: a piece's load, a bound and the ranking, the
-// last arrival half way through; then the merge's sums of rows, candidates, bound and ranking.  256 rows in fp16, n = 16, some finished: 30 us, 2.5 TB/s, of which the reading is 18.
+// 4 rows of 151552 fp32 logits, n = 8: 12.3 us, a chain of latencies beside 0.5 us of traffic: a piece's load 2.1, a bound and the ranking
+// 1.8, the last arrival 1.9, then the merge 5.9 (sums of rows 2.3, candidates, bound and ranking 3.6).  256 rows in fp16, n = 16, a fifth of
+// them finished and not read: 30 us, of which the last logits come at 18.4 (62 MB, 3.4 TB/s) and the last sequence's merge starts at 22.3.
 #include "hx_gemv.hpp"
 #include "hx_kernels.hpp"
 
@@ -184,7 +189,7 @@ constexpr float LOG2E = 1.44269504f, REF_MAX = 2e38f;
 HX_INLINE bool ref_fits(float top) { return fabsf(top) < REF_MAX; }
 HX_INLINE float ref_rest(float top) { return ref_fits(top) ? __builtin_fmaf(top, LOG2E, -(top * LOG2E)) : 0.0f; }
 // Factor that takes a sum relative to `from` to one relative to the larger `to`.  The references are the rounded products: one fused
-// into the subtraction would leave its rounding in the sum, 4e-6 of it for logits near 100 and 3e-3 near 60000.
+// into the subtraction would leave its rounding in the sum, up to 5e-6 of it for logits near 100 and 2.7e-3 near 60000.
 HX_INLINE float rescale(float from, float to)
 {
 #pragma clang fp contract(off)
@@ -734,7 +739,8 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(const char* src, cons
 namespace {
 
 // Few large pieces are divided among workgroups, 8 per CU in all, into no less than one access per thread: 4 pieces of 64 MiB 111 us, 4.9
-// TB/s, undivided 6980; 32 of 8 MiB 110 and 920.  A cache's pieces (42 layers of 32 rows, 3.1 GB both ways) 550 us, 5.6 TB/s.
+// TB/s, undivided 6980; 32 of 8 MiB 110 and 920.  A cache's pieces (42 layers of 32 rows, a
+// sequence's 8 having 5.25 distinct parents in the mean: 1.02 GB to read once, 1.55 to write) 551 us, 4.65 TB/s.
 template <typename V>
 hipError_t reorder_launch(const char* src, const int64_t* parents, char* dst, const ReorderArgs& p, hipStream_t st)
 {

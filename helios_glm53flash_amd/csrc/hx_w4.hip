@@ -298,10 +298,12 @@ __global__ __launch_bounds__(64 * WAVES) void w4_rows_kernel(const _Float16* x, 
 // with an LDS destination (256 consecutive bytes of a row); 16-byte piece u of row m lies at piece u ^ (m & 15), so the 16
 // rows of a fragment read touch all banks.  The words go from memory into registers, as many steps ahead, and become operands
 // there: no wave decodes a weight that another wave of the workgroup uses.
-// With few rows the address unit is the busiest (70 % of a step of 64 x 64 outputs by 256 k in groups of 64: x takes 512 of its 1900 cycles,
-// the words 264, scales and zero points 248), the VALU half as much: 45 rows of 4096 -> 12288 15.5 us, 29 MB.  With many it is the
+// With few rows the address unit is the busiest, by its counter 70 % of the time: of the 1900 cycles of a step of 64 x 64 outputs by 256 k in
+// groups of 64, x takes 512, the words 264, scales and zero points 248, which is 54 %; the rest it holds requests that wait.  The VALU
+// is busy half as much: 45 rows of 4096 -> 12288 15.6 us, 29 MB.  With many it is the
 // matrix instructions at what clock the power limit leaves (1.7 GHz, 52 % busy): 2000 rows of 4096 -> 24576 in groups of 128
-// 383 us, 1.05 PFLOP/s, where the library's fp16 product of 8192^3 runs at 1.26.
+// 382 to 396 us, 1.02 to 1.05 PFLOP/s, where the library's fp16 product of 8192^3 runs at 1.26.  Groups of 32 have four products to scale where
+// those have one: the same with zero points 510 us, vector instructions in 69 % of the cycles (53) and the matrix pipe in 37 % (54).
 struct W4Split {
     int splits, steps;  // workgroups that share a tile's K, steps of each
     hx_f4* partial;     // [tiles][splits][RB][NT][4][64]

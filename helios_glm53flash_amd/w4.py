@@ -136,8 +136,8 @@ def call_workspace(nbytes: int, device: torch.device, st: int) -> torch.Tensor:
 
 
 def gemm(y: torch.Tensor, x: torch.Tensor, w: W4Words, M: int, N: int, K: int, y_fp32: bool = False, stream=None) -> None:
-    """y[m][n] = sum_k x[m][k] W[n][k]: x fp16 [M][K], y fp32 or fp16 [M][N], any M (M = 0 is a no-op).  Shapes that split K
-    over workgroups do so in the stream's workspace (exl3.workspace, which never grows for it)."""
+    """y[m][n] = sum_k x[m][k] W[n][k]: x fp16 [M][K], y fp32 or fp16 [M][N], any M (M = 0 is a no-op); y may not
+    overlap x.  Shapes that split K over workgroups do so in the stream's workspace (exl3.workspace, which never grows for it)."""
     _need(x, "x", (torch.float16,))
     _need(y, "y", (torch.float32,) if y_fp32 else (torch.float16,))
     if M >> 31:

@@ -247,8 +247,8 @@ typedef struct hx_w4_words {
     int group;
 } hx_w4_words;
 
-/* y[M][N] = x W^T: x fp16 [M][K] (16-byte aligned), y fp32 (y_fp32) or fp16, fp32 sums rounded once.  The codes and zero
- * points enter the products exactly and the scales are applied to fp32 sums.  M == 0 is a no-op (x and y may
+/* y[M][N] = x W^T: x fp16 [M][K] (16-byte aligned), y fp32 (y_fp32) or fp16, fp32 sums rounded once; y may not
+ * overlap x.  The codes and zero points enter the products exactly and the scales are applied to fp32 sums.  M == 0 is a no-op (x and y may
  * then be NULL).  The workspace is optional: a call with at least hx_w4_gemm_workspace_size(M, N, K) bytes (0: the shape has no
  * use for it; at most 64 KiB + 4 MiB) splits K over more workgroups where there are few (up to three times as fast from 9 rows on),
  * with the fp32 sums in another order than without; NULL or fewer bytes do without. */
@@ -256,8 +256,8 @@ size_t hx_w4_gemm_workspace_size(int M, int N, int K);
 int hx_w4_gemm(void* y, const void* x, const hx_w4_words* w, int M, int N, int K, int y_fp32, hx_stream_t stream,
                void* workspace, size_t workspace_bytes);
 
-/* out[t][:] = scale * W[tokens[t]][:] for t < n, fp32 (out_fp32) or fp16 rows of K (16-byte aligned); a token outside
- * [0, N) gives a row of zeros. */
+/* out[t][:] = scale * W[tokens[t]][:] for t < n, fp32 (out_fp32) or fp16 rows of K (16-byte aligned), rounded once to fp32 and
+ * once more to fp16; a token outside [0, N) gives a row of zeros. */
 int hx_w4_embed(const hx_w4_words* w, const int64_t* tokens, void* out, int n, int N, int K, float scale, int out_fp32,
                 hx_stream_t stream);
 
@@ -267,8 +267,11 @@ int hx_w4_embed(const hx_w4_words* w, const int64_t* tokens, void* out, int n, i
  * b * beams + w of logits (fp16 or fp32 by dtype, HX_DTYPE_*; ld elements from row to row) is beam w of sequence b:
  *   score(w, v) = cum[b][w] + logits[w][v] - logsumexp(logits[w][0 .. vocab))
  * and scores / parents / tokens [batch][n] receive the n best (score, w, v) of each sequence in descending order, the
- * lowest w * vocab + v first among equal scores; fp32 scores rounded once from 64 bits.  A beam with done != 0 (done may be
- * NULL) has the one candidate (w, eos) with score cum.  A logit of -inf is no candidate; a beam whose cum is not finite, whose
+ * lowest w * vocab + v first among equal scores.  Exponentials, and their sums over the p pieces of 4096 logits that one
+ * workgroup takes, are fp32, all after them 64 bits, and the score is rounded to fp32 at the end: beside that rounding it is off by at
+ * most 4e-6 + 3e-7 p, p = ceil(ceil(vocab / 4096) / max(1, floor(1024 / (batch * beams)))), whatever the logits' size.  Within a
+ * beam the order is that of its logits; candidates of different beams closer than the error may change places.
+ * A beam with done != 0 (done may be NULL) has the one candidate (w, eos) with score cum.  A logit of -inf is no candidate; a beam whose cum is not finite, whose
  * logits hold a NaN or +inf, or are all -inf, has none.  Places without a candidate get score -inf, parent -1, token -1.
  * scores may be cum itself where n == beams; otherwise outputs and inputs may not overlap.
  * batch <= 4096, beams <= 1024, vocab <= 2^30, n <= 128.  batch == 0 is a no-op. */
