@@ -34,6 +34,10 @@ class W4WordsC(C.Structure):
     _fields_ = [("words", C.c_void_p), ("scales", C.c_void_p), ("zeros", C.c_void_p), ("group", C.c_int)]
 
 
+class F8BlocksC(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p)]
+
+
 class ExpertLayoutC(C.Structure):
     _fields_ = [("off", C.c_uint64 * 12), ("piece", C.c_uint64 * 12), ("bits", C.c_int * 3), ("stride", C.c_uint64)]
 
@@ -87,6 +91,14 @@ SIGNATURES: dict[str, tuple] = {
     "hx_w4_gemm_workspace_size": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
     "hx_w4_embed": (C.c_int, [C.POINTER(W4WordsC), C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_float, C.c_int,
                               C.c_void_p]),
+    "hx_f8_quantize": (C.c_int, [C.c_void_p] * 3 + [C.c_int] * 2 + [C.c_int64, C.c_int, C.c_void_p]),
+    "hx_f8_rms_norm": (C.c_int, [C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int] +
+                       [C.c_void_p] * 3 + [C.c_int, C.c_int, C.c_float, C.c_void_p]),
+    "hx_f8_gemm_workspace_size": (C.c_size_t, [C.c_int] * 3),
+    "hx_f8_gemm": (C.c_int, [C.c_void_p] * 3 + [C.POINTER(F8BlocksC)] + [C.c_int] * 4 + [C.c_void_p, C.c_void_p, C.c_size_t]),
+    "hx_f8_gate_up_workspace_size": (C.c_size_t, [C.c_int] * 3),
+    "hx_f8_gate_up": (C.c_int, [C.c_void_p] * 4 + [C.POINTER(F8BlocksC)] * 2 + [C.c_int] * 3 +
+                      [C.c_float, C.c_void_p, C.c_void_p, C.c_size_t]),
     "hx_beam_select_workspace_size": (C.c_size_t, [C.c_int] * 4),
     "hx_beam_select": (C.c_int, [C.c_void_p] * 6 + [C.c_int] * 4 + [C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
                                                                    C.c_size_t]),

@@ -38,7 +38,7 @@ HIP_FLAGS = [
 # k step copies them back and forth (3 extra VALU moves per MFMA on gfx950, measured in the
 # generated code).
 _VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
-FILE_FLAGS = {f: _VGPR_FORM for f in ("hx_moe_prefill.hip", "hx_gemm.hip", "hx_w4.hip", *(f"hx_gemm_b{b}.hip" for b in range(1, 9)))}
+FILE_FLAGS = {f: _VGPR_FORM for f in ("hx_moe_prefill.hip", "hx_gemm.hip", "hx_w4.hip", "hx_f8.hip", *(f"hx_gemm_b{b}.hip" for b in range(1, 9)))}
 
 
 def _compile(src: Path) -> Path:

@@ -552,6 +552,156 @@ int hx_w4_embed(const hx_w4_words* w, const int64_t* tokens, void* out, int n, i
     return hip_status(hx::launch_w4_embed(a, tokens, out, n, scale, out_fp32 != 0, (hipStream_t)stream), "hx_w4_embed");
 }
 
+// ------------------------------------------------------------------ 8-bit floating point in blocks of 128
+
+namespace {
+
+constexpr int F8_MAX_K = 1 << 22, F8_MAX_N = 1 << 28;
+
+int f8_fail(const char* who, const char* what)
+{
+    snprintf(g_err, sizeof(g_err), "%s: %s", who, what);
+    return HX_ERR_INVALID;
+}
+
+const char* f8_extents(int M, int K)
+{
+    if (M < 0) return "negative M";
+    if (K <= 0 || K % 16) return "K must be a positive multiple of 16";
+    if (K > F8_MAX_K) return "K must be at most 2^22";
+    return nullptr;
+}
+
+const char* f8_blocks(const hx_f8_blocks* w, int N)
+{
+    if (!w || !w->codes || !w->scales) return "null pointer";
+    if (N <= 0 || N > F8_MAX_N) return "N must be positive and at most 2^28";
+    if ((uintptr_t)w->codes & 15) return "codes must be 16-byte aligned";
+    if ((uintptr_t)w->scales & 3) return "scales must be 4-byte aligned";
+    return nullptr;
+}
+
+// A call's buffer: rows rows of `width` elements, ld apart.
+struct F8Span {
+    uintptr_t at;
+    __int128 bytes;
+};
+F8Span f8_span(const void* p, int64_t rows, int64_t width, int64_t ld, int size)
+{
+    return {(uintptr_t)p, p && rows > 0 ? ((__int128)(rows - 1) * ld + width) * size : 0};
+}
+bool f8_apart(const F8Span& a, const F8Span& b)
+{
+    return !a.bytes || !b.bytes || a.at + a.bytes <= (__int128)b.at || b.at + b.bytes <= (__int128)a.at;
+}
+
+}  // namespace
+
+int hx_f8_quantize(const void* x, void* q, float* scales, int M, int K, int64_t ld, int dtype, hx_stream_t stream)
+{
+    static const char who[] = "hx_f8_quantize";
+    if (const char* what = f8_extents(M, K)) return f8_fail(who, what);
+    if (dtype != HX_DTYPE_HALF && dtype != HX_DTYPE_FLOAT) return f8_fail(who, "dtype must be HX_DTYPE_HALF or HX_DTYPE_FLOAT");
+    if (ld < K || ld % 8 || ld >> 40) return f8_fail(who, "ld must be a multiple of 8, at least K and below 2^40");
+    if (M == 0) return 0;
+    if (!x || !q || !scales) return f8_fail(who, "null pointer");
+    if (((uintptr_t)x | (uintptr_t)q) & 15) return f8_fail(who, "x and q must be 16-byte aligned");
+    if ((uintptr_t)scales & 3) return f8_fail(who, "scales must be 4-byte aligned");
+    const int kb = (K + 127) / 128;
+    const F8Span in = f8_span(x, M, K, ld, dtype == HX_DTYPE_FLOAT ? 4 : 2), oq = f8_span(q, M, K, K, 1), os = f8_span(scales, M, kb, kb, 4);
+    if (!f8_apart(in, oq) || !f8_apart(in, os) || !f8_apart(oq, os)) return f8_fail(who, "x, q and scales overlap");
+    return hip_status(hx::launch_f8_quantize(x, dtype == HX_DTYPE_FLOAT, static_cast<uint8_t*>(q), scales, M, K, (long)ld, (hipStream_t)stream), who);
+}
+
+int hx_f8_rms_norm(const void* x, int64_t ld, int x_dtype, const void* residual, void* out, int residual_dtype, const void* weight,
+                   int weight_dtype, void* y, void* q, float* scales, int M, int K, float eps, hx_stream_t stream)
+{
+    static const char who[] = "hx_f8_rms_norm";
+    if (const char* what = f8_extents(M, K)) return f8_fail(who, what);
+    for (int t : {x_dtype, residual_dtype, weight_dtype})
+        if (t != HX_DTYPE_HALF && t != HX_DTYPE_FLOAT) return f8_fail(who, "a dtype is neither HX_DTYPE_HALF nor HX_DTYPE_FLOAT");
+    if (ld < K || ld % 8 || ld >> 40) return f8_fail(who, "ld must be a multiple of 8, at least K and below 2^40");
+    if (!(eps >= 0.0f)) return f8_fail(who, "eps must not be negative");
+    if (M == 0) return 0;
+    if (!x || !weight) return f8_fail(who, "null pointer");
+    if (!residual != !out || !q != !scales) return f8_fail(who, "residual and out, and q and scales, are given together");
+    if (!y && !q) return f8_fail(who, "neither y nor q is asked for");
+    if (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)out | (uintptr_t)weight | (uintptr_t)y | (uintptr_t)q) & 15)
+        return f8_fail(who, "x, residual, out, weight, y and q must be 16-byte aligned");
+    if ((uintptr_t)scales & 3) return f8_fail(who, "scales must be 4-byte aligned");
+    const auto size = [](int t) { return t == HX_DTYPE_FLOAT ? 4 : 2; };
+    const int kb = (K + 127) / 128;
+    const F8Span in[] = {f8_span(x, M, K, ld, size(x_dtype)), f8_span(weight, 1, K, K, size(weight_dtype)), f8_span(residual, M, K, K, size(residual_dtype))};
+    const F8Span to[] = {f8_span(out, M, K, K, size(residual_dtype)), f8_span(y, M, K, K, 2), f8_span(q, M, K, K, 1), f8_span(scales, M, kb, kb, 4)};
+    for (int i = 0; i < 4; ++i) {
+        for (int j = 0; j < 3; ++j)
+            if (!(i == 0 && j == 2 && out == residual) && !f8_apart(to[i], in[j])) return f8_fail(who, "an output overlaps an input");
+        for (int j = 0; j < i; ++j)
+            if (!f8_apart(to[i], to[j])) return f8_fail(who, "outputs overlap");
+    }
+    const hx::F8NormArgs a{x, residual, out, weight, y, q, scales, (long)ld, K, eps, weight_dtype == HX_DTYPE_FLOAT};
+    return hip_status(hx::launch_f8_norm(a, M, x_dtype == HX_DTYPE_FLOAT, residual_dtype == HX_DTYPE_FLOAT, (hipStream_t)stream), who);
+}
+
+size_t hx_f8_gemm_workspace_size(int M, int N, int K)
+{
+    if (M <= 0 || N <= 0 || N > F8_MAX_N || f8_extents(M, K)) return 0;
+    return hx::f8_gemm_workspace_bytes(M, N, K);
+}
+
+int hx_f8_gemm(void* y, const void* x, const float* x_scales, const hx_f8_blocks* w, int M, int N, int K, int y_fp32,
+               hx_stream_t stream, void* workspace, size_t workspace_bytes)
+{
+    static const char who[] = "hx_f8_gemm";
+    if (const char* what = f8_extents(M, K)) return f8_fail(who, what);
+    if (const char* what = f8_blocks(w, N)) return f8_fail(who, what);
+    if (M == 0) return 0;
+    if (!y || !x || !x_scales) return f8_fail(who, "null pointer");
+    if ((uintptr_t)x & 15) return f8_fail(who, "x must be 16-byte aligned");
+    if (((uintptr_t)x_scales & 3) || ((uintptr_t)y & (y_fp32 ? 3 : 1))) return f8_fail(who, "x_scales or y is not aligned to its type");
+    if ((uintptr_t)workspace & 15) return fail(HX_ERR_WORKSPACE, "hx_f8_gemm: workspace must be 16-byte aligned");
+    const int kb = (K + 127) / 128;
+    const F8Span to = f8_span(y, M, N, N, y_fp32 ? 4 : 2);
+    if (!f8_apart(to, f8_span(x, M, K, K, 1)) || !f8_apart(to, f8_span(x_scales, M, kb, kb, 4))) return f8_fail(who, "y overlaps x or x_scales");
+    return hip_status(hx::launch_f8_gemm(static_cast<const uint8_t*>(x), x_scales, {static_cast<const uint8_t*>(w->codes), w->scales}, y, M, N, K,
+                                         y_fp32 != 0, workspace, workspace_bytes, (hipStream_t)stream),
+                      who);
+}
+
+size_t hx_f8_gate_up_workspace_size(int M, int N, int K)
+{
+    if (M <= 0 || N <= 0 || N > F8_MAX_N || N % 16 || f8_extents(M, K)) return 0;
+    return hx::f8_gate_up_workspace_bytes(M, N, K);
+}
+
+int hx_f8_gate_up(void* q, float* scales, const void* x, const float* x_scales, const hx_f8_blocks* gate, const hx_f8_blocks* up,
+                  int M, int N, int K, float limit, hx_stream_t stream, void* workspace, size_t workspace_bytes)
+{
+    static const char who[] = "hx_f8_gate_up";
+    if (const char* what = f8_extents(M, K)) return f8_fail(who, what);
+    for (const hx_f8_blocks* w : {gate, up})
+        if (const char* what = f8_blocks(w, N)) return f8_fail(who, what);
+    if (N % 16) return f8_fail(who, "N must be a multiple of 16");
+    if (!(limit > 0.0f)) return f8_fail(who, "limit must be positive");
+    if (M == 0) return 0;
+    if (!q || !scales || !x || !x_scales) return f8_fail(who, "null pointer");
+    if (((uintptr_t)x | (uintptr_t)q) & 15) return f8_fail(who, "x and q must be 16-byte aligned");
+    if (((uintptr_t)x_scales | (uintptr_t)scales) & 3) return f8_fail(who, "scales must be 4-byte aligned");
+    const int kb = (K + 127) / 128, nb = (N + 127) / 128;
+    const F8Span in[] = {f8_span(x, M, K, K, 1), f8_span(x_scales, M, kb, kb, 4)}, to[] = {f8_span(q, M, N, N, 1), f8_span(scales, M, nb, nb, 4)};
+    for (const F8Span& o : to)
+        for (const F8Span& i : in)
+            if (!f8_apart(o, i)) return f8_fail(who, "an output overlaps an input");
+    if (!f8_apart(to[0], to[1])) return f8_fail(who, "outputs overlap");
+    const size_t need = hx::f8_gate_up_workspace_bytes(M, N, K);
+    if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))
+        return fail(HX_ERR_WORKSPACE, "hx_f8_gate_up: workspace missing, not 16-byte aligned or smaller than hx_f8_gate_up_workspace_size");
+    return hip_status(hx::launch_f8_gate_up(static_cast<const uint8_t*>(x), x_scales, {static_cast<const uint8_t*>(gate->codes), gate->scales},
+                                            {static_cast<const uint8_t*>(up->codes), up->scales}, static_cast<uint8_t*>(q), scales, M, N, K,
+                                            limit, workspace, workspace_bytes, (hipStream_t)stream),
+                      who);
+}
+
 // ------------------------------------------------------------------ beam search
 
 size_t hx_beam_select_workspace_size(int batch, int beams, int vocab, int n)

@@ -96,6 +96,31 @@ hipError_t launch_w4_gemm(const _Float16* x, const W4Args& a, void* y, int M, bo
 hipError_t launch_w4_embed(const W4Args& a, const int64_t* tokens, void* out, int n, float scale, bool out_fp32,
                            hipStream_t st);
 
+// 8-bit floating point in blocks of 128 (hx_f8.hpp): activations (hx_f8_act.hip), linear and gated pair (hx_f8.hip)
+struct F8NormArgs {
+    const void *x, *residual;  // [M] rows, ld elements from one of x to the next; residual [M][K], or null
+    void* out;                 // [M][K]: x + residual
+    const void* weight;        // [K], fp32 or fp16
+    void *y, *q;               // [M][K] fp16 and e4m3, or null
+    float* scales;             // [M][ceil(K / 128)], of q
+    long ld;
+    int K;
+    float eps;
+    bool weight32;
+};
+hipError_t launch_f8_norm(const F8NormArgs& a, int M, bool x32, bool r32, hipStream_t st);
+hipError_t launch_f8_quantize(const void* x, bool x32, uint8_t* q, float* scales, int M, int K, long ld, hipStream_t st);
+struct F8Blocks {
+    const uint8_t* codes;  // [N][K]
+    const float* scales;   // [ceil(N / 128)][ceil(K / 128)]
+};
+size_t f8_gemm_workspace_bytes(int M, int N, int K);
+hipError_t launch_f8_gemm(const uint8_t* x, const float* xs, const F8Blocks& w, void* y, int M, int N, int K, bool y_fp32, void* ws,
+                          size_t ws_bytes, hipStream_t st);
+size_t f8_gate_up_workspace_bytes(int M, int N, int K);
+hipError_t launch_f8_gate_up(const uint8_t* x, const float* xs, const F8Blocks& gate, const F8Blocks& up, uint8_t* q, float* scales,
+                             int M, int N, int K, float limit, void* ws, size_t ws_bytes, hipStream_t st);
+
 // beam search's selection and reordering of states (hx_beam.hip)
 struct BeamArgs {
     const float* cum;     // [batch * beams]

@@ -261,6 +261,47 @@ int hx_w4_gemm(void* y, const void* x, const hx_w4_words* w, int M, int N, int K
 int hx_w4_embed(const hx_w4_words* w, const int64_t* tokens, void* out, int n, int N, int K, float scale, int out_fp32,
                 hx_stream_t stream);
 
+/* ---- 8-bit floating point in blocks of 128 --------------------------------------------------- */
+
+/* Values in e4m3 (4 exponent bits, 3 mantissa bits, largest 448) with an fp32 scale for each block of 128 consecutive k of an input
+ * row, or of 128 x 128 weights; the last blocks may be short (no counterpart in the reference):
+ *   a = max(largest |v| of the block, 2^-100)   scale = a / 448   code = e4m3(v * (448 / a)), fp32 operations, ties to even
+ * A block with a NaN or an infinity stands for NaN throughout.  K % 16 == 0, K <= 2^22 in all calls of this section; M == 0 is a
+ * no-op (the pointers may then be NULL); outputs overlap neither inputs nor each other but where that is said. */
+
+/* q uint8 [M][K] and scales fp32 [M][ceil(K / 128)] of x (fp16 or fp32 by dtype, HX_DTYPE_*; rows ld elements apart, ld % 8 == 0).
+ * x and q 16-byte aligned. */
+int hx_f8_quantize(const void* x, void* q, float* scales, int M, int K, int64_t ld, int dtype, hx_stream_t stream);
+
+/* h = x + residual, rounded to residual's type; n = h / sqrt(mean over K of h^2 + eps) * weight in fp32 (fp32 sums); y = fp16(n);
+ * q, scales = blocks of n before that rounding.  x (x_dtype) as in hx_f8_quantize; residual and out [M][K] (residual_dtype), out receives h and
+ * may be residual itself; both NULL: h = x.  weight [K] (weight_dtype).  y fp16 [M][K], or NULL; q and scales as in hx_f8_quantize, or
+ * both NULL.  All 16-byte aligned but scales. */
+int hx_f8_rms_norm(const void* x, int64_t ld, int x_dtype, const void* residual, void* out, int residual_dtype, const void* weight,
+                   int weight_dtype, void* y, void* q, float* scales, int M, int K, float eps, hx_stream_t stream);
+
+/* One linear W[N][K]: codes uint8 [N][K] (16-byte aligned), scales fp32 [ceil(N / 128)][ceil(K / 128)].  N <= 2^28. */
+typedef struct hx_f8_blocks {
+    const void* codes;
+    const float* scales;
+} hx_f8_blocks;
+
+/* y[M][N] = x W^T: x and x_scales as hx_f8_quantize gives them, y fp32 (y_fp32) or fp16: fp32 sums rounded once.  The codes' products
+ * are exact, and a block's scales are applied to its fp32 sum.  The workspace is optional: a call with at least hx_f8_gemm_workspace_size(M, N, K)
+ * bytes (0: the shape has no use for it) splits K over more workgroups where there are few, with the fp32 sums in another order
+ * than without; NULL or fewer bytes do without. */
+size_t hx_f8_gemm_workspace_size(int M, int N, int K);
+int hx_f8_gemm(void* y, const void* x, const float* x_scales, const hx_f8_blocks* w, int M, int N, int K, int y_fp32,
+               hx_stream_t stream, void* workspace, size_t workspace_bytes);
+
+/* Gate and up projections of a feed-forward block and its activation: with g = x gate^T, u = x up^T (fp32),
+ *   v = silu(min(g, limit)) * clamp(u, -limit, limit)      q, scales = blocks of v along N, ready for the down projection
+ * gate, up: W[N][K], N % 16 == 0; limit > 0 (infinity: no clamp).  A NaN stays a NaN.  The workspace is needed where
+ * hx_f8_gate_up_workspace_size(M, N, K) is not 0. */
+size_t hx_f8_gate_up_workspace_size(int M, int N, int K);
+int hx_f8_gate_up(void* q, float* scales, const void* x, const float* x_scales, const hx_f8_blocks* gate, const hx_f8_blocks* up,
+                  int M, int N, int K, float limit, hx_stream_t stream, void* workspace, size_t workspace_bytes);
+
 /* ---- beam search ---------------------------------------------------------------------------- */
 
 /* Selection over beams and vocabulary (no counterpart in the reference, which samples one sequence).  Row
