@@ -106,10 +106,10 @@ HX_INLINE void f8_finish_block(const F8Call& c, const float* v, int rows, int m0
 // The 16 columns of a matrix instruction are R = 16 / S weight rows by S consecutive blocks of 128 k: column s R + r is row r, block s, and
 // row s R + t of the other operand is input row t, block s.  Of the products those with equal s are wanted; with few rows of x the
 // others buy whole cache lines of each weight row and S times as many pieces of work.  S = 4 serves 4 rows of x, 2 serves 8, 1 serves 16.
-// A wave owns NS spans (S blocks each) of every WK NS, keeps x for them in registers as fp16 and goes over tiles of NT R weight rows
+// A wave owns NS spans (S blocks each) of every WK NS, keeps x for them in registers and goes over tiles of NT R weight rows
 // (of a gated pair: NT / 2 of gate and as many of up); codes are replaced by the next tile's as soon as they are converted.
 template <int S, int WAVES, int NS, int NT, bool PAIR>
-__global__ __launch_bounds__(64 * WAVES) void f8_rows_kernel(F8Call a, int wk)
+__global__ __launch_bounds__(64 * WAVES, 2) void f8_rows_kernel(F8Call a, int wk)
 {
     constexpr int R = 16 / S, H = 4 / S, NP = PAIR ? NT / 2 : NT;  // weight rows of a load; 4-row pieces of x in a column; loads of rows
     __shared__ float red[WAVES][NT][4 * H][16];
@@ -120,24 +120,21 @@ __global__ __launch_bounds__(64 * WAVES) void f8_rows_kernel(F8Call a, int wk)
     const int rows_wg = wr * NP * R, tiles = (a.N + rows_wg - 1) / rows_wg;  // rows_wg: a power of two up to 128
 
     const __amdgpu_buffer_rsrc_t rx = mf_rsrc(a.x, (size_t)a.M * a.K), rxs = mf_rsrc(a.xs, (size_t)a.M * a.kb * 4);
-    F8Half xa[NS];
+    F8Raw xr[NS];
     float sx[NS][4];
     auto block = [&](int i, int kb) { return ((kb * NS + i) * wk + kw) * S + s; };
     auto load_x = [&](int kb) {
-        F8Raw raw[NS];
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             const int b = block(i, kb), k = b * F8_BLOCK + 16 * kg;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-                raw[i].p[h] = __builtin_bit_cast(f8_u4, __builtin_amdgcn_raw_buffer_load_b128(rx, k + 64 * h < a.K ? r * a.K + k + 64 * h : F8_NONE, 0, 0));
+                xr[i].p[h] = __builtin_bit_cast(f8_u4, __builtin_amdgcn_raw_buffer_load_b128(rx, k + 64 * h < a.K ? r * a.K + k + 64 * h : F8_NONE, 0, 0));
 #pragma unroll
             for (int e = 0; e < 4; ++e)  // of the input rows whose products this lane gets
                 sx[i][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
                                                          rxs, kg / H == s && b < a.kb ? ((kg % H * 4 + e) * a.kb + b) * 4 : F8_NONE, 0, 0));
         }
-#pragma unroll
-        for (int i = 0; i < NS; ++i) xa[i] = f8_half(raw[i]);
     };
     F8Raw w[NS][NT];
     float sw[NS][PAIR ? 2 : 1];
@@ -177,6 +174,7 @@ __global__ __launch_bounds__(64 * WAVES) void f8_rows_kernel(F8Call a, int wk)
             if (wrap) aim(tile + gridDim.x);
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
+                const F8Half xa = f8_half(xr[i]);
                 float f[PAIR ? 2 : 1][4];
 #pragma unroll
                 for (int p = 0; p < (PAIR ? 2 : 1); ++p)
@@ -189,7 +187,7 @@ __global__ __launch_bounds__(64 * WAVES) void f8_rows_kernel(F8Call a, int wk)
                     __builtin_amdgcn_sched_barrier(0);  // the loads stay here, ahead of these codes' products
                     hx_f4 t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(xa[i].k[j], b.k[j], t, 0, 0, 0);
+                    for (int j = 0; j < 4; ++j) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(xa.k[j], b.k[j], t, 0, 0, 0);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[n][e] = __builtin_fmaf(f[PAIR ? n & 1 : 0][e], t[e], acc[n][e]);
                 }
@@ -236,28 +234,32 @@ __global__ __launch_bounds__(64 * WAVES) void f8_rows_kernel(F8Call a, int wk)
 //
 // A workgroup of WN x WM waves computes BN = 16 WN TN weight rows (of a pair: BN / 2 of gate and as many of up) by BM = 16 WM TM input
 // rows; the weights are the operand whose rows become the products' rows, so that a lane has four consecutive outputs of one input
-// row and needs one scale of x for them.  A step takes a block of 128 k: BN + BM rows of 128 bytes and the scales of x, in a ring of PF
-// LDS stages that buffer loads fill directly.  16-byte piece u of row r lies at piece u ^ (r & 7), so that the 16 rows of a fragment
-// read touch all banks.
+// row and needs one scale of x for them.  A step takes a block of 128 k: BN + BM rows of 128 bytes, which buffer loads put into LDS
+// directly, PF stages in turn.  16-byte piece u of row r lies at piece u ^ (r & 7), so that the 16 rows of a fragment
+// read touch all banks (245 bytes a cycle; 64 without).
+// The scales of x come for four steps at a time, 16 rows a load, two groups ahead: with a load from 64 rows a step, 2000 rows of 4096 -> 24576
+// took 273 us where 224 were without any.
 struct F8Split {
     int splits, steps;  // workgroups that share a tile's K, steps of each
 };
 
-template <int WN, int WM, int TN, int TM>
+template <int WN, int WM, int TN, int TM, int PF>
 struct F8TileSize {
     static constexpr int WAVES = WN * WM, BN = 16 * WN * TN, BM = 16 * WM * TM;
-    static constexpr int CODES = (BN + BM) * F8_BLOCK, STAGE = CODES + WAVES * 256;  // bytes; the scales of 64 rows a wave
-    static constexpr int NL = CODES / (1024 * WAVES);  // code loads of a wave a step
-    static_assert(CODES % (1024 * WAVES) == 0 && BM <= 64 * WAVES);
+    static constexpr int X = PF * BN * F8_BLOCK, SCALES = X + PF * BM * F8_BLOCK;  // where they begin in LDS
+    static constexpr int GROUP = BM * 16, NOTHING = SCALES + 3 * GROUP, BYTES = NOTHING + 256 * WAVES;  // of scales: [rows][4]; where loads of none go
+    static constexpr int NW = BN / (8 * WAVES), NX = BM / (8 * WAVES);  // loads of a wave a step
+    static_assert(BN % (8 * WAVES) == 0 && BM % (8 * WAVES) == 0 && BM <= 64 * WAVES && PF <= 8);
 };
 
 template <int WN, int WM, int TN, int TM, int PF, bool EXACT, bool PAIR>
 __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split sp)
 {
-    using Z = F8TileSize<WN, WM, TN, TM>;
-    constexpr int BN = Z::BN, BM = Z::BM, NL = Z::NL, WAVES = Z::WAVES;
+    using Z = F8TileSize<WN, WM, TN, TM, PF>;
+    constexpr int BN = Z::BN, BM = Z::BM, NW = Z::NW, NX = Z::NX, WAVES = Z::WAVES;
+    static_assert(!PAIR || NW % 2 == 0);
     constexpr int CN = PAIR ? BN / 2 : BN, TP = PAIR ? TN / 2 : TN;  // outputs of a tile along N; a wave's row blocks of them
-    extern __shared__ __align__(16) uint8_t f8_lds[];  // [PF][STAGE]
+    extern __shared__ __align__(16) uint8_t f8_lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wn = wave % WN, wm = wave / WN, col = lane & 15, kg = lane >> 4;
     const int tile = (int)(blockIdx.x / sp.splits), split = (int)(blockIdx.x % sp.splits);
@@ -268,22 +270,42 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
     const int m0 = (xcd ? (tile >> 3) % mt : tile % mt) * BM, n0 = (xcd ? (tile >> 3) / mt * 8 + (tile & 7) : tile / mt) * CN;
     const int nrows = min(a.N - n0, CN), mrows = min(a.M - m0, BM);
 
-    // Loads of a wave: 8 rows of 128 bytes each.  LDS rows: the weights' (of a pair: gate, up), then x.
+    // A wave's load i takes 8 rows of 128 bytes, rows 8 (i WAVES + wave) and behind of the weights (of a pair: gate, then up) or of x.  The
+    // descriptors move on with the steps and end with the matrix; behind the last step they are empty.
+    typedef __attribute__((address_space(3))) void* lds_t;
+    const long lrow = 8 * wave;
+    const uint8_t* base[3] = {a.w[0].codes + (n0 + lrow) * a.K, PAIR ? a.w[1].codes + (n0 + lrow) * a.K : nullptr, a.x + (m0 + lrow) * a.K};
+    const long bytes[2] = {(nrows - lrow) * a.K, (mrows - lrow) * a.K};
     const int lane_off = (lane >> 3) * a.K + 16 * ((lane & 7) ^ (lane >> 3));
-    auto load = [&](int i, int slot, int c) {
-        const int r = 8 * (wave * NL + i);  // first LDS row
-        const int part = r >= BN ? 2 : PAIR && r >= CN ? 1 : 0, row = r - (part == 2 ? BN : part * CN);
-        const uint8_t* base = part == 2 ? a.x + (size_t)m0 * a.K : (part == 1 ? a.w[1].codes : a.w[0].codes) + (size_t)n0 * a.K;
-        const long at = (long)row * a.K + (long)c * F8_BLOCK, bytes = (long)(part == 2 ? mrows : nrows) * a.K;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(mf_rsrc(base + at, (size_t)(c < steps ? max(bytes - at, 0l) : 0l)),
-                                                 (__attribute__((address_space(3))) void*)(f8_lds + slot * Z::STAGE + r * F8_BLOCK), 16, lane_off, 0, 0, 0);
+    auto desc = [&](int p, int c) {
+        const long at = (long)c * F8_BLOCK;
+        return mf_rsrc(base[p] + at, (size_t)(c < steps ? max(bytes[p >> 1] - at, 0l) : 0l));
     };
-    const int scale_off = (64 * wave + lane) * a.kb * 4;
-    auto load_scales = [&](int slot, int c) {
-        const float* base = a.xs + (size_t)m0 * a.kb + c;
-        const size_t bytes = c < steps ? ((size_t)mrows * a.kb - c) * 4 : 0;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(mf_rsrc(base, bytes),
-                                                 (__attribute__((address_space(3))) void*)(f8_lds + slot * Z::STAGE + Z::CODES + wave * 256), 4, scale_off, 0, 0, 0);
+    auto load_w = [&](int slot, int c) {
+        const __amdgpu_buffer_rsrc_t d[2] = {desc(0, c), desc(PAIR ? 1 : 0, c)};
+        uint8_t* st = f8_lds + (slot * BN + 8 * wave) * F8_BLOCK;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            const int r = 8 * WAVES * i, up = PAIR && r >= CN ? 1 : 0;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(d[up], (lds_t)(st + r * F8_BLOCK), 16, lane_off + (r - up * CN) * a.K, 0, 0, 0);
+        }
+    };
+    auto load_x = [&](int slot, int c) {
+        const __amdgpu_buffer_rsrc_t d = desc(2, c);
+        uint8_t* st = f8_lds + Z::X + (slot * BM + 8 * wave) * F8_BLOCK;
+#pragma unroll
+        for (int i = 0; i < NX; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lds_t)(st + 8 * WAVES * i * F8_BLOCK), 16, lane_off + 8 * WAVES * i * a.K, 0, 0, 0);
+    };
+    // Part s of group g of the scales: 16 rows a wave from 16 (s WAVES + wave) on, of steps first + 4 g and the three behind.  Loads that touch no
+    // memory write zeros.
+    const float* xs = a.xs + (size_t)m0 * a.kb + first;
+    auto load_scales = [&](int buf, int g, int s) {
+        const int row = 16 * (s * WAVES + wave);
+        const bool any = row < BM && first + 4 * g < steps;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(mf_rsrc(xs + 4 * g, any ? ((size_t)mrows * a.kb - first - 4 * g) * 4 : 0),
+                                                 (lds_t)(f8_lds + (row < BM ? Z::SCALES + buf * Z::GROUP + row * 16 : Z::NOTHING + 256 * wave)), 4,
+                                                 any ? ((row + (lane >> 2)) * a.kb + (lane & 3)) * 4 : F8_NONE, 0, 0, 0);
     };
     hx_f4 acc[TN][TM];
 #pragma unroll
@@ -291,85 +313,120 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
 #pragma unroll
         for (int j = 0; j < TM; ++j) acc[i][j] = hx_f4{0.f, 0.f, 0.f, 0.f};
     // LDS offsets of a lane's pieces of the first row block on either side
-    const int pa = (wn * TP * 16 + col) * F8_BLOCK + 16 * (kg ^ (col & 7)), pb = (BN + wm * TM * 16 + col) * F8_BLOCK + 16 * (kg ^ (col & 7));
-    const float* ws0 = a.w[0].scales + (size_t)(n0 / F8_BLOCK) * a.kb;
-    const float* ws1 = PAIR ? a.w[1].scales + (size_t)(n0 / F8_BLOCK) * a.kb : nullptr;
+    const int piece = 16 * (kg ^ (col & 7)), pa = (wn * TP * 16 + col) * F8_BLOCK + piece, pb = (wm * TM * 16 + col) * F8_BLOCK + piece;
     // rows of a tile of more than 128 lie in several blocks of weights
-    const int wblock = CN > F8_BLOCK ? min(n0 + wn * TP * 16, a.N - 1) / F8_BLOCK - n0 / F8_BLOCK : 0;
+    const int wblock = CN > F8_BLOCK ? min(n0 + wn * TP * 16, a.N - 1) / F8_BLOCK : n0 / F8_BLOCK;
     static_assert(CN <= F8_BLOCK || TP * 16 <= F8_BLOCK);
+    // Scales of the weights by scalar loads, a step ahead: as vector loads, to which they turn by themselves between the barriers, their
+    // wait is one for all loads in flight.
+    typedef const __attribute__((address_space(4))) float* scalar_t;
+    const scalar_t ws[2] = {(scalar_t)(a.w[0].scales + (size_t)wblock * a.kb), PAIR ? (scalar_t)(a.w[1].scales + (size_t)wblock * a.kb) : nullptr};
+    float wnext[2] = {ws[0][first], PAIR ? ws[1][first] : 0.0f};
 
-    auto step = [&](int slot, int c) {
-        const uint8_t* st = f8_lds + slot * Z::STAGE;
-        const int left = a.K - c * F8_BLOCK;  // of K in this block and behind
-        auto fragment = [&](int off) {
+    auto step = [&](const uint8_t* sw, const uint8_t* sx, const float* sc, int c, auto whole) {
+        auto fragment = [&](const uint8_t* p) {
             F8Raw v;
-            v.p[0] = *reinterpret_cast<const f8_u4*>(st + off);
-            v.p[1] = *reinterpret_cast<const f8_u4*>(st + (off ^ 64));
-            if (left < F8_BLOCK) {  // what lies behind a row's K counts as 0
+            v.p[0] = *reinterpret_cast<const f8_u4*>(p);
+            v.p[1] = *reinterpret_cast<const f8_u4*>(f8_lds + ((p - f8_lds) ^ 64));
+            if constexpr (!decltype(whole)::value) {  // what lies behind a row's K counts as 0
+                const int left = a.K - c * F8_BLOCK;
                 if (16 * kg >= left) v.p[0] = f8_u4{};
                 if (64 + 16 * kg >= left) v.p[1] = f8_u4{};
             }
             return v;
         };
-        const float* sxs = reinterpret_cast<const float*>(st + Z::CODES) + wm * TM * 16 + col;
-        float f0[TM], f1[TM];
-        const float s0 = ws0[(size_t)wblock * a.kb + c], s1 = PAIR ? ws1[c] : 0.0f;
+        auto weights = [&](int i) { return fragment(sw + pa + (PAIR ? i / TP * CN + i % TP * 16 : i * 16) * F8_BLOCK); };
+        const float s[2] = {wnext[0], wnext[1]};
+        const int next = min(c + 1, a.kb - 1);
+        wnext[0] = ws[0][next];
+        if constexpr (PAIR) wnext[1] = ws[1][next];
+        F8Raw w, x[TM];
+        float f[TM];
 #pragma unroll
-        for (int j = 0; j < TM; ++j) f0[j] = sxs[16 * j] * s0, f1[j] = sxs[16 * j] * s1;
+        for (int j = 0; j < TM; ++j) x[j] = fragment(sx + pb + j * 16 * F8_BLOCK);
+        w = weights(0);
+#pragma unroll
+        for (int j = 0; j < TM; ++j) f[j] = sc[(wm * TM * 16 + 16 * j + col) * 4];
         if constexpr (EXACT) {
             F8Half b[TM];
 #pragma unroll
-            for (int j = 0; j < TM; ++j) b[j] = f8_half(fragment(pb + j * 16 * F8_BLOCK));
+            for (int j = 0; j < TM; ++j) b[j] = f8_half(x[j]);
 #pragma unroll
             for (int i = 0; i < TN; ++i) {
-                const F8Half w = f8_half(fragment(pa + (PAIR ? i / TP * CN + i % TP * 16 : i * 16) * F8_BLOCK));
+                __builtin_amdgcn_sched_barrier(0);
                 hx_f4 t[TM];
 #pragma unroll
-                for (int j = 0; j < TM; ++j) t[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.k[0], b[j].k[0], hx_f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                for (int h = 0; h < 2; ++h) {
+                    const hx_h8 k0 = f8_half8(w.p[h][0], w.p[h][1]), k1 = f8_half8(w.p[h][2], w.p[h][3]);
+                    if (h == 1 && i + 1 < TN) w = weights(i + 1);
 #pragma unroll
-                for (int k = 1; k < 4; ++k)
+                    for (int j = 0; j < TM; ++j) t[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, b[j].k[2 * h], h ? t[j] : hx_f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
-                    for (int j = 0; j < TM; ++j) t[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.k[k], b[j].k[k], t[j], 0, 0, 0);
-#pragma unroll
-                for (int j = 0; j < TM; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(PAIR && i >= TP ? f1[j] : f0[j], t[j][e], acc[i][j][e]);
-            }
-        } else {
-            F8Raw b[TM];
-#pragma unroll
-            for (int j = 0; j < TM; ++j) b[j] = fragment(pb + j * 16 * F8_BLOCK);
-#pragma unroll
-            for (int i = 0; i < TN; ++i) {
-                const F8Raw w = fragment(pa + (PAIR ? i / TP * CN + i % TP * 16 : i * 16) * F8_BLOCK);
+                    for (int j = 0; j < TM; ++j) t[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, b[j].k[2 * h + 1], t[j], 0, 0, 0);
+                }
 #pragma unroll
                 for (int j = 0; j < TM; ++j) {
-                    const hx_f4 t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(f8_v8, w), __builtin_bit_cast(f8_v8, b[j]),
-                                                                                     hx_f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+                    const float r = f[j] * s[PAIR && i >= TP];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(PAIR && i >= TP ? f1[j] : f0[j], t[e], acc[i][j][e]);
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(r, t[j][e], acc[i][j][e]);
                 }
             }
+        } else {
+            // One product and four of the sums of the row block before at a time: a wave's vector instructions fit behind its own products.
+            hx_f4 t[2][TM];
+            auto scaled = [&](int i, int j) {
+                const float r = f[j] * s[PAIR && i >= TP];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(r, t[i & 1][j][e], acc[i][j][e]);
+            };
+#pragma unroll
+            for (int i = 0; i < TN; ++i) {
+                const F8Raw v = w;
+                if (i + 1 < TN) w = weights(i + 1);
+#pragma unroll
+                for (int j = 0; j < TM; ++j) {
+                    t[i & 1][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(f8_v8, v), __builtin_bit_cast(f8_v8, x[j]),
+                                                                                   hx_f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (i > 0) scaled(i - 1, j);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < TM; ++j) scaled(TN - 1, j);
         }
     };
+    constexpr int NS = (BM + 16 * WAVES - 1) / (16 * WAVES);  // parts of a group of scales
+    static_assert(NS <= 4);
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int u = 0; u < NS; ++u) load_scales(g, g, u);
 #pragma unroll
     for (int u = 0; u < PF - 1; ++u) {
-#pragma unroll
-        for (int i = 0; i < NL; ++i) load(i, u, first + u);
-        load_scales(u, first + u);
-    }
-    int slot = 0;
-    for (int c = first; c < steps; ++c) {
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(qt_vmcnt((PF - 2) * (NL + 1)));  // this step's loads of this wave have arrived
+        load_x(u, first + u);
+        load_w(u, first + u);
+    }
+    int slot = 0, group = 0;  // of weights (and x), of scales
+    auto round = [&](int c, auto whole) {
+        const int d = c - first;
+        // This step's loads of this wave have arrived, once at most those of the PF - 2 steps before it are outstanding.
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(qt_vmcnt((PF - 2) * (NW + NX + 1)));
         hx_lds_barrier();  // and the other waves'; the stage of the step before is no longer read
         const int ahead = slot == 0 ? PF - 1 : slot - 1;
-#pragma unroll
-        for (int i = 0; i < NL; ++i) load(i, ahead, c + PF - 1);
-        load_scales(ahead, c + PF - 1);
-        step(slot, c);
+        load_scales(group == 0 ? 2 : group - 1, (d >> 2) + 2, d & 3);
+        load_x(ahead, c + PF - 1);
+        load_w(ahead, c + PF - 1);
+        step(f8_lds + slot * BN * F8_BLOCK, f8_lds + Z::X + slot * BM * F8_BLOCK,
+             reinterpret_cast<const float*>(f8_lds + Z::SCALES + group * Z::GROUP) + (d & 3), c, whole);
         slot = slot + 1 == PF ? 0 : slot + 1;
-    }
+        if ((d & 3) == 3) group = group == 2 ? 0 : group + 1;
+    };
+    const int whole = min(steps, a.K / F8_BLOCK);  // the end of the steps without a part past K
+    for (int c = first; c < whole; ++c) round(c, std::true_type{});
+    if (whole < steps) round(whole, std::false_type{});
     // the accesses behind the last step are done with the stages too
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(qt_vmcnt(0));
@@ -395,14 +452,24 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
             }
     }
     if constexpr (!PAIR) {
+        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+        const size_t size = a.y_fp32 ? 4 : 2;
+        const bool four = a.N % 4 == 0 && reinterpret_cast<uintptr_t>(a.y) % (4 * size) == 0;  // four outputs of a row in one store
 #pragma unroll
         for (int i = 0; i < TN; ++i)
 #pragma unroll
             for (int j = 0; j < TM; ++j) {
                 const int n = n0 + (wn * TN + i) * 16 + 4 * kg, m = m0 + (wm * TM + j) * 16 + col;
+                const size_t at = (size_t)m * a.N + n;
+                if (m >= a.M || n >= a.N) continue;
+                if (four) {
+                    if (a.y_fp32) *reinterpret_cast<hx_f4*>(static_cast<float*>(a.y) + at) = acc[i][j];
+                    else *reinterpret_cast<h4*>(static_cast<_Float16*>(a.y) + at) = __builtin_convertvector(acc[i][j], h4);
+                } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (m < a.M && n + e < a.N) f8_store(a.y, (size_t)m * a.N + n + e, acc[i][j][e], a.y_fp32);
+                    for (int e = 0; e < 4; ++e)
+                        if (n + e < a.N) f8_store(a.y, at + e, acc[i][j][e], a.y_fp32);
+                }
             }
     } else {
         const int nb = (a.N + F8_BLOCK - 1) / F8_BLOCK, block = n0 / F8_BLOCK;
@@ -526,9 +593,10 @@ hipError_t rows_launch(const F8Call& c, hipStream_t st)
 template <int WN, int WM, int TN, int TM, int PF, bool EXACT, bool PAIR>
 hipError_t tile_launch(const F8Call& c, const F8Plan& p, hipStream_t st)
 {
-    using Z = F8TileSize<WN, WM, TN, TM>;
-    hipLaunchKernelGGL((f8_tile_kernel<WN, WM, TN, TM, PF, EXACT, PAIR>), dim3((unsigned)(p.tiles * p.splits)), dim3(64 * Z::WAVES),
-                       PF * Z::STAGE, st, c, F8Split{p.splits, p.steps});
+    using Z = F8TileSize<WN, WM, TN, TM, PF>;
+    static_assert(Z::BYTES <= 160 * 1024);
+    hipLaunchKernelGGL((f8_tile_kernel<WN, WM, TN, TM, PF, EXACT, PAIR>), dim3((unsigned)(p.tiles * p.splits)), dim3(64 * Z::WAVES), Z::BYTES, st, c,
+                       F8Split{p.splits, p.steps});
     return hipGetLastError();
 }
 
