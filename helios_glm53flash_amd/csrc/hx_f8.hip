@@ -61,6 +61,20 @@ HX_INLINE void f8_store(void* y, size_t i, float v, bool y_fp32)
     else static_cast<_Float16*>(y)[i] = (_Float16)v;
 }
 
+// Sum over the S parts of a span (f8_rows_kernel): lane 16 s H + s R + l holds part s of what lane l gets.
+template <int S>
+HX_INLINE float f8_parts_sum(float v)
+{
+    auto turned = [](uint32_t x, auto ctrl) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xf, 0xf, false)); };
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    v += turned(__builtin_amdgcn_permlane32_swap(u, u, false, false)[1], std::integral_constant<int, 0x128>{});  // lane + 40: the upper half, row_ror:8
+    if constexpr (S == 4) {
+        const uint32_t q = __builtin_bit_cast(uint32_t, v);
+        v += turned(__builtin_amdgcn_permlane16_swap(q, q, false, false)[1], std::integral_constant<int, 0x12c>{});  // lane + 20: the odd row, row_ror:12
+    }
+    return v;
+}
+
 // A call.  w[1] is the up projection of a gated pair (w[0] the gate), else unused.
 struct F8Call {
     const uint8_t* x;
@@ -103,58 +117,84 @@ HX_INLINE void f8_finish_block(const F8Call& c, const float* v, int rows, int m0
 
 // ---- up to 16 rows
 //
-// The 16 columns of a matrix instruction are R = 16 / S weight rows by S consecutive blocks of 128 k: column s R + r is row r, block s, and
-// row s R + t of the other operand is input row t, block s.  Of the products those with equal s are wanted; with few rows of x the
-// others buy whole cache lines of each weight row and S times as many pieces of work.  S = 4 serves 4 rows of x, 2 serves 8, 1 serves 16.
-// A wave owns NS spans (S blocks each) of every WK NS, keeps x for them in registers and goes over tiles of NT R weight rows
-// (of a gated pair: NT / 2 of gate and as many of up); codes are replaced by the next tile's as soon as they are converted.
-template <int S, int WAVES, int NS, int NT, bool PAIR>
-__global__ __launch_bounds__(64 * WAVES, 2) void f8_rows_kernel(F8Call a, int wk)
+// The 16 columns of a matrix instruction are R = 16 / S weight rows by S parts of a span of S blocks of K: column s R + r is part s of
+// row r, and row s R + t of the other operand is part s of input row t.  Of the products those of equal parts are wanted; with few
+// rows of x the others buy whole cache lines of each weight row, which a load from 16 rows by 64 bytes does not get (15 bytes a cycle and
+// CU; 45 from 8 rows by 128), and S times as many pieces of work.  Load h of a lane takes the 16 bytes 4 s + kg of the span's half h, so
+// that its 4 S lanes of a row are consecutive; they belong to block s / 2 + h S / 2 of the span.  S = 4 serves 4 rows of x, S = 2 8 rows, or 16 in
+// two groups (TG).
+// A wave owns NS spans of every WK NS, keeps x for them in registers and goes over tiles of NT R weight rows (of a gated pair: NT / 2 of gate and
+// as many of up); codes are replaced by the next tile's as soon as they are converted.
+template <int S, int TG, int WAVES, int NS, int NT, bool PAIR>
+__global__ __launch_bounds__(64 * WAVES) void f8_rows_kernel(F8Call a, int wk_log2)
 {
-    constexpr int R = 16 / S, H = 4 / S, NP = PAIR ? NT / 2 : NT;  // weight rows of a load; 4-row pieces of x in a column; loads of rows
-    __shared__ float red[WAVES][NT][4 * H][16];
+    constexpr int R = 16 / S, H = R / 4, P = PAIR ? 2 : 1, NP = NT / P;  // weight rows of a load; lane groups that hold a part's products
+    constexpr int TOKENS = TG * R, HALF = 64 * S;                       // bytes of a half span
+    constexpr bool KEPT = TG * NS <= 2;                                 // x stays in registers as fp16
+    __shared__ __align__(16) float red[2][NT * TOKENS * R * WAVES];     // of this tile and the next: [row part][n][token][r][wave in K]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kw = wave & (wk - 1), rw = wave / wk, wr = WAVES / wk;  // the wave's place in K and in rows
+    const int wk = 1 << wk_log2, kw = wave & (wk - 1), rw = wave >> wk_log2, wr = WAVES >> wk_log2;  // the wave's place in K and in rows
     const int col = lane & 15, kg = lane >> 4, s = col / R, r = col % R;
     const int nkb = ((a.kb + S - 1) / S + wk * NS - 1) / (wk * NS);  // rounds over K
     const int rows_wg = wr * NP * R, tiles = (a.N + rows_wg - 1) / rows_wg;  // rows_wg: a power of two up to 128
+    const int other = kg / H == s ? 0 : F8_NONE;  // this lane's products are of unequal parts: it needs no scales
 
     const __amdgpu_buffer_rsrc_t rx = mf_rsrc(a.x, (size_t)a.M * a.K), rxs = mf_rsrc(a.xs, (size_t)a.M * a.kb * 4);
-    F8Raw xr[NS];
-    float sx[NS][4];
-    auto block = [&](int i, int kb) { return ((kb * NS + i) * wk + kw) * S + s; };
+    F8Raw xr[TG][NS];
+    F8Half xh[KEPT ? TG : 1][KEPT ? NS : 1];
+    float sx[TG][NS][2][4];
+    auto span = [&](int i, int kb) { return (kb * NS + i) * wk + kw; };
     auto load_x = [&](int kb) {
 #pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            const int b = block(i, kb), k = b * F8_BLOCK + 16 * kg;
+        for (int i = 0; i < NS; ++i)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                xr[i].p[h] = __builtin_bit_cast(f8_u4, __builtin_amdgcn_raw_buffer_load_b128(rx, k + 64 * h < a.K ? r * a.K + k + 64 * h : F8_NONE, 0, 0));
+            for (int h = 0; h < 2; ++h) {
+                const int k = span(i, kb) * 2 * HALF + h * HALF + 16 * (4 * s + kg), b = span(i, kb) * S + s / 2 + h * (S / 2);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)  // of the input rows whose products this lane gets
-                sx[i][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
-                                                         rxs, kg / H == s && b < a.kb ? ((kg % H * 4 + e) * a.kb + b) * 4 : F8_NONE, 0, 0));
-        }
+                for (int g = 0; g < TG; ++g)
+                    xr[g][i].p[h] = __builtin_bit_cast(f8_u4, __builtin_amdgcn_raw_buffer_load_b128(rx, k < a.K ? (g * R + r) * a.K + k : F8_NONE, 0, 0));
+#pragma unroll
+                for (int g = 0; g < TG; ++g)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        sx[g][i][h][e] = __builtin_bit_cast(
+                            float, __builtin_amdgcn_raw_buffer_load_b32(rxs, ((g * R + kg % H * 4 + e) * a.kb + b) * 4 | (b < a.kb ? other : F8_NONE), 0, 0));
+            }
     };
+    auto keep_x = [&] {
+        if constexpr (KEPT)
+#pragma unroll
+            for (int g = 0; g < TG; ++g)
+#pragma unroll
+                for (int i = 0; i < NS; ++i) xh[g][i] = f8_half(xr[g][i]);
+    };
+    // The codes by vector loads, the scales, which all lanes share but for s, by scalar ones.
+    typedef const __attribute__((address_space(4))) float* scalar_t;
     F8Raw w[NS][NT];
-    float sw[NS][PAIR ? 2 : 1];
-    __amdgpu_buffer_rsrc_t rw_[PAIR ? 2 : 1], rs[PAIR ? 2 : 1];
+    float sw[NS][P][S];
+    __amdgpu_buffer_rsrc_t rw_[P];
+    scalar_t ws[P];
     auto aim = [&](int tile) {  // descriptors of the tile's rows (nothing left of the matrix: every load is 0)
         const long row0 = ((long)tile * wr + rw) * NP * R, left = tile < tiles ? max(min(a.N - row0, (long)NP * R), 0l) : 0;
 #pragma unroll
-        for (int p = 0; p < (PAIR ? 2 : 1); ++p) {
+        for (int p = 0; p < P; ++p) {
             rw_[p] = mf_rsrc(a.w[p].codes + row0 * a.K, (size_t)(left * a.K));
-            rs[p] = mf_rsrc(a.w[p].scales + row0 / F8_BLOCK * a.kb, left ? (size_t)a.kb * 4 : 0);
+            ws[p] = (scalar_t)(a.w[p].scales + (left ? row0 / F8_BLOCK * a.kb : 0));
         }
     };
-    const int lane_off = r * a.K + 16 * kg;
+    const int lane_off = r * a.K + 16 * (4 * s + kg);
     auto load_w = [&](int i, int n, int kb) {
-        const int b = block(i, kb), k = b * F8_BLOCK + 16 * kg, p = PAIR ? n & 1 : 0;
+        const int p = n % P, at = span(i, kb) * 2 * HALF;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
             w[i][n].p[h] = __builtin_bit_cast(f8_u4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                         rw_[p], k + 64 * h < a.K ? lane_off + (PAIR ? n >> 1 : n) * R * a.K + b * F8_BLOCK + 64 * h : F8_NONE, 0, 0));
-        if (n == p) sw[i][p] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs[p], b < a.kb ? b * 4 : F8_NONE, 0, 0));
+                                                         rw_[p], at + h * HALF + 16 * (4 * s + kg) < a.K ? n / P * R * a.K + lane_off + at + h * HALF : F8_NONE, 0, 0));
+        if (n == p)
+#pragma unroll
+            for (int q = 0; q < S; ++q) {
+                const int b = span(i, kb) * S + q;
+                sw[i][p][q] = ws[p][min(b, a.kb - 1)];
+            }
     };
     int tile = blockIdx.x;
     aim(tile);
@@ -163,70 +203,105 @@ __global__ __launch_bounds__(64 * WAVES, 2) void f8_rows_kernel(F8Call a, int wk
     for (int i = 0; i < NS; ++i)
 #pragma unroll
         for (int n = 0; n < NT; ++n) load_w(i, n, 0);
-    for (; tile < tiles; tile += gridDim.x) {
-        hx_f4 acc[NT];
+    keep_x();
+    for (int turn = 0; tile < tiles; tile += gridDim.x, turn ^= 1) {
+        hx_f4 acc[NT][TG];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) acc[n] = hx_f4{0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int g = 0; g < TG; ++g) acc[n][g] = hx_f4{0.f, 0.f, 0.f, 0.f};
         for (int kb = 0; kb < nkb; ++kb) {
-            if (nkb > 1) load_x(kb);
+            if (nkb > 1) load_x(kb), keep_x();
             const bool wrap = kb + 1 == nkb;
             const int next_kb = wrap ? 0 : kb + 1;
             if (wrap) aim(tile + gridDim.x);
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
-                const F8Half xa = f8_half(xr[i]);
-                float f[PAIR ? 2 : 1][4];
+                float f[P][TG][2][4];
 #pragma unroll
-                for (int p = 0; p < (PAIR ? 2 : 1); ++p)
+                for (int p = 0; p < P; ++p)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) f[p][e] = sx[i][e] * sw[i][p];
+                    for (int h = 0; h < 2; ++h) {
+                        // one of two by masks: a choice between two places of an array became an index into LDS, where the compiler put the array
+                        // (13 us a call: the kernel then reads its dispatch packet)
+                        uint32_t bits = __builtin_bit_cast(uint32_t, sw[i][p][h * (S / 2)]);
+                        if constexpr (S == 4) bits = (bits & (s / 2 ? 0u : ~0u)) | (__builtin_bit_cast(uint32_t, sw[i][p][2 * h + 1]) & (s / 2 ? ~0u : 0u));
+                        const float q = __builtin_bit_cast(float, bits);
+#pragma unroll
+                        for (int g = 0; g < TG; ++g)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) f[p][g][h][e] = sx[g][i][h][e] * q;
+                    }
+                F8Half x[TG];
+#pragma unroll
+                for (int g = 0; g < TG; ++g) {
+                    if constexpr (KEPT) x[g] = xh[g][i];
+                    else x[g] = f8_half(xr[g][i]);
+                }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const F8Half b = f8_half(w[i][n]);
                     load_w(i, n, next_kb);
                     __builtin_amdgcn_sched_barrier(0);  // the loads stay here, ahead of these codes' products
-                    hx_f4 t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(xa.k[j], b.k[j], t, 0, 0, 0);
+                    for (int g = 0; g < TG; ++g) {
+                        hx_f4 t[2];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[n][e] = __builtin_fmaf(f[PAIR ? n & 1 : 0][e], t[e], acc[n][e]);
+                        for (int h = 0; h < 2; ++h) t[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[g].k[2 * h], b.k[2 * h], hx_f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) t[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[g].k[2 * h + 1], b.k[2 * h + 1], t[h], 0, 0, 0);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[n][g][e] = __builtin_fmaf(f[n % P][g][h][e], t[h][e], acc[n][g][e]);
+                    }
                 }
             }
         }
-        // lane: column col, rows 4 kg + e of the products; wanted where their blocks agree
-        if (kg / H == s)
+        // A wave's parts, then the waves' sums, which lie together.
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) red[wave][n][kg % H * 4 + e][col] = acc[n][e];
-        hx_lds_barrier();
-        constexpr int ITEMS = NP * 4 * H * R;  // outputs per row part of the workgroup
-        auto sum = [&](int part, int n, int t, int rr) {
-            float v = 0.0f;
-            for (int k = 0; k < wk; ++k)
+            for (int g = 0; g < TG; ++g)
 #pragma unroll
-                for (int ss = 0; ss < S; ++ss) v += red[part * wk + k][n][t][ss * R + rr];
-            return v;
-        };
-        for (int i = threadIdx.x; i < ITEMS * wr; i += 64 * WAVES) {
-            const int part = i / ITEMS, q = i % ITEMS, rr = q % R, n = q / R % NP, t = q / R / NP;
-            const int row = (tile * wr + part) * NP * R + n * R + rr;
-            if constexpr (PAIR) {
-                const float v = f8_gated(sum(part, 2 * n, t, rr), sum(part, 2 * n + 1, t, rr), a.limit);
-                if (row < a.N && t < a.M)
-                    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), coherent_rsrc(a.products + (size_t)(tile * rows_wg / F8_BLOCK) * (16 * F8_BLOCK)),
-                                                          (t * F8_BLOCK + row % F8_BLOCK) * 4, 0, HX_BUF_SC1);
-            } else {
-                const float v = sum(part, n, t, rr);
-                if (row < a.N && t < a.M) f8_store(a.y, (size_t)t * a.N + row, v, a.y_fp32);
+                for (int e = 0; e < 4; ++e) {
+                    const float v = f8_parts_sum<S>(acc[n][g][e]);
+                    if (kg < H && s == 0) red[turn][((((rw * NT + n) * TOKENS + g * R + kg * 4 + e) * R + r) << wk_log2) + kw] = v;
+                }
+        hx_lds_barrier();  // also: the sums of the tile before are read
+        constexpr int OUT = NP * TOKENS * R;  // of a row part
+        for (int i = threadIdx.x; i < OUT * wr; i += 64 * WAVES) {
+            const int rr = i % R, t = i / R % TOKENS, n = i / R / TOKENS % NP, part = i / OUT;
+            float v[P];
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                const float* from = red[turn] + ((((part * NT + n * P + p) * TOKENS + t) * R + rr) << wk_log2);
+                float sum = 0.0f;
+                if (wk == WAVES) {
+                    const hx_f4* four = reinterpret_cast<const hx_f4*>(from);
+                    hx_f4 u = four[0];
+#pragma unroll
+                    for (int k = 1; k < WAVES / 4; ++k) u += four[k];
+                    sum = (u[0] + u[1]) + (u[2] + u[3]);
+                } else {
+                    for (int k = 0; k < wk; ++k) sum += from[k];
+                }
+                v[p] = sum;
             }
+            const int row = (tile * wr + part) * NP * R + n * R + rr;
+            if (row >= a.N || t >= a.M) continue;
+            if constexpr (PAIR)
+                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, f8_gated(v[0], v[1], a.limit)),
+                                                      coherent_rsrc(a.products + (size_t)(tile * rows_wg / F8_BLOCK) * (16 * F8_BLOCK)),
+                                                      (t * F8_BLOCK + row % F8_BLOCK) * 4, 0, HX_BUF_SC1);
+            else
+                f8_store(a.y, (size_t)t * a.N + row, v[0], a.y_fp32);
         }
         if constexpr (PAIR) {  // the last tile of a block of 128 outputs to arrive scales it
             const int b = tile * rows_wg / F8_BLOCK, per = F8_BLOCK / rows_wg;
             if (arrive_last(a.counters + b, min(per, tiles - b * per)))
                 f8_finish_block<64 * WAVES>(a, a.products + (size_t)b * (16 * F8_BLOCK), 16, 0, b);
         }
-        hx_lds_barrier();  // the sums are read before the next tile's overwrite them
     }
 }
 
@@ -405,6 +480,7 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
 #pragma unroll
     for (int u = 0; u < PF - 1; ++u) {
         asm volatile("" ::: "memory");
+        load_scales(0, 0, 4);  // of none: the waits below count this many loads for every step
         load_x(u, first + u);
         load_w(u, first + u);
     }
@@ -579,14 +655,14 @@ F8Plan f8_plan(int M, int N, int K, bool pair, bool split)
     return p;
 }
 
-template <int S, int WAVES, int NS, int NT, bool PAIR>
+template <int S, int TG, int WAVES, int NS, int NT, bool PAIR>
 hipError_t rows_launch(const F8Call& c, hipStream_t st)
 {
     const int spans = (c.kb + S - 1) / S;
-    int wk = 1;  // waves along K: as many as have spans, up to all
-    while (wk < WAVES && wk * NS < spans) wk *= 2;
-    const long rows = WAVES / wk * (PAIR ? NT / 2 : NT) * 16 / S, tiles = (c.N + rows - 1) / rows;
-    hipLaunchKernelGGL((f8_rows_kernel<S, WAVES, NS, NT, PAIR>), dim3(tiles < 2 * F8_CUS ? tiles : 2 * F8_CUS), dim3(64 * WAVES), 0, st, c, wk);
+    int log2 = 0;  // waves along K: as many as have spans, up to all
+    while (1 << log2 < WAVES && NS << log2 < spans) ++log2;
+    const long rows = (WAVES >> log2) * (PAIR ? NT / 2 : NT) * 16 / S, tiles = (c.N + rows - 1) / rows;
+    hipLaunchKernelGGL((f8_rows_kernel<S, TG, WAVES, NS, NT, PAIR>), dim3(tiles < 2 * F8_CUS ? tiles : 2 * F8_CUS), dim3(64 * WAVES), 0, st, c, log2);
     return hipGetLastError();
 }
 
@@ -608,9 +684,9 @@ hipError_t f8_launch(F8Call c, const F8Plan& p, void* ws, hipStream_t st)
     c.products = reinterpret_cast<float*>(static_cast<char*>(ws) + HX_COUNTER_BYTES + p.partial);
     switch (p.kind) {
         case F8Plan::ROWS:
-            if (c.M <= 4) return rows_launch<4, 8, 1, 4, PAIR>(c, st);
-            if (c.M <= 8) return rows_launch<2, 8, 2, 2, PAIR>(c, st);
-            return rows_launch<1, 8, 2, 2, PAIR>(c, st);
+            if (c.M <= 4) return rows_launch<4, 1, 8, 1, 2, PAIR>(c, st);
+            if (c.M <= 8) return rows_launch<2, 1, 8, 2, 2, PAIR>(c, st);
+            return rows_launch<2, 2, 8, 2, 2, PAIR>(c, st);
         case F8Plan::TILE64x32: return tile_launch<2, 2, 2, 1, 6, true, PAIR>(c, p, st);
         case F8Plan::TILE64x64: return tile_launch<2, 2, 2, 2, 4, true, PAIR>(c, p, st);
         case F8Plan::TILE128x128: return tile_launch<2, 2, 4, 4, 2, true, PAIR>(c, p, st);
