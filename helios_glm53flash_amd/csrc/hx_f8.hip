@@ -9,11 +9,14 @@
 //   exact  the codes become fp16 (no rounding), v_mfma_f32_16x16x32_f16: products exact, sums fp32
 //   fast   v_mfma_f32_16x16x128_f8f6f4, twice the rate.  It adds 8 consecutive k (a lane's octets) after shifting each product to the
 //          largest exponent among them, and drops what lies 2^13 and more below; from there on sums are fp32.  The result is off by some
-//          2^-16 of its size (measured 1.6e-5 rms), so it serves fp16 outputs only, whose rounding is 2^-11.
+//          2^-16 of its size (measured 1.6e-5 rms), so it serves fp16 outputs only, whose rounding is 2^-11.  (The gated pair's scales
+//          are fp32.)
 //
-//   M <= 16  f8_rows_kernel: the waves of a workgroup split K and keep their part of x in registers; they walk over the weight rows,
-//            every code read once from memory into operands, and add their sums through LDS.
-//   M > 16   f8_tile_kernel: tiles, both sides through a ring of LDS stages.
+//   M <= 8  f8_rows_kernel: the waves of a workgroup split K and keep their part of x in registers; they walk over the weight rows,
+//           every code read once from memory into operands, and add their sums through LDS.  exact
+//   M > 8   f8_tile_kernel: tiles, both sides through a ring of LDS stages.  fast for fp16 outputs, else exact
+#include <algorithm>
+
 #include "hx_f8.hpp"
 #include "hx_kernels.hpp"
 #include "hx_mfma.hpp"
@@ -41,12 +44,17 @@ struct F8Raw {
 struct F8Half {
     hx_h8 k[4];
 };
+template <int NS>
+struct F8Spans {
+    F8Raw of[NS];
+};
 HX_INLINE F8Half f8_half(const F8Raw& r)
 {
     return {{f8_half8(r.p[0][0], r.p[0][1]), f8_half8(r.p[0][2], r.p[0][3]), f8_half8(r.p[1][0], r.p[1][1]), f8_half8(r.p[1][2], r.p[1][3])}};
 }
 
 constexpr int F8_NONE = 0x7ffffff0;  // an offset behind every descriptor
+constexpr int F8_ROWS = 8, F8_ROWS_THREADS = 1024;  // most rows of f8_rows_kernel; its workgroup
 
 HX_INLINE float f8_gated(float g, float u, float limit)
 {
@@ -61,18 +69,11 @@ HX_INLINE void f8_store(void* y, size_t i, float v, bool y_fp32)
     else static_cast<_Float16*>(y)[i] = (_Float16)v;
 }
 
-// Sum over the S parts of a span (f8_rows_kernel): lane 16 s H + s R + l holds part s of what lane l gets.
-template <int S>
+// Sum over the two parts of a span (f8_rows_kernel): lane 40 + l holds part 1 of what lane l gets (its upper half, row_ror:8).
 HX_INLINE float f8_parts_sum(float v)
 {
-    auto turned = [](uint32_t x, auto ctrl) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xf, 0xf, false)); };
     const uint32_t u = __builtin_bit_cast(uint32_t, v);
-    v += turned(__builtin_amdgcn_permlane32_swap(u, u, false, false)[1], std::integral_constant<int, 0x128>{});  // lane + 40: the upper half, row_ror:8
-    if constexpr (S == 4) {
-        const uint32_t q = __builtin_bit_cast(uint32_t, v);
-        v += turned(__builtin_amdgcn_permlane16_swap(q, q, false, false)[1], std::integral_constant<int, 0x12c>{});  // lane + 20: the odd row, row_ror:12
-    }
-    return v;
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, (int)__builtin_amdgcn_permlane32_swap(u, u, false, false)[1], 0x128, 0xf, 0xf, false));
 }
 
 // A call.  w[1] is the up projection of a gated pair (w[0] the gate), else unused.
@@ -94,188 +95,179 @@ struct F8Call {
     float* products;
 };
 
-// Codes and scales of products v[rows][128] in memory (device-coherent; columns n0 .. of N, rows m0 .. of M): 32 lanes a row.
-template <int THREADS>
+// Four outputs of a row from n on, in one store where rows and y allow it.
+HX_INLINE void f8_store4(const F8Call& c, int m, int n, hx_f4 v)
+{
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    if (m >= c.M || n >= c.N) return;
+    const size_t at = (size_t)m * c.N + n;
+    if (c.N % 4 == 0 && reinterpret_cast<uintptr_t>(c.y) % (c.y_fp32 ? 16 : 8) == 0) {
+        if (c.y_fp32) *reinterpret_cast<hx_f4*>(static_cast<float*>(c.y) + at) = v;
+        else *reinterpret_cast<h4*>(static_cast<_Float16*>(c.y) + at) = __builtin_convertvector(v, h4);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < c.N) f8_store(c.y, at + e, v[e], c.y_fp32);
+    }
+}
+
+// Codes and scales of products v[rows][128] in memory (device-coherent; block of N, rows m0 .. of M): 32 lanes a row, THREADS threads, the loads
+// of BATCH rows each ahead of their use (one at a time, each is a round trip of over a us).
+template <int THREADS, int BATCH>
 HX_INLINE void f8_finish_block(const F8Call& c, const float* v, int rows, int m0, int block)
 {
-    const int n = block * F8_BLOCK + 4 * (threadIdx.x & 31), nb = (c.N + F8_BLOCK - 1) / F8_BLOCK;
+    const int thread = threadIdx.x % THREADS, n = block * F8_BLOCK + 4 * (thread & 31), nb = (c.N + F8_BLOCK - 1) / F8_BLOCK;
     const __amdgpu_buffer_rsrc_t r = coherent_rsrc(v);
-    for (int i = threadIdx.x >> 5; i < rows && m0 + i < c.M; i += THREADS / 32) {
-        hx_f4 t{0.f, 0.f, 0.f, 0.f};
-        if (n < c.N) t = coherent_load4(r, (i * F8_BLOCK + 4 * (int)(threadIdx.x & 31)) * 4);
-        uint32_t a = max(max(f8_abs_bits(t[0]), f8_abs_bits(t[1])), max(f8_abs_bits(t[2]), f8_abs_bits(t[3])));
-        a = f8_row_max(a);
-        a = max(a, (uint32_t)__shfl_xor((int)a, 16, 64));
-        const F8Scale s = f8_scale(a);
-        if (n < c.N)
-            *reinterpret_cast<uint32_t*>(c.q + (size_t)(m0 + i) * c.N + n) = f8_codes(t[0] * s.factor, t[1] * s.factor, t[2] * s.factor, t[3] * s.factor);
-        if ((threadIdx.x & 31) == 0) c.scales[(size_t)(m0 + i) * nb + block] = s.scale;
+    rows = min(rows, c.M - m0);
+    for (int i0 = thread >> 5; i0 < rows; i0 += BATCH * (THREADS / 32)) {
+        hx_f4 t[BATCH];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) t[j] = coherent_load4(r, (min(i0 + j * (THREADS / 32), rows - 1) * F8_BLOCK + 4 * (thread & 31)) * 4);
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+            const int i = i0 + j * (THREADS / 32);
+            if (n >= c.N) t[j] = hx_f4{0.f, 0.f, 0.f, 0.f};
+            uint32_t a = max(max(f8_abs_bits(t[j][0]), f8_abs_bits(t[j][1])), max(f8_abs_bits(t[j][2]), f8_abs_bits(t[j][3])));
+            a = f8_row_max(a);
+            a = max(a, (uint32_t)__shfl_xor((int)a, 16, 64));
+            const F8Scale s = f8_scale(a);
+            if (i < rows && n < c.N)
+                *reinterpret_cast<uint32_t*>(c.q + (size_t)(m0 + i) * c.N + n) = f8_codes(t[j][0] * s.factor, t[j][1] * s.factor, t[j][2] * s.factor, t[j][3] * s.factor);
+            if (i < rows && (thread & 31) == 0) c.scales[(size_t)(m0 + i) * nb + block] = s.scale;
+        }
     }
 }
 
 }  // namespace
 
-// ---- up to 16 rows
+// ---- up to 8 rows
 //
-// The 16 columns of a matrix instruction are R = 16 / S weight rows by S parts of a span of S blocks of K: column s R + r is part s of
-// row r, and row s R + t of the other operand is part s of input row t.  Of the products those of equal parts are wanted; with few
-// rows of x the others buy whole cache lines of each weight row, which a load from 16 rows by 64 bytes does not get (15 bytes a cycle and
-// CU; 45 from 8 rows by 128), and S times as many pieces of work.  Load h of a lane takes the 16 bytes 4 s + kg of the span's half h, so
-// that its 4 S lanes of a row are consecutive; they belong to block s / 2 + h S / 2 of the span.  S = 4 serves 4 rows of x, S = 2 8 rows, or 16 in
-// two groups (TG).
-// A wave owns NS spans of every WK NS, keeps x for them in registers and goes over tiles of NT R weight rows (of a gated pair: NT / 2 of gate and
-// as many of up); codes are replaced by the next tile's as soon as they are converted.
-template <int S, int TG, int WAVES, int NS, int NT, bool PAIR>
-__global__ __launch_bounds__(64 * WAVES) void f8_rows_kernel(F8Call a, int wk_log2)
+// The 16 columns of a matrix instruction are 8 weight rows by the two parts of a span of two blocks of K: column 8 s + r is part s of row
+// r, and row 8 s + t of the other operand is part s of input row t.  Of the products those of equal parts are wanted; the others buy whole
+// cache lines of each weight row, which a load from 16 rows by 64 bytes does not get (15 bytes a cycle and CU; 45 from 8 rows by 128), and
+// twice as many pieces of work.  Load h of a lane takes the 16 bytes 4 s + kg of the span's half h, so that its 8 lanes of a row are
+// consecutive: half h is block h of the span.
+// A workgroup's waves split K (all WAVES of them, if it has as many spans; else they also split the tile's rows), each owns NS spans of every
+// WK NS, keeps x for them in registers and goes over tiles of 8 weight rows (of a gated pair: 8 of gate and 8 of up); codes are replaced
+// by the next tile's as soon as they are converted.  One workgroup of 16 waves a CU: 8 rows of 4096 -> 12288 take 12.5 us, 15.1 with two workgroups
+// and 17.8 with two of 8 waves; one row of 4096 -> 151552 96.7 us (6.4 TB/s).
+template <int NS, bool PAIR>
+__global__ __launch_bounds__(F8_ROWS_THREADS) void f8_rows_kernel(F8Call a, int wk_log2)
 {
-    constexpr int R = 16 / S, H = R / 4, P = PAIR ? 2 : 1, NP = NT / P;  // weight rows of a load; lane groups that hold a part's products
-    constexpr int TOKENS = TG * R, HALF = 64 * S;                       // bytes of a half span
-    constexpr bool KEPT = TG * NS <= 2;                                 // x stays in registers as fp16
-    __shared__ __align__(16) float red[2][NT * TOKENS * R * WAVES];     // of this tile and the next: [row part][n][token][r][wave in K]
+    constexpr int WAVES = F8_ROWS_THREADS / 64, R = F8_ROWS, P = PAIR ? 2 : 1;
+    __shared__ __align__(16) float red[2][P * R * R * WAVES];  // of this tile and the next: [row part][p][token][r][wave in K]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wk = 1 << wk_log2, kw = wave & (wk - 1), rw = wave >> wk_log2, wr = WAVES >> wk_log2;  // the wave's place in K and in rows
     const int col = lane & 15, kg = lane >> 4, s = col / R, r = col % R;
-    const int nkb = ((a.kb + S - 1) / S + wk * NS - 1) / (wk * NS);  // rounds over K
-    const int rows_wg = wr * NP * R, tiles = (a.N + rows_wg - 1) / rows_wg;  // rows_wg: a power of two up to 128
-    const int other = kg / H == s ? 0 : F8_NONE;  // this lane's products are of unequal parts: it needs no scales
+    const int nkb = ((a.kb + 1) / 2 + wk * NS - 1) / (wk * NS);               // rounds over K
+    const int rows_wg = wr * R, tiles = (a.N + rows_wg - 1) / rows_wg;        // rows_wg: a power of two up to 128
+    const int other = kg / 2 == s ? 0 : F8_NONE;  // this lane's products are of unequal parts: it needs no scales
 
     const __amdgpu_buffer_rsrc_t rx = mf_rsrc(a.x, (size_t)a.M * a.K), rxs = mf_rsrc(a.xs, (size_t)a.M * a.kb * 4);
-    F8Raw xr[TG][NS];
-    F8Half xh[KEPT ? TG : 1][KEPT ? NS : 1];
-    float sx[TG][NS][2][4];
+    F8Half x[NS];
+    float sx[NS][2][4];
     auto span = [&](int i, int kb) { return (kb * NS + i) * wk + kw; };
+    const int in_span = 16 * (4 * s + kg);  // of this lane's first piece
     auto load_x = [&](int kb) {
+        F8Spans<NS> raw;
 #pragma unroll
         for (int i = 0; i < NS; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int k = span(i, kb) * 2 * HALF + h * HALF + 16 * (4 * s + kg), b = span(i, kb) * S + s / 2 + h * (S / 2);
+                const int b = 2 * span(i, kb) + h, k = b * F8_BLOCK + in_span;
+                raw.of[i].p[h] = __builtin_bit_cast(f8_u4, __builtin_amdgcn_raw_buffer_load_b128(rx, k < a.K ? r * a.K + k : F8_NONE, 0, 0));
 #pragma unroll
-                for (int g = 0; g < TG; ++g)
-                    xr[g][i].p[h] = __builtin_bit_cast(f8_u4, __builtin_amdgcn_raw_buffer_load_b128(rx, k < a.K ? (g * R + r) * a.K + k : F8_NONE, 0, 0));
-#pragma unroll
-                for (int g = 0; g < TG; ++g)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        sx[g][i][h][e] = __builtin_bit_cast(
-                            float, __builtin_amdgcn_raw_buffer_load_b32(rxs, ((g * R + kg % H * 4 + e) * a.kb + b) * 4 | (b < a.kb ? other : F8_NONE), 0, 0));
+                for (int e = 0; e < 4; ++e)
+                    sx[i][h][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rxs, ((kg % 2 * 4 + e) * a.kb + b) * 4 | (b < a.kb ? other : F8_NONE), 0, 0));
             }
+        return raw;
     };
-    auto keep_x = [&] {
-        if constexpr (KEPT)
+    auto keep_x = [&](const F8Spans<NS>& raw) {
 #pragma unroll
-            for (int g = 0; g < TG; ++g)
-#pragma unroll
-                for (int i = 0; i < NS; ++i) xh[g][i] = f8_half(xr[g][i]);
+        for (int i = 0; i < NS; ++i) x[i] = f8_half(raw.of[i]);
     };
-    // The codes by vector loads, the scales, which all lanes share but for s, by scalar ones.
+    // The codes by vector loads, the scales, which all lanes share, by scalar ones.
     typedef const __attribute__((address_space(4))) float* scalar_t;
-    F8Raw w[NS][NT];
-    float sw[NS][P][S];
+    F8Raw w[NS][P];
+    float sw[NS][P][2];
     __amdgpu_buffer_rsrc_t rw_[P];
     scalar_t ws[P];
     auto aim = [&](int tile) {  // descriptors of the tile's rows (nothing left of the matrix: every load is 0)
-        const long row0 = ((long)tile * wr + rw) * NP * R, left = tile < tiles ? max(min(a.N - row0, (long)NP * R), 0l) : 0;
+        const long row0 = ((long)tile * wr + rw) * R, left = tile < tiles ? max(min(a.N - row0, (long)R), 0l) : 0;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             rw_[p] = mf_rsrc(a.w[p].codes + row0 * a.K, (size_t)(left * a.K));
             ws[p] = (scalar_t)(a.w[p].scales + (left ? row0 / F8_BLOCK * a.kb : 0));
         }
     };
-    const int lane_off = r * a.K + 16 * (4 * s + kg);
-    auto load_w = [&](int i, int n, int kb) {
-        const int p = n % P, at = span(i, kb) * 2 * HALF;
+    auto load_w = [&](int i, int p, int kb) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-            w[i][n].p[h] = __builtin_bit_cast(f8_u4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                         rw_[p], at + h * HALF + 16 * (4 * s + kg) < a.K ? n / P * R * a.K + lane_off + at + h * HALF : F8_NONE, 0, 0));
-        if (n == p)
-#pragma unroll
-            for (int q = 0; q < S; ++q) {
-                const int b = span(i, kb) * S + q;
-                sw[i][p][q] = ws[p][min(b, a.kb - 1)];
-            }
+        for (int h = 0; h < 2; ++h) {
+            const int b = 2 * span(i, kb) + h, k = b * F8_BLOCK + in_span;
+            w[i][p].p[h] = __builtin_bit_cast(f8_u4, __builtin_amdgcn_raw_buffer_load_b128(rw_[p], k < a.K ? r * a.K + k : F8_NONE, 0, 0));
+            sw[i][p][h] = ws[p][min(b, a.kb - 1)];
+        }
     };
     int tile = blockIdx.x;
     aim(tile);
-    load_x(0);
+    {
+        const F8Spans<NS> raw = load_x(0);
 #pragma unroll
-    for (int i = 0; i < NS; ++i)
+        for (int i = 0; i < NS; ++i)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) load_w(i, n, 0);
-    keep_x();
+            for (int p = 0; p < P; ++p) load_w(i, p, 0);
+        keep_x(raw);
+    }
     for (int turn = 0; tile < tiles; tile += gridDim.x, turn ^= 1) {
-        hx_f4 acc[NT][TG];
+        hx_f4 acc[P];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int g = 0; g < TG; ++g) acc[n][g] = hx_f4{0.f, 0.f, 0.f, 0.f};
+        for (int p = 0; p < P; ++p) acc[p] = hx_f4{0.f, 0.f, 0.f, 0.f};
         for (int kb = 0; kb < nkb; ++kb) {
-            if (nkb > 1) load_x(kb), keep_x();
+            if (nkb > 1) keep_x(load_x(kb));
             const bool wrap = kb + 1 == nkb;
             const int next_kb = wrap ? 0 : kb + 1;
             if (wrap) aim(tile + gridDim.x);
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
-                float f[P][TG][2][4];
+                float f[P][2][4];
 #pragma unroll
                 for (int p = 0; p < P; ++p)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        // one of two by masks: a choice between two places of an array became an index into LDS, where the compiler put the array
-                        // (13 us a call: the kernel then reads its dispatch packet)
-                        uint32_t bits = __builtin_bit_cast(uint32_t, sw[i][p][h * (S / 2)]);
-                        if constexpr (S == 4) bits = (bits & (s / 2 ? 0u : ~0u)) | (__builtin_bit_cast(uint32_t, sw[i][p][2 * h + 1]) & (s / 2 ? ~0u : 0u));
-                        const float q = __builtin_bit_cast(float, bits);
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int g = 0; g < TG; ++g)
+                        for (int e = 0; e < 4; ++e) f[p][h][e] = sx[i][h][e] * sw[i][p][h];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) f[p][g][h][e] = sx[g][i][h][e] * q;
-                    }
-                F8Half x[TG];
-#pragma unroll
-                for (int g = 0; g < TG; ++g) {
-                    if constexpr (KEPT) x[g] = xh[g][i];
-                    else x[g] = f8_half(xr[g][i]);
-                }
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const F8Half b = f8_half(w[i][n]);
-                    load_w(i, n, next_kb);
+                for (int p = 0; p < P; ++p) {
+                    const F8Half b = f8_half(w[i][p]);
+                    load_w(i, p, next_kb);
                     __builtin_amdgcn_sched_barrier(0);  // the loads stay here, ahead of these codes' products
+                    hx_f4 t[2];
 #pragma unroll
-                    for (int g = 0; g < TG; ++g) {
-                        hx_f4 t[2];
+                    for (int h = 0; h < 2; ++h) t[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[i].k[2 * h], b.k[2 * h], hx_f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) t[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[g].k[2 * h], b.k[2 * h], hx_f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    for (int h = 0; h < 2; ++h) t[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[i].k[2 * h + 1], b.k[2 * h + 1], t[h], 0, 0, 0);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) t[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[g].k[2 * h + 1], b.k[2 * h + 1], t[h], 0, 0, 0);
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) acc[n][g][e] = __builtin_fmaf(f[n % P][g][h][e], t[h][e], acc[n][g][e]);
-                    }
+                        for (int e = 0; e < 4; ++e) acc[p][e] = __builtin_fmaf(f[p][h][e], t[h][e], acc[p][e]);
                 }
             }
         }
-        // A wave's parts, then the waves' sums, which lie together.
+        // A wave's two parts, then the waves' sums, which lie together.
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int p = 0; p < P; ++p)
 #pragma unroll
-            for (int g = 0; g < TG; ++g)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float v = f8_parts_sum<S>(acc[n][g][e]);
-                    if (kg < H && s == 0) red[turn][((((rw * NT + n) * TOKENS + g * R + kg * 4 + e) * R + r) << wk_log2) + kw] = v;
-                }
+            for (int e = 0; e < 4; ++e) {
+                const float v = f8_parts_sum(acc[p][e]);
+                if (kg < 2 && s == 0) red[turn][((((rw * P + p) * R + kg * 4 + e) * R + r) << wk_log2) + kw] = v;
+            }
         hx_lds_barrier();  // also: the sums of the tile before are read
-        constexpr int OUT = NP * TOKENS * R;  // of a row part
-        for (int i = threadIdx.x; i < OUT * wr; i += 64 * WAVES) {
-            const int rr = i % R, t = i / R % TOKENS, n = i / R / TOKENS % NP, part = i / OUT;
+        for (int i = threadIdx.x; i < R * R * wr; i += F8_ROWS_THREADS) {
+            const int rr = i % R, t = i / R % R, part = i / (R * R);
             float v[P];
 #pragma unroll
             for (int p = 0; p < P; ++p) {
-                const float* from = red[turn] + ((((part * NT + n * P + p) * TOKENS + t) * R + rr) << wk_log2);
+                const float* from = red[turn] + ((((part * P + p) * R + t) * R + rr) << wk_log2);
                 float sum = 0.0f;
                 if (wk == WAVES) {
                     const hx_f4* four = reinterpret_cast<const hx_f4*>(from);
@@ -288,19 +280,42 @@ __global__ __launch_bounds__(64 * WAVES) void f8_rows_kernel(F8Call a, int wk_lo
                 }
                 v[p] = sum;
             }
-            const int row = (tile * wr + part) * NP * R + n * R + rr;
+            const int row = (tile * wr + part) * R + rr;
             if (row >= a.N || t >= a.M) continue;
             if constexpr (PAIR)
                 __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, f8_gated(v[0], v[1], a.limit)),
-                                                      coherent_rsrc(a.products + (size_t)(tile * rows_wg / F8_BLOCK) * (16 * F8_BLOCK)),
+                                                      coherent_rsrc(a.products + (size_t)(row / F8_BLOCK) * (R * F8_BLOCK)),
                                                       (t * F8_BLOCK + row % F8_BLOCK) * 4, 0, HX_BUF_SC1);
             else
                 f8_store(a.y, (size_t)t * a.N + row, v[0], a.y_fp32);
         }
-        if constexpr (PAIR) {  // the last tile of a block of 128 outputs to arrive scales it
-            const int b = tile * rows_wg / F8_BLOCK, per = F8_BLOCK / rows_wg;
-            if (arrive_last(a.counters + b, min(per, tiles - b * per)))
-                f8_finish_block<64 * WAVES>(a, a.products + (size_t)b * (16 * F8_BLOCK), 16, 0, b);
+    }
+    if constexpr (PAIR) {
+        // The last tile of a block of 128 outputs to arrive scales it.  A workgroup's tiles arrive together at its end: one by one, each waits for
+        // the codes in flight (one row of 4096 -> 12288, 6 tiles a workgroup: 27.6 us).
+        int* full = reinterpret_cast<int*>(red);
+        static_assert(F8_ROWS_THREADS * sizeof(int) <= sizeof(red));
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        const int per = F8_BLOCK / rows_wg;
+        for (long t0 = blockIdx.x; t0 < tiles; t0 += (long)F8_ROWS_THREADS * gridDim.x) {
+            const long t = t0 + (long)threadIdx.x * gridDim.x;
+            int block = -1;
+            if (t < tiles) {
+                const int b = (int)(t / per), all = min(per, tiles - b * per);
+                if (__hip_atomic_fetch_add(a.counters + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == all - 1) {
+                    __hip_atomic_store(a.counters + b, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
+                    block = b;
+                }
+            }
+            full[threadIdx.x] = block;
+            __syncthreads();
+            const long here = (tiles - t0 + gridDim.x - 1) / gridDim.x;
+            for (int i = wave; i < min(here, (long)F8_ROWS_THREADS); i += WAVES) {
+                const int b = __builtin_amdgcn_readfirstlane(full[i]);
+                if (b >= 0) f8_finish_block<64, R / 2>(a, a.products + (size_t)b * (R * F8_BLOCK), R, 0, b);
+            }
+            __syncthreads();
         }
     }
 }
@@ -324,7 +339,24 @@ struct F8TileSize {
     static constexpr int X = PF * BN * F8_BLOCK, SCALES = X + PF * BM * F8_BLOCK;  // where they begin in LDS
     static constexpr int GROUP = BM * 16, NOTHING = SCALES + 3 * GROUP, BYTES = NOTHING + 256 * WAVES;  // of scales: [rows][4]; where loads of none go
     static constexpr int NW = BN / (8 * WAVES), NX = BM / (8 * WAVES);  // loads of a wave a step
+    static constexpr bool SPLITS = TN * TM <= 16;  // K may be split: its sums take few registers next to a split's
     static_assert(BN % (8 * WAVES) == 0 && BM % (8 * WAVES) == 0 && BM <= 64 * WAVES && PF <= 8);
+};
+
+// What a buffer load may read; a step's loads of a wave and where in LDS they go; a step's operands in LDS.
+struct F8Rows {
+    const void* from;
+    size_t bytes;
+};
+struct F8Loads {
+    F8Rows w[2], x, scales;
+    uint8_t *into_w, *into_x, *into_scales;
+    int scales_off;
+};
+struct F8Stage {
+    const uint8_t *w, *x;
+    const float* scales;
+    int left;  // of K from this block on
 };
 
 template <int WN, int WM, int TN, int TM, int PF, bool EXACT, bool PAIR>
@@ -332,7 +364,6 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
 {
     using Z = F8TileSize<WN, WM, TN, TM, PF>;
     constexpr int BN = Z::BN, BM = Z::BM, NW = Z::NW, NX = Z::NX, WAVES = Z::WAVES;
-    static_assert(!PAIR || NW % 2 == 0);
     constexpr int CN = PAIR ? BN / 2 : BN, TP = PAIR ? TN / 2 : TN;  // outputs of a tile along N; a wave's row blocks of them
     extern __shared__ __align__(16) uint8_t f8_lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -348,39 +379,41 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
     // A wave's load i takes 8 rows of 128 bytes, rows 8 (i WAVES + wave) and behind of the weights (of a pair: gate, then up) or of x.  The
     // descriptors move on with the steps and end with the matrix; behind the last step they are empty.
     typedef __attribute__((address_space(3))) void* lds_t;
+    static_assert(!PAIR || NW % 2 == 0);
     const long lrow = 8 * wave;
     const uint8_t* base[3] = {a.w[0].codes + (n0 + lrow) * a.K, PAIR ? a.w[1].codes + (n0 + lrow) * a.K : nullptr, a.x + (m0 + lrow) * a.K};
     const long bytes[2] = {(nrows - lrow) * a.K, (mrows - lrow) * a.K};
     const int lane_off = (lane >> 3) * a.K + 16 * ((lane & 7) ^ (lane >> 3));
-    auto desc = [&](int p, int c) {
+    auto rows = [&](int p, int c) {
         const long at = (long)c * F8_BLOCK;
-        return mf_rsrc(base[p] + at, (size_t)(c < steps ? max(bytes[p >> 1] - at, 0l) : 0l));
+        return F8Rows{base[p] + at, (size_t)(c < steps ? max(bytes[p >> 1] - at, 0l) : 0l)};
     };
-    auto load_w = [&](int slot, int c) {
-        const __amdgpu_buffer_rsrc_t d[2] = {desc(0, c), desc(PAIR ? 1 : 0, c)};
-        uint8_t* st = f8_lds + (slot * BN + 8 * wave) * F8_BLOCK;
-#pragma unroll
-        for (int i = 0; i < NW; ++i) {
-            const int r = 8 * WAVES * i, up = PAIR && r >= CN ? 1 : 0;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(d[up], (lds_t)(st + r * F8_BLOCK), 16, lane_off + (r - up * CN) * a.K, 0, 0, 0);
-        }
-    };
-    auto load_x = [&](int slot, int c) {
-        const __amdgpu_buffer_rsrc_t d = desc(2, c);
-        uint8_t* st = f8_lds + Z::X + (slot * BM + 8 * wave) * F8_BLOCK;
-#pragma unroll
-        for (int i = 0; i < NX; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lds_t)(st + 8 * WAVES * i * F8_BLOCK), 16, lane_off + 8 * WAVES * i * a.K, 0, 0, 0);
-    };
-    // Part s of group g of the scales: 16 rows a wave from 16 (s WAVES + wave) on, of steps first + 4 g and the three behind.  Loads that touch no
-    // memory write zeros.
+    // A step's loads of a wave, LOADS of them: one of scales, then x, then the weights.  Loads that touch no memory write zeros.
     const float* xs = a.xs + (size_t)m0 * a.kb + first;
-    auto load_scales = [&](int buf, int g, int s) {
+    // Into stage `slot`, block c; of the scales part s of group g into group buffer `buf`: 16 rows a wave from 16 (s WAVES + wave) on, steps first + 4 g
+    // and the three behind.
+    auto loads = [&](int slot, int c, int buf, int g, int s) {
         const int row = 16 * (s * WAVES + wave);
         const bool any = row < BM && first + 4 * g < steps;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(mf_rsrc(xs + 4 * g, any ? ((size_t)mrows * a.kb - first - 4 * g) * 4 : 0),
-                                                 (lds_t)(f8_lds + (row < BM ? Z::SCALES + buf * Z::GROUP + row * 16 : Z::NOTHING + 256 * wave)), 4,
-                                                 any ? ((row + (lane >> 2)) * a.kb + (lane & 3)) * 4 : F8_NONE, 0, 0, 0);
+        return F8Loads{{rows(0, c), rows(PAIR ? 1 : 0, c)},
+                     rows(2, c),
+                     {xs + 4 * g, any ? ((size_t)mrows * a.kb - first - 4 * g) * 4 : 0},
+                     f8_lds + (slot * BN + 8 * wave) * F8_BLOCK,
+                     f8_lds + Z::X + (slot * BM + 8 * wave) * F8_BLOCK,
+                     f8_lds + (row < BM ? Z::SCALES + buf * Z::GROUP + row * 16 : Z::NOTHING + 256 * wave),
+                     any ? ((row + (lane >> 2)) * a.kb + (lane & 3)) * 4 : F8_NONE};
+    };
+    constexpr int LOADS = 1 + NX + NW;
+    auto load = [&](const F8Loads& l, int i) {
+        if (i == 0) {
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(mf_rsrc(l.scales.from, l.scales.bytes), (lds_t)l.into_scales, 4, l.scales_off, 0, 0, 0);
+        } else if (i <= NX) {
+            const int r = 8 * WAVES * (i - 1);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(mf_rsrc(l.x.from, l.x.bytes), (lds_t)(l.into_x + r * F8_BLOCK), 16, lane_off + r * a.K, 0, 0, 0);
+        } else {
+            const int r = 8 * WAVES * (i - 1 - NX), up = PAIR && r >= CN ? 1 : 0;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(mf_rsrc(l.w[up].from, l.w[up].bytes), (lds_t)(l.into_w + r * F8_BLOCK), 16, lane_off + (r - up * CN) * a.K, 0, 0, 0);
+        }
     };
     hx_f4 acc[TN][TM];
 #pragma unroll
@@ -398,30 +431,35 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
     const scalar_t ws[2] = {(scalar_t)(a.w[0].scales + (size_t)wblock * a.kb), PAIR ? (scalar_t)(a.w[1].scales + (size_t)wblock * a.kb) : nullptr};
     float wnext[2] = {ws[0][first], PAIR ? ws[1][first] : 0.0f};
 
-    auto step = [&](const uint8_t* sw, const uint8_t* sx, const float* sc, int c, auto whole) {
+    // One step, with the loads for a later one first: between the products, where a wave's vector instructions would alternate with its
+    // matrix instructions, they cost 8000 rows of 4096 -> 4096 163 us where 151 were.
+    auto step = [&](const F8Stage& g, const F8Loads& l, auto whole) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) load(l, i);
         auto fragment = [&](const uint8_t* p) {
             F8Raw v;
             v.p[0] = *reinterpret_cast<const f8_u4*>(p);
             v.p[1] = *reinterpret_cast<const f8_u4*>(f8_lds + ((p - f8_lds) ^ 64));
             if constexpr (!decltype(whole)::value) {  // what lies behind a row's K counts as 0
-                const int left = a.K - c * F8_BLOCK;
-                if (16 * kg >= left) v.p[0] = f8_u4{};
-                if (64 + 16 * kg >= left) v.p[1] = f8_u4{};
+                if (16 * kg >= g.left) v.p[0] = f8_u4{};
+                if (64 + 16 * kg >= g.left) v.p[1] = f8_u4{};
             }
             return v;
         };
-        auto weights = [&](int i) { return fragment(sw + pa + (PAIR ? i / TP * CN + i % TP * 16 : i * 16) * F8_BLOCK); };
+        auto weights = [&](int i) { return fragment(g.w + pa + (PAIR ? i / TP * CN + i % TP * 16 : i * 16) * F8_BLOCK); };
         const float s[2] = {wnext[0], wnext[1]};
-        const int next = min(c + 1, a.kb - 1);
-        wnext[0] = ws[0][next];
-        if constexpr (PAIR) wnext[1] = ws[1][next];
-        F8Raw w, x[TM];
+        F8Raw x[TM];
         float f[TM];
+        F8Raw w = weights(0);
 #pragma unroll
-        for (int j = 0; j < TM; ++j) x[j] = fragment(sx + pb + j * 16 * F8_BLOCK);
-        w = weights(0);
+        for (int j = 0; j < TM; ++j) x[j] = fragment(g.x + pb + j * 16 * F8_BLOCK);
 #pragma unroll
-        for (int j = 0; j < TM; ++j) f[j] = sc[(wm * TM * 16 + 16 * j + col) * 4];
+        for (int j = 0; j < TM; ++j) f[j] = g.scales[(wm * TM * 16 + 16 * j + col) * 4];
+        auto sums = [&](int i, int j, const hx_f4& t) {  // of one product
+            const float q = f[j] * s[PAIR && i >= TP];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(q, t[e], acc[i][j][e]);
+        };
         if constexpr (EXACT) {
             F8Half b[TM];
 #pragma unroll
@@ -440,35 +478,27 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
                     for (int j = 0; j < TM; ++j) t[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, b[j].k[2 * h + 1], t[j], 0, 0, 0);
                 }
 #pragma unroll
-                for (int j = 0; j < TM; ++j) {
-                    const float r = f[j] * s[PAIR && i >= TP];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(r, t[j][e], acc[i][j][e]);
-                }
+                for (int j = 0; j < TM; ++j) sums(i, j, t[j]);
             }
         } else {
             // One product and four of the sums of the row block before at a time: a wave's vector instructions fit behind its own products.
             hx_f4 t[2][TM];
-            auto scaled = [&](int i, int j) {
-                const float r = f[j] * s[PAIR && i >= TP];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(r, t[i & 1][j][e], acc[i][j][e]);
-            };
+            F8Raw ahead[2] = {w, weights(1)};
 #pragma unroll
             for (int i = 0; i < TN; ++i) {
-                const F8Raw v = w;
-                if (i + 1 < TN) w = weights(i + 1);
+                const F8Raw v = ahead[i & 1];
+                if (i + 2 < TN) ahead[i & 1] = weights(i + 2);
 #pragma unroll
                 for (int j = 0; j < TM; ++j) {
                     t[i & 1][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(f8_v8, v), __builtin_bit_cast(f8_v8, x[j]),
                                                                                    hx_f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
                     __builtin_amdgcn_sched_barrier(0);
-                    if (i > 0) scaled(i - 1, j);
+                    if (i > 0) sums(i - 1, j, t[(i - 1) & 1][j]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
 #pragma unroll
-            for (int j = 0; j < TM; ++j) scaled(TN - 1, j);
+            for (int j = 0; j < TM; ++j) sums(TN - 1, j, t[(TN - 1) & 1][j]);
         }
     };
     constexpr int NS = (BM + 16 * WAVES - 1) / (16 * WAVES);  // parts of a group of scales
@@ -476,27 +506,27 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
 #pragma unroll
     for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int u = 0; u < NS; ++u) load_scales(g, g, u);
+        for (int u = 0; u < NS; ++u) load(loads(0, first, g, g, u), 0);
 #pragma unroll
     for (int u = 0; u < PF - 1; ++u) {
         asm volatile("" ::: "memory");
-        load_scales(0, 0, 4);  // of none: the waits below count this many loads for every step
-        load_x(u, first + u);
-        load_w(u, first + u);
+        const F8Loads l = loads(u, first + u, 0, 0, 4);  // with scales of no rows: the waits below count LOADS for every step
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) load(l, i);
     }
-    int slot = 0, group = 0;  // of weights (and x), of scales
+    int slot = 0, group = 0;  // of codes, of scales
     auto round = [&](int c, auto whole) {
         const int d = c - first;
         // This step's loads of this wave have arrived, once at most those of the PF - 2 steps before it are outstanding.
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(qt_vmcnt((PF - 2) * (NW + NX + 1)));
+        __builtin_amdgcn_s_waitcnt(qt_vmcnt((PF - 2) * LOADS));
         hx_lds_barrier();  // and the other waves'; the stage of the step before is no longer read
-        const int ahead = slot == 0 ? PF - 1 : slot - 1;
-        load_scales(group == 0 ? 2 : group - 1, (d >> 2) + 2, d & 3);
-        load_x(ahead, c + PF - 1);
-        load_w(ahead, c + PF - 1);
-        step(f8_lds + slot * BN * F8_BLOCK, f8_lds + Z::X + slot * BM * F8_BLOCK,
-             reinterpret_cast<const float*>(f8_lds + Z::SCALES + group * Z::GROUP) + (d & 3), c, whole);
+        const F8Stage g{f8_lds + slot * BN * F8_BLOCK, f8_lds + Z::X + slot * BM * F8_BLOCK,
+                        reinterpret_cast<const float*>(f8_lds + Z::SCALES + group * Z::GROUP) + (d & 3), a.K - c * F8_BLOCK};
+        step(g, loads(slot == 0 ? PF - 1 : slot - 1, c + PF - 1, group == 0 ? 2 : group - 1, (d >> 2) + 2, d & 3), whole);
+        const int next = min(c + 1, a.kb - 1);
+        wnext[0] = ws[0][next];
+        if constexpr (PAIR) wnext[1] = ws[1][next];
         slot = slot + 1 == PF ? 0 : slot + 1;
         if ((d & 3) == 3) group = group == 2 ? 0 : group + 1;
     };
@@ -508,7 +538,7 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
     __builtin_amdgcn_s_waitcnt(qt_vmcnt(0));
     hx_lds_barrier();
 
-    if (sp.splits > 1) {  // the splits' sums, in order: the last workgroup of a tile to arrive adds them
+    if (Z::SPLITS && sp.splits > 1) {  // the splits' sums, in order: the last workgroup of a tile to arrive adds them
         constexpr int PIECES = TN * TM * 64 * WAVES;
         hx_f4* mine = a.partial + (size_t)tile * sp.splits * PIECES;
         const __amdgpu_buffer_rsrc_t rp = coherent_rsrc(mine);
@@ -517,36 +547,35 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
 #pragma unroll
             for (int j = 0; j < TM; ++j) coherent_store4(rp, (split * PIECES + ((i * TM + j) * WAVES + wave) * 64 + lane) * 16, acc[i][j]);
         if (!arrive_last(a.counters + tile, sp.splits)) return;
+        // several splits' loads in flight: one at a time, each is a round trip of over a us
+        constexpr int BATCH = Z::SPLITS ? 16 / (TN * TM) : 1;
 #pragma unroll
         for (int i = 0; i < TN; ++i)
 #pragma unroll
-            for (int j = 0; j < TM; ++j) {
-                const int at = (((i * TM + j) * WAVES + wave) * 64 + lane) * 16;
-                hx_f4 v = coherent_load4(rp, at);
-                for (int p = 1; p < sp.splits; ++p) v += coherent_load4(rp, at + p * PIECES * 16);
-                acc[i][j] = v;
-            }
+            for (int j = 0; j < TM; ++j) acc[i][j] = hx_f4{0.f, 0.f, 0.f, 0.f};
+        for (int p0 = 0; p0 < sp.splits; p0 += BATCH) {
+            hx_f4 t[BATCH][TN][TM];
+#pragma unroll
+            for (int p = 0; p < BATCH; ++p)
+#pragma unroll
+                for (int i = 0; i < TN; ++i)
+#pragma unroll
+                    for (int j = 0; j < TM; ++j)
+                        t[p][i][j] = coherent_load4(rp, (min(p0 + p, sp.splits - 1) * PIECES + ((i * TM + j) * WAVES + wave) * 64 + lane) * 16);
+#pragma unroll
+            for (int p = 0; p < BATCH; ++p)
+                if (p0 + p < sp.splits)
+#pragma unroll
+                    for (int i = 0; i < TN; ++i)
+#pragma unroll
+                        for (int j = 0; j < TM; ++j) acc[i][j] += t[p][i][j];
+        }
     }
     if constexpr (!PAIR) {
-        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-        const size_t size = a.y_fp32 ? 4 : 2;
-        const bool four = a.N % 4 == 0 && reinterpret_cast<uintptr_t>(a.y) % (4 * size) == 0;  // four outputs of a row in one store
 #pragma unroll
         for (int i = 0; i < TN; ++i)
 #pragma unroll
-            for (int j = 0; j < TM; ++j) {
-                const int n = n0 + (wn * TN + i) * 16 + 4 * kg, m = m0 + (wm * TM + j) * 16 + col;
-                const size_t at = (size_t)m * a.N + n;
-                if (m >= a.M || n >= a.N) continue;
-                if (four) {
-                    if (a.y_fp32) *reinterpret_cast<hx_f4*>(static_cast<float*>(a.y) + at) = acc[i][j];
-                    else *reinterpret_cast<h4*>(static_cast<_Float16*>(a.y) + at) = __builtin_convertvector(acc[i][j], h4);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (n + e < a.N) f8_store(a.y, at + e, acc[i][j][e], a.y_fp32);
-                }
-            }
+            for (int j = 0; j < TM; ++j) f8_store4(a, m0 + (wm * TM + j) * 16 + col, n0 + (wn * TN + i) * 16 + 4 * kg, acc[i][j]);
     } else {
         const int nb = (a.N + F8_BLOCK - 1) / F8_BLOCK, block = n0 / F8_BLOCK;
         hx_f4 v[TP][TM];
@@ -598,71 +627,88 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
 #pragma unroll
                 for (int j = 0; j < TM; ++j)
                     coherent_store4(rd, (((wm * TM + j) * 16 + col) * F8_BLOCK + n0 % F8_BLOCK + (wn * TP + i) * 16 + 4 * kg) * 4, v[i][j]);
-            if (arrive_last(a.counters + mt * nt + at, min(per, nt - block * per))) f8_finish_block<64 * WAVES>(a, dst, BM, m0, block);
+            if (arrive_last(a.counters + mt * nt + at, min(per, nt - block * per))) f8_finish_block<64 * WAVES, BM / (2 * WAVES) < 8 ? BM / (2 * WAVES) : 8>(a, dst, BM, m0, block);
         }
     }
 }
 
 namespace {
 
-// Which kernel takes a call.
+// Which kernel takes a call, and the parts of K.
 struct F8Plan {
-    enum Kind { ROWS, TILE64x32, TILE64x64, TILE128x128, TILE256x256 } kind;
+    enum Kind { ROWS, TILE64x32, TILE64x64, TILE128x64, TILE128x128, TILE256x256, NONE } kind;
     int splits, steps;
     long tiles;
     size_t partial, products;  // bytes of workspace
 };
-struct F8Tile {
-    int bn, bm;
-};
-constexpr F8Tile F8_TILES[] = {{0, 0}, {64, 32}, {64, 64}, {128, 128}, {256, 256}};
+enum F8Sums { F8_FAST, F8_EXACT, F8_GATED };  // fp16 outputs; fp32 outputs; gated pair (exact)
 constexpr int F8_CUS = 256, F8_COUNTERS = (int)(HX_COUNTER_BYTES / sizeof(int));
-constexpr size_t F8_MOST_PRODUCTS = 48u << 20;  // with the sums of parts of K
+constexpr size_t F8_MOST_PRODUCTS = 48u << 20;
 
-F8Plan f8_plan(int M, int N, int K, bool pair, bool split)
+// A tile, how many of its workgroups a CU holds, and what it costs, in us: to begin and end; a step of a workgroup at least; a step of each
+// workgroup on a CU; where K is split, for the join and for each split of it.  Fitted to some 200 calls of either sort (20 to 1000 rows, K and N 2048 to 12288),
+// the model is within 8 % rms, and its choice takes 1 % longer than the best of the tiles and splits on average, 10 % at most.
+struct F8Tile {
+    int bn, bm, resident;
+    float start, step, each, join, split;
+};
+constexpr F8Tile F8_TILES[2][6] = {
+    {{}, {64, 32, 2, 2.8f, 0.40f, 0.33f, 2.7f, 0.13f}, {64, 64, 3, 3.2f, 0.44f, 0.30f, 2.5f, 0.31f}, {128, 64, 2, 3.5f, 0.58f, 0.44f, 2.1f, 0.69f},
+     {128, 128, 1, 4.2f, 0.68f, 0.71f, 2.0f, 1.15f}, {256, 256, 1, 9.4f, 1.69f, 1.69f, 0.f, 0.f}},
+    {{}, {64, 32, 2, 2.6f, 0.51f, 0.39f, 2.8f, 0.15f}, {64, 64, 3, 3.4f, 0.56f, 0.385f, 2.3f, 0.31f}, {128, 64, 2, 4.0f, 0.80f, 0.59f, 1.8f, 0.65f},
+     {}, {256, 256, 1, 9.6f, 3.11f, 3.11f, 0.f, 0.f}}};  // exact, 128 x 128 is at most 3 % before 128 x 64
+
+F8Plan f8_plan(int M, int N, int K, F8Sums sums, bool split)
 {
     F8Plan p{};
+    const bool pair = sums == F8_GATED;
     const long nb = ((long)N + F8_BLOCK - 1) / F8_BLOCK;
     const int kb = (K + F8_BLOCK - 1) / F8_BLOCK;
+    const size_t few = (size_t)nb * F8_ROWS * F8_BLOCK * sizeof(float);
     p.splits = 1;
     p.steps = kb;
-    const size_t few = (size_t)nb * 16 * F8_BLOCK * sizeof(float);
-    if (M <= 16 && !(pair && (nb > F8_COUNTERS || few > F8_MOST_PRODUCTS))) {
+    if (M <= F8_ROWS && !(pair && (nb > F8_COUNTERS || few > F8_MOST_PRODUCTS))) {
         p.kind = F8Plan::ROWS;
         if (pair) p.products = few;
         return p;
     }
-    auto tiles = [&](int kind) { return ((long)M + F8_TILES[kind].bm - 1) / F8_TILES[kind].bm * (((long)N * (pair ? 2 : 1) + F8_TILES[kind].bn - 1) / F8_TILES[kind].bn); };
-    p.kind = M <= 32 ? F8Plan::TILE64x32 : M <= 64 || tiles(F8Plan::TILE128x128) < F8_CUS ? F8Plan::TILE64x64 : F8Plan::TILE128x128;
-    if (M > 128 && tiles(F8Plan::TILE256x256) >= F8_CUS) p.kind = F8Plan::TILE256x256;
-    const F8Tile t = F8_TILES[p.kind];
-    p.tiles = tiles(p.kind);
-    const long pieces = ((long)M + t.bm - 1) / t.bm * nb;  // blocks of 128 outputs by BM rows
-    const size_t products = (size_t)pieces * t.bm * F8_BLOCK * sizeof(float);
-    if (pair && t.bn < 2 * F8_BLOCK && (p.tiles + pieces > F8_COUNTERS || products > F8_MOST_PRODUCTS)) {
-        p.kind = F8Plan::TILE256x256;
-        p.tiles = tiles(p.kind);
-        return p;
+    float least = 0.0f;
+    p.kind = F8Plan::NONE;
+    for (int kind = F8Plan::TILE64x32; kind <= F8Plan::TILE256x256; ++kind) {
+        const F8Tile& t = F8_TILES[sums != F8_FAST][kind];
+        if (!t.bn) continue;
+        const long mt = ((long)M + t.bm - 1) / t.bm, tiles = mt * (((long)N * (pair ? 2 : 1) + t.bn - 1) / t.bn);
+        const bool whole = !pair || t.bn == 2 * F8_BLOCK;  // no blocks of outputs in parts, to be scaled later
+        const size_t products = whole ? 0 : (size_t)(mt * nb) * t.bm * F8_BLOCK * sizeof(float);
+        if (!whole && (tiles + mt * nb > F8_COUNTERS || products > F8_MOST_PRODUCTS)) continue;
+        for (int s = 1; s <= 8; s *= 2) {
+            const int steps = (kb + s - 1) / s;
+            if (s > 1 && (!split || t.join == 0.f || kb < 2 * s || tiles * s > (long)F8_CUS * t.resident)) break;  // all are at work at once
+            const float each = (float)((tiles * s + F8_CUS - 1) / F8_CUS);
+            const float us = t.start + (pair ? whole ? 2.0f : 3.4f : 0.0f) + steps * std::max(t.step, each * t.each) + (s > 1 ? t.join + t.split * each * s : 0.0f);
+            if (p.kind != F8Plan::NONE && us >= least) continue;
+            least = us;
+            p.kind = (F8Plan::Kind)kind;
+            p.tiles = tiles;
+            p.steps = steps;
+            p.splits = (kb + steps - 1) / steps;
+            p.partial = p.splits > 1 ? (size_t)tiles * p.splits * t.bn * t.bm * sizeof(float) : 0;
+            p.products = products;
+        }
     }
-    if (split && p.kind != F8Plan::TILE256x256) {
-        int s = 1;
-        while (p.tiles * s * 2 <= 2 * F8_CUS && s < 8 && kb / (2 * s) >= 4) s *= 2;
-        p.steps = (kb + s - 1) / s;
-        p.splits = (kb + p.steps - 1) / p.steps;
-        if (p.splits > 1) p.partial = (size_t)p.tiles * p.splits * t.bn * t.bm * sizeof(float);
-    }
-    if (pair && t.bn < 2 * F8_BLOCK) p.products = products;
     return p;
 }
 
-template <int S, int TG, int WAVES, int NS, int NT, bool PAIR>
+// One workgroup a CU; waves along K as there are spans of two blocks, up to all.
+template <int NS, bool PAIR>
 hipError_t rows_launch(const F8Call& c, hipStream_t st)
 {
-    const int spans = (c.kb + S - 1) / S;
-    int log2 = 0;  // waves along K: as many as have spans, up to all
+    constexpr int WAVES = F8_ROWS_THREADS / 64;
+    const int spans = (c.kb + 1) / 2;
+    int log2 = 0;
     while (1 << log2 < WAVES && NS << log2 < spans) ++log2;
-    const long rows = (WAVES >> log2) * (PAIR ? NT / 2 : NT) * 16 / S, tiles = (c.N + rows - 1) / rows;
-    hipLaunchKernelGGL((f8_rows_kernel<S, TG, WAVES, NS, NT, PAIR>), dim3(tiles < 2 * F8_CUS ? tiles : 2 * F8_CUS), dim3(64 * WAVES), 0, st, c, log2);
+    const long rows = (WAVES >> log2) * F8_ROWS, tiles = (c.N + rows - 1) / rows;
+    hipLaunchKernelGGL((f8_rows_kernel<NS, PAIR>), dim3(tiles < F8_CUS ? tiles : F8_CUS), dim3(F8_ROWS_THREADS), 0, st, c, log2);
     return hipGetLastError();
 }
 
@@ -676,24 +722,28 @@ hipError_t tile_launch(const F8Call& c, const F8Plan& p, hipStream_t st)
     return hipGetLastError();
 }
 
-template <bool PAIR>
+template <F8Sums SUMS>
 hipError_t f8_launch(F8Call c, const F8Plan& p, void* ws, hipStream_t st)
 {
     c.counters = static_cast<int*>(ws);
     c.partial = reinterpret_cast<hx_f4*>(static_cast<char*>(ws) + HX_COUNTER_BYTES);
     c.products = reinterpret_cast<float*>(static_cast<char*>(ws) + HX_COUNTER_BYTES + p.partial);
+    constexpr bool FAST = SUMS == F8_FAST, PAIR = SUMS == F8_GATED;
     switch (p.kind) {
         case F8Plan::ROWS:
-            if (c.M <= 4) return rows_launch<4, 1, 8, 1, 2, PAIR>(c, st);
-            if (c.M <= 8) return rows_launch<2, 1, 8, 2, 2, PAIR>(c, st);
-            return rows_launch<2, 2, 8, 2, 2, PAIR>(c, st);
-        case F8Plan::TILE64x32: return tile_launch<2, 2, 2, 1, 6, true, PAIR>(c, p, st);
-        case F8Plan::TILE64x64: return tile_launch<2, 2, 2, 2, 4, true, PAIR>(c, p, st);
-        case F8Plan::TILE128x128: return tile_launch<2, 2, 4, 4, 2, true, PAIR>(c, p, st);
-        default:
+            // two spans a wave where 16 waves have them: 8 rows of 8192 -> 4096 10.8 us, 13.3 in two rounds over K (the pair's codes would not fit: 41 us
+            // where 28 are)
             if constexpr (!PAIR)
-                if (!c.y_fp32) return tile_launch<2, 4, 8, 4, 2, false, PAIR>(c, p, st);
-            return tile_launch<2, 4, 8, 4, 2, true, PAIR>(c, p, st);
+                if (c.kb > 2 * F8_ROWS_THREADS / 64) return rows_launch<2, PAIR>(c, st);
+            return rows_launch<1, PAIR>(c, st);
+        case F8Plan::TILE64x32: return tile_launch<2, 2, 2, 1, 6, !FAST, PAIR>(c, p, st);
+        case F8Plan::TILE64x64: return tile_launch<2, 2, 2, 2, 3, !FAST, PAIR>(c, p, st);
+        case F8Plan::TILE128x64: return tile_launch<2, 2, 4, 2, 3, !FAST, PAIR>(c, p, st);
+        case F8Plan::TILE128x128:
+            if constexpr (FAST) return tile_launch<2, 4, 4, 2, 3, false, false>(c, p, st);
+            return hipErrorInvalidValue;
+        case F8Plan::TILE256x256: return tile_launch<2, 4, 8, 4, 2, !FAST, PAIR>(c, p, st);
+        default: return hipErrorInvalidValue;
     }
 }
 
@@ -707,12 +757,12 @@ int f8_most_rows(int N, bool pair)
 }
 
 // Of the launches that a call is made of.
-size_t f8_call_workspace(int M, int N, int K, bool pair)
+size_t f8_call_workspace(int M, int N, int K, F8Sums sums)
 {
-    const int most = f8_most_rows(N, pair);
-    size_t need = f8_workspace(f8_plan(M < most ? M : most, N, K, pair, true));
+    const int most = f8_most_rows(N, sums == F8_GATED);
+    size_t need = f8_workspace(f8_plan(M < most ? M : most, N, K, sums, true));
     if (M > most && M % most) {
-        const size_t last = f8_workspace(f8_plan(M % most, N, K, pair, true));
+        const size_t last = f8_workspace(f8_plan(M % most, N, K, sums, true));
         if (last > need) need = last;
     }
     return need;
@@ -720,8 +770,8 @@ size_t f8_call_workspace(int M, int N, int K, bool pair)
 
 }  // namespace
 
-size_t f8_gemm_workspace_bytes(int M, int N, int K) { return f8_call_workspace(M, N, K, false); }
-size_t f8_gate_up_workspace_bytes(int M, int N, int K) { return f8_call_workspace(M, N, K, true); }
+size_t f8_gemm_workspace_bytes(int M, int N, int K) { return std::max(f8_call_workspace(M, N, K, F8_FAST), f8_call_workspace(M, N, K, F8_EXACT)); }
+size_t f8_gate_up_workspace_bytes(int M, int N, int K) { return f8_call_workspace(M, N, K, F8_GATED); }
 
 hipError_t launch_f8_gemm(const uint8_t* x, const float* xs, const F8Blocks& w, void* y, int M, int N, int K, bool y_fp32, void* ws,
                           size_t ws_bytes, hipStream_t st)
@@ -729,12 +779,13 @@ hipError_t launch_f8_gemm(const uint8_t* x, const float* xs, const F8Blocks& w, 
     const int kb = (K + F8_BLOCK - 1) / F8_BLOCK, most = f8_most_rows(N, false);
     for (long m = 0; m < M; m += most) {
         const int rows = (int)(M - m < most ? M - m : most);
-        F8Plan p = f8_plan(rows, N, K, false, true);
-        if (p.partial && (!ws || ws_bytes < f8_workspace(p))) p = f8_plan(rows, N, K, false, false);
+        const F8Sums sums = y_fp32 ? F8_EXACT : F8_FAST;
+        F8Plan p = f8_plan(rows, N, K, sums, true);
+        if (p.partial && (!ws || ws_bytes < f8_workspace(p))) p = f8_plan(rows, N, K, sums, false);
         F8Call c{x + m * K, xs + m * kb, {w, {}}, rows, N, K, kb};
         c.y = static_cast<char*>(y) + m * N * (y_fp32 ? 4 : 2);
         c.y_fp32 = y_fp32;
-        const hipError_t e = f8_launch<false>(c, p, ws, st);
+        const hipError_t e = y_fp32 ? f8_launch<F8_EXACT>(c, p, ws, st) : f8_launch<F8_FAST>(c, p, ws, st);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
@@ -750,7 +801,7 @@ hipError_t launch_f8_gate_up(const uint8_t* x, const float* xs, const F8Blocks& 
         c.q = q + m * N;
         c.scales = scales + m * nb;
         c.limit = limit;
-        const hipError_t e = f8_launch<true>(c, f8_plan(rows, N, K, true, true), ws, st);
+        const hipError_t e = f8_launch<F8_GATED>(c, f8_plan(rows, N, K, F8_GATED, true), ws, st);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
