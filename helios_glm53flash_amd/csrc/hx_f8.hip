@@ -338,9 +338,12 @@ struct F8TileSize {
     static constexpr int WAVES = WN * WM, BN = 16 * WN * TN, BM = 16 * WM * TM;
     static constexpr int X = PF * BN * F8_BLOCK, SCALES = X + PF * BM * F8_BLOCK;  // where they begin in LDS
     static constexpr int GROUP = BM * 16, NOTHING = SCALES + 3 * GROUP, BYTES = NOTHING + 256 * WAVES;  // of scales: [rows][4]; where loads of none go
-    static constexpr int NW = BN / (8 * WAVES), NX = BM / (8 * WAVES);  // loads of a wave a step
+    // Waves that load.  With two waves a SIMD it is one of them: the other computes meanwhile (a wave takes some 1000 cycles to issue its loads,
+    // while the address units are busy; all 8 loading, 2000 rows of 4096 -> 24576 took 209 us where 203 are, fp32 outputs 341 where 333 are).
+    static constexpr int LW = WAVES == 8 ? 4 : WAVES;
+    static constexpr int NW = BN / (8 * LW), NX = BM / (8 * LW);  // their loads a step
     static constexpr bool SPLITS = TN * TM <= 16;  // K may be split: its sums take few registers next to a split's
-    static_assert(BN % (8 * WAVES) == 0 && BM % (8 * WAVES) == 0 && BM <= 64 * WAVES && PF <= 8);
+    static_assert(BN % (8 * LW) == 0 && BM % (8 * LW) == 0 && BM <= 64 * WAVES && PF <= 8);
 };
 
 // What a buffer load may read; a step's loads of a wave and where in LDS they go; a step's operands in LDS.
@@ -363,7 +366,7 @@ template <int WN, int WM, int TN, int TM, int PF, bool EXACT, bool PAIR>
 __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split sp)
 {
     using Z = F8TileSize<WN, WM, TN, TM, PF>;
-    constexpr int BN = Z::BN, BM = Z::BM, NW = Z::NW, NX = Z::NX, WAVES = Z::WAVES;
+    constexpr int BN = Z::BN, BM = Z::BM, NW = Z::NW, NX = Z::NX, WAVES = Z::WAVES, LW = Z::LW;
     constexpr int CN = PAIR ? BN / 2 : BN, TP = PAIR ? TN / 2 : TN;  // outputs of a tile along N; a wave's row blocks of them
     extern __shared__ __align__(16) uint8_t f8_lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -393,7 +396,7 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
     // Into stage `slot`, block c; of the scales part s of group g into group buffer `buf`: 16 rows a wave from 16 (s WAVES + wave) on, steps first + 4 g
     // and the three behind.
     auto loads = [&](int slot, int c, int buf, int g, int s) {
-        const int row = 16 * (s * WAVES + wave);
+        const int row = 16 * (s * LW + wave);
         const bool any = row < BM && first + 4 * g < steps;
         return F8Loads{{rows(0, c), rows(PAIR ? 1 : 0, c)},
                      rows(2, c),
@@ -408,10 +411,10 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
         if (i == 0) {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(mf_rsrc(l.scales.from, l.scales.bytes), (lds_t)l.into_scales, 4, l.scales_off, 0, 0, 0);
         } else if (i <= NX) {
-            const int r = 8 * WAVES * (i - 1);
+            const int r = 8 * LW * (i - 1);
             __builtin_amdgcn_raw_ptr_buffer_load_lds(mf_rsrc(l.x.from, l.x.bytes), (lds_t)(l.into_x + r * F8_BLOCK), 16, lane_off + r * a.K, 0, 0, 0);
         } else {
-            const int r = 8 * WAVES * (i - 1 - NX), up = PAIR && r >= CN ? 1 : 0;
+            const int r = 8 * LW * (i - 1 - NX), up = PAIR && r >= CN ? 1 : 0;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(mf_rsrc(l.w[up].from, l.w[up].bytes), (lds_t)(l.into_w + r * F8_BLOCK), 16, lane_off + (r - up * CN) * a.K, 0, 0, 0);
         }
     };
@@ -435,7 +438,8 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
     // matrix instructions, they cost 8000 rows of 4096 -> 4096 163 us where 151 were.
     auto step = [&](const F8Stage& g, const F8Loads& l, auto whole) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) load(l, i);
+        for (int i = 0; i < LOADS; ++i)
+            if (LW == WAVES || wave < LW) load(l, i);
         auto fragment = [&](const uint8_t* p) {
             F8Raw v;
             v.p[0] = *reinterpret_cast<const f8_u4*>(p);
@@ -501,18 +505,20 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
             for (int j = 0; j < TM; ++j) sums(TN - 1, j, t[(TN - 1) & 1][j]);
         }
     };
-    constexpr int NS = (BM + 16 * WAVES - 1) / (16 * WAVES);  // parts of a group of scales
+    constexpr int NS = (BM + 16 * LW - 1) / (16 * LW);  // parts of a group of scales
     static_assert(NS <= 4);
 #pragma unroll
     for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int u = 0; u < NS; ++u) load(loads(0, first, g, g, u), 0);
+        for (int u = 0; u < NS; ++u)
+            if (LW == WAVES || wave < LW) load(loads(0, first, g, g, u), 0);
 #pragma unroll
     for (int u = 0; u < PF - 1; ++u) {
         asm volatile("" ::: "memory");
         const F8Loads l = loads(u, first + u, 0, 0, 4);  // with scales of no rows: the waits below count LOADS for every step
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) load(l, i);
+        for (int i = 0; i < LOADS; ++i)
+            if (LW == WAVES || wave < LW) load(l, i);
     }
     int slot = 0, group = 0;  // of codes, of scales
     auto round = [&](int c, auto whole) {
@@ -654,9 +660,9 @@ struct F8Tile {
 };
 constexpr F8Tile F8_TILES[2][6] = {
     {{}, {64, 32, 2, 2.8f, 0.40f, 0.33f, 2.7f, 0.13f}, {64, 64, 3, 3.2f, 0.44f, 0.30f, 2.5f, 0.31f}, {128, 64, 2, 3.5f, 0.58f, 0.44f, 2.1f, 0.69f},
-     {128, 128, 1, 4.2f, 0.68f, 0.71f, 2.0f, 1.15f}, {256, 256, 1, 9.4f, 1.69f, 1.69f, 0.f, 0.f}},
+     {128, 128, 1, 4.2f, 0.68f, 0.71f, 2.0f, 1.15f}, {256, 256, 1, 9.4f, 1.66f, 1.66f, 0.f, 0.f}},
     {{}, {64, 32, 2, 2.6f, 0.51f, 0.39f, 2.8f, 0.15f}, {64, 64, 3, 3.4f, 0.56f, 0.385f, 2.3f, 0.31f}, {128, 64, 2, 4.0f, 0.80f, 0.59f, 1.8f, 0.65f},
-     {}, {256, 256, 1, 9.6f, 3.11f, 3.11f, 0.f, 0.f}}};  // exact, 128 x 128 is at most 3 % before 128 x 64
+     {}, {256, 256, 1, 9.6f, 3.0f, 3.0f, 0.f, 0.f}}};  // exact, 128 x 128 is at most 3 % before 128 x 64
 
 F8Plan f8_plan(int M, int N, int K, F8Sums sums, bool split)
 {
