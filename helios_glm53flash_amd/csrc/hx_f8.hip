@@ -292,7 +292,7 @@ __global__ __launch_bounds__(F8_ROWS_THREADS) void f8_rows_kernel(F8Call a, int 
     }
     if constexpr (PAIR) {
         // The last tile of a block of 128 outputs to arrive scales it.  A workgroup's tiles arrive together at its end: one by one, each waits for
-        // the codes in flight (one row of 4096 -> 12288, 6 tiles a workgroup: 27.6 us).
+        // the codes in flight (one row of 4096 -> 12288, 6 tiles a workgroup: 27.6 us where 24.1 are).
         int* full = reinterpret_cast<int*>(red);
         static_assert(F8_ROWS_THREADS * sizeof(int) <= sizeof(red));
         __builtin_amdgcn_s_waitcnt(0);
@@ -650,6 +650,7 @@ struct F8Plan {
 enum F8Sums { F8_FAST, F8_EXACT, F8_GATED };  // fp16 outputs; fp32 outputs; gated pair (exact)
 constexpr int F8_CUS = 256, F8_COUNTERS = (int)(HX_COUNTER_BYTES / sizeof(int));
 constexpr size_t F8_MOST_PRODUCTS = 48u << 20;
+constexpr long F8_MOST_TILES = 1l << 22;  // of at most 512 threads
 
 // A tile, how many of its workgroups a CU holds, and what it costs, in us: to begin and end; a step of a workgroup at least; a step of each
 // workgroup on a CU; where K is split, for the join and for each split of it.  Fitted to some 200 calls of either sort (20 to 1000 rows, K and N 2048 to 12288),
@@ -684,6 +685,7 @@ F8Plan f8_plan(int M, int N, int K, F8Sums sums, bool split)
         const F8Tile& t = F8_TILES[sums != F8_FAST][kind];
         if (!t.bn) continue;
         const long mt = ((long)M + t.bm - 1) / t.bm, tiles = mt * (((long)N * (pair ? 2 : 1) + t.bn - 1) / t.bn);
+        if (tiles > F8_MOST_TILES) continue;
         const bool whole = !pair || t.bn == 2 * F8_BLOCK;  // no blocks of outputs in parts, to be scaled later
         const size_t products = whole ? 0 : (size_t)(mt * nb) * t.bm * F8_BLOCK * sizeof(float);
         if (!whole && (tiles + mt * nb > F8_COUNTERS || products > F8_MOST_PRODUCTS)) continue;
@@ -755,11 +757,11 @@ hipError_t f8_launch(F8Call c, const F8Plan& p, void* ws, hipStream_t st)
 
 size_t f8_workspace(const F8Plan& p) { return p.partial || p.products ? HX_COUNTER_BYTES + p.partial + p.products : 0; }
 
-// Rows of a launch, a multiple of 256: 2^22 tiles of at most 512 threads.
+// Rows of a launch, a multiple of 256: 2^22 tiles of 256 x 256.
 int f8_most_rows(int N, bool pair)
 {
-    const long columns = ((long)N * (pair ? 2 : 1) + 63) / 64;
-    return 256 * (int)(columns < 1l << 21 ? (1l << 21) / columns : 1);
+    const long columns = ((long)N * (pair ? 2 : 1) + 255) / 256, rows = F8_MOST_TILES / columns;  // columns <= 2^21
+    return 256 * (int)std::min(rows, 1l << 22);
 }
 
 // Of the launches that a call is made of.
