@@ -12,7 +12,7 @@
 //          2^-16 of its size (measured 1.6e-5 rms), so it serves fp16 outputs only, whose rounding is 2^-11.  (The gated pair's scales
 //          are fp32.)
 //
-//   M <= 8  f8_rows_kernel: the waves of a workgroup split K and keep their part of x in registers; they walk over the weight rows,
+//   M <= 8  f8_rows_kernel: the waves of a workgroup split K and keep x in registers or LDS; they walk over the weight rows,
 //           every code read once from memory into operands, and add their sums through LDS.  exact
 //   M > 8   f8_tile_kernel: tiles, both sides through a ring of LDS stages.  fast for fp16 outputs, else exact
 #include <algorithm>
@@ -43,10 +43,6 @@ struct F8Raw {
 };
 struct F8Half {
     hx_h8 k[4];
-};
-template <int NS>
-struct F8Spans {
-    F8Raw of[NS];
 };
 HX_INLINE F8Half f8_half(const F8Raw& r)
 {
@@ -147,49 +143,41 @@ HX_INLINE void f8_finish_block(const F8Call& c, const float* v, int rows, int m0
 // cache lines of each weight row, which a load from 16 rows by 64 bytes does not get (15 bytes a cycle and CU; 45 from 8 rows by 128), and
 // twice as many pieces of work.  Load h of a lane takes the 16 bytes 4 s + kg of the span's half h, so that its 8 lanes of a row are
 // consecutive: half h is block h of the span.
-// A workgroup's waves split K (all WAVES of them, if it has as many spans; else they also split the tile's rows), each owns NS spans of every
-// WK NS, keeps x for them in registers and goes over tiles of 8 weight rows (of a gated pair: 8 of gate and 8 of up); codes are replaced
-// by the next tile's as soon as they are converted.  One workgroup of 16 waves a CU: 8 rows of 4096 -> 12288 take 12.5 us, 15.1 with two workgroups
-// and 17.8 with two of 8 waves; one row of 4096 -> 151552 96.7 us (6.4 TB/s).
-template <int NS, bool PAIR>
+// A workgroup's waves split K, a span each (with fewer spans than waves they also split the tile's rows), and go over tiles of 8 weight rows
+// (of a gated pair: 8 of gate and 8 of up); codes are replaced by the next piece's as soon as they are converted.  One workgroup of 16 waves
+// a CU: 8 rows of 4096 -> 12288 took 12.5 us, 15.1 with two workgroups and 17.8 with two of 8 waves; now 11.4, and 8 rows of 4096 -> 151552 97 us
+// (6.4 TB/s).
+// x stays in registers as fp16 where a round of spans is all of K, up to 4096 (from LDS: 1 row of 4096 -> 12288 the same, the pair of 8 rows of
+// 4096 -> 2048 12.2 us where 11.4 are).  Where it is not (FAR), x stays in LDS as codes, piece u of a block of row r at piece u ^ (r & 7), rows a
+// multiple of 1 KB, then its scales, [block][8]: 8 rows of 12288 -> 4096 12.8 us; 20.8 with x loaded again in every round.  (Two spans a wave, so that
+// K up to 8192 is one round, took 10.9 us for 8 rows of 8192 -> 4096 where this takes 10.0.)
+constexpr int f8_far_row(int K) { return (K + 1023) / 1024 * 1024; }
+constexpr int f8_far_blocks(int kb) { return (kb + 31) / 32 * 32; }  // whole rounds of 16 spans: zeros behind K
+inline size_t f8_far_bytes(int M, int K) { return (size_t)M * f8_far_row(K) + f8_far_blocks((K + F8_BLOCK - 1) / F8_BLOCK) * F8_ROWS * sizeof(float); }
+
+template <bool PAIR, bool FAR>
 __global__ __launch_bounds__(F8_ROWS_THREADS) void f8_rows_kernel(F8Call a, int wk_log2)
 {
     constexpr int WAVES = F8_ROWS_THREADS / 64, R = F8_ROWS, P = PAIR ? 2 : 1;
     __shared__ __align__(16) float red[2][P * R * R * WAVES];  // of this tile and the next: [row part][p][token][r][wave in K]
+    extern __shared__ __align__(16) uint8_t f8_lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wk = 1 << wk_log2, kw = wave & (wk - 1), rw = wave >> wk_log2, wr = WAVES >> wk_log2;  // the wave's place in K and in rows
     const int col = lane & 15, kg = lane >> 4, s = col / R, r = col % R;
-    const int nkb = ((a.kb + 1) / 2 + wk * NS - 1) / (wk * NS);               // rounds over K
+    const int rounds = FAR ? ((a.kb + 1) / 2 + wk - 1) >> wk_log2 : 1;        // over K
     const int rows_wg = wr * R, tiles = (a.N + rows_wg - 1) / rows_wg;        // rows_wg: a power of two up to 128
-    const int other = kg / 2 == s ? 0 : F8_NONE;  // this lane's products are of unequal parts: it needs no scales
+    const int far_row = f8_far_row(a.K), far_r = min(r, a.M - 1);             // rows behind M: any
+    float* far_scales = reinterpret_cast<float*>(f8_lds + a.M * far_row);
 
-    const __amdgpu_buffer_rsrc_t rx = mf_rsrc(a.x, (size_t)a.M * a.K), rxs = mf_rsrc(a.xs, (size_t)a.M * a.kb * 4);
-    F8Half x[NS];
-    float sx[NS][2][4];
-    auto span = [&](int i, int kb) { return (kb * NS + i) * wk + kw; };
+    const __amdgpu_buffer_rsrc_t rx = mf_rsrc(a.x, (size_t)a.M * a.K);
+    F8Half x;
+    float sx[2][4];  // of the input rows of this lane's products of equal parts; its other products are not used
     const int in_span = 16 * (4 * s + kg);  // of this lane's first piece
-    auto load_x = [&](int kb) {
-        F8Spans<NS> raw;
-#pragma unroll
-        for (int i = 0; i < NS; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int b = 2 * span(i, kb) + h, k = b * F8_BLOCK + in_span;
-                raw.of[i].p[h] = __builtin_bit_cast(f8_u4, __builtin_amdgcn_raw_buffer_load_b128(rx, k < a.K ? r * a.K + k : F8_NONE, 0, 0));
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    sx[i][h][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rxs, ((kg % 2 * 4 + e) * a.kb + b) * 4 | (b < a.kb ? other : F8_NONE), 0, 0));
-            }
-        return raw;
-    };
-    auto keep_x = [&](const F8Spans<NS>& raw) {
-#pragma unroll
-        for (int i = 0; i < NS; ++i) x[i] = f8_half(raw.of[i]);
-    };
-    // The codes by vector loads, the scales, which all lanes share, by scalar ones.
+    auto block = [&](int round, int h) { return 2 * (round * wk + kw) + h; };
+    // The codes by vector loads, the scales, which all lanes share, by scalar ones; behind K the codes are 0 and the scales any.
     typedef const __attribute__((address_space(4))) float* scalar_t;
-    F8Raw w[NS][P];
-    float sw[NS][P][2];
+    F8Raw w[P];
+    float sw[P][2];
     __amdgpu_buffer_rsrc_t rw_[P];
     scalar_t ws[P];
     auto aim = [&](int tile) {  // descriptors of the tile's rows (nothing left of the matrix: every load is 0)
@@ -200,57 +188,90 @@ __global__ __launch_bounds__(F8_ROWS_THREADS) void f8_rows_kernel(F8Call a, int 
             ws[p] = (scalar_t)(a.w[p].scales + (left ? row0 / F8_BLOCK * a.kb : 0));
         }
     };
-    auto load_w = [&](int i, int p, int kb) {
+    auto load_w = [&](int p, int round) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int b = 2 * span(i, kb) + h, k = b * F8_BLOCK + in_span;
-            w[i][p].p[h] = __builtin_bit_cast(f8_u4, __builtin_amdgcn_raw_buffer_load_b128(rw_[p], k < a.K ? r * a.K + k : F8_NONE, 0, 0));
-            sw[i][p][h] = ws[p][min(b, a.kb - 1)];
+            const int b = block(round, h), k = b * F8_BLOCK + in_span;
+            w[p].p[h] = __builtin_bit_cast(f8_u4, __builtin_amdgcn_raw_buffer_load_b128(rw_[p], k < a.K ? r * a.K + k : F8_NONE, 0, 0));
+            sw[p][h] = ws[p][min(b, a.kb - 1)];
         }
     };
-    int tile = blockIdx.x;
+    // Workgroups go to the 8 XCDs in turn: neighbouring tiles, which share lines of y, go to one (8 rows of 4096 -> 151552, fp32 outputs: 97 us; 106
+    // where each XCD writes parts of all lines).
+    const int tile0 = gridDim.x % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
+    int tile = tile0;
     aim(tile);
-    {
-        const F8Spans<NS> raw = load_x(0);
+    if constexpr (!FAR) {
+        const __amdgpu_buffer_rsrc_t rxs = mf_rsrc(a.xs, (size_t)a.M * a.kb * 4);
+        F8Raw v;
 #pragma unroll
-        for (int i = 0; i < NS; ++i)
+        for (int h = 0; h < 2; ++h) {
+            const int b = block(0, h), k = b * F8_BLOCK + in_span;
+            v.p[h] = __builtin_bit_cast(f8_u4, __builtin_amdgcn_raw_buffer_load_b128(rx, k < a.K ? r * a.K + k : F8_NONE, 0, 0));
 #pragma unroll
-            for (int p = 0; p < P; ++p) load_w(i, p, 0);
-        keep_x(raw);
+            for (int e = 0; e < 4; ++e)
+                sx[h][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rxs, b < a.kb ? ((kg % 2 * 4 + e) * a.kb + b) * 4 : F8_NONE, 0, 0));
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) load_w(p, 0);
+        x = f8_half(v);
+    } else {
+        typedef __attribute__((address_space(3))) void* lds_t;
+        const int parts = far_row / 1024;  // of a row, a load of a wave each
+        for (int i = wave; i < a.M * parts; i += WAVES) {
+            const int row = i / parts, k = 16 * ((i % parts * 64 + lane) ^ (row & 7));
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_t)(f8_lds + i * 1024), 16, k < a.K ? row * a.K + k : F8_NONE, 0, 0, 0);
+        }
+        for (int i = threadIdx.x; i < f8_far_blocks(a.kb) * R; i += F8_ROWS_THREADS)
+            far_scales[i] = i % R < a.M && i / R < a.kb ? a.xs[i % R * a.kb + i / R] : 0.0f;
+#pragma unroll
+        for (int p = 0; p < P; ++p) load_w(p, 0);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(qt_vmcnt(0));
+        hx_lds_barrier();
     }
     for (int turn = 0; tile < tiles; tile += gridDim.x, turn ^= 1) {
         hx_f4 acc[P];
 #pragma unroll
         for (int p = 0; p < P; ++p) acc[p] = hx_f4{0.f, 0.f, 0.f, 0.f};
-        for (int kb = 0; kb < nkb; ++kb) {
-            if (nkb > 1) keep_x(load_x(kb));
-            const bool wrap = kb + 1 == nkb;
-            const int next_kb = wrap ? 0 : kb + 1;
+        for (int round = 0; round < rounds; ++round) {
+            const bool wrap = round + 1 == rounds;
             if (wrap) aim(tile + gridDim.x);
+            if constexpr (FAR) {
+                F8Raw v;
 #pragma unroll
-            for (int i = 0; i < NS; ++i) {
-                float f[P][2][4];
+                for (int h = 0; h < 2; ++h) {
+                    const int b = block(round, h);
+                    v.p[h] = *reinterpret_cast<const f8_u4*>(f8_lds + far_r * far_row + min(b, a.kb - 1) * F8_BLOCK + 16 * ((4 * s + kg) ^ far_r));
+                    const hx_f4 t = *reinterpret_cast<const hx_f4*>(far_scales + b * R + kg % 2 * 4);
 #pragma unroll
-                for (int p = 0; p < P; ++p)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) f[p][h][e] = sx[i][h][e] * sw[i][p][h];
-#pragma unroll
-                for (int p = 0; p < P; ++p) {
-                    const F8Half b = f8_half(w[i][p]);
-                    load_w(i, p, next_kb);
-                    __builtin_amdgcn_sched_barrier(0);  // the loads stay here, ahead of these codes' products
-                    hx_f4 t[2];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) t[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[i].k[2 * h], b.k[2 * h], hx_f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) t[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[i].k[2 * h + 1], b.k[2 * h + 1], t[h], 0, 0, 0);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[p][e] = __builtin_fmaf(f[p][h][e], t[h][e], acc[p][e]);
+                    for (int e = 0; e < 4; ++e) sx[h][e] = t[e];
                 }
+                x = f8_half(v);
+            }
+            float f[P][2][4];
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float q = block(round, h) < a.kb ? sw[p][h] : 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) f[p][h][e] = sx[h][e] * q;
+                }
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                const F8Half b = f8_half(w[p]);
+                load_w(p, wrap ? 0 : round + 1);
+                __builtin_amdgcn_sched_barrier(0);  // the loads stay here, ahead of these codes' products
+                hx_f4 t[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) t[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.k[2 * h], b.k[2 * h], hx_f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) t[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.k[2 * h + 1], b.k[2 * h + 1], t[h], 0, 0, 0);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[p][e] = __builtin_fmaf(f[p][h][e], t[h][e], acc[p][e]);
             }
         }
         // A wave's two parts, then the waves' sums, which lie together.
@@ -298,7 +319,7 @@ __global__ __launch_bounds__(F8_ROWS_THREADS) void f8_rows_kernel(F8Call a, int 
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
         const int per = F8_BLOCK / rows_wg;
-        for (long t0 = blockIdx.x; t0 < tiles; t0 += (long)F8_ROWS_THREADS * gridDim.x) {
+        for (long t0 = tile0; t0 < tiles; t0 += (long)F8_ROWS_THREADS * gridDim.x) {
             const long t = t0 + (long)threadIdx.x * gridDim.x;
             int block = -1;
             if (t < tiles) {
@@ -650,6 +671,8 @@ struct F8Plan {
 enum F8Sums { F8_FAST, F8_EXACT, F8_GATED };  // fp16 outputs; fp32 outputs; gated pair (exact)
 constexpr int F8_CUS = 256, F8_COUNTERS = (int)(HX_COUNTER_BYTES / sizeof(int));
 constexpr size_t F8_MOST_PRODUCTS = 48u << 20;
+constexpr size_t F8_FAR_BYTES = (160 - 16) * 1024;  // next to the rows kernel's sums
+constexpr int F8_NEAR = 2 * F8_ROWS_THREADS / 64;  // blocks of K whose spans are one round of the rows kernel's waves
 constexpr long F8_MOST_TILES = 1l << 22;  // of at most 512 threads
 
 // A tile, how many of its workgroups a CU holds, and what it costs, in us: to begin and end; a step of a workgroup at least; a step of each
@@ -674,7 +697,7 @@ F8Plan f8_plan(int M, int N, int K, F8Sums sums, bool split)
     const size_t few = (size_t)nb * F8_ROWS * F8_BLOCK * sizeof(float);
     p.splits = 1;
     p.steps = kb;
-    if (M <= F8_ROWS && !(pair && (nb > F8_COUNTERS || few > F8_MOST_PRODUCTS))) {
+    if (M <= F8_ROWS && !(pair && (nb > F8_COUNTERS || few > F8_MOST_PRODUCTS)) && (kb <= F8_NEAR || f8_far_bytes(M, K) <= F8_FAR_BYTES)) {
         p.kind = F8Plan::ROWS;
         if (pair) p.products = few;
         return p;
@@ -707,16 +730,16 @@ F8Plan f8_plan(int M, int N, int K, F8Sums sums, bool split)
     return p;
 }
 
-// One workgroup a CU; waves along K as there are spans of two blocks, up to all.
-template <int NS, bool PAIR>
+template <bool PAIR>
 hipError_t rows_launch(const F8Call& c, hipStream_t st)
 {
     constexpr int WAVES = F8_ROWS_THREADS / 64;
-    const int spans = (c.kb + 1) / 2;
-    int log2 = 0;
-    while (1 << log2 < WAVES && NS << log2 < spans) ++log2;
+    int log2 = 0;  // waves along K: as there are spans, up to all
+    while (1 << log2 < WAVES && 1 << log2 < (c.kb + 1) / 2) ++log2;
     const long rows = (WAVES >> log2) * F8_ROWS, tiles = (c.N + rows - 1) / rows;
-    hipLaunchKernelGGL((f8_rows_kernel<NS, PAIR>), dim3(tiles < F8_CUS ? tiles : F8_CUS), dim3(F8_ROWS_THREADS), 0, st, c, log2);
+    const dim3 grid(tiles < F8_CUS ? tiles : F8_CUS);
+    if (c.kb <= F8_NEAR) hipLaunchKernelGGL((f8_rows_kernel<PAIR, false>), grid, dim3(F8_ROWS_THREADS), 0, st, c, log2);
+    else hipLaunchKernelGGL((f8_rows_kernel<PAIR, true>), grid, dim3(F8_ROWS_THREADS), f8_far_bytes(c.M, c.K), st, c, log2);
     return hipGetLastError();
 }
 
@@ -738,12 +761,7 @@ hipError_t f8_launch(F8Call c, const F8Plan& p, void* ws, hipStream_t st)
     c.products = reinterpret_cast<float*>(static_cast<char*>(ws) + HX_COUNTER_BYTES + p.partial);
     constexpr bool FAST = SUMS == F8_FAST, PAIR = SUMS == F8_GATED;
     switch (p.kind) {
-        case F8Plan::ROWS:
-            // two spans a wave where 16 waves have them: 8 rows of 8192 -> 4096 10.8 us, 13.3 in two rounds over K (the pair's codes would not fit: 41 us
-            // where 28 are)
-            if constexpr (!PAIR)
-                if (c.kb > 2 * F8_ROWS_THREADS / 64) return rows_launch<2, PAIR>(c, st);
-            return rows_launch<1, PAIR>(c, st);
+        case F8Plan::ROWS: return rows_launch<PAIR>(c, st);
         case F8Plan::TILE64x32: return tile_launch<2, 2, 2, 1, 6, !FAST, PAIR>(c, p, st);
         case F8Plan::TILE64x64: return tile_launch<2, 2, 2, 2, 3, !FAST, PAIR>(c, p, st);
         case F8Plan::TILE128x64: return tile_launch<2, 2, 4, 2, 3, !FAST, PAIR>(c, p, st);

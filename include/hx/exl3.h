@@ -266,7 +266,7 @@ int hx_w4_embed(const hx_w4_words* w, const int64_t* tokens, void* out, int n, i
 /* Values in e4m3 (4 exponent bits, 3 mantissa bits, largest 448) with an fp32 scale for each block of 128 consecutive k of an input
  * row, or of 128 x 128 weights; the last blocks may be short (no counterpart in the reference):
  *   a = max(largest |v| of the block, 2^-100)   scale = a / 448   code = e4m3(v * (448 / a)), fp32 operations, ties to even
- * A block with a NaN or an infinity stands for NaN throughout.  K % 16 == 0, K <= 2^22 in all calls of this section; M == 0 is a
+ * A block with a NaN or an infinity stands for NaN throughout, and what reads a scale that is not finite is not finite.  K % 16 == 0, K <= 2^22 in all calls of this section; M == 0 is a
  * no-op (the pointers may then be NULL); outputs overlap neither inputs nor each other but where that is said. */
 
 /* q uint8 [M][K] and scales fp32 [M][ceil(K / 128)] of x (fp16 or fp32 by dtype, HX_DTYPE_*; rows ld elements apart, ld % 8 == 0).
@@ -286,10 +286,12 @@ typedef struct hx_f8_blocks {
     const float* scales;
 } hx_f8_blocks;
 
-/* y[M][N] = x W^T: x and x_scales as hx_f8_quantize gives them, y fp32 (y_fp32) or fp16: fp32 sums rounded once.  The codes' products
- * are exact, and a block's scales are applied to its fp32 sum.  The workspace is optional: a call with at least hx_f8_gemm_workspace_size(M, N, K)
- * bytes (0: the shape has no use for it) splits K over more workgroups where there are few, with the fp32 sums in another order
- * than without; NULL or fewer bytes do without. */
+/* y[M][N] = x W^T: x and x_scales as hx_f8_quantize gives them, y fp32 (y_fp32) or fp16: fp32 sums rounded once.  A block's scales are
+ * applied to the fp32 sum of its codes' products.  These are exact for fp32 outputs and M <= 8; with more rows and fp16 outputs, 8
+ * consecutive k (from a multiple of 8) are first added to 2^-13 of the largest of their 8 products, so that y is off by at most 7 * 2^-13
+ * times the sum of those largest ones beside its rounding (1.6e-5 of the outputs' size, rms, where the values are random).  The workspace
+ * is optional: a call with at least hx_f8_gemm_workspace_size(M, N, K) bytes (0: the shape has no use for it) splits K over more
+ * workgroups where there are few, with the fp32 sums in another order than without; NULL or fewer bytes do without. */
 size_t hx_f8_gemm_workspace_size(int M, int N, int K);
 int hx_f8_gemm(void* y, const void* x, const float* x_scales, const hx_f8_blocks* w, int M, int N, int K, int y_fp32,
                hx_stream_t stream, void* workspace, size_t workspace_bytes);

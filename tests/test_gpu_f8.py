@@ -536,6 +536,71 @@ def test_gate_up_with_nans_behind_every_edge(f8, M):
     check_guard(gs)
 
 
+def inside_nans(t, rows=3):
+    """A copy of t between rows of NaN."""
+    import torch
+    whole = torch.full((t.shape[0] + 2 * rows, t.shape[1]), float("nan"), device="cuda").to(t.dtype)
+    whole.view(torch.uint8)[rows:-rows] = t.view(torch.uint8)
+    return whole[rows:-rows]
+
+
+LONG_K = [4096, 4112, 4224, 6160, 8192, 12288, 16384, 17408, 17424, 32016]
+
+
+@pytest.mark.parametrize("M", [1, 3, 8])
+@pytest.mark.parametrize("K", LONG_K)
+def test_gemm_of_few_long_rows(f8, M, K):
+    """As test_gemm_of_integers_is_exact, with NaNs around all inputs."""
+    import torch
+    N = 72
+    assert K * 16 * 4 < 2 ** 21
+    w, w64 = weights(f8, M + K, N, K, True)
+    x, xs, x64 = inputs(K + 1, M, K, True)
+    w, x, xs = f8.F8Blocks(inside_nans(w.codes), inside_nans(w.scales)), inside_nans(x), inside_nans(xs)
+    for dt in (torch.float32, torch.float16):
+        whole, y = guarded((M, N), dt)
+        f8.gemm(y, x, xs, w, M, N, K, dt == torch.float32)
+        with np.errstate(over="ignore"):
+            want = (x64 @ w64.T).astype(np.float32 if dt == torch.float32 else np.float16)
+        assert np.array_equal(y.cpu().numpy(), want)
+        check_guard(whole)
+
+
+@pytest.mark.parametrize("M", [1, 3, 8])
+@pytest.mark.parametrize("K", LONG_K)
+def test_gate_up_of_few_long_rows(f8, M, K):
+    import torch
+    N = 144
+    (gw, gw64), (uw, uw64), (x, xs, x64) = weights(f8, 1, N, K, False), weights(f8, 2, N, K, False), inputs(3, M, K, False)
+    gw, uw = f8.F8Blocks(inside_nans(gw.codes), inside_nans(gw.scales)), f8.F8Blocks(inside_nans(uw.codes), inside_nans(uw.scales))
+    gq, q = guarded((M, N), torch.float8_e4m3fn)
+    gs, s = guarded((M, nblocks(N)), torch.float32)
+    f8.gate_up(q, s, inside_nans(x), inside_nans(xs), gw, uw, M, N, K)
+    check_blocks(q, s, *gated(x64, gw64, uw64, 10.0))
+    check_guard(gq)
+    check_guard(gs)
+
+
+@pytest.mark.parametrize("fp32", [True, False])
+@pytest.mark.parametrize("M", [1, 8, 9, 40, 300])
+@pytest.mark.parametrize("K", [384, 400, 4224, 12416])
+def test_gemm_of_infinite_scales(f8, M, K, fp32):
+    """Positive values and an infinite scale of the last block on either side: what it reaches is not finite (infinity, or NaN where a
+    part of the block without values is scaled: K = 400, 0 * infinity), the other rows are as they would be."""
+    import torch
+    N = 40
+    x, w = torch.ones((M, K), device="cuda").to(torch.float8_e4m3fn), torch.ones((N, K), device="cuda").to(torch.float8_e4m3fn)
+    xs, ws = torch.ones((M, nblocks(K)), device="cuda"), torch.ones((1, nblocks(K)), device="cuda")
+    ys = torch.empty((2, M, N), dtype=torch.float32 if fp32 else torch.float16, device="cuda")
+    xs[M // 2, -1] = float("inf")
+    f8.gemm(ys[0], x, xs, f8.F8Blocks(w, ws), M, N, K, fp32)
+    ws[0, -1] = float("inf")
+    f8.gemm(ys[1], x, xs, f8.F8Blocks(w, ws), M, N, K, fp32)
+    assert not bool(ys[0, M // 2].isfinite().any()) and not bool(ys[1].isfinite().any())
+    ys[0, M // 2] = K
+    assert bool((ys[0] == K).all())
+
+
 @pytest.mark.parametrize("M", [1, 7, 16, 45, 300])
 def test_gate_up_repeats(f8, M):
     import torch
