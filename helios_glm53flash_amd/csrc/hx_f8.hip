@@ -572,7 +572,8 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
 #pragma unroll
         for (int i = 0; i < TN; ++i)
 #pragma unroll
-            for (int j = 0; j < TM; ++j) coherent_store4(rp, (split * PIECES + ((i * TM + j) * WAVES + wave) * 64 + lane) * 16, acc[i][j]);
+            for (int j = 0; j < TM; ++j)
+                if (m0 + (wm * TM + j) * 16 < a.M) coherent_store4(rp, (split * PIECES + ((i * TM + j) * WAVES + wave) * 64 + lane) * 16, acc[i][j]);
         if (!arrive_last(a.counters + tile, sp.splits)) return;
         // several splits' loads in flight: one at a time, each is a round trip of over a us
         constexpr int BATCH = Z::SPLITS ? 16 / (TN * TM) : 1;
@@ -581,14 +582,15 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
 #pragma unroll
             for (int j = 0; j < TM; ++j) acc[i][j] = hx_f4{0.f, 0.f, 0.f, 0.f};
         for (int p0 = 0; p0 < sp.splits; p0 += BATCH) {
-            hx_f4 t[BATCH][TN][TM];
+            hx_f4 t[BATCH][TN][TM] = {};
 #pragma unroll
             for (int p = 0; p < BATCH; ++p)
 #pragma unroll
                 for (int i = 0; i < TN; ++i)
 #pragma unroll
                     for (int j = 0; j < TM; ++j)
-                        t[p][i][j] = coherent_load4(rp, (min(p0 + p, sp.splits - 1) * PIECES + ((i * TM + j) * WAVES + wave) * 64 + lane) * 16);
+                        if (m0 + (wm * TM + j) * 16 < a.M)
+                            t[p][i][j] = coherent_load4(rp, (min(p0 + p, sp.splits - 1) * PIECES + ((i * TM + j) * WAVES + wave) * 64 + lane) * 16);
 #pragma unroll
             for (int p = 0; p < BATCH; ++p)
                 if (p0 + p < sp.splits)
