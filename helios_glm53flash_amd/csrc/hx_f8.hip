@@ -12,9 +12,10 @@
 //          2^-16 of its size (measured 1.6e-5 rms), so it serves fp16 outputs only, whose rounding is 2^-11.  (The gated pair's scales
 //          are fp32.)
 //
-//   M <= 8  f8_rows_kernel: the waves of a workgroup split K and keep x in registers or LDS; they walk over the weight rows,
-//           every code read once from memory into operands, and add their sums through LDS.  exact
+//   M <= 8  f8_rows_kernel: the waves of a workgroup split K and keep x in registers or LDS; they walk over the weight rows, every code read
+//           once from memory into operands, and add their sums through LDS.  exact
 //   M > 8   f8_tile_kernel: tiles, both sides through a ring of LDS stages.  fast for fp16 outputs, else exact
+// (Few rows that fit neither registers nor LDS take exact tiles.)
 #include <algorithm>
 
 #include "hx_f8.hpp"
@@ -128,7 +129,8 @@ HX_INLINE void f8_finish_block(const F8Call& c, const float* v, int rows, int m0
             a = max(a, (uint32_t)__shfl_xor((int)a, 16, 64));
             const F8Scale s = f8_scale(a);
             if (i < rows && n < c.N)
-                *reinterpret_cast<uint32_t*>(c.q + (size_t)(m0 + i) * c.N + n) = f8_codes(t[j][0] * s.factor, t[j][1] * s.factor, t[j][2] * s.factor, t[j][3] * s.factor);
+                *reinterpret_cast<uint32_t*>(c.q + (size_t)(m0 + i) * c.N + n) =
+                    f8_codes(t[j][0] * s.factor, t[j][1] * s.factor, t[j][2] * s.factor, t[j][3] * s.factor);
             if (i < rows && (thread & 31) == 0) c.scales[(size_t)(m0 + i) * nb + block] = s.scale;
         }
     }
@@ -400,7 +402,7 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
     const int m0 = (xcd ? (tile >> 3) % mt : tile % mt) * BM, n0 = (xcd ? (tile >> 3) / mt * 8 + (tile & 7) : tile / mt) * CN;
     const int nrows = min(a.N - n0, CN), mrows = min(a.M - m0, BM);
 
-    // A wave's load i takes 8 rows of 128 bytes, rows 8 (i WAVES + wave) and behind of the weights (of a pair: gate, then up) or of x.  The
+    // A wave's load i takes 8 rows of 128 bytes, rows 8 (i LW + wave) and behind of the weights (of a pair: gate, then up) or of x.  The
     // descriptors move on with the steps and end with the matrix; behind the last step they are empty.
     typedef __attribute__((address_space(3))) void* lds_t;
     static_assert(!PAIR || NW % 2 == 0);
@@ -414,7 +416,7 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
     };
     // A step's loads of a wave, LOADS of them: one of scales, then x, then the weights.  Loads that touch no memory write zeros.
     const float* xs = a.xs + (size_t)m0 * a.kb + first;
-    // Into stage `slot`, block c; of the scales part s of group g into group buffer `buf`: 16 rows a wave from 16 (s WAVES + wave) on, steps first + 4 g
+    // Into stage `slot`, block c; of the scales part s of group g into group buffer `buf`: 16 rows a wave from 16 (s LW + wave) on, steps first + 4 g
     // and the three behind.
     auto loads = [&](int slot, int c, int buf, int g, int s) {
         const int row = 16 * (s * LW + wave);
@@ -436,7 +438,8 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
             __builtin_amdgcn_raw_ptr_buffer_load_lds(mf_rsrc(l.x.from, l.x.bytes), (lds_t)(l.into_x + r * F8_BLOCK), 16, lane_off + r * a.K, 0, 0, 0);
         } else {
             const int r = 8 * LW * (i - 1 - NX), up = PAIR && r >= CN ? 1 : 0;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(mf_rsrc(l.w[up].from, l.w[up].bytes), (lds_t)(l.into_w + r * F8_BLOCK), 16, lane_off + (r - up * CN) * a.K, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(mf_rsrc(l.w[up].from, l.w[up].bytes), (lds_t)(l.into_w + r * F8_BLOCK), 16,
+                                                     lane_off + (r - up * CN) * a.K, 0, 0, 0);
         }
     };
     hx_f4 acc[TN][TM];
@@ -498,7 +501,8 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
                     const hx_h8 k0 = f8_half8(w.p[h][0], w.p[h][1]), k1 = f8_half8(w.p[h][2], w.p[h][3]);
                     if (h == 1 && i + 1 < TN) w = weights(i + 1);
 #pragma unroll
-                    for (int j = 0; j < TM; ++j) t[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, b[j].k[2 * h], h ? t[j] : hx_f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    for (int j = 0; j < TM; ++j)
+                        t[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, b[j].k[2 * h], h ? t[j] : hx_f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
                     for (int j = 0; j < TM; ++j) t[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, b[j].k[2 * h + 1], t[j], 0, 0, 0);
                 }
@@ -656,7 +660,8 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
 #pragma unroll
                 for (int j = 0; j < TM; ++j)
                     coherent_store4(rd, (((wm * TM + j) * 16 + col) * F8_BLOCK + n0 % F8_BLOCK + (wn * TP + i) * 16 + 4 * kg) * 4, v[i][j]);
-            if (arrive_last(a.counters + mt * nt + at, min(per, nt - block * per))) f8_finish_block<64 * WAVES, BM / (2 * WAVES) < 8 ? BM / (2 * WAVES) : 8>(a, dst, BM, m0, block);
+            constexpr int BATCH = BM / (2 * WAVES) < 8 ? BM / (2 * WAVES) : 8;
+            if (arrive_last(a.counters + mt * nt + at, min(per, nt - block * per))) f8_finish_block<64 * WAVES, BATCH>(a, dst, BM, m0, block);
         }
     }
 }
@@ -670,7 +675,7 @@ struct F8Plan {
     long tiles;
     size_t partial, products;  // bytes of workspace
 };
-enum F8Sums { F8_FAST, F8_EXACT, F8_GATED };  // fp16 outputs; fp32 outputs; gated pair (exact)
+enum F8Sums { F8_FAST, F8_EXACT, F8_GATED };  // fp16 outputs; fp32 outputs, and few rows; gated pair (exact)
 constexpr int F8_CUS = 256, F8_COUNTERS = (int)(HX_COUNTER_BYTES / sizeof(int));
 constexpr size_t F8_MOST_PRODUCTS = 48u << 20;
 constexpr size_t F8_FAR_BYTES = (160 - 16) * 1024;  // next to the rows kernel's sums
@@ -678,8 +683,10 @@ constexpr int F8_NEAR = 2 * F8_ROWS_THREADS / 64;  // blocks of K whose spans ar
 constexpr long F8_MOST_TILES = 1l << 22;  // of at most 512 threads
 
 // A tile, how many of its workgroups a CU holds, and what it costs, in us: to begin and end; a step of a workgroup at least; a step of each
-// workgroup on a CU; where K is split, for the join and for each split of it.  Fitted to some 200 calls of either sort (20 to 1000 rows, K and N 2048 to 12288),
-// the model is within 8 % rms, and its choice takes 1 % longer than the best of the tiles and splits on average, 10 % at most.
+// workgroup on a CU; where K is split, for the join and for each split of it.  Fitted to some 200 calls of either sort (20 to 1000 rows, K and
+// N 2048 to 12288), the model is within 8 % rms, and its choice takes 1 % longer than the best of the tiles and splits on average, 10 % at most.
+// (45 rows of 8192 -> 4096: 64 x 64 in 4 parts 14.1 us, in 2 parts 20.3, 128 x 64 in 8 parts 15.6; 1000 rows of 4096 -> 4096: 128 x 128 27.9, 64 x 64 40.5,
+// 256 x 256 63.2.)
 struct F8Tile {
     int bn, bm, resident;
     float start, step, each, join, split;
@@ -699,7 +706,8 @@ F8Plan f8_plan(int M, int N, int K, F8Sums sums, bool split)
     const size_t few = (size_t)nb * F8_ROWS * F8_BLOCK * sizeof(float);
     p.splits = 1;
     p.steps = kb;
-    if (M <= F8_ROWS && !(pair && (nb > F8_COUNTERS || few > F8_MOST_PRODUCTS)) && (kb <= F8_NEAR || f8_far_bytes(M, K) <= F8_FAR_BYTES)) {
+    const bool fits = !(pair && (nb > F8_COUNTERS || few > F8_MOST_PRODUCTS)) && (kb <= F8_NEAR || f8_far_bytes(M, K) <= F8_FAR_BYTES);
+    if (M <= F8_ROWS && fits) {
         p.kind = F8Plan::ROWS;
         if (pair) p.products = few;
         return p;
@@ -718,7 +726,8 @@ F8Plan f8_plan(int M, int N, int K, F8Sums sums, bool split)
             const int steps = (kb + s - 1) / s;
             if (s > 1 && (!split || t.join == 0.f || kb < 2 * s || tiles * s > (long)F8_CUS * t.resident)) break;  // all are at work at once
             const float each = (float)((tiles * s + F8_CUS - 1) / F8_CUS);
-            const float us = t.start + (pair ? whole ? 2.0f : 3.4f : 0.0f) + steps * std::max(t.step, each * t.each) + (s > 1 ? t.join + t.split * each * s : 0.0f);
+            const float join = s > 1 ? t.join + t.split * each * s : 0.0f, scaling = !pair ? 0.0f : whole ? 2.0f : 3.4f;
+            const float us = t.start + steps * std::max(t.step, each * t.each) + join + scaling;
             if (p.kind != F8Plan::NONE && us >= least) continue;
             least = us;
             p.kind = (F8Plan::Kind)kind;
@@ -807,13 +816,13 @@ hipError_t launch_f8_gemm(const uint8_t* x, const float* xs, const F8Blocks& w, 
     const int kb = (K + F8_BLOCK - 1) / F8_BLOCK, most = f8_most_rows(N, false);
     for (long m = 0; m < M; m += most) {
         const int rows = (int)(M - m < most ? M - m : most);
-        const F8Sums sums = y_fp32 ? F8_EXACT : F8_FAST;
+        const F8Sums sums = y_fp32 || rows <= F8_ROWS ? F8_EXACT : F8_FAST;
         F8Plan p = f8_plan(rows, N, K, sums, true);
         if (p.partial && (!ws || ws_bytes < f8_workspace(p))) p = f8_plan(rows, N, K, sums, false);
         F8Call c{x + m * K, xs + m * kb, {w, {}}, rows, N, K, kb};
         c.y = static_cast<char*>(y) + m * N * (y_fp32 ? 4 : 2);
         c.y_fp32 = y_fp32;
-        const hipError_t e = y_fp32 ? f8_launch<F8_EXACT>(c, p, ws, st) : f8_launch<F8_FAST>(c, p, ws, st);
+        const hipError_t e = sums == F8_EXACT ? f8_launch<F8_EXACT>(c, p, ws, st) : f8_launch<F8_FAST>(c, p, ws, st);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;

@@ -266,8 +266,9 @@ int hx_w4_embed(const hx_w4_words* w, const int64_t* tokens, void* out, int n, i
 /* Values in e4m3 (4 exponent bits, 3 mantissa bits, largest 448) with an fp32 scale for each block of 128 consecutive k of an input
  * row, or of 128 x 128 weights; the last blocks may be short (no counterpart in the reference):
  *   a = max(largest |v| of the block, 2^-100)   scale = a / 448   code = e4m3(v * (448 / a)), fp32 operations, ties to even
- * A block with a NaN or an infinity stands for NaN throughout, and what reads a scale that is not finite is not finite.  K % 16 == 0, K <= 2^22 in all calls of this section; M == 0 is a
- * no-op (the pointers may then be NULL); outputs overlap neither inputs nor each other but where that is said. */
+ * A block with a NaN or an infinity stands for NaN throughout, and what reads a scale that is not finite is not finite.  K % 16 == 0
+ * and K <= 2^22 in all calls of this section; M == 0 is a no-op (the pointers may then be NULL); outputs overlap neither inputs nor each
+ * other but where that is said. */
 
 /* q uint8 [M][K] and scales fp32 [M][ceil(K / 128)] of x (fp16 or fp32 by dtype, HX_DTYPE_*; rows ld elements apart, ld % 8 == 0).
  * x and q 16-byte aligned. */
