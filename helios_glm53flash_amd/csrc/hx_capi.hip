@@ -662,7 +662,10 @@ int hx_f8_gemm(void* y, const void* x, const float* x_scales, const hx_f8_blocks
     if ((uintptr_t)workspace & 15) return fail(HX_ERR_WORKSPACE, "hx_f8_gemm: workspace must be 16-byte aligned");
     const int kb = (K + 127) / 128;
     const F8Span to = f8_span(y, M, N, N, y_fp32 ? 4 : 2);
-    if (!f8_apart(to, f8_span(x, M, K, K, 1)) || !f8_apart(to, f8_span(x_scales, M, kb, kb, 4))) return f8_fail(who, "y overlaps x or x_scales");
+    const F8Span in[] = {f8_span(x, M, K, K, 1), f8_span(x_scales, M, kb, kb, 4), f8_span(w->codes, N, K, K, 1),
+                         f8_span(w->scales, (N + 127) / 128, kb, kb, 4)};
+    for (const F8Span& i : in)
+        if (!f8_apart(to, i)) return f8_fail(who, "y overlaps an input");
     return hip_status(hx::launch_f8_gemm(static_cast<const uint8_t*>(x), x_scales, {static_cast<const uint8_t*>(w->codes), w->scales}, y, M, N, K,
                                          y_fp32 != 0, workspace, workspace_bytes, (hipStream_t)stream),
                       who);
@@ -688,7 +691,9 @@ int hx_f8_gate_up(void* q, float* scales, const void* x, const float* x_scales, 
     if (((uintptr_t)x | (uintptr_t)q) & 15) return f8_fail(who, "x and q must be 16-byte aligned");
     if (((uintptr_t)x_scales | (uintptr_t)scales) & 3) return f8_fail(who, "scales must be 4-byte aligned");
     const int kb = (K + 127) / 128, nb = (N + 127) / 128;
-    const F8Span in[] = {f8_span(x, M, K, K, 1), f8_span(x_scales, M, kb, kb, 4)}, to[] = {f8_span(q, M, N, N, 1), f8_span(scales, M, nb, nb, 4)};
+    const F8Span in[] = {f8_span(x, M, K, K, 1), f8_span(x_scales, M, kb, kb, 4), f8_span(gate->codes, N, K, K, 1), f8_span(gate->scales, nb, kb, kb, 4),
+                         f8_span(up->codes, N, K, K, 1), f8_span(up->scales, nb, kb, kb, 4)};
+    const F8Span to[] = {f8_span(q, M, N, N, 1), f8_span(scales, M, nb, nb, 4)};
     for (const F8Span& o : to)
         for (const F8Span& i : in)
             if (!f8_apart(o, i)) return f8_fail(who, "an output overlaps an input");

@@ -175,6 +175,8 @@ __global__ __launch_bounds__(OPT == 0 ? 1024 : 512) void f8_norm_kernel(F8NormAr
 
 namespace {
 
+constexpr size_t F8_NORM_ROWS = 1u << 21;  // of a launch: 2^31 threads
+
 template <typename T, typename R>
 void norm_launch(const F8NormArgs& a, int M, hipStream_t st)
 {
@@ -198,9 +200,20 @@ void norm_launch(const F8NormArgs& a, int M, bool r32, hipStream_t st)
 
 hipError_t launch_f8_norm(const F8NormArgs& a, int M, bool x32, bool r32, hipStream_t st)
 {
-    if (M <= 0) return hipSuccess;
-    if (x32) norm_launch<float>(a, M, r32, st);
-    else norm_launch<_Float16>(a, M, r32, st);
+    const size_t kb = (size_t)(a.K + F8_BLOCK - 1) / F8_BLOCK;
+    auto behind = [](const void* p, size_t bytes) { return p ? static_cast<const char*>(p) + bytes : nullptr; };
+    for (size_t m = 0; m < (size_t)M; m += F8_NORM_ROWS) {
+        F8NormArgs c = a;
+        c.x = behind(a.x, m * a.ld * (x32 ? 4 : 2));
+        c.residual = behind(a.residual, m * a.K * (r32 ? 4 : 2));
+        c.out = const_cast<char*>(behind(a.out, m * a.K * (r32 ? 4 : 2)));
+        c.y = const_cast<char*>(behind(a.y, m * a.K * 2));
+        c.q = const_cast<char*>(behind(a.q, m * a.K));
+        if (a.scales) c.scales = a.scales + m * kb;
+        const int rows = (int)((size_t)M - m < F8_NORM_ROWS ? (size_t)M - m : F8_NORM_ROWS);
+        if (x32) norm_launch<float>(c, rows, r32, st);
+        else norm_launch<_Float16>(c, rows, r32, st);
+    }
     return hipGetLastError();
 }
 

@@ -82,7 +82,8 @@ WEIGHTS = [(dict(w=dict(null=True)), "null"), (dict(w=dict(codes=None)), "null")
 @pytest.mark.parametrize("bad,text", EXTENTS + WEIGHTS + [
     (dict(y=None), "null"), (dict(x=None), "null"), (dict(xs=None), "null"), (dict(x=2 * FAR + 8), "16-byte"), (dict(xs=2), "aligned"),
     (dict(y=FAR + 2), "aligned"), (dict(y=FAR + 1, fp32=0), "aligned"), (dict(y=2 * FAR), "overlap"), (dict(y=2 * FAR - 1596), "overlap"),
-    (dict(y=2 * FAR + 1020), "overlap"), (dict(y=3 * FAR + 28), "overlap")])
+    (dict(y=2 * FAR + 1020), "overlap"), (dict(y=3 * FAR + 28), "overlap"),
+    (dict(y=4 * FAR + 25584), "overlap"), (dict(y=5 * FAR + 4), "overlap")])
 def test_gemm_refusals(bad, text):
     refused(gemm(**bad), text)
 
@@ -103,7 +104,8 @@ def gate_up(w=None, w2=None, **kw):
     (dict(limit=float("nan")), "limit"), (dict(limit=-1.0), "limit"), (dict(q=None), "null"), (dict(scales=None), "null"),
     (dict(x=None), "null"), (dict(xs=None), "null"), (dict(q=FAR + 8), "16-byte"), (dict(scales=6 * FAR + 1), "4-byte"),
     (dict(q=2 * FAR - 16), "an output overlaps an input"), (dict(scales=3 * FAR + 28), "an output overlaps an input"),
-    (dict(scales=FAR + 1020), "outputs overlap")])
+    (dict(scales=FAR + 1020), "outputs overlap"), (dict(q=4 * FAR + 65520), "an output overlaps an input"),
+    (dict(scales=5 * FAR + 12), "an output overlaps an input"), (dict(w2=dict(codes=FAR - 65520)), "an output overlaps an input")])
 def test_gate_up_refusals(bad, text):
     refused(gate_up(**bad), text)
 

@@ -155,6 +155,19 @@ def test_quantize_of_the_smallest_and_largest(f8, value):
     assert same(s.cpu().numpy(), ws) and same(host(q), want)
 
 
+def test_quantize_of_more_rows_than_a_launch_takes(f8):
+    import torch
+    M, K = (1 << 27) + 7, 16
+    x = torch.randn((1 << 20, K), device="cuda").half().repeat((M >> 20) + 1, 1)[:M].contiguous()
+    q, s = torch.empty((M, K), dtype=torch.float8_e4m3fn, device="cuda"), torch.empty((M, 1), device="cuda")
+    f8.quantize(x, q, s, M, K)
+    one = torch.empty((1 << 20, K), dtype=torch.float8_e4m3fn, device="cuda"), torch.empty((1 << 20, 1), device="cuda")
+    f8.quantize(x, *one, 1 << 20, K)
+    for at in (0, 64 << 20, 127 << 20, 1 << 27):
+        n = min(1 << 20, M - at)
+        assert torch.equal(q[at:at + n].view(torch.uint8), one[0][:n].view(torch.uint8)) and torch.equal(s[at:at + n], one[1][:n])
+
+
 def test_quantize_rounds_ties_to_even(f8):
     """Every halfway value between two codes, and its neighbours in fp32, in a block whose largest value is 448 (factor 1)."""
     import torch
@@ -250,6 +263,22 @@ def test_norm_rows_of_zeros_infinities_and_nans(f8, K):
     assert np.isnan(got[3, K - 1]) and (got[3, :K - 1] == 0).all()
     ok = [0, 1, 4]
     check_norm(x[ok].astype(np.float64), w, 1e-5, y[ok], q[ok], s[ok])
+
+
+def test_norm_of_more_rows_than_a_launch_takes(f8):
+    import torch
+    M, K = (1 << 21) + 5, 16
+    x = torch.randn((M, K), device="cuda").half()
+    h, out, w = torch.randn((M, K), device="cuda"), torch.empty((M, K), device="cuda"), torch.rand((K,), device="cuda")
+    whole = [torch.empty((M, K), dtype=torch.float16, device="cuda"), torch.empty((M, K), dtype=torch.float8_e4m3fn, device="cuda"),
+             torch.empty((M, 1), device="cuda")]
+    f8.rms_norm(x, w, M, K, 1e-5, residual=h, out=out, y=whole[0], q=whole[1], scales=whole[2])
+    assert torch.equal(out, x.float() + h)
+    for a, b in ((0, 1 << 20), (1 << 20, 1 << 21), ((1 << 21) - 3, M)):
+        part = [torch.empty_like(t[a:b]) for t in whole]
+        f8.rms_norm(x[a:b], w, b - a, K, 1e-5, residual=h[a:b], out=torch.empty_like(out[a:b]), y=part[0], q=part[1], scales=part[2])
+        for t, p in zip(whole, part):
+            assert torch.equal(t[a:b].view(torch.uint8), p.view(torch.uint8))
 
 
 # ------------------------------------------------------------------ linear
@@ -441,6 +470,30 @@ def test_gemm_large_offsets(f8):
         for at in (0, N // 2000 * 1000, N - 1000):
             assert np.array_equal(y[:, at:at + 1000].cpu().numpy(), part[:m])
         del y
+
+
+def test_gemm_of_more_rows_than_a_launch_takes(f8):
+    """2^30 rows and some: codes past 2^34 bytes, outputs past 2^34 elements."""
+    import torch
+    M, K, N = (1 << 30) + 300, 16, 16
+    free, _ = torch.cuda.mem_get_info()
+    if free < 70 << 30:
+        pytest.skip("not enough memory")
+    w, w64 = weights(f8, 1, N, K, True)
+    some = inputs(2, 1000, K, True)[0]
+    x = torch.zeros((M, K), dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    xs = torch.ones((M, 1), device="cuda")
+    places = [0, (1 << 27) - 500, (1 << 28) - 500, M - 1000]
+    for at in places:
+        x.view(torch.uint8)[at:at + 1000] = some.view(torch.uint8)
+    y = torch.full((M, N), float("nan"), dtype=torch.float16, device="cuda")
+    f8.gemm(y, x, xs, w, M, N, K)
+    want = (host(some) @ w64.T).astype(np.float16)
+    for at in places:
+        assert np.array_equal(y[at:at + 1000].cpu().numpy(), want)
+        y[at:at + 1000] = 0
+    for at in range(0, M, 1 << 27):
+        assert not bool(y[at:at + (1 << 27)].any())
 
 
 # ------------------------------------------------------------------ gated pair
