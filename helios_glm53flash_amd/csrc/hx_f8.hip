@@ -161,11 +161,12 @@ template <bool PAIR, bool FAR>
 __global__ __launch_bounds__(F8_ROWS_THREADS) void f8_rows_kernel(F8Call a, int wk_log2)
 {
     constexpr int WAVES = F8_ROWS_THREADS / 64, R = F8_ROWS, P = PAIR ? 2 : 1;
-    __shared__ __align__(16) float red[2][P * R * R * WAVES];  // of this tile and the next: [row part][p][token][r][wave in K]
+    __shared__ __align__(16) float red[2][P * R * R * (WAVES + 4)];  // of this tile and the next: [row part][p][token][r][wave in K]
     extern __shared__ __align__(16) uint8_t f8_lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wk = 1 << wk_log2, kw = wave & (wk - 1), rw = wave >> wk_log2, wr = WAVES >> wk_log2;  // the wave's place in K and in rows
     const int col = lane & 15, kg = lane >> 4, s = col / R, r = col % R;
+    const int sums = wk == WAVES ? WAVES + 4 : wk;  // apart in red, where all waves share K: without the 4, banks cost some 500 cycles a tile
     const int rounds = FAR ? ((a.kb + 1) / 2 + wk - 1) >> wk_log2 : 1;        // over K
     const int rows_wg = wr * R, tiles = (a.N + rows_wg - 1) / rows_wg;        // rows_wg: a power of two up to 128
     const int far_row = f8_far_row(a.K), far_r = min(r, a.M - 1);             // rows behind M: any
@@ -282,7 +283,7 @@ __global__ __launch_bounds__(F8_ROWS_THREADS) void f8_rows_kernel(F8Call a, int 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float v = f8_parts_sum(acc[p][e]);
-                if (kg < 2 && s == 0) red[turn][((((rw * P + p) * R + kg * 4 + e) * R + r) << wk_log2) + kw] = v;
+                if (kg < 2 && s == 0) red[turn][(((rw * P + p) * R + kg * 4 + e) * R + r) * sums + kw] = v;
             }
         hx_lds_barrier();  // also: the sums of the tile before are read
         for (int i = threadIdx.x; i < R * R * wr; i += F8_ROWS_THREADS) {
@@ -290,7 +291,7 @@ __global__ __launch_bounds__(F8_ROWS_THREADS) void f8_rows_kernel(F8Call a, int 
             float v[P];
 #pragma unroll
             for (int p = 0; p < P; ++p) {
-                const float* from = red[turn] + ((((part * P + p) * R + t) * R + rr) << wk_log2);
+                const float* from = red[turn] + (((part * P + p) * R + t) * R + rr) * sums;
                 float sum = 0.0f;
                 if (wk == WAVES) {
                     const hx_f4* four = reinterpret_cast<const hx_f4*>(from);
@@ -678,24 +679,24 @@ struct F8Plan {
 enum F8Sums { F8_FAST, F8_EXACT, F8_GATED };  // fp16 outputs; fp32 outputs, and few rows; gated pair (exact)
 constexpr int F8_CUS = 256, F8_COUNTERS = (int)(HX_COUNTER_BYTES / sizeof(int));
 constexpr size_t F8_MOST_PRODUCTS = 48u << 20;
-constexpr size_t F8_FAR_BYTES = (160 - 16) * 1024;  // next to the rows kernel's sums
+constexpr size_t F8_FAR_BYTES = (160 - 20) * 1024;  // next to the rows kernel's sums
 constexpr int F8_NEAR = 2 * F8_ROWS_THREADS / 64;  // blocks of K whose spans are one round of the rows kernel's waves
 constexpr long F8_MOST_TILES = 1l << 22;  // of at most 512 threads
 
 // A tile, how many of its workgroups a CU holds, and what it costs, in us: to begin and end; a step of a workgroup at least; a step of each
-// workgroup on a CU; where K is split, for the join and for each split of it.  Fitted to some 200 calls of either sort (20 to 1000 rows, K and
-// N 2048 to 12288), the model is within 8 % rms, and its choice takes 1 % longer than the best of the tiles and splits on average, 10 % at most.
-// (45 rows of 8192 -> 4096: 64 x 64 in 4 parts 14.1 us, in 2 parts 20.3, 128 x 64 in 8 parts 15.6; 1000 rows of 4096 -> 4096: 128 x 128 27.9, 64 x 64 40.5,
-// 256 x 256 63.2.)
+// workgroup on a CU; where K is split, for the join and for each part of it, beside .31 us for each MB of sums.  Fitted to some 400 calls of fp16
+// outputs and 240 of fp32 outputs (12 to 1500 rows, K and N 2048 to 12288), the model is within 5 % rms, and its choice takes 1 % longer than
+// the best of the tiles and splits on average, 11 % at most.  (45 rows of 8192 -> 4096: 64 x 64 in 4 parts 13.9 us, in 2 parts 20.3, 128 x 64 in 8
+// parts 15.6; 1000 rows of 4096 -> 4096: 128 x 128 26.9, 64 x 64 40.5, 256 x 256 63.2.)
 struct F8Tile {
     int bn, bm, resident;
-    float start, step, each, join, split;
+    float start, step, each, join, part;
 };
 constexpr F8Tile F8_TILES[2][6] = {
-    {{}, {64, 32, 2, 2.8f, 0.40f, 0.33f, 2.7f, 0.13f}, {64, 64, 3, 3.2f, 0.44f, 0.30f, 2.5f, 0.31f}, {128, 64, 2, 3.5f, 0.58f, 0.44f, 2.1f, 0.69f},
-     {128, 128, 1, 4.2f, 0.68f, 0.71f, 2.0f, 1.15f}, {256, 256, 1, 9.4f, 1.66f, 1.66f, 0.f, 0.f}},
-    {{}, {64, 32, 2, 2.6f, 0.51f, 0.39f, 2.8f, 0.15f}, {64, 64, 3, 3.4f, 0.56f, 0.385f, 2.3f, 0.31f}, {128, 64, 2, 4.0f, 0.80f, 0.59f, 1.8f, 0.65f},
-     {}, {256, 256, 1, 9.6f, 3.0f, 3.0f, 0.f, 0.f}}};  // exact, 128 x 128 is at most 3 % before 128 x 64
+    {{}, {64, 32, 4, 2.2f, 0.44f, 0.286f, 2.0f, 0.29f}, {64, 64, 3, 3.0f, 0.458f, 0.30f, 0.9f, 0.43f}, {128, 64, 2, 3.75f, 0.57f, 0.437f, 0.5f, 0.64f},
+     {128, 128, 1, 4.2f, 0.70f, 0.705f, 0.f, 0.6f}, {256, 256, 1, 11.0f, 1.57f, 1.57f, 0.f, 0.f}},
+    {{}, {64, 32, 4, 3.4f, 0.46f, 0.308f, 1.7f, 0.19f}, {64, 64, 3, 3.45f, 0.56f, 0.376f, 1.0f, 0.36f}, {128, 64, 2, 4.4f, 0.79f, 0.593f, 0.2f, 0.59f},
+     {}, {256, 256, 1, 10.5f, 2.99f, 2.99f, 0.f, 0.f}}};  // exact, 128 x 128 is at most 3 % before 128 x 64
 
 F8Plan f8_plan(int M, int N, int K, F8Sums sums, bool split)
 {
@@ -724,9 +725,10 @@ F8Plan f8_plan(int M, int N, int K, F8Sums sums, bool split)
         if (!whole && (tiles + mt * nb > F8_COUNTERS || products > F8_MOST_PRODUCTS)) continue;
         for (int s = 1; s <= 8; s *= 2) {
             const int steps = (kb + s - 1) / s;
-            if (s > 1 && (!split || t.join == 0.f || kb < 2 * s || tiles * s > (long)F8_CUS * t.resident)) break;  // all are at work at once
-            const float each = (float)((tiles * s + F8_CUS - 1) / F8_CUS);
-            const float join = s > 1 ? t.join + t.split * each * s : 0.0f, scaling = !pair ? 0.0f : whole ? 2.0f : 3.4f;
+            if (s > 1 && (!split || t.part == 0.f || steps < 4 || tiles * s > (long)F8_CUS * t.resident)) break;  // all are at work at once
+            const float each = (float)((tiles * s + F8_CUS - 1) / F8_CUS), scaling = !pair ? 0.0f : whole ? 2.4f : 3.3f;
+            const float sums_mb = (float)(tiles * s * t.bn * std::min(t.bm, (M + 15) / 16 * 16)) * 4e-6f;
+            const float join = s > 1 ? t.join + t.part * s + 0.31f * sums_mb : 0.0f;
             const float us = t.start + steps * std::max(t.step, each * t.each) + join + scaling;
             if (p.kind != F8Plan::NONE && us >= least) continue;
             least = us;
@@ -773,7 +775,7 @@ hipError_t f8_launch(F8Call c, const F8Plan& p, void* ws, hipStream_t st)
     constexpr bool FAST = SUMS == F8_FAST, PAIR = SUMS == F8_GATED;
     switch (p.kind) {
         case F8Plan::ROWS: return rows_launch<PAIR>(c, st);
-        case F8Plan::TILE64x32: return tile_launch<2, 2, 2, 1, 6, !FAST, PAIR>(c, p, st);
+        case F8Plan::TILE64x32: return tile_launch<2, 2, 2, 1, 3, !FAST, PAIR>(c, p, st);
         case F8Plan::TILE64x64: return tile_launch<2, 2, 2, 2, 3, !FAST, PAIR>(c, p, st);
         case F8Plan::TILE128x64: return tile_launch<2, 2, 4, 2, 3, !FAST, PAIR>(c, p, st);
         case F8Plan::TILE128x128:
