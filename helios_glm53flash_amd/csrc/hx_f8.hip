@@ -73,6 +73,13 @@ HX_INLINE float f8_parts_sum(float v)
     return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, (int)__builtin_amdgcn_permlane32_swap(u, u, false, false)[1], 0x128, 0xf, 0xf, false));
 }
 
+HX_INLINE __amdgpu_buffer_rsrc_t f8_rsrc(const void* base, int bytes)
+{
+    const uint64_t u = reinterpret_cast<uint64_t>(base);
+    const uint64_t b = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(u >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)u);
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(b), 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
+}
+
 // A call.  w[1] is the up projection of a gated pair (w[0] the gate), else unused.
 struct F8Call {
     const uint8_t* x;
@@ -370,19 +377,15 @@ struct F8TileSize {
     static_assert(BN % (8 * LW) == 0 && BM % (8 * LW) == 0 && BM <= 64 * WAVES && PF <= 8);
 };
 
-// What a buffer load may read; a step's loads of a wave and where in LDS they go; a step's operands in LDS.
-struct F8Rows {
-    const void* from;
-    size_t bytes;
-};
+// A step's loads of a wave: from where, how many bytes are left there, and where in LDS they go.  A step's operands in LDS.
 struct F8Loads {
-    F8Rows w[2], x, scales;
-    uint8_t *into_w, *into_x, *into_scales;
-    int scales_off;
+    const uint8_t *w[2], *x;
+    const float* scales;
+    int w_left, x_left, scales_left;
+    int into_w, into_x, into_scales;
 };
 struct F8Stage {
-    const uint8_t *w, *x;
-    const float* scales;
+    int w, x, scales;
     int left;  // of K from this block on
 };
 
@@ -409,37 +412,36 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
     static_assert(!PAIR || NW % 2 == 0);
     const long lrow = 8 * wave;
     const uint8_t* base[3] = {a.w[0].codes + (n0 + lrow) * a.K, PAIR ? a.w[1].codes + (n0 + lrow) * a.K : nullptr, a.x + (m0 + lrow) * a.K};
-    const long bytes[2] = {(nrows - lrow) * a.K, (mrows - lrow) * a.K};
+    const int bytes[2] = {(int)(nrows - lrow) * a.K, (int)(mrows - lrow) * a.K};  // at most 2^30, or negative
     const int lane_off = (lane >> 3) * a.K + 16 * ((lane & 7) ^ (lane >> 3));
-    auto rows = [&](int p, int c) {
-        const long at = (long)c * F8_BLOCK;
-        return F8Rows{base[p] + at, (size_t)(c < steps ? max(bytes[p >> 1] - at, 0l) : 0l)};
-    };
     // A step's loads of a wave, LOADS of them: one of scales, then x, then the weights.  Loads that touch no memory write zeros.
-    const float* xs = a.xs + (size_t)m0 * a.kb + first;
+    const float* xs = a.xs + (size_t)(m0 + 16 * wave) * a.kb + first;
+    const int xs_off = ((lane >> 2) * a.kb + (lane & 3)) * 4;
     // Into stage `slot`, block c; of the scales part s of group g into group buffer `buf`: 16 rows a wave from 16 (s LW + wave) on, steps first + 4 g
     // and the three behind.
     auto loads = [&](int slot, int c, int buf, int g, int s) {
-        const int row = 16 * (s * LW + wave);
+        const int row = 16 * (s * LW + wave), at = c * F8_BLOCK, skip = 16 * s * LW * a.kb + 4 * g;
         const bool any = row < BM && first + 4 * g < steps;
-        return F8Loads{{rows(0, c), rows(PAIR ? 1 : 0, c)},
-                     rows(2, c),
-                     {xs + 4 * g, any ? ((size_t)mrows * a.kb - first - 4 * g) * 4 : 0},
-                     f8_lds + (slot * BN + 8 * wave) * F8_BLOCK,
-                     f8_lds + Z::X + (slot * BM + 8 * wave) * F8_BLOCK,
-                     f8_lds + (row < BM ? Z::SCALES + buf * Z::GROUP + row * 16 : Z::NOTHING + 256 * wave),
-                     any ? ((row + (lane >> 2)) * a.kb + (lane & 3)) * 4 : F8_NONE};
+        return F8Loads{{base[0] + at, base[1] + at},
+                       base[2] + at,
+                       xs + skip,
+                       c < steps ? max(bytes[0] - at, 0) : 0,
+                       c < steps ? max(bytes[1] - at, 0) : 0,
+                       any ? max((mrows - 16 * wave) * a.kb - first - skip, 0) * 4 : 0,
+                       (slot * BN + 8 * wave) * F8_BLOCK,
+                       Z::X + (slot * BM + 8 * wave) * F8_BLOCK,
+                       row < BM ? Z::SCALES + buf * Z::GROUP + row * 16 : Z::NOTHING + 256 * wave};
     };
     constexpr int LOADS = 1 + NX + NW;
     auto load = [&](const F8Loads& l, int i) {
         if (i == 0) {
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(mf_rsrc(l.scales.from, l.scales.bytes), (lds_t)l.into_scales, 4, l.scales_off, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(f8_rsrc(l.scales, l.scales_left), (lds_t)(f8_lds + l.into_scales), 4, xs_off, 0, 0, 0);
         } else if (i <= NX) {
             const int r = 8 * LW * (i - 1);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(mf_rsrc(l.x.from, l.x.bytes), (lds_t)(l.into_x + r * F8_BLOCK), 16, lane_off + r * a.K, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(f8_rsrc(l.x, l.x_left), (lds_t)(f8_lds + l.into_x + r * F8_BLOCK), 16, lane_off + r * a.K, 0, 0, 0);
         } else {
             const int r = 8 * LW * (i - 1 - NX), up = PAIR && r >= CN ? 1 : 0;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(mf_rsrc(l.w[up].from, l.w[up].bytes), (lds_t)(l.into_w + r * F8_BLOCK), 16,
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(f8_rsrc(l.w[up], l.w_left), (lds_t)(f8_lds + l.into_w + r * F8_BLOCK), 16,
                                                      lane_off + (r - up * CN) * a.K, 0, 0, 0);
         }
     };
@@ -449,7 +451,7 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
 #pragma unroll
         for (int j = 0; j < TM; ++j) acc[i][j] = hx_f4{0.f, 0.f, 0.f, 0.f};
     // LDS offsets of a lane's pieces of the first row block on either side
-    const int piece = 16 * (kg ^ (col & 7)), pa = (wn * TP * 16 + col) * F8_BLOCK + piece, pb = (wm * TM * 16 + col) * F8_BLOCK + piece;
+    const int piece = 16 * (kg ^ (col & 7)), pa = (wn * TP * 16 + col) * F8_BLOCK, pb = (wm * TM * 16 + col) * F8_BLOCK;
     // rows of a tile of more than 128 lie in several blocks of weights
     const int wblock = CN > F8_BLOCK ? min(n0 + wn * TP * 16, a.N - 1) / F8_BLOCK : n0 / F8_BLOCK;
     static_assert(CN <= F8_BLOCK || TP * 16 <= F8_BLOCK);
@@ -465,25 +467,29 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
             if (LW == WAVES || wave < LW) load(l, i);
-        auto fragment = [&](const uint8_t* p) {
+        auto fragment = [&](int at, int at2) {
             F8Raw v;
-            v.p[0] = *reinterpret_cast<const f8_u4*>(p);
-            v.p[1] = *reinterpret_cast<const f8_u4*>(f8_lds + ((p - f8_lds) ^ 64));
+            v.p[0] = *reinterpret_cast<const f8_u4*>(f8_lds + at);
+            v.p[1] = *reinterpret_cast<const f8_u4*>(f8_lds + at2);
             if constexpr (!decltype(whole)::value) {  // what lies behind a row's K counts as 0
                 if (16 * kg >= g.left) v.p[0] = f8_u4{};
                 if (64 + 16 * kg >= g.left) v.p[1] = f8_u4{};
             }
             return v;
         };
-        auto weights = [&](int i) { return fragment(g.w + pa + (PAIR ? i / TP * CN + i % TP * 16 : i * 16) * F8_BLOCK); };
+        const int wa = g.w + pa + piece, wa2 = g.w + pa + (piece ^ 64), xa = g.x + pb + piece, xa2 = g.x + pb + (piece ^ 64);
+        auto weights = [&](int i) {
+            const int row = (PAIR ? i / TP * CN + i % TP * 16 : i * 16) * F8_BLOCK;
+            return fragment(wa + row, Z::SPLITS ? wa2 + row : (wa + row) ^ 64);
+        };
         const float s[2] = {wnext[0], wnext[1]};
         F8Raw x[TM];
         float f[TM];
         F8Raw w = weights(0);
 #pragma unroll
-        for (int j = 0; j < TM; ++j) x[j] = fragment(g.x + pb + j * 16 * F8_BLOCK);
+        for (int j = 0; j < TM; ++j) x[j] = fragment(xa + j * 16 * F8_BLOCK, Z::SPLITS ? xa2 + j * 16 * F8_BLOCK : (xa + j * 16 * F8_BLOCK) ^ 64);
 #pragma unroll
-        for (int j = 0; j < TM; ++j) f[j] = g.scales[(wm * TM * 16 + 16 * j + col) * 4];
+        for (int j = 0; j < TM; ++j) f[j] = *reinterpret_cast<const float*>(f8_lds + g.scales + (wm * TM * 16 + 16 * j + col) * 16);
         auto sums = [&](int i, int j, const hx_f4& t) {  // of one product
             const float q = f[j] * s[PAIR && i >= TP];
 #pragma unroll
@@ -547,20 +553,30 @@ __global__ __launch_bounds__(64 * WN * WM) void f8_tile_kernel(F8Call a, F8Split
             if (LW == WAVES || wave < LW) load(l, i);
     }
     int slot = 0, group = 0;  // of codes, of scales
+    // A step's loads: into the stage of the step before.
+    auto loads_of = [&](int c) {
+        const int d = c - first;
+        return loads(slot == 0 ? PF - 1 : slot - 1, c + PF - 1, group == 0 ? 2 : group - 1, (d >> 2) + 2, d & 3);
+    };
+    // Small tiles make them out a step ahead: behind the barrier some 50 dependent scalar instructions hold them up (45 rows of 8192 -> 4096 14.1 us
+    // where 13.1 are).  The largest has no registers to spare for it.
+    F8Loads ahead;
+    if constexpr (Z::SPLITS) ahead = loads_of(first);
     auto round = [&](int c, auto whole) {
         const int d = c - first;
+        const F8Stage g{slot * BN * F8_BLOCK, Z::X + slot * BM * F8_BLOCK, Z::SCALES + group * Z::GROUP + (d & 3) * 4, a.K - c * F8_BLOCK};
         // This step's loads of this wave have arrived, once at most those of the PF - 2 steps before it are outstanding.
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(qt_vmcnt((PF - 2) * LOADS));
         hx_lds_barrier();  // and the other waves'; the stage of the step before is no longer read
-        const F8Stage g{f8_lds + slot * BN * F8_BLOCK, f8_lds + Z::X + slot * BM * F8_BLOCK,
-                        reinterpret_cast<const float*>(f8_lds + Z::SCALES + group * Z::GROUP) + (d & 3), a.K - c * F8_BLOCK};
-        step(g, loads(slot == 0 ? PF - 1 : slot - 1, c + PF - 1, group == 0 ? 2 : group - 1, (d >> 2) + 2, d & 3), whole);
+        if constexpr (!Z::SPLITS) ahead = loads_of(c);
+        step(g, ahead, whole);
         const int next = min(c + 1, a.kb - 1);
         wnext[0] = ws[0][next];
         if constexpr (PAIR) wnext[1] = ws[1][next];
         slot = slot + 1 == PF ? 0 : slot + 1;
         if ((d & 3) == 3) group = group == 2 ? 0 : group + 1;
+        if constexpr (Z::SPLITS) ahead = loads_of(c + 1);
     };
     const int whole = min(steps, a.K / F8_BLOCK);  // the end of the steps without a part past K
     for (int c = first; c < whole; ++c) round(c, std::true_type{});
@@ -686,17 +702,17 @@ constexpr long F8_MOST_TILES = 1l << 22;  // of at most 512 threads
 // A tile, how many of its workgroups a CU holds, and what it costs, in us: to begin and end; a step of a workgroup at least; a step of each
 // workgroup on a CU; where K is split, for the join and for each part of it, beside .31 us for each MB of sums.  Fitted to some 400 calls of fp16
 // outputs and 240 of fp32 outputs (12 to 1500 rows, K and N 2048 to 12288), the model is within 5 % rms, and its choice takes 1 % longer than
-// the best of the tiles and splits on average, 11 % at most.  (45 rows of 8192 -> 4096: 64 x 64 in 4 parts 13.9 us, in 2 parts 20.3, 128 x 64 in 8
-// parts 15.6; 1000 rows of 4096 -> 4096: 128 x 128 26.9, 64 x 64 40.5, 256 x 256 63.2.)
+// the best of the tiles and splits on average, 10 % at most.  (45 rows of 8192 -> 4096: 64 x 64 in 4 parts 12.9 us, in 2 parts 18.2, 128 x 64 in 8
+// parts 14.7; 1000 rows of 4096 -> 4096: 128 x 128 25.7, 64 x 64 38.8, 256 x 256 55.7.)
 struct F8Tile {
     int bn, bm, resident;
     float start, step, each, join, part;
 };
 constexpr F8Tile F8_TILES[2][6] = {
-    {{}, {64, 32, 4, 2.2f, 0.44f, 0.286f, 2.0f, 0.29f}, {64, 64, 3, 3.0f, 0.458f, 0.30f, 0.9f, 0.43f}, {128, 64, 2, 3.75f, 0.57f, 0.437f, 0.5f, 0.64f},
-     {128, 128, 1, 4.2f, 0.70f, 0.705f, 0.f, 0.6f}, {256, 256, 1, 11.0f, 1.57f, 1.57f, 0.f, 0.f}},
-    {{}, {64, 32, 4, 3.4f, 0.46f, 0.308f, 1.7f, 0.19f}, {64, 64, 3, 3.45f, 0.56f, 0.376f, 1.0f, 0.36f}, {128, 64, 2, 4.4f, 0.79f, 0.593f, 0.2f, 0.59f},
-     {}, {256, 256, 1, 10.5f, 2.99f, 2.99f, 0.f, 0.f}}};  // exact, 128 x 128 is at most 3 % before 128 x 64
+    {{}, {64, 32, 4, 2.2f, 0.38f, 0.26f, 1.8f, 0.31f}, {64, 64, 3, 2.7f, 0.413f, 0.29f, 0.95f, 0.445f}, {128, 64, 2, 3.4f, 0.52f, 0.435f, 0.65f, 0.66f},
+     {128, 128, 1, 3.9f, 0.65f, 0.66f, 0.f, 0.61f}, {256, 256, 1, 10.9f, 1.49f, 1.49f, 0.f, 0.f}},
+    {{}, {64, 32, 4, 3.1f, 0.43f, 0.292f, 1.65f, 0.2f}, {64, 64, 3, 3.2f, 0.552f, 0.37f, 0.93f, 0.38f}, {128, 64, 2, 4.25f, 0.80f, 0.596f, 0.2f, 0.62f},
+     {}, {256, 256, 1, 9.6f, 2.94f, 2.94f, 0.f, 0.f}}};  // exact, 128 x 128 is at most 3 % before 128 x 64
 
 F8Plan f8_plan(int M, int N, int K, F8Sums sums, bool split)
 {
@@ -726,7 +742,7 @@ F8Plan f8_plan(int M, int N, int K, F8Sums sums, bool split)
         for (int s = 1; s <= 8; s *= 2) {
             const int steps = (kb + s - 1) / s;
             if (s > 1 && (!split || t.part == 0.f || steps < 4 || tiles * s > (long)F8_CUS * t.resident)) break;  // all are at work at once
-            const float each = (float)((tiles * s + F8_CUS - 1) / F8_CUS), scaling = !pair ? 0.0f : whole ? 2.4f : 3.3f;
+            const float each = (float)((tiles * s + F8_CUS - 1) / F8_CUS), scaling = !pair ? 0.0f : whole ? 3.0f : 3.3f;
             const float sums_mb = (float)(tiles * s * t.bn * std::min(t.bm, (M + 15) / 16 * 16)) * 4e-6f;
             const float join = s > 1 ? t.join + t.part * s + 0.31f * sums_mb : 0.0f;
             const float us = t.start + steps * std::max(t.step, each * t.each) + join + scaling;
