@@ -73,6 +73,7 @@ HX_INLINE float f8_parts_sum(float v)
     return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, (int)__builtin_amdgcn_permlane32_swap(u, u, false, false)[1], 0x128, 0xf, 0xf, false));
 }
 
+// Of at most 2^31 - 1 bytes (a 64-bit size costs vector instructions).
 HX_INLINE __amdgpu_buffer_rsrc_t f8_rsrc(const void* base, int bytes)
 {
     const uint64_t u = reinterpret_cast<uint64_t>(base);
@@ -154,7 +155,7 @@ HX_INLINE void f8_finish_block(const F8Call& c, const float* v, int rows, int m0
 // consecutive: half h is block h of the span.
 // A workgroup's waves split K, a span each (with fewer spans than waves they also split the tile's rows), and go over tiles of 8 weight rows
 // (of a gated pair: 8 of gate and 8 of up); codes are replaced by the next piece's as soon as they are converted.  One workgroup of 16 waves
-// a CU: 8 rows of 4096 -> 12288 took 12.5 us, 15.1 with two workgroups and 17.8 with two of 8 waves; now 11.4, and 8 rows of 4096 -> 151552 97 us
+// a CU: 8 rows of 4096 -> 12288 took 12.5 us, 15.1 with two workgroups and 17.8 with two of 8 waves; now 11.5, and 8 rows of 4096 -> 151552 97 us
 // (6.4 TB/s).
 // x stays in registers as fp16 where a round of spans is all of K, up to 4096 (from LDS: 1 row of 4096 -> 12288 the same, the pair of 8 rows of
 // 4096 -> 2048 12.2 us where 11.4 are).  Where it is not (FAR), x stays in LDS as codes, piece u of a block of row r at piece u ^ (r & 7), rows a
@@ -174,9 +175,10 @@ __global__ __launch_bounds__(F8_ROWS_THREADS) void f8_rows_kernel(F8Call a, int 
     const int wk = 1 << wk_log2, kw = wave & (wk - 1), rw = wave >> wk_log2, wr = WAVES >> wk_log2;  // the wave's place in K and in rows
     const int col = lane & 15, kg = lane >> 4, s = col / R, r = col % R;
     const int sums = wk == WAVES ? WAVES + 4 : wk;  // apart in red, where all waves share K: without the 4, banks cost some 500 cycles a tile
-    const int rounds = FAR ? ((a.kb + 1) / 2 + wk - 1) >> wk_log2 : 1;        // over K
-    const int rows_wg = wr * R, tiles = (a.N + rows_wg - 1) / rows_wg;        // rows_wg: a power of two up to 128
-    const int far_row = f8_far_row(a.K), far_r = min(r, a.M - 1);             // rows behind M: any
+    // Rounds over K; 1 if not FAR, which stays unsaid: without the loop 8 rows of 4096 -> 151552 take 99 us where 97 are.
+    const int rounds = ((a.kb + 1) / 2 + wk - 1) >> wk_log2;
+    const int rows_wg = wr * R, tiles = (a.N + rows_wg - 1) / rows_wg;  // rows_wg: a power of two up to 128
+    const int far_row = f8_far_row(a.K), far_r = min(r, a.M - 1);       // rows behind M: any
     float* far_scales = reinterpret_cast<float*>(f8_lds + a.M * far_row);
 
     const __amdgpu_buffer_rsrc_t rx = mf_rsrc(a.x, (size_t)a.M * a.K);
@@ -191,11 +193,11 @@ __global__ __launch_bounds__(F8_ROWS_THREADS) void f8_rows_kernel(F8Call a, int 
     __amdgpu_buffer_rsrc_t rw_[P];
     scalar_t ws[P];
     auto aim = [&](int tile) {  // descriptors of the tile's rows (nothing left of the matrix: every load is 0)
-        const long row0 = ((long)tile * wr + rw) * R, left = tile < tiles ? max(min(a.N - row0, (long)R), 0l) : 0;
+        const int row0 = (tile * wr + rw) * R, left = tile < tiles ? max(min(a.N - row0, R), 0) : 0;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            rw_[p] = mf_rsrc(a.w[p].codes + row0 * a.K, (size_t)(left * a.K));
-            ws[p] = (scalar_t)(a.w[p].scales + (left ? row0 / F8_BLOCK * a.kb : 0));
+            rw_[p] = f8_rsrc(a.w[p].codes + (size_t)row0 * a.K, left * a.K);
+            ws[p] = (scalar_t)(a.w[p].scales + (left ? (size_t)(row0 / F8_BLOCK) * a.kb : 0));
         }
     };
     auto load_w = [&](int p, int round) {
