@@ -689,7 +689,7 @@ namespace {
 
 // Which kernel takes a call, and the parts of K.
 struct F8Plan {
-    enum Kind { ROWS, TILE64x32, TILE64x64, TILE128x64, TILE128x128, TILE256x256, NONE } kind;
+    enum Kind { ROWS, TILE64x32, TILE64x64, TILE128x64, TILE128x128, TILE256x32, TILE256x64, TILE256x256, NONE } kind;
     int splits, steps;
     long tiles;
     size_t partial, products;  // bytes of workspace
@@ -702,19 +702,24 @@ constexpr int F8_NEAR = 2 * F8_ROWS_THREADS / 64;  // blocks of K whose spans ar
 constexpr long F8_MOST_TILES = 1l << 22;  // of at most 512 threads
 
 // A tile, how many of its workgroups a CU holds, and what it costs, in us: to begin and end; a step of a workgroup at least; a step of each
-// workgroup on a CU; where K is split, for the join and for each part of it, beside .31 us for each MB of sums.  Fitted to some 400 calls of fp16
-// outputs and 240 of fp32 outputs (12 to 1500 rows, K and N 2048 to 12288), the model is within 5 % rms, and its choice takes 1 % longer than
-// the best of the tiles and splits on average, 10 % at most.  (45 rows of 8192 -> 4096: 64 x 64 in 4 parts 12.9 us, in 2 parts 18.2, 128 x 64 in 8
-// parts 14.7; 1000 rows of 4096 -> 4096: 128 x 128 25.7, 64 x 64 38.8, 256 x 256 55.7.)
+// workgroup on a CU; where K is split, for the join and for each part of it, beside .36 us for each MB of sums.  Fitted to some 400 calls of fp16
+// outputs, 240 of fp32 outputs and 480 of the gated pair (12 to 1500 rows, K and N 2048 to 12288), the model is within 5 % rms, and its choice
+// takes 1 % longer than the best of the tiles and splits on average, 10 % at most.  (45 rows of 8192 -> 4096: 64 x 64 in 4 parts 12.9 us, in 2 parts
+// 18.2, 128 x 64 in 8 parts 14.7; 1000 rows of 4096 -> 4096: 128 x 128 25.7, 64 x 64 38.8, 256 x 256 55.7.)
 struct F8Tile {
     int bn, bm, resident;
     float start, step, each, join, part;
 };
-constexpr F8Tile F8_TILES[2][6] = {
+constexpr F8Tile F8_TILES[3][8] = {
     {{}, {64, 32, 4, 2.2f, 0.38f, 0.26f, 1.8f, 0.31f}, {64, 64, 3, 2.7f, 0.413f, 0.29f, 0.95f, 0.445f}, {128, 64, 2, 3.4f, 0.52f, 0.435f, 0.65f, 0.66f},
-     {128, 128, 1, 3.9f, 0.65f, 0.66f, 0.f, 0.61f}, {256, 256, 1, 10.9f, 1.49f, 1.49f, 0.f, 0.f}},
+     {128, 128, 1, 3.9f, 0.65f, 0.66f, 0.f, 0.61f}, {}, {}, {256, 256, 1, 10.9f, 1.49f, 1.49f, 0.f, 0.f}},
+    // exact, 128 x 128 is at most 3 % before 128 x 64
     {{}, {64, 32, 4, 3.1f, 0.43f, 0.292f, 1.65f, 0.2f}, {64, 64, 3, 3.2f, 0.552f, 0.37f, 0.93f, 0.38f}, {128, 64, 2, 4.25f, 0.80f, 0.596f, 0.2f, 0.62f},
-     {}, {256, 256, 1, 9.6f, 2.94f, 2.94f, 0.f, 0.f}}};  // exact, 128 x 128 is at most 3 % before 128 x 64
+     {}, {}, {}, {256, 256, 1, 9.6f, 2.94f, 2.94f, 0.f, 0.f}},
+    // with the scaling; tiles of whole blocks of outputs do without products in memory (20 rows of 4096 -> 12288: 256 x 32 24.3 us, 64 x 32 26.7; 45
+    // rows: 256 x 64 28.8, 64 x 64 30.3)
+    {{}, {64, 32, 4, 6.2f, 0.446f, 0.333f, 0.93f, 0.16f}, {64, 64, 3, 7.4f, 0.543f, 0.39f, 0.62f, 0.16f}, {128, 64, 2, 7.2f, 0.867f, 0.649f, 0.1f, 0.56f},
+     {}, {256, 32, 1, 4.5f, 1.0f, 1.0f, 0.94f, 0.65f}, {256, 64, 1, 6.0f, 1.17f, 1.17f, 0.46f, 0.5f}, {256, 256, 1, 11.6f, 2.9f, 2.9f, 0.f, 0.f}}};
 
 F8Plan f8_plan(int M, int N, int K, F8Sums sums, bool split)
 {
@@ -734,7 +739,7 @@ F8Plan f8_plan(int M, int N, int K, F8Sums sums, bool split)
     float least = 0.0f;
     p.kind = F8Plan::NONE;
     for (int kind = F8Plan::TILE64x32; kind <= F8Plan::TILE256x256; ++kind) {
-        const F8Tile& t = F8_TILES[sums != F8_FAST][kind];
+        const F8Tile& t = F8_TILES[sums][kind];
         if (!t.bn) continue;
         const long mt = ((long)M + t.bm - 1) / t.bm, tiles = mt * (((long)N * (pair ? 2 : 1) + t.bn - 1) / t.bn);
         if (tiles > F8_MOST_TILES) continue;
@@ -744,10 +749,10 @@ F8Plan f8_plan(int M, int N, int K, F8Sums sums, bool split)
         for (int s = 1; s <= 8; s *= 2) {
             const int steps = (kb + s - 1) / s;
             if (s > 1 && (!split || t.part == 0.f || steps < 4 || tiles * s > (long)F8_CUS * t.resident)) break;  // all are at work at once
-            const float each = (float)((tiles * s + F8_CUS - 1) / F8_CUS), scaling = !pair ? 0.0f : whole ? 3.0f : 3.3f;
+            const float each = (float)((tiles * s + F8_CUS - 1) / F8_CUS);
             const float sums_mb = (float)(tiles * s * t.bn * std::min(t.bm, (M + 15) / 16 * 16)) * 4e-6f;
-            const float join = s > 1 ? t.join + t.part * s + 0.31f * sums_mb : 0.0f;
-            const float us = t.start + steps * std::max(t.step, each * t.each) + join + scaling;
+            const float join = s > 1 ? t.join + t.part * s + 0.36f * sums_mb : 0.0f;
+            const float us = t.start + steps * std::max(t.step, each * t.each) + join;
             if (p.kind != F8Plan::NONE && us >= least) continue;
             least = us;
             p.kind = (F8Plan::Kind)kind;
@@ -798,6 +803,12 @@ hipError_t f8_launch(F8Call c, const F8Plan& p, void* ws, hipStream_t st)
         case F8Plan::TILE128x64: return tile_launch<2, 2, 4, 2, 3, !FAST, PAIR>(c, p, st);
         case F8Plan::TILE128x128:
             if constexpr (FAST) return tile_launch<2, 4, 4, 2, 3, false, false>(c, p, st);
+            return hipErrorInvalidValue;
+        case F8Plan::TILE256x32:
+            if constexpr (PAIR) return tile_launch<4, 1, 4, 2, 3, true, true>(c, p, st);
+            return hipErrorInvalidValue;
+        case F8Plan::TILE256x64:
+            if constexpr (PAIR) return tile_launch<4, 2, 4, 2, 3, true, true>(c, p, st);
             return hipErrorInvalidValue;
         case F8Plan::TILE256x256: return tile_launch<2, 4, 8, 4, 2, !FAST, PAIR>(c, p, st);
         default: return hipErrorInvalidValue;

@@ -59,7 +59,7 @@ def test_every_step_is_complete_at_its_barrier(tmp_path, monkeypatch):
         __graft_entry__.build()
     monkeypatch.setattr(waits, "KERNELS", ("f8_tile_kernel",))
     kernels = waits.tile_kernels(waits.LIB, tmp_path)
-    assert len(kernels) == 5 + 4 + 4  # fp16 outputs, fp32 outputs, gated pair
+    assert len(kernels) == 5 + 4 + 6  # fp16 outputs, fp32 outputs, gated pair
     for name, bb in kernels.items():
         fault = follow(loading(bb), min(bb), *ring(name))
         assert fault is None, f"{name}: {fault}"

@@ -502,6 +502,7 @@ GSHAPES = [  # M, K, N
     (1, 16, 16), (1, 4096, 2048), (2, 144, 48), (3, 1056, 272), (4, 4096, 512), (5, 2048, 1040), (8, 8208, 144), (9, 512, 128),
     (16, 4096, 384), (17, 272, 112), (33, 1024, 640), (45, 4096, 1024), (64, 2048, 272), (100, 4096, 2048), (129, 144, 400), (300, 2048, 1040),
     (513, 512, 256), (1030, 256, 528)]
+GWIDE = [(17, 144, 16400), (33, 272, 8208), (45, 528, 12304), (70, 1040, 12304), (20, 4112, 12304), (48, 4112, 8208)]  # many outputs
 
 
 def gated(x, gw, uw, limit):
@@ -527,8 +528,7 @@ def check_blocks(q, s, v, ev):
     assert (err <= tol).all(), float((err / tol).max())
 
 
-@pytest.mark.parametrize("limit", [10.0, 0.5, float("inf")])
-@pytest.mark.parametrize("M,K,N", GSHAPES)
+@pytest.mark.parametrize("M,K,N,limit", [(*g, limit) for g in GSHAPES for limit in (10.0, 0.5, float("inf"))] + [(*g, 10.0) for g in GWIDE])
 def test_gate_up(f8, M, K, N, limit):
     import torch
     gw, gw64 = weights(f8, M + K, N, K, False)
