@@ -288,9 +288,11 @@ typedef struct hx_f8_blocks {
 } hx_f8_blocks;
 
 /* y[M][N] = x W^T: x and x_scales as hx_f8_quantize gives them, y fp32 (y_fp32) or fp16: fp32 sums rounded once.  A block's scales are
- * applied to the fp32 sum of its codes' products.  These are exact for fp32 outputs and M <= 8; with more rows and fp16 outputs, 8
- * consecutive k (from a multiple of 8) are first added to 2^-13 of the largest of their 8 products, so that y is off by at most 7 * 2^-13
- * times the sum of those largest ones beside its rounding (1.6e-5 of the outputs' size, rms, where the values are random).  The workspace
+ * applied to the fp32 sum of its codes' products.  These are exact for fp32 outputs and M <= 8; with more rows and fp16 outputs the products
+ * of 8 consecutive k (from a multiple of 8) are first cut to multiples of 2^(e - 13), e the largest sum of two multiplied codes' exponents
+ * there (a code below 2^-6 counts with -6, a product of 0 not at all), so that y is off by at most 7 * 2^-13 times the sum of the octets' 2^e
+ * (with their scales) beside its rounding: 1.6e-5 of the outputs' size, rms, where the values are random.  2^e is at most the octet's largest
+ * product where no code is below 2^-6, up to 8 times it (64 times) where the product of the largest e has one such code (two).  The workspace
  * is optional: a call with at least hx_f8_gemm_workspace_size(M, N, K) bytes (0: the shape has no use for it) splits K over more
  * workgroups where there are few, with the fp32 sums in another order than without; NULL or fewer bytes do without. */
 size_t hx_f8_gemm_workspace_size(int M, int N, int K);

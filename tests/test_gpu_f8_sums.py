@@ -1,0 +1,53 @@
+"""Accuracy of the 8-bit linear's sums, and of the norm at its smallest inputs, against the definitions in 64 bits."""
+import numpy as np
+import pytest
+
+from test_gpu_f8 import E4M3, U16, codes, dev, f8, host, inputs, nblocks, product_tolerance, weights  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+SUBNORMAL, NORMAL = E4M3[1:8], E4M3[8:127]
+
+
+def power(v):
+    """2 to the exponent of codes, of those below 2^-6 to -6; 0 of 0."""
+    return np.where(v == 0, 0.0, 2.0 ** np.maximum(np.floor(np.log2(np.maximum(np.abs(v), 2.0 ** -9))), -6))
+
+
+def octet_loss(x, w):
+    """What an octet may lose: its products become multiples of 2^-13 of its largest power of two.  Those with this exponent are such multiples
+    (two significands of 3 bits behind the point make 6), so that at most 7 lose, less than one such multiple each."""
+    most = np.zeros((len(x), len(w)))
+    for k in range(0, x.shape[1], 8):
+        t = np.zeros_like(most)
+        for j in range(k, k + 8):
+            t = np.maximum(t, power(x[:, j])[:, None] * power(w[:, j])[None])
+        most += t
+    return 7 * 2.0 ** -13 * most
+
+
+@pytest.mark.parametrize("signs", [False, True])
+@pytest.mark.parametrize("kx,kw", [(NORMAL, NORMAL), (NORMAL, SUBNORMAL), (SUBNORMAL, NORMAL), (SUBNORMAL, SUBNORMAL)],
+                         ids=["normal", "subnormal_w", "subnormal_x", "subnormal"])
+def test_octets_of_unlike_products(f8, kx, kw, signs):
+    """fp16 outputs of more than 8 rows: in each octet one product of any codes, normal or not, beside seven of codes up to 1.4.  A second octet
+    takes the one away again, so that the outputs are sums of the seven and show what these lost."""
+    import torch
+    M, N, K, up = 64, 256, 16, 2.0 ** 8
+    r = np.random.default_rng(len(kx) + 2 * len(kw) + signs)
+    worst = 0.0
+    for _ in range(10):
+        x, w = np.zeros((M, K)), np.zeros((N, K))
+        x[:, 0], w[:, 0] = r.choice(kx, M), r.choice(kw, N)
+        x[:, 1:8], w[:, 1:8] = r.choice(E4M3[:60], (M, 7)), r.choice(E4M3[:60], (N, 7))
+        if signs:
+            x[:, :8] *= r.choice([-1, 1], (M, 8))
+            w[:, :8] *= r.choice([-1, 1], (N, 8))
+        x[:, 8], w[:, 8] = -x[:, 0], w[:, 0]
+        y = torch.empty((M, N), dtype=torch.float16, device="cuda")
+        f8.gemm(y, codes(x), torch.full((M, 1), up, device="cuda"), f8.F8Blocks(codes(w), torch.ones((2, 1), device="cuda")), M, N, K)
+        ref = up * (x @ w.T)
+        tol = product_tolerance(up * x, w) + up * octet_loss(x, w)
+        tol = tol * (1 + U16) + U16 * np.abs(ref) + 2.0 ** -25
+        worst = max(worst, float((np.abs(host(y) - ref) / tol).max()))
+    assert worst <= 1, worst
