@@ -96,6 +96,7 @@ SIGNATURES: dict[str, tuple] = {
                        [C.c_void_p] * 3 + [C.c_int, C.c_int, C.c_float, C.c_void_p]),
     "hx_f8_gemm_workspace_size": (C.c_size_t, [C.c_int] * 3),
     "hx_f8_gemm": (C.c_int, [C.c_void_p] * 3 + [C.POINTER(F8BlocksC)] + [C.c_int] * 4 + [C.c_void_p, C.c_void_p, C.c_size_t]),
+    "hx_f8_gemm_exact": (C.c_int, [C.c_void_p] * 3 + [C.POINTER(F8BlocksC)] + [C.c_int] * 4 + [C.c_void_p, C.c_void_p, C.c_size_t]),
     "hx_f8_gate_up_workspace_size": (C.c_size_t, [C.c_int] * 3),
     "hx_f8_gate_up": (C.c_int, [C.c_void_p] * 4 + [C.POINTER(F8BlocksC)] * 2 + [C.c_int] * 3 +
                       [C.c_float, C.c_void_p, C.c_void_p, C.c_size_t]),

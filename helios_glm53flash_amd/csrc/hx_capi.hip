@@ -649,17 +649,21 @@ size_t hx_f8_gemm_workspace_size(int M, int N, int K)
     return hx::f8_gemm_workspace_bytes(M, N, K);
 }
 
-int hx_f8_gemm(void* y, const void* x, const float* x_scales, const hx_f8_blocks* w, int M, int N, int K, int y_fp32,
-               hx_stream_t stream, void* workspace, size_t workspace_bytes)
+namespace {
+
+int f8_gemm(const char* who, void* y, const void* x, const float* x_scales, const hx_f8_blocks* w, int M, int N, int K, int y_fp32, bool exact,
+            hx_stream_t stream, void* workspace, size_t workspace_bytes)
 {
-    static const char who[] = "hx_f8_gemm";
     if (const char* what = f8_extents(M, K)) return f8_fail(who, what);
     if (const char* what = f8_blocks(w, N)) return f8_fail(who, what);
     if (M == 0) return 0;
     if (!y || !x || !x_scales) return f8_fail(who, "null pointer");
     if ((uintptr_t)x & 15) return f8_fail(who, "x must be 16-byte aligned");
     if (((uintptr_t)x_scales & 3) || ((uintptr_t)y & (y_fp32 ? 3 : 1))) return f8_fail(who, "x_scales or y is not aligned to its type");
-    if ((uintptr_t)workspace & 15) return fail(HX_ERR_WORKSPACE, "hx_f8_gemm: workspace must be 16-byte aligned");
+    if ((uintptr_t)workspace & 15) {
+        f8_fail(who, "workspace must be 16-byte aligned");
+        return HX_ERR_WORKSPACE;
+    }
     const int kb = (K + 127) / 128;
     const F8Span to = f8_span(y, M, N, N, y_fp32 ? 4 : 2);
     const F8Span in[] = {f8_span(x, M, K, K, 1), f8_span(x_scales, M, kb, kb, 4), f8_span(w->codes, N, K, K, 1),
@@ -667,8 +671,22 @@ int hx_f8_gemm(void* y, const void* x, const float* x_scales, const hx_f8_blocks
     for (const F8Span& i : in)
         if (!f8_apart(to, i)) return f8_fail(who, "y overlaps an input");
     return hip_status(hx::launch_f8_gemm(static_cast<const uint8_t*>(x), x_scales, {static_cast<const uint8_t*>(w->codes), w->scales}, y, M, N, K,
-                                         y_fp32 != 0, workspace, workspace_bytes, (hipStream_t)stream),
+                                         y_fp32 != 0, exact, workspace, workspace_bytes, (hipStream_t)stream),
                       who);
+}
+
+}  // namespace
+
+int hx_f8_gemm(void* y, const void* x, const float* x_scales, const hx_f8_blocks* w, int M, int N, int K, int y_fp32,
+               hx_stream_t stream, void* workspace, size_t workspace_bytes)
+{
+    return f8_gemm("hx_f8_gemm", y, x, x_scales, w, M, N, K, y_fp32, false, stream, workspace, workspace_bytes);
+}
+
+int hx_f8_gemm_exact(void* y, const void* x, const float* x_scales, const hx_f8_blocks* w, int M, int N, int K, int y_fp32,
+                     hx_stream_t stream, void* workspace, size_t workspace_bytes)
+{
+    return f8_gemm("hx_f8_gemm_exact", y, x, x_scales, w, M, N, K, y_fp32, true, stream, workspace, workspace_bytes);
 }
 
 size_t hx_f8_gate_up_workspace_size(int M, int N, int K)

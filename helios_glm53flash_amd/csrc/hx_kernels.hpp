@@ -115,8 +115,8 @@ struct F8Blocks {
     const float* scales;   // [ceil(N / 128)][ceil(K / 128)]
 };
 size_t f8_gemm_workspace_bytes(int M, int N, int K);
-hipError_t launch_f8_gemm(const uint8_t* x, const float* xs, const F8Blocks& w, void* y, int M, int N, int K, bool y_fp32, void* ws,
-                          size_t ws_bytes, hipStream_t st);
+hipError_t launch_f8_gemm(const uint8_t* x, const float* xs, const F8Blocks& w, void* y, int M, int N, int K, bool y_fp32, bool exact,
+                          void* ws, size_t ws_bytes, hipStream_t st);
 size_t f8_gate_up_workspace_bytes(int M, int N, int K);
 hipError_t launch_f8_gate_up(const uint8_t* x, const float* xs, const F8Blocks& gate, const F8Blocks& up, uint8_t* q, float* scales,
                              int M, int N, int K, float limit, void* ws, size_t ws_bytes, hipStream_t st);

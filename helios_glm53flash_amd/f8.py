@@ -144,9 +144,10 @@ def _gate_up_workspace_bytes(M: int, N: int, K: int) -> int:
 
 
 def gemm(y: torch.Tensor, x: torch.Tensor, x_scales: torch.Tensor, w: F8Blocks, M: int, N: int, K: int, y_fp32: bool = False,
-         stream=None) -> None:
+         stream=None, exact: bool = False) -> None:
     """y[m][n] = sum_k x[m][k] W[n][k] over the values that the codes and scales stand for: x and x_scales as quantize gives them,
-    y fp32 or fp16 [M][N], any M (M = 0 is a no-op).  Shapes that split K over workgroups do so in the stream's workspace."""
+    y fp32 or fp16 [M][N], any M (M = 0 is a no-op).  fp32 outputs, and up to 8 rows, come from exact products; fp16 outputs of more rows cut those
+    of 8 consecutive k at 2^-13 of their largest (some 2^-16 of the outputs' size), but where `exact` asks for the others' way.  Shapes that split K over workgroups do so in the stream's workspace."""
     kb = _extents("gemm", M, K)
     _codes("gemm", x, x_scales, M, K, kb)
     _need(y, "y", (torch.float32,) if y_fp32 else (torch.float16,))
@@ -157,8 +158,9 @@ def gemm(y: torch.Tensor, x: torch.Tensor, x_scales: torch.Tensor, w: F8Blocks, 
     st = _stream(stream)
     need = _gemm_workspace_bytes(M, N, K)
     ws = call_workspace(need, x.device, st) if need else None
-    check(lib.hx_f8_gemm(y.data_ptr(), x.data_ptr(), x_scales.data_ptr(), C.byref(w.c()), M, N, K, int(y_fp32), st, _ptr(ws),
-                         ws.numel() if ws is not None else 0), "hx_f8_gemm")
+    entry, name = (lib.hx_f8_gemm_exact, "hx_f8_gemm_exact") if exact else (lib.hx_f8_gemm, "hx_f8_gemm")
+    check(entry(y.data_ptr(), x.data_ptr(), x_scales.data_ptr(), C.byref(w.c()), M, N, K, int(y_fp32), st, _ptr(ws),
+                ws.numel() if ws is not None else 0), name)
 
 
 def gate_up(q: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, x_scales: torch.Tensor, gate: F8Blocks, up: F8Blocks, M: int,

@@ -51,3 +51,32 @@ def test_octets_of_unlike_products(f8, kx, kw, signs):
         tol = tol * (1 + U16) + U16 * np.abs(ref) + 2.0 ** -25
         worst = max(worst, float((np.abs(host(y) - ref) / tol).max()))
     assert worst <= 1, worst
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 400, 70), (8, 4224, 200), (9, 2048, 96), (20, 4096, 1024), (45, 8192, 512), (70, 528, 1201), (300, 1040, 640),
+                                   (700, 272, 2064)])
+def test_exact_products_of_fp16_outputs(f8, M, K, N):
+    """exact=True: the fp32 outputs rounded once, bit for bit, whatever M; fp32 outputs are the same with it."""
+    import torch
+    w, w64 = weights(f8, M, N, K, False)
+    x, xs, x64 = inputs(K, M, K, False)
+    y32, same32, y16 = torch.empty((M, N), device="cuda"), torch.empty((M, N), device="cuda"), torch.empty((M, N), dtype=torch.float16, device="cuda")
+    f8.gemm(y32, x, xs, w, M, N, K, True)
+    f8.gemm(same32, x, xs, w, M, N, K, True, exact=True)
+    f8.gemm(y16, x, xs, w, M, N, K, exact=True)
+    assert (np.abs(host(y32) - x64 @ w64.T) <= product_tolerance(x64, w64)).all()
+    assert torch.equal(same32, y32) and torch.equal(y16, y32.half())
+
+
+def test_exact_products_of_subnormal_codes(f8):
+    """Where the cut of 8 consecutive k is coarsest: one product of a subnormal code on one side, 448 on the other, beside smaller ones."""
+    import torch
+    M, N, K = 16, 32, 16
+    x, w = np.full((M, K), 2.0 ** -6), np.full((N, K), 2.0 ** -6)
+    x[:, 0], w[:, 0], x[:, 8], w[:, 8] = 448, 2.0 ** -9, -448, 2.0 ** -9
+    y = torch.empty((2, M, N), dtype=torch.float16, device="cuda")
+    one = torch.ones((M, 1), device="cuda")
+    for i in range(2):
+        f8.gemm(y[i], codes(x), one, f8.F8Blocks(codes(w), one[:1]), M, N, K, exact=bool(i))
+    assert (host(y[1]) == 14 * 2.0 ** -12).all()
+    assert (np.abs(host(y[0]) - 14 * 2.0 ** -12) <= octet_loss(x, w) + 2.0 ** -25).all()
