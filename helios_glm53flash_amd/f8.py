@@ -108,7 +108,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, M: int, K: int, eps: float, 
              scales: Optional[torch.Tensor] = None, stream=None) -> None:
     """h = x + residual, rounded to residual's type, into out (residual itself: in place); n = h / sqrt(mean(h^2) + eps) * weight;
     y (fp16) = n; q and scales: blocks of n before that rounding.  x as in quantize; residual and out fp16 or fp32 [M][K], or neither
-    (h = x); weight fp16 or fp32 [K]; y, or q and scales, or all three."""
+    (h = x); weight fp16 or fp32 [K]; y, or q and scales, or all three.  Rows of zeros give zeros, but NaN where eps is 0."""
     kb = _extents("rms_norm", M, K)
     ld = _rows("rms_norm", x, M, K)
     _need(weight, "weight", (torch.float16, torch.float32))

@@ -277,7 +277,9 @@ int hx_f8_quantize(const void* x, void* q, float* scales, int M, int K, int64_t 
 /* h = x + residual, rounded to residual's type; n = h / sqrt(mean over K of h^2 + eps) * weight in fp32 (fp32 sums); y = fp16(n);
  * q, scales = blocks of n before that rounding.  x (x_dtype) as in hx_f8_quantize; residual and out [M][K] (residual_dtype), out receives h and
  * may be residual itself; both NULL: h = x.  weight [K] (weight_dtype).  y fp16 [M][K], or NULL; q and scales as in hx_f8_quantize, or
- * both NULL.  All 16-byte aligned but scales. */
+ * both NULL.  All 16-byte aligned but scales.  eps >= 0: any above 0 makes a row of zeros zeros; with eps == 0 a row whose squares are all 0
+ * in fp32 (zeros, values below 2^-75) has 0 / 0 = NaN of its zeros and infinities of its other values.  A row of finite values whose squares
+ * add to 2^128 or more has n = 0. */
 int hx_f8_rms_norm(const void* x, int64_t ld, int x_dtype, const void* residual, void* out, int residual_dtype, const void* weight,
                    int weight_dtype, void* y, void* q, float* scales, int M, int K, float eps, hx_stream_t stream);
 

@@ -80,3 +80,30 @@ def test_exact_products_of_subnormal_codes(f8):
         f8.gemm(y[i], codes(x), one, f8.F8Blocks(codes(w), one[:1]), M, N, K, exact=bool(i))
     assert (host(y[1]) == 14 * 2.0 ** -12).all()
     assert (np.abs(host(y[0]) - 14 * 2.0 ** -12) <= octet_loss(x, w) + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("K", [16, 256, 5008, 16400])
+def test_norm_at_the_ends_of_its_squares(f8, K):
+    """Rows of zeros, of values whose squares are 0 in fp32, and of values whose squares' sum is not finite there, at eps from 0 on; an
+    ordinary row beside them is as it would be."""
+    import torch
+    x = np.repeat(np.float32([0, 2.0 ** -80, 2.0 ** 70, 0.5]), K).reshape(4, K)
+    x[1, K // 2:] = 0
+    w = np.ones(K, np.float32)
+    for eps in (0.0, 2.0 ** -149, 2.0 ** -126, 1e-30, 1e-5):
+        y, q, s = (torch.empty((4, K), dtype=torch.float16, device="cuda"), torch.empty((4, K), dtype=torch.float8_e4m3fn, device="cuda"),
+                   torch.empty((4, nblocks(K)), device="cuda"))
+        f8.rms_norm(dev(x), dev(w), 4, K, eps, y=y, q=q, scales=s)
+        got = host(y)
+        with np.errstate(invalid="ignore"):
+            blocks = host(q) * np.repeat(s.cpu().numpy().astype(np.float64), 128, axis=1)[:, :K]
+        if eps == 0:
+            assert np.isnan(got[0]).all() and np.isnan(blocks[0]).all()
+            assert np.isinf(got[1, :K // 2]).all() and np.isnan(got[1, K // 2:]).all()
+        else:
+            assert (got[0] == 0).all() and (blocks[0] == 0).all()
+            n = 2.0 ** -80 / np.sqrt(eps)  # the squares add nothing to eps
+            assert (np.abs(got[1, :K // 2] - n) <= U16 * n + 2.0 ** -24).all() and (got[1, K // 2:] == 0).all()
+        assert (got[2] == 0).all() and (blocks[2] == 0).all()
+        n = 0.5 / np.sqrt(0.25 + eps)
+        assert (np.abs(got[3] - n) <= (U16 + (K + 20) * 2.0 ** -24) * n).all()
