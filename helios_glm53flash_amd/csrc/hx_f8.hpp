@@ -7,11 +7,11 @@
 // floor keeps 448 / a finite; a block of zeros has codes 0.  A NaN or an infinity makes the scale NaN or infinite and with it every value
 // that the block stands for NaN: codes are NaN, or 0 times an infinite scale.
 #pragma once
+#include "hx_f8_plan.hpp"
 #include "hx_gemv.hpp"
 
 namespace hx {
 
-constexpr int F8_BLOCK = 128;
 constexpr float F8_TOP = 448.0f, F8_TINY = 0x1p-100f;
 
 // Largest of a u32 over each row of 16 lanes, in all of them.
