@@ -118,3 +118,27 @@ def test_gated_pair(f8, outputs, tile, parts, size):
         got.append((q, s))
     check_blocks(*got[0], *gated(x64, gw64, uw64, 10.0))
     assert torch.equal(got[0][0].view(torch.uint8), got[1][0].view(torch.uint8)) and torch.equal(got[0][1], got[1][1])
+
+
+def test_large_offsets_with_scales(f8):
+    """Codes past 2^32 bytes under scales that differ from block to block."""
+    import torch
+    K, N, M = 4112, 1_050_000, 2100
+    free, _ = torch.cuda.mem_get_info()
+    if free < 20 << 30:
+        pytest.skip("not enough memory")
+    r = np.random.default_rng(0)
+    c = torch.randint(-4, 5, (1000, K), device="cuda").float().to(torch.float8_e4m3fn)
+    s = (2.0 ** r.integers(-2, 2, (nblocks(N), nblocks(K)))).astype(np.float32)
+    w = f8.F8Blocks(c.view(torch.uint8).repeat(N // 1000, 1).view(torch.float8_e4m3fn), torch.from_numpy(s).cuda())
+    x, xs, x64 = inputs(2, M, K, True)
+    c64 = host(c)
+    for m in (1, 16, 40, M):
+        y = torch.empty((m, N), dtype=torch.float16, device="cuda")
+        f8.gemm(y, x[:m], xs[:m], w, m, N, K)
+        for at in (0, N // 2000 * 1000, N - 1000):
+            scales = spread(s[(np.arange(at, at + 1000)) // 128].astype(np.float64), K)
+            with np.errstate(over="ignore"):
+                want = (x64[:m] @ (c64 * scales).T).astype(np.float16)
+            assert np.array_equal(y[:, at:at + 1000].cpu().numpy(), want)
+        del y
