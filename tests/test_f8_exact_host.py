@@ -30,3 +30,14 @@ def test_python_checks():
     codes, scales = torch.zeros((4, 32), dtype=torch.float8_e4m3fn), torch.ones((1, 1))
     with pytest.raises(ValueError, match="32 bits"):
         f8.gemm(scales, codes, scales, None, 1 << 31, 4, 32, exact=True)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 2048, 4096), (8, 16, 16), (12, 144, 400), (33, 1040, 2704)])
+def test_gated_pair_without_its_workspace(M, N, K):
+    """Sizes whose blocks of outputs meet in memory: the size is not 0, and a call with less, none or a misaligned one is refused."""
+    need = _lib.lib.hx_f8_gate_up_workspace_size(M, N, K)
+    assert need > 64 * 1024
+    w = C.byref(_lib.F8BlocksC(400 * FAR, 500 * FAR))
+    for ws, size in ((None, need), (700 * FAR + 8, need), (700 * FAR, need - 1), (700 * FAR, 0)):
+        r = _lib.lib.hx_f8_gate_up(FAR, 100 * FAR, 200 * FAR, 300 * FAR, w, w, M, N, K, 10.0, None, ws, size)
+        assert r == _lib.HX_ERR_WORKSPACE and "hx_f8_gate_up_workspace_size" in err(), (ws, size, err())
