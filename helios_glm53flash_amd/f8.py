@@ -86,11 +86,11 @@ def _rows(who: str, x: torch.Tensor, M: int, K: int) -> int:
     return ld
 
 
-def _codes(who: str, q: torch.Tensor, scales: torch.Tensor, M: int, K: int, kb: int) -> None:
-    _need(q, "q", (F8,))
-    _need(scales, "scales", (torch.float32,))
+def _codes(who: str, q: torch.Tensor, scales: torch.Tensor, M: int, K: int, kb: int, name: str = "q", scales_name: str = "scales") -> None:
+    _need(q, name, (F8,))
+    _need(scales, scales_name, (torch.float32,))
     if q.numel() < M * K or scales.numel() < M * kb:
-        raise ValueError(f"{who}: codes / scales smaller than M * K / M * ceil(K / 128)")
+        raise ValueError(f"{who}: codes / scales smaller than M * K / M * ceil(K / 128): {name}, {scales_name}")
 
 
 def quantize(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, M: int, K: int, stream=None) -> None:
@@ -149,7 +149,7 @@ def gemm(y: torch.Tensor, x: torch.Tensor, x_scales: torch.Tensor, w: F8Blocks, 
     y fp32 or fp16 [M][N], any M (M = 0 is a no-op).  fp32 outputs, and up to 8 rows, come from exact products; fp16 outputs of more rows cut those
     of 8 consecutive k at 2^-13 of their largest (some 2^-16 of the outputs' size), but where `exact` asks for the others' way.  Shapes that split K over workgroups do so in the stream's workspace."""
     kb = _extents("gemm", M, K)
-    _codes("gemm", x, x_scales, M, K, kb)
+    _codes("gemm", x, x_scales, M, K, kb, "x", "x_scales")
     _need(y, "y", (torch.float32,) if y_fp32 else (torch.float16,))
     if y.numel() < M * N:
         raise ValueError("gemm: y smaller than M * N")
@@ -170,7 +170,7 @@ def gate_up(q: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, x_scales: to
     16; limit = inf does not clamp."""
     kb = _extents("gate_up", M, K)
     nb = _extents("gate_up", M, N)
-    _codes("gate_up", x, x_scales, M, K, kb)
+    _codes("gate_up", x, x_scales, M, K, kb, "x", "x_scales")
     _codes("gate_up", q, scales, M, N, nb)
     _blocks_here(gate, N, K)
     _blocks_here(up, N, K)

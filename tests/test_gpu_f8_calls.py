@@ -140,7 +140,7 @@ REFUSALS = {  # name: (raised, its text, call of f8 and a maker of zeros)
     "gemm_into_the_other_type": (ValueError, "y", lambda f8, e: f8.gemm(e((4, 32)), e((4, 256), F), e((4, 2)), blocks(f8, e), 4, 32, 256)),
     "exact_gemm_into_the_other_type": (ValueError, "y",
         lambda f8, e: f8.gemm(e((4, 32)), e((4, 256), F), e((4, 2)), blocks(f8, e), 4, 32, 256, exact=True)),
-    "gemm_of_fp32": (ValueError, "q", lambda f8, e: f8.gemm(e((4, 32)), e((4, 256)), e((4, 2)), blocks(f8, e), 4, 32, 256, True)),
+    "gemm_of_fp32": (ValueError, "dtype", lambda f8, e: f8.gemm(e((4, 32)), e((4, 256)), e((4, 2)), blocks(f8, e), 4, 32, 256, True)),
     "gemm_into_few_rows": (ValueError, "y smaller", lambda f8, e: f8.gemm(e((3, 32)), e((4, 256), F), e((4, 2)), blocks(f8, e), 4, 32, 256, True)),
     "gemm_of_negative_rows": (ValueError, "32 bits", lambda f8, e: f8.gemm(e((4, 32)), e((4, 256), F), e((4, 2)), blocks(f8, e), -1, 32, 256, True)),
     "gemm_over_its_input": (HxError, "overlap", lambda f8, e: gemm_over(f8, e((4, 256), F), e)),
@@ -163,6 +163,16 @@ REFUSALS = {  # name: (raised, its text, call of f8 and a maker of zeros)
     "quantize_of_a_first_column_off_alignment": (HxError, "16-byte",
         lambda f8, e: f8.quantize(e((4, 264))[:, 2:258], e((4, 256), F), e((4, 2)), 4, 256)),
     "quantize_of_short_k": (HxError, "multiple of 16", lambda f8, e: f8.quantize(e((4, 40)), e((4, 40), F), e((4, 1)), 4, 40)),
+    # messages name the argument
+    "gemm_of_codes_in_fp32": (ValueError, "^x has dtype", lambda f8, e: f8.gemm(e((4, 32)), e((4, 256)), e((4, 2)), blocks(f8, e), 4, 32, 256, True)),
+    "gemm_of_fp16_scales": (ValueError, "^x_scales has dtype",
+        lambda f8, e: f8.gemm(e((4, 32)), e((4, 256), F), e((4, 2), H), blocks(f8, e), 4, 32, 256, True)),
+    "gemm_of_few_scales_of_x": (ValueError, ": x, x_scales$",
+        lambda f8, e: f8.gemm(e((4, 32)), e((4, 256), F), e((3, 2)), blocks(f8, e), 4, 32, 256, True)),
+    "pair_of_codes_in_fp32": (ValueError, "^x has dtype",
+        lambda f8, e: f8.gate_up(e((4, 32), F), e((4, 1)), e((4, 256)), e((4, 2)), blocks(f8, e), blocks(f8, e), 4, 32, 256)),
+    "pair_into_fp16_scales": (ValueError, "^scales has dtype",
+        lambda f8, e: f8.gate_up(e((4, 32), F), e((4, 1), H), e((4, 256), F), e((4, 2)), blocks(f8, e), blocks(f8, e), 4, 32, 256)),
     "norm_with_a_short_weight": (ValueError, "K values", lambda f8, e: f8.rms_norm(e((4, 256)), e((255,)), 4, 256, 1e-5, y=e((4, 256), H))),
     "norm_without_out": (ValueError, "together",
         lambda f8, e: f8.rms_norm(e((4, 256)), e((256,)), 4, 256, 1e-5, residual=e((4, 256)), y=e((4, 256), H))),
