@@ -153,8 +153,8 @@ HX_INLINE void f8_finish_block(const F8Call& c, const float* v, int rows, int m0
 // consecutive: half h is block h of the span.
 // A workgroup's waves split K, a span each (with fewer spans than waves they also split the tile's rows), and go over tiles of 8 weight rows
 // (of a gated pair: 8 of gate and 8 of up); codes are replaced by the next piece's as soon as they are converted.  One workgroup of 16 waves
-// a CU: 8 rows of 4096 -> 12288 took 12.5 us, 15.1 with two workgroups and 17.8 with two of 8 waves; now 11.5, and 8 rows of 4096 -> 151552 97 us
-// (6.4 TB/s).
+// a CU: 8 rows of 4096 -> 12288 took 12.5 us, 15.1 with two workgroups and 17.8 with two of 8 waves; now 11.4, and 8 rows of 4096 -> 151552
+// 98 us with fp16 outputs (6.3 TB/s), 102 with fp32 outputs.
 // x stays in registers as fp16 where a round of spans is all of K, up to 4096 (from LDS: 1 row of 4096 -> 12288 the same, the pair of 8 rows of
 // 4096 -> 2048 12.2 us where 11.4 are).  Where it is not (FAR), x stays in LDS as codes, piece u of a block of row r at piece u ^ (r & 7), rows a
 // multiple of 1 KB, then its scales, [block][8]: 8 rows of 12288 -> 4096 12.8 us; 20.8 with x loaded again in every round.  (Two spans a wave, so that
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(F8_ROWS_THREADS) void f8_rows_kernel(F8Call a, int 
     const int wk = 1 << wk_log2, kw = wave & (wk - 1), rw = wave >> wk_log2, wr = WAVES >> wk_log2;  // the wave's place in K and in rows
     const int col = lane & 15, kg = lane >> 4, s = col / R, r = col % R;
     const int sums = wk == WAVES ? WAVES + 4 : wk;  // apart in red, where all waves share K: without the 4, banks cost some 500 cycles a tile
-    // Rounds over K; 1 if not FAR, which stays unsaid: without the loop 8 rows of 4096 -> 151552 take 99 us where 97 are.
+    // Rounds over K; 1 if not FAR, which stays unsaid: without the loop 8 rows of 4096 -> 151552 (fp16 outputs) take 99 us where 97 are.
     const int rounds = ((a.kb + 1) / 2 + wk - 1) >> wk_log2;
     const int rows_wg = wr * R, tiles = (a.N + rows_wg - 1) / rows_wg;  // rows_wg: a power of two up to 128
     const int far_row = f8_far_row(a.K), far_r = min(r, a.M - 1);       // rows behind M: any
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(F8_ROWS_THREADS) void f8_rows_kernel(F8Call a, int 
             sw[p][h] = ws[p][min(b, a.kb - 1)];
         }
     };
-    // Workgroups go to the 8 XCDs in turn: neighbouring tiles, which share lines of y, go to one (8 rows of 4096 -> 151552: 97 us; 106 where each
+    // Workgroups go to the 8 XCDs in turn: neighbouring tiles, which share lines of y, go to one (8 rows of 4096 -> 151552, fp16 outputs: 97 us; 106 where each
     // XCD writes parts of all lines).
     const int tile0 = gridDim.x % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
     int tile = tile0;

@@ -30,8 +30,11 @@ constexpr long F8_MOST_TILES = 1l << 22;  // of at most 512 threads
 
 // A tile, how many of its workgroups a CU holds, and what it costs, in us: to begin and end; a step of a workgroup at least; a step of each
 // workgroup on a CU; where K is split, for the join and for each part of it, beside .36 us for each MB of sums.  Fitted to some 400 calls of fp16
-// outputs, 240 of fp32 outputs and 480 of the gated pair (12 to 1500 rows, K and N 2048 to 12288), the model is within 5 % rms, and its choice
-// takes 1 % longer than the best of the tiles and splits on average, 10 % at most.  (45 rows of 8192 -> 4096: 64 x 64 in 4 parts 12.9 us, in 2 parts
+// outputs, 240 of fp32 outputs and 480 of the gated pair (12 to 1500 rows, K and N 2048 to 12288), the model is within 5 % rms there, and its
+// choice takes 1 % longer than the best of the tiles and splits on average, 10 % at most.  Beyond, 45 to 8000 rows with N from 2048 to 24576: from K = 2048 on
+// at most 3 % longer, also over several rounds of tiles; at K = 1024 1 % on average and 13 % at most, at 512 4 and 30 %, at 128 13 and 46 % (2000 rows of
+// 128 -> 8192, gated: 256 x 64 44.7 us, 256 x 256 30.7).  There `start`, charged once, is most of a call, and where tiles go in several rounds the times
+// themselves are too low (8000 rows of 4096 -> 4096: 106 us, 143 to 150 measured).  (45 rows of 8192 -> 4096: 64 x 64 in 4 parts 12.9 us, in 2 parts
 // 18.2, 128 x 64 in 8 parts 14.7; 1000 rows of 4096 -> 4096: 128 x 128 25.7, 64 x 64 38.8, 256 x 256 55.7.)
 struct F8Tile {
     int bn, bm, resident;
