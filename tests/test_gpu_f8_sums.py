@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_gpu_f8 import E4M3, U16, codes, dev, f8, host, inputs, nblocks, product_tolerance, weights  # noqa: F401
+from test_gpu_f8 import E4M3, U16, codes, dev, exact_codes, f8, host, inputs, nblocks, product_tolerance, weights  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +107,76 @@ def test_norm_at_the_ends_of_its_squares(f8, K):
         assert (got[2] == 0).all() and (blocks[2] == 0).all()
         n = 0.5 / np.sqrt(0.25 + eps)
         assert (np.abs(got[3] - n) <= (U16 + (K + 20) * 2.0 ** -24) * n).all()
+
+
+def every_code():
+    """Values of the 256 codes and a tensor of them."""
+    import torch
+    c = torch.arange(256, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    v = np.concatenate([E4M3, [np.nan], -E4M3, [np.nan]])
+    assert np.array_equal(host(c), v, equal_nan=True)
+    return v, c
+
+
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -12])
+@pytest.mark.parametrize("M", [8, 9, 45, 256])
+def test_every_code_by_every_code(f8, M, scale):
+    """One product an output: exact, and in fp16 rounded once, also to values below its smallest normal one."""
+    import torch
+    v, c = every_code()
+    for k in (0, 7, 8, 77):
+        K = 112
+        x, w = (torch.zeros((256, K), dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2))
+        x[:, k], w[:, k] = c, c
+        blocks = f8.F8Blocks(w, torch.full((2, 1), scale, device="cuda"))
+        for m in range(0, 256 - M + 1, M):
+            with np.errstate(invalid="ignore", over="ignore"):
+                want = v[m:m + M, None] * v[None] * scale
+                for dt, nt, exact in ((torch.float32, np.float32, False), (torch.float16, np.float16, False), (torch.float16, np.float16, True)):
+                    y = torch.empty((M, 256), dtype=dt, device="cuda")
+                    f8.gemm(y, x[m:m + M], torch.ones((M, 1), device="cuda"), blocks, M, 256, K, dt == torch.float32, exact=exact)
+                    assert np.array_equal(y.cpu().numpy(), want.astype(nt), equal_nan=True)
+
+
+def test_quantize_of_every_fp16_value(f8):
+    """Each of them beside a largest value of every size, bit for bit."""
+    import torch
+    bits = np.arange(65536, dtype=np.uint16).view(np.float16)
+    v = bits[np.isfinite(bits)]
+    v = np.concatenate([v, np.zeros(-len(v) % 127, np.float16)]).reshape(-1, 127)
+    for top in 2.0 ** np.arange(-24, 16, 3):
+        x = np.concatenate([v, np.full((len(v), 1), top, np.float16)], axis=1)
+        q, s = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device="cuda"), torch.empty((len(x), 1), device="cuda")
+        f8.quantize(dev(x), q, s, len(x), 128)
+        want, ws = exact_codes(x.astype(np.float32))
+        assert np.array_equal(s.cpu().numpy(), ws) and np.array_equal(host(q), want)
+
+
+@pytest.mark.parametrize("M", [9, 45, 300])
+def test_exact_products_in_a_graph(f8, M):
+    """Captured with fp32 outputs and 8-bit products beside them, replayed with eager calls between: every replay as the eager result."""
+    import torch
+    K, N = 4096, 1024
+    w, _ = weights(f8, M, N, K, False)
+    x, xs, _ = inputs(K, M, K, False)
+    ys = [torch.empty((M, N), dtype=t, device="cuda") for t in (torch.float32, torch.float16, torch.float16)]
+
+    def calls():
+        f8.gemm(ys[0], x, xs, w, M, N, K, True)
+        f8.gemm(ys[1], x, xs, w, M, N, K)
+        f8.gemm(ys[2], x, xs, w, M, N, K, exact=True)
+    calls()
+    want = [y.clone() for y in ys]
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        calls()
+    for _ in range(4):
+        for y in ys:
+            y.fill_(7)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(ys, want))
+        calls()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(ys, want))
