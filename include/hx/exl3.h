@@ -309,7 +309,7 @@ int hx_f8_gemm_exact(void* y, const void* x, const float* x_scales, const hx_f8_
 /* Gate and up projections of a feed-forward block and its activation: with g = x gate^T, u = x up^T (fp32),
  *   v = silu(min(g, limit)) * clamp(u, -limit, limit)      q, scales = blocks of v along N, ready for the down projection
  * gate, up: W[N][K], N % 16 == 0; limit > 0 (infinity: no clamp).  g, u from exact products; silu's exponential is the fast one, which puts v off
- * by up to (2 |g| + 8) 2^-24 of its size, |g| after the clamp.  A NaN stays a NaN.  The workspace is needed where
+ * by up to (2 |g| + 8) 2^-24 of its size, and makes silu 0 from g = -88.8 down, where it is below 2^-121.  A NaN stays a NaN.  The workspace is needed where
  * hx_f8_gate_up_workspace_size(M, N, K) is not 0. */
 size_t hx_f8_gate_up_workspace_size(int M, int N, int K);
 int hx_f8_gate_up(void* q, float* scales, const void* x, const float* x_scales, const hx_f8_blocks* gate, const hx_f8_blocks* up,

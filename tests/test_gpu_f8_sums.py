@@ -180,3 +180,25 @@ def test_exact_products_in_a_graph(f8, M):
         calls()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(ys, want))
+
+
+@pytest.mark.parametrize("M", [8, 200])
+def test_gate_over_its_range(f8, M):
+    """silu(g) u by its scales, which keep the one value of a block to two roundings: g of either sign from 2^-20 to 100, u = 2^100 |g|, no clamp.
+    The exponential, sum, quotient and product are off by (2 |g| + 8) 2^-24, and 0 where the exponential passes fp32's range (its last finite value is
+    below exp(88.73)); the scale is rounded twice."""
+    import torch
+    K, N = 16, 16
+    g = np.concatenate([np.geomspace(2.0 ** -20, 100, M - 8), [1, 2, 86, 87, 88, 88.5, 88.9, 99]]).astype(np.float32)[:M]
+    for sign in (-1.0, 1.0):
+        x, gw, uw = np.zeros((M, K)), np.zeros((N, K)), np.zeros((N, K))
+        x[:, 3], gw[:, 3], uw[:, 3] = 1, sign, 1
+        one = torch.ones((1, 1), device="cuda")
+        q, s = torch.empty((M, N), dtype=torch.float8_e4m3fn, device="cuda"), torch.empty((M, 1), device="cuda")
+        f8.gate_up(q, s, codes(x), dev(g[:, None]), f8.F8Blocks(codes(gw), one), f8.F8Blocks(codes(uw), 2.0 ** 100 * one), M, N, K, float("inf"))
+        g64 = sign * g.astype(np.float64)
+        v = np.abs(g64 / (1 + np.exp(-g64)) * g) * 2.0 ** 100
+        got = s.cpu().numpy()[:, 0].astype(np.float64)
+        want = np.where(g64 < -88.73, 2.0 ** -100, v) / 448
+        assert (np.abs(got - want) <= (2 * np.abs(g64) + 10) * 2.0 ** -24 * want).all()
+        assert (np.abs(host(q)[:, 0]) == np.where(g64 < -88.73, 0, 448)).all()
